@@ -230,6 +230,90 @@ JYHIP_API void jyhip_wmat_free(jyhip_wmat* w);
 JYHIP_API int jyhip_wmat_matmul(jyhip_wmat* w, int m, const float* A, float* C);
 JYHIP_API int jyhip_wmat_time(jyhip_wmat* w, const float* x, int iters, double* avg_us);
 
+/* ---- Operators of a decode step over several sequences at once: a paged
+ * key/value cache written and read back, attention of one new token per sequence over it, and
+ * sampling.  The reference decodes one sequence at a time over a contiguous int8 cache
+ * (libs/date_libs/date.h:89-147, libs/model_libs/attention/attention_q8.h:12-184) and samples
+ * by temperature alone on the host (libs/model_libs/generate.h:36, :50-77); these have no
+ * counterpart there.
+ *
+ * All buffers are the caller's and in device memory.  Calls enqueue work on `stream` (a
+ * hipStream_t, NULL for the device's default stream) and return without waiting; they allocate
+ * nothing and can be recorded into a HIP graph.  A call's buffers, its workspace among them,
+ * have to stay as they are until its work is done, and two calls that may run at the same time
+ * need a workspace each.  Status 0, or -1 with the reason in jyhip_last_error(); a refused call
+ * has enqueued nothing.  `device` is the device that the buffers are on; a stream of another
+ * device is refused. */
+
+/* element types */
+enum { JYHIP_T_F32 = 0, JYHIP_T_F16 = 1, JYHIP_T_BF16 = 2, JYHIP_T_I8 = 3 };
+
+/* One layer's pool of pages, `page_size` positions each:
+ *   k, v              [num_pages][num_kv_heads][page_size][head_dim] of `type`
+ *   k_scale, v_scale  fp32 [num_pages][num_kv_heads][page_size] with JYHIP_T_I8, else NULL
+ * head_dim: a multiple of 16 up to 256; page_size: 16, 32, 64, 128 or 256; type: JYHIP_T_I8,
+ * JYHIP_T_F16 or JYHIP_T_BF16.  k and v are aligned to 16 bytes.  An int8 vector holds
+ * q * scale by the rule of jyhip_kv (libs/model_libs/attention/attention_q8.h:29-35): scale =
+ * absmax / 127, q = rint(x * (127 / absmax)), both fp32; zeros where absmax <= 1e-8.  A vector
+ * with an infinity or a NaN in it is held as NaN (scale NaN), all of it. */
+typedef struct jyhip_pages {
+    void* k;
+    void* v;
+    float* k_scale;
+    float* v_scale;
+    int num_pages;
+    int page_size;
+    int num_kv_heads;
+    int head_dim;
+    int type;
+    int device;
+} jyhip_pages;
+
+/* Which page holds a sequence's positions: position p of sequence s lies in slot p % page_size
+ * of page tables[s * table_stride + p / page_size].  An id outside [0, num_pages) is a hole: its
+ * positions do not exist (they are not written, read as zeros, and attention leaves them out).
+ * The same page may stand in several sequences' tables (a shared prefix).  The tables are read on
+ * the device. */
+typedef struct jyhip_page_tables {
+    const int* tables;
+    int num_seqs;
+    int table_stride; /* pages per sequence */
+} jyhip_page_tables;
+
+/* Vectors [row][head][head_dim]: element (r, h, i) at data[r * row_stride + h * head_stride + i]
+ * (strides in elements, not negative). */
+typedef struct jyhip_vectors {
+    void* data;
+    long long row_stride;
+    long long head_stride;
+} jyhip_vectors;
+
+/* Write the keys and values k, v (elements of `type`: JYHIP_T_F32, _F16 or _BF16) of `rows`
+ * positions: row r is position pos[r] of sequence seq[r] (seq NULL: of sequence r).  A row whose
+ * sequence or position does not exist (negative, past the table, a hole) is skipped: so the idle
+ * rows of a padded batch have position -1.  The rows of one call are different positions; where
+ * two name the same slot, that slot's contents are unspecified. */
+JYHIP_API int jyhip_pages_write(const jyhip_pages* pages, const jyhip_page_tables* tables, int rows, const int* seq,
+                                const int* pos, const jyhip_vectors* k, const jyhip_vectors* v, int type,
+                                void* stream);
+
+/* Read the same positions back as values of `type` (zeros for a row that does not exist). */
+JYHIP_API int jyhip_pages_read(const jyhip_pages* pages, const jyhip_page_tables* tables, int rows, const int* seq,
+                               const int* pos, const jyhip_vectors* k, const jyhip_vectors* v, int type, void* stream);
+
+/* Attention of one query row per sequence over the first lens[s] positions of every sequence s of
+ * `tables`: out[s][h] = sum_j softmax_j(scale q[s][h] . k_j) v_j, head h reading kv head
+ * h / (num_heads / num_kv_heads).  q and out are of `type` (JYHIP_T_F32, _F16, _BF16); scores,
+ * softmax and sums are held in fp32.  A sequence without any position (lens[s] <= 0, only holes)
+ * gives zeros.  max_len is an upper bound of lens known on the host: it sizes the launch, and a
+ * longer lens[s] is cut to it.  The workspace needs jyhip_pages_attend_workspace() bytes, aligned
+ * to 16. */
+JYHIP_API int jyhip_pages_attend(const jyhip_pages* pages, const jyhip_page_tables* tables, const int* lens,
+                                 int max_len, int num_heads, float scale, const jyhip_vectors* q,
+                                 const jyhip_vectors* out, int type, void* workspace, size_t workspace_bytes,
+                                 void* stream);
+JYHIP_API size_t jyhip_pages_attend_workspace(const jyhip_pages* pages, int num_seqs, int num_heads, int max_len);
+
 #ifdef __cplusplus
 }
 #endif

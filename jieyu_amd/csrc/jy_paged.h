@@ -1,0 +1,37 @@
+// jy_paged.h — launchers of the paged cache's kernels (jy_paged.hip, jy_paged_attention.hip).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "jieyu_amd.h"
+
+namespace jy {
+
+// which position each row is, and where it lies (jyhip_page_tables with the rows' indices)
+struct PageMap {
+    const int* tables = nullptr;
+    int nseq = 0, stride = 0;
+    const int* seq = nullptr;
+    const int* pos = nullptr;
+};
+
+void launch_paged_write(const jyhip_pages& P, const PageMap& M, int rows, const jyhip_vectors& k,
+                        const jyhip_vectors& v, int type, hipStream_t st);
+void launch_paged_read(const jyhip_pages& P, const PageMap& M, int rows, const jyhip_vectors& k,
+                       const jyhip_vectors& v, int type, hipStream_t st);
+
+struct PagedAttn {
+    jyhip_pages P;
+    PageMap M;                   // tables only: sequence s is row s
+    const int* lens = nullptr;
+    int max_len = 0, nh = 0;
+    float scale = 1.0f;
+    jyhip_vectors q{}, out{};
+    int type = 0;
+    float* part = nullptr;       // paged_attend_part_floats() floats
+};
+size_t paged_attend_part_floats(const jyhip_pages& P, int nseq, int nh, int max_len);
+void launch_paged_attend(const PagedAttn& A, hipStream_t st);
+
+}  // namespace jy

@@ -1,0 +1,182 @@
+// jy_paged.hip — writing and reading the paged key/value cache.
+//
+// A vector (one row's key or value of one head, head_dim elements) belongs to 16 lanes, DL
+// consecutive elements each, so its absolute maximum takes four DPP moves within a row of
+// lanes and its bytes leave as one contiguous run.  Both kernels move each byte once.
+#include <hip/hip_runtime.h>
+
+#include "jy_device.h"
+#include "jy_paged_device.h"
+
+namespace jy {
+
+namespace {
+
+struct Moved {
+    jyhip_pages P;
+    PageMap M;
+    int rows;
+    jyhip_vectors k, v;
+};
+
+// the vector of this group of 16 lanes: (row, K or V, head), heads fastest; false past the end
+struct Item {
+    int row, which, head;
+};
+__device__ __forceinline__ bool item_of(const Moved& A, Item& it) {
+    const int64_t i = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+    const int nkv = A.P.num_kv_heads;
+    if (i >= (int64_t)A.rows * 2 * nkv) return false;
+    it.head = (int)(i % nkv);
+    const int64_t r = i / nkv;
+    it.which = (int)(r & 1);
+    it.row = (int)(r >> 1);
+    return true;
+}
+
+template <int PT, int T, int DL, bool VEC>
+__global__ __launch_bounds__(256) void paged_write_kernel(Moved A) {
+    typedef elem_t<PT> PE;
+    typedef elem_t<T> E;
+    Item it;
+    if (!item_of(A, it)) return;
+    const jyhip_pages& P = A.P;
+    const int lane = threadIdx.x & 15;
+    const int d0 = lane * DL;
+    const bool on = d0 < P.head_dim;
+    const jyhip_vectors& src = it.which ? A.v : A.k;
+    float x[DL];
+    if (on) {
+        load_n<E, DL, VEC>(static_cast<const E*>(src.data) + it.row * src.row_stride + it.head * src.head_stride + d0, x);
+    } else {
+#pragma unroll
+        for (int i = 0; i < DL; i++) x[i] = 0.0f;
+    }
+    const int64_t slot = slot_of(A.M, P.num_pages, P.page_size, A.M.seq ? A.M.seq[it.row] : it.row, A.M.pos[it.row]);
+    if (slot < 0) return;
+    const int64_t page = slot / P.page_size;
+    const int64_t vec = (page * P.num_kv_heads + it.head) * P.page_size + slot % P.page_size;
+    PE* dst = static_cast<PE*>(it.which ? P.v : P.k) + vec * P.head_dim + d0;
+    if constexpr (PT == JYHIP_T_I8) {
+        float a = 0.0f;
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < DL; i++) {
+            a = fmaxf(a, fabsf(x[i]));
+            bad |= !(fabsf(x[i]) <= 3.402823466e38f);
+        }
+        a = fmaxf(a, dpp_f<0xB1>(a));
+        a = fmaxf(a, dpp_f<0x4E>(a));
+        a = fmaxf(a, dpp_f<0x124>(a));
+        a = fmaxf(a, dpp_f<0x128>(a));
+        const unsigned group = threadIdx.x & 48u;
+        bad = ((__ballot(bad) >> group) & 0xffffull) != 0;
+        const float inv = quant_inv(a);
+        if (on) {
+            int8_t q[DL];
+#pragma unroll
+            for (int i = 0; i < DL; i++) q[i] = bad ? (int8_t)0 : quant_i8(x[i], inv);
+            typedef int words __attribute__((ext_vector_type(DL / 4)));
+            *reinterpret_cast<words*>(dst) = __builtin_bit_cast(words, q);
+        }
+        if (lane == 0) (it.which ? P.v_scale : P.k_scale)[vec] = bad ? __builtin_nanf("") : quant_scale(a);
+    } else if (on) {
+        store_n<PE, DL, true>(dst, x);
+    }
+}
+
+template <int PT, int T, int DL, bool VEC>
+__global__ __launch_bounds__(256) void paged_read_kernel(Moved A) {
+    typedef elem_t<PT> PE;
+    typedef elem_t<T> E;
+    Item it;
+    if (!item_of(A, it)) return;
+    const jyhip_pages& P = A.P;
+    const int d0 = (threadIdx.x & 15) * DL;
+    if (d0 >= P.head_dim) return;
+    const int64_t slot = slot_of(A.M, P.num_pages, P.page_size, A.M.seq ? A.M.seq[it.row] : it.row, A.M.pos[it.row]);
+    float x[DL];
+#pragma unroll
+    for (int i = 0; i < DL; i++) x[i] = 0.0f;
+    if (slot >= 0) {
+        const int64_t page = slot / P.page_size;
+        const int64_t vec = (page * P.num_kv_heads + it.head) * P.page_size + slot % P.page_size;
+        load_n<PE, DL, true>(static_cast<const PE*>(it.which ? P.v : P.k) + vec * P.head_dim + d0, x);
+        if constexpr (PT == JYHIP_T_I8) {
+            const float s = (it.which ? P.v_scale : P.k_scale)[vec];
+#pragma unroll
+            for (int i = 0; i < DL; i++) x[i] *= s;
+        }
+    }
+    const jyhip_vectors& dst = it.which ? A.v : A.k;
+    store_n<E, DL, VEC>(static_cast<E*>(dst.data) + it.row * dst.row_stride + it.head * dst.head_stride + d0, x);
+}
+
+// whether every vector starts at a multiple of 16 bytes
+bool aligned(const jyhip_vectors& x, int type) {
+    const long long e = type == JYHIP_T_F32 ? 4 : 2;
+    return ((uintptr_t)x.data | (uintptr_t)(x.row_stride * e) | (uintptr_t)(x.head_stride * e)) % 16 == 0;
+}
+
+template <bool WRITE, int PT, int T, int DL>
+void launch_vec(const Moved& A, bool vec, unsigned grid, hipStream_t st) {
+    if constexpr (WRITE) {
+        if (vec)
+            paged_write_kernel<PT, T, DL, true><<<grid, 256, 0, st>>>(A);
+        else
+            paged_write_kernel<PT, T, DL, false><<<grid, 256, 0, st>>>(A);
+    } else {
+        if (vec)
+            paged_read_kernel<PT, T, DL, true><<<grid, 256, 0, st>>>(A);
+        else
+            paged_read_kernel<PT, T, DL, false><<<grid, 256, 0, st>>>(A);
+    }
+}
+
+template <bool WRITE, int PT, int T>
+void launch_dl(const Moved& A, bool vec, unsigned grid, hipStream_t st) {
+    if (A.P.head_dim <= 64)
+        launch_vec<WRITE, PT, T, 4>(A, vec, grid, st);
+    else if (A.P.head_dim <= 128)
+        launch_vec<WRITE, PT, T, 8>(A, vec, grid, st);
+    else
+        launch_vec<WRITE, PT, T, 16>(A, vec, grid, st);
+}
+
+template <bool WRITE, int PT>
+void launch_io(const Moved& A, int type, bool vec, unsigned grid, hipStream_t st) {
+    if (type == JYHIP_T_F32)
+        launch_dl<WRITE, PT, JYHIP_T_F32>(A, vec, grid, st);
+    else if (type == JYHIP_T_F16)
+        launch_dl<WRITE, PT, JYHIP_T_F16>(A, vec, grid, st);
+    else
+        launch_dl<WRITE, PT, JYHIP_T_BF16>(A, vec, grid, st);
+}
+
+template <bool WRITE>
+void launch_moved(const jyhip_pages& P, const PageMap& M, int rows, const jyhip_vectors& k, const jyhip_vectors& v,
+                  int type, hipStream_t st) {
+    const Moved A{P, M, rows, k, v};
+    const bool vec = aligned(k, type) && aligned(v, type);
+    const unsigned grid = (unsigned)(((int64_t)rows * 2 * P.num_kv_heads + 15) / 16);
+    if (P.type == JYHIP_T_I8)
+        launch_io<WRITE, JYHIP_T_I8>(A, type, vec, grid, st);
+    else if (P.type == JYHIP_T_F16)
+        launch_io<WRITE, JYHIP_T_F16>(A, type, vec, grid, st);
+    else
+        launch_io<WRITE, JYHIP_T_BF16>(A, type, vec, grid, st);
+}
+
+}  // namespace
+
+void launch_paged_write(const jyhip_pages& P, const PageMap& M, int rows, const jyhip_vectors& k,
+                        const jyhip_vectors& v, int type, hipStream_t st) {
+    launch_moved<true>(P, M, rows, k, v, type, st);
+}
+
+void launch_paged_read(const jyhip_pages& P, const PageMap& M, int rows, const jyhip_vectors& k,
+                       const jyhip_vectors& v, int type, hipStream_t st) {
+    launch_moved<false>(P, M, rows, k, v, type, st);
+}
+
+}  // namespace jy

@@ -15,6 +15,7 @@
 #include <vector>
 
 #include "jieyu_amd.h"
+#include "jy_guard.h"
 #include "jy_kernels.h"
 #include "jy_stage.h"
 
@@ -26,20 +27,6 @@ using namespace jy;
 static __device__ __align__(256) unsigned char scratch[JYHIP_NOALLOC_SCRATCH_BYTES];
 
 namespace {
-
-thread_local std::string g_err;
-
-struct Error {
-    std::string msg;
-};
-
-void fail(const std::string& m) { throw Error{m}; }
-
-void ck(hipError_t e, const char* what) {
-    if (e != hipSuccess) fail(std::string(what) + ": " + hipGetErrorString(e));
-}
-
-#define CK(x) ck((x), #x)
 
 template <class T>
 T* dalloc(size_t n, bool zero = true) {
@@ -1712,21 +1699,6 @@ int forward_noalloc(jyhip_model* m, jyhip_kv* kv, float* X, int seq, int start_p
     check_persist(m);
     kv->current_len = start_pos + seq;
     return 0;
-}
-
-template <class F>
-auto guarded(F&& f, decltype(f()) bad) -> decltype(f()) {
-    try {
-        g_err.clear();
-        return f();
-    } catch (const Error& e) {
-        g_err = e.msg;
-    } catch (const std::exception& e) {
-        g_err = e.what();
-    } catch (...) {
-        g_err = "unknown error";
-    }
-    return bad;
 }
 
 }  // namespace
