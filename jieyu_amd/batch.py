@@ -188,7 +188,7 @@ class PagePool:
             raise JyError("attend: one query row for each sequence of the tables")
         if not batch:
             return out
-        need = b.attend_workspace(pages, batch, heads, min(max_len, T.table_stride * self.page_size))
+        need = b.attend_workspace(pages, batch, heads, max_len)
         ws = q.new_empty(need, dtype=b.torch.uint8) if need else None
         if b.attend(pages, T, n, max_len, heads, 1.0 / math.sqrt(self.hd) if scale is None else scale, Q, O, code,
                     ws.data_ptr() if need else None, need, b.stream(self.device).cuda_stream) != 0:

@@ -128,7 +128,7 @@ JYHIP_API int jyhip_pages_read(const jyhip_pages* pages, const jyhip_page_tables
 }
 
 JYHIP_API size_t jyhip_pages_attend_workspace(const jyhip_pages* pages, int num_seqs, int num_heads, int max_len) {
-    if (!pages || num_seqs < 1 || num_heads < 1 || max_len < 1) return 0;
+    if (!pages || num_seqs < 1 || num_heads < 1 || pages->num_kv_heads < 1 || max_len < 1) return 0;
     return paged_attend_part_floats(*pages, num_seqs, num_heads, max_len) * sizeof(float);
 }
 
@@ -151,17 +151,19 @@ JYHIP_API int jyhip_pages_attend(const jyhip_pages* pages, const jyhip_page_tabl
         A.P = *pages;
         A.M = map_of(tables, nullptr, nullptr);
         A.lens = lens;
-        // (positions past the table do not exist)
-        A.max_len = (int)std::min<int64_t>(max_len, (int64_t)tables->table_stride * pages->page_size);
+        A.max_len = max_len;
+        A.cap = (int)std::min<int64_t>(max_len, (int64_t)tables->table_stride * pages->page_size);
         A.nh = num_heads;
         A.scale = scale;
         A.q = *q;
         A.out = *out;
         A.type = type;
         A.part = static_cast<float*>(workspace);
-        const size_t need = paged_attend_part_floats(*pages, tables->num_seqs, num_heads, std::max(A.max_len, 1)) * sizeof(float);
+        const size_t need = paged_attend_part_floats(*pages, tables->num_seqs, num_heads, max_len) * sizeof(float);
         if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
             fail("attend: the workspace must hold " + std::to_string(need) + " bytes, aligned to 16");
+        if (paged_attend_blocks(*pages, tables->num_seqs, num_heads, max_len) >= (1 << 24))
+            fail("attend: too many sequences and heads for one call");
         const OnDevice on(pages->device, (hipStream_t)stream);
         launch_paged_attend(A, (hipStream_t)stream);
         CK(hipGetLastError());

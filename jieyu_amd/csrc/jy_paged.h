@@ -25,13 +25,17 @@ struct PagedAttn {
     jyhip_pages P;
     PageMap M;                   // tables only: sequence s is row s
     const int* lens = nullptr;
-    int max_len = 0, nh = 0;
+    int max_len = 0;             // sizes the launch
+    int cap = 0;                 // positions past it do not exist: the smaller of max_len and the table's
+    int nh = 0;
     float scale = 1.0f;
     jyhip_vectors q{}, out{};
     int type = 0;
     float* part = nullptr;       // paged_attend_part_floats() floats
 };
 size_t paged_attend_part_floats(const jyhip_pages& P, int nseq, int nh, int max_len);
+// workgroups of the larger of its launches (256 threads each)
+int64_t paged_attend_blocks(const jyhip_pages& P, int nseq, int nh, int max_len);
 void launch_paged_attend(const PagedAttn& A, hipStream_t st);
 
 }  // namespace jy
