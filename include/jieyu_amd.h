@@ -314,6 +314,27 @@ JYHIP_API int jyhip_pages_attend(const jyhip_pages* pages, const jyhip_page_tabl
                                  void* stream);
 JYHIP_API size_t jyhip_pages_attend_workspace(const jyhip_pages* pages, int num_seqs, int num_heads, int max_len);
 
+/* One token id for each of `rows` rows of `vocab` logits (of `type`, row r at logits + r *
+ * row_stride elements), from the row's own settings and a given random number u[r] in [0, 1):
+ *   temperature  T <= 0: the largest logit (the lowest index of equal ones), the rest unused;
+ *                else token i has mass e_i = exp((x_i - max x) / T), and the tokens stand in order
+ *                of falling logits, equal ones by index
+ *   top_k        k > 0: the first k stay
+ *   top_p        p < 1: of those, the ones before which less than p of their mass lies (the first
+ *                always stays)
+ *   min_p        m > 0: of those, the ones with e_i >= m (at most 1)
+ * and the id is the lowest index at which the running sum of the staying tokens' masses, in order of
+ * indices, exceeds u[r] times their total.  Masses are fp64, added up as whole numbers (a step is
+ * at most 2^-40 of the largest mass), so a row's id does not depend on the order of additions.
+ * A logit that is NaN or -infinity is never picked; a row of nothing else gives -1.  With +infinity
+ * among the logits, those alone have mass.  Each of temperature, top_k, top_p and min_p may be
+ * NULL: 1, off, off, off.  u outside [0, 1) counts as the nearest value in it, NaN as 0.  vocab is
+ * at most 2^22.  The workspace needs jyhip_sample_workspace() bytes, aligned to 16. */
+JYHIP_API int jyhip_sample(const void* logits, int type, int rows, int vocab, long long row_stride, const float* u,
+                           const float* temperature, const int* top_k, const float* top_p, const float* min_p,
+                           int* ids, void* workspace, size_t workspace_bytes, int device, void* stream);
+JYHIP_API size_t jyhip_sample_workspace(int rows, int vocab);
+
 #ifdef __cplusplus
 }
 #endif

@@ -55,6 +55,8 @@ class _Bound:
         self.attend = proto("jyhip_pages_attend", I, ref(_Pages), ref(_Tables), P, I, I, C.c_float, ref(_Vectors),
                             ref(_Vectors), I, P, C.c_size_t, P)
         self.attend_workspace = proto("jyhip_pages_attend_workspace", C.c_size_t, ref(_Pages), I, I, I)
+        self.sample = proto("jyhip_sample", I, P, I, I, I, LL, P, P, P, P, P, P, P, C.c_size_t, I, P)
+        self.sample_workspace = proto("jyhip_sample_workspace", C.c_size_t, I, I)
         self.error = L.jyhip_last_error
 
 
@@ -196,4 +198,43 @@ class PagePool:
         return out
 
 
-__all__ = ["PagePool"]
+def _settings(b, t, rows, device, dtype, name):
+    """The address of one setting per row (None: off)."""
+    if t is None:
+        return None
+    if t.dtype is not dtype or t.dim() != 1 or t.shape[0] != rows or t.device != device or not t.is_contiguous():
+        raise JyError(f"sample: {name} must be {rows} contiguous {dtype} values on {device}")
+    return t.data_ptr()
+
+
+def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, out=None):
+    """One token id (int32) for each row of logits [rows][vocab] (float32, float16 or bfloat16) from
+    the rows' random numbers u in [0, 1) and settings, device tensors of one value per row: float32
+    temperature (<= 0: the largest logit; None: 1), int32 top_k (<= 0 or None: off), float32 top_p
+    (>= 1 or None: off) and min_p (<= 0 or None: off), applied in this order.  -1 for a row without
+    any logit above -infinity.  jyhip_sample in include/jieyu_amd.h says it to the letter."""
+    b = _bind()
+    torch, dev = b.torch, logits.device
+    code = b.io.get(logits.dtype)
+    if code is None or logits.dim() != 2 or not logits.is_cuda:
+        raise JyError("sample: logits are a device tensor [rows][vocab] in float32, float16 or bfloat16")
+    rows, vocab = logits.shape
+    if vocab and logits.stride(1) != 1:
+        raise JyError("sample: a row's logits must lie side by side")
+    if out is None:
+        out = logits.new_empty(rows, dtype=torch.int32)
+    f = torch.float32
+    args = [_settings(b, u, rows, dev, f, "u"), _settings(b, temperature, rows, dev, f, "temperature"),
+            _settings(b, top_k, rows, dev, torch.int32, "top_k"), _settings(b, top_p, rows, dev, f, "top_p"),
+            _settings(b, min_p, rows, dev, f, "min_p"), _settings(b, out, rows, dev, torch.int32, "out")]
+    if not rows:
+        return out
+    need = b.sample_workspace(rows, vocab)
+    ws = logits.new_empty(need, dtype=torch.uint8) if need else None
+    if b.sample(logits.data_ptr(), code, rows, vocab, logits.stride(0), *args, ws.data_ptr() if need else None, need,
+                dev.index, b.stream(dev).cuda_stream) != 0:
+        _failed(b)
+    return out
+
+
+__all__ = ["PagePool", "sample"]

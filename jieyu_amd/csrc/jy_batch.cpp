@@ -10,6 +10,7 @@
 #include "jieyu_amd.h"
 #include "jy_guard.h"
 #include "jy_paged.h"
+#include "jy_sample.h"
 
 using namespace jy;
 
@@ -166,6 +167,46 @@ JYHIP_API int jyhip_pages_attend(const jyhip_pages* pages, const jyhip_page_tabl
             fail("attend: too many sequences and heads for one call");
         const OnDevice on(pages->device, (hipStream_t)stream);
         launch_paged_attend(A, (hipStream_t)stream);
+        CK(hipGetLastError());
+        return 0;
+    }, -1);
+}
+
+JYHIP_API size_t jyhip_sample_workspace(int rows, int vocab) {
+    if (rows < 1 || vocab < 1 || vocab > SAMPLE_MAX_VOCAB) return 0;
+    return sample_workspace_bytes(rows, vocab);
+}
+
+JYHIP_API int jyhip_sample(const void* logits, int type, int rows, int vocab, long long row_stride, const float* u,
+                           const float* temperature, const int* top_k, const float* top_p, const float* min_p,
+                           int* ids, void* workspace, size_t workspace_bytes, int device, void* stream) {
+    return guarded([&]() {
+        check_type(type);
+        if (rows < 0) fail("rows must not be negative");
+        if (rows == 0) return 0;
+        if (vocab < 1 || vocab > SAMPLE_MAX_VOCAB) fail("sample: vocab must be between 1 and 2^22");
+        if (rows >= 1 << 21) fail("sample: too many rows for one call");
+        if (!logits || !u || !ids) fail("sample: NULL logits, u or ids");
+        if ((uintptr_t)logits % (type == JYHIP_T_F32 ? 4 : 2)) fail("sample: logits are not aligned to their elements");
+        if (row_stride < 0) fail("sample: a negative row stride");
+        SampleArgs A;
+        A.logits = logits;
+        A.row_stride = row_stride;
+        A.type = type;
+        A.rows = rows;
+        A.vocab = vocab;
+        A.u = u;
+        A.temperature = temperature;
+        A.top_k = top_k;
+        A.top_p = top_p;
+        A.min_p = min_p;
+        A.ids = ids;
+        A.ws = static_cast<unsigned char*>(workspace);
+        const size_t need = sample_workspace_bytes(rows, vocab);
+        if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
+            fail("sample: the workspace must hold " + std::to_string(need) + " bytes, aligned to 16");
+        const OnDevice on(device, (hipStream_t)stream);
+        launch_sample(A, (hipStream_t)stream);
         CK(hipGetLastError());
         return 0;
     }, -1);
