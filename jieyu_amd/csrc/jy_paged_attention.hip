@@ -42,24 +42,36 @@ typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
 typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
 
 constexpr float kNone = -3.0e38f;       // the running maximum before any score
+constexpr int kMaxChunk = 4096;          // 64 groups of 16 positions per wave: one lane holds each one's page
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct AttnPlan {
-    int chunk = 0;   // positions per workgroup, a multiple of 128
+    int chunk = 0;   // positions per workgroup, a multiple of 32
     int splits = 1;  // chunks of the longest sequence the launch may see
     int tiles = 1;   // groups of 16 query heads per kv head
 };
 
+// The chunk by the launch's upper bound of its lengths (the lengths themselves are on the device).
+// A workgroup's own start and end cost about as much as 300 positions, two run on a CU at a time,
+// and chunks that one sequence has and another has not are what balances a ragged batch:
+//   up to 1024 positions in one piece: no join (32 x 800 positions of int8 12.1 us, in two 13.7)
+//   512 at least; 1024 where those still make 768 workgroups (16 x 6000 positions of 8 heads of 128
+//   int8 46.3 us against 50.7 with 512; 32 of up to 1500 20.0 us against 18.2, so not there)
+//   2048 workgroups where the batch is longer (64 of 200 to 8190 in bf16: 137 us, with half as
+//   many 145, with twice as many 135; 16 x 12000 84, 81, 84 us)
 AttnPlan plan_of(const jyhip_pages& P, int nseq, int nh, int max_len) {
     AttnPlan p;
     p.tiles = (nh / P.num_kv_heads + 15) / 16;
-    // chunks small enough that the launch has several workgroups per CU to balance sequences of
-    // different lengths, not so small that the joining costs more than it spreads
     const int64_t base = (int64_t)nseq * P.num_kv_heads * p.tiles;
-    const int64_t want = std::max<int64_t>(1, (2048 + base - 1) / base);
-    const int64_t chunk = (max_len + want - 1) / want;
-    p.chunk = (int)std::max<int64_t>(256, (chunk + 127) / 128 * 128);
-    p.splits = std::max(1, (max_len + p.chunk - 1) / p.chunk);
+    if (max_len <= 1024) {
+        p.chunk = 1024;
+        return p;
+    }
+    const int64_t want = std::max<int64_t>(1, 2048 / base);
+    const int64_t least = base * ((max_len + 1023) / 1024) >= 768 ? 1024 : 512;
+    const int64_t chunk = std::max<int64_t>(least, ((max_len + want - 1) / want + 31) / 32 * 32);
+    p.chunk = (int)std::min<int64_t>(chunk, kMaxChunk);
+    p.splits = (max_len + p.chunk - 1) / p.chunk;
     return p;
 }
 
@@ -95,18 +107,37 @@ __device__ __forceinline__ float head_sum(float v) {
     return v;
 }
 
-__device__ __forceinline__ float load_io(const void* p, int64_t i, int type) {
-    return type == JYHIP_T_F32   ? static_cast<const float*>(p)[i]
-           : type == JYHIP_T_F16 ? (float)static_cast<const _Float16*>(p)[i]
-                                 : (float)static_cast<const __bf16*>(p)[i];
+// this lane's elements of a query row p: STEP from STEP (4 c + lane >> 4) for each c, zeros past hd
+// (`on` false: all zeros)
+template <class E, int KC, int STEP>
+__device__ __forceinline__ void load_query(const E* p, int hd, bool on, float (&x)[KC * STEP]) {
+    const int d0 = ((threadIdx.x & 63) >> 4) * STEP;
+#pragma unroll
+    for (int c = 0; c < KC; c++) {
+        const int d = c * 4 * STEP + d0;
+        const E* at = p + (d < hd ? d : 0);  // (hd is a multiple of 16)
+        E v[STEP];
+#pragma unroll
+        for (int e = 0; e < STEP; e++) v[e] = at[e];
+#pragma unroll
+        for (int e = 0; e < STEP; e++) x[c * STEP + e] = on && d < hd ? (float)v[e] : 0.0f;
+    }
 }
-__device__ __forceinline__ void store_io(void* p, int64_t i, int type, float v) {
-    if (type == JYHIP_T_F32)
-        static_cast<float*>(p)[i] = v;
-    else if (type == JYHIP_T_F16)
-        static_cast<_Float16*>(p)[i] = (_Float16)v;
-    else
-        static_cast<__bf16*>(p)[i] = (__bf16)v;
+// o / sum as dims d .. d + 3 of the output of head h of sequence b (zeros without any weight)
+__device__ __forceinline__ void store_out(const PagedAttn& A, int b, int h, int d, const f4_t& o, float sum) {
+    const int64_t at = b * A.out.row_stride + h * A.out.head_stride + d;
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = sum == 0.0f ? 0.0f : o[i] / sum;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if (A.type == JYHIP_T_F32)
+            static_cast<float*>(A.out.data)[at + i] = v[i];
+        else if (A.type == JYHIP_T_F16)
+            static_cast<_Float16*>(A.out.data)[at + i] = (_Float16)v[i];
+        else
+            static_cast<__bf16*>(A.out.data)[at + i] = (__bf16)v[i];
+    }
 }
 
 // the top 16 bits of two fp32 values as a pair of bf16 (truncated): a in the low half
@@ -118,13 +149,13 @@ __device__ __forceinline__ float bf16_cut(float a) {
 }
 
 // The query of 16 heads as B operands of q.k, and the factor that turns their products into
-// scores: PARTS operands for each 16 bytes of a key.
-template <int PT, int KC>
+// scores.  Without WIDE one 16-bit operand holds the query (fp16 or bf16 ones against fp16 keys:
+// scaled, they lose only what lies 2^-40 below the largest element; bf16 ones against bf16 keys).
+template <int PT, int KC, bool WIDE>
 struct Query;
 
-template <int KC>
-struct Query<JYHIP_T_I8, KC> {
-    static constexpr int PARTS = 3;
+template <int KC, bool WIDE>
+struct Query<JYHIP_T_I8, KC, WIDE> {
     i4_t q[KC][3];
     __device__ __forceinline__ void load(const float* x, float amax) {  // x: KC x 16 elements of this lane
         const float inv = amax > 0.0f ? 8323072.0f / amax : 0.0f;       // 127 * 65536
@@ -155,9 +186,10 @@ struct Query<JYHIP_T_I8, KC> {
     }
 };
 
-template <int KC>
-struct Query<JYHIP_T_F16, KC> {
-    h8_t q[KC][2];
+template <int KC, bool WIDE>
+struct Query<JYHIP_T_F16, KC, WIDE> {
+    static constexpr int PARTS = WIDE ? 2 : 1;
+    h8_t q[KC][PARTS];
     // scaled by the power of two that puts the largest element in [2^14, 2^15)
     static __device__ __forceinline__ int exponent(float amax) {
         return amax > 0.0f ? 15 - (int)((__builtin_bit_cast(uint32_t, amax) >> 23) - 126) : 0;
@@ -171,14 +203,14 @@ struct Query<JYHIP_T_F16, KC> {
                 const float v = __builtin_ldexpf(x[c * 8 + e], e2);
                 const _Float16 hi = (_Float16)v;
                 q[c][0][e] = hi;
-                q[c][1][e] = (_Float16)(v - (float)hi);
+                if constexpr (WIDE) q[c][1][e] = (_Float16)(v - (float)hi);
             }
     }
     static __device__ __forceinline__ float factor(float amax) { return __builtin_ldexpf(1.0f, -exponent(amax)); }
     __device__ __forceinline__ void dot(const i4_t (&k)[KC], float (&s)[4]) const {
         f4_t d = {};
 #pragma unroll
-        for (int p = 1; p >= 0; p--)
+        for (int p = PARTS - 1; p >= 0; p--)
 #pragma unroll
             for (int c = 0; c < KC; c++)
                 d = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, k[c]), q[c][p], d, 0, 0, 0);
@@ -187,32 +219,33 @@ struct Query<JYHIP_T_F16, KC> {
     }
 };
 
-template <int KC>
-struct Query<JYHIP_T_BF16, KC> {
-    b8_t q[KC][3];
+template <int KC, bool WIDE>
+struct Query<JYHIP_T_BF16, KC, WIDE> {
+    static constexpr int PARTS = WIDE ? 3 : 1;
+    b8_t q[KC][PARTS];
     __device__ __forceinline__ void load(const float* x, float) {
 #pragma unroll
         for (int c = 0; c < KC; c++) {
-            uint32_t w[3][4];
+            uint32_t w[PARTS][4];
 #pragma unroll
             for (int e = 0; e < 8; e += 2) {
                 float a = x[c * 8 + e], b = x[c * 8 + e + 1];
 #pragma unroll
-                for (int p = 0; p < 3; p++) {
+                for (int p = 0; p < PARTS; p++) {
                     w[p][e >> 1] = bf16_pair(a, b);
                     a -= bf16_cut(a);
                     b -= bf16_cut(b);
                 }
             }
 #pragma unroll
-            for (int p = 0; p < 3; p++) q[c][p] = __builtin_bit_cast(b8_t, u4_t{w[p][0], w[p][1], w[p][2], w[p][3]});
+            for (int p = 0; p < PARTS; p++) q[c][p] = __builtin_bit_cast(b8_t, u4_t{w[p][0], w[p][1], w[p][2], w[p][3]});
         }
     }
     static __device__ __forceinline__ float factor(float) { return 1.0f; }
     __device__ __forceinline__ void dot(const i4_t (&k)[KC], float (&s)[4]) const {
         f4_t d = {};
 #pragma unroll
-        for (int p = 2; p >= 0; p--)
+        for (int p = PARTS - 1; p >= 0; p--)
 #pragma unroll
             for (int c = 0; c < KC; c++)
                 d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8_t, k[c]), q[c][p], d, 0, 0, 0);
@@ -444,10 +477,11 @@ struct State {
     }
 };
 
-template <int PT, int NC>
-__global__ __launch_bounds__(256) void paged_attend_kernel(AttnKernelArgs K) {
+template <int PT, int NC, bool WIDE>
+__global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void paged_attend_kernel(AttnKernelArgs K) {
 #if defined(__HIP_DEVICE_COMPILE__)
     typedef Tile<PT, NC> T;
+    typedef Query<PT, T::KC, WIDE> Q;
     constexpr int DL = 4 * NC, ES = T::ES, STEP = 16 / ES;
     constexpr int ROW = 64 * NC + 4;
     __shared__ float so[4][16][ROW];
@@ -456,61 +490,45 @@ __global__ __launch_bounds__(256) void paged_attend_kernel(AttnKernelArgs K) {
     const jyhip_pages& P = A.P;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int hd = P.head_dim, nkv = P.num_kv_heads, per = A.nh / nkv;
-    // blocks: chunks fastest, then head groups, kv heads, sequences
+    // Blocks: heads fastest, then sequences, then chunks.  Blocks go round the XCDs in turn, and
+    // short sequences have first chunks alone: with chunks fastest those met on two of the eight.
     unsigned id = blockIdx.x;
-    const int split = id % K.plan.splits;
-    id /= K.plan.splits;
-    const int tile = id % K.plan.tiles;
-    id /= K.plan.tiles;
-    const int kvh = id % nkv, b = id / nkv;
-    const int n = min(A.lens[b], A.cap);
+    const int hg = id % (nkv * K.plan.tiles);
+    id /= nkv * K.plan.tiles;
+    const int b = id % A.M.nseq, split = id / A.M.nseq;
+    const int kvh = hg / K.plan.tiles, tile = hg % K.plan.tiles;
     const int c0 = split * K.plan.chunk;
-    if (c0 >= n && !(split == 0)) return;
-    const int end = min(n, c0 + K.plan.chunk);
     const int h0 = kvh * per + tile * 16, heads = min(16, per - tile * 16);
 
-    // the query: this lane's head, its dims of every 16-byte step
-    Query<PT, T::KC> q;
-    float qf;
+    // the page of each of the wave's groups of 16 positions: lane 2i + g has that of group g of its
+    // i-th tile (past the sequence's end as well: whether a position exists is settled below)
+    int ids = -1;
     {
-        float x[T::KC * STEP];
-        float amax = 0.0f;
-        bool bad = false;
-        const bool on = (lane & 15) < heads;
-        const int64_t base = b * A.q.row_stride + (h0 + (on ? lane & 15 : 0)) * A.q.head_stride;
-#pragma unroll
-        for (int c = 0; c < T::KC; c++)
-#pragma unroll
-            for (int e = 0; e < STEP; e++) {
-                const int d = c * 4 * STEP + (lane >> 4) * STEP + e;
-                const float v = on && d < hd ? load_io(A.q.data, base + d, A.type) : 0.0f;
-                x[c * STEP + e] = v;
-                amax = fmaxf(amax, fabsf(v));
-                bad |= !(fabsf(v) <= 3.402823466e38f);
-            }
-        amax = head_max(amax);
-        bad = head_max(bad ? 1.0f : 0.0f) > 0.0f;
-        if (bad) {
-#pragma unroll
-            for (int i = 0; i < T::KC * STEP; i++) x[i] = 0.0f;
-            amax = 0.0f;
-        }
-        q.load(x, amax);
-        qf = bad ? __builtin_nanf("") : q.factor(amax) * (A.scale * kLog2e);
+        const int at = (c0 + (wave + 4 * (lane >> 1)) * 32 + 16 * (lane & 1)) >> K.ps_log2;
+        if (at < A.M.stride) ids = A.M.tables[(int64_t)b * A.M.stride + at];
     }
+    const int n = min(A.lens[b], A.cap);
+    const bool on = (lane & 15) < heads;
+    const int64_t qbase = b * A.q.row_stride + (h0 + (on ? lane & 15 : 0)) * A.q.head_stride;
+    float x[T::KC * STEP];
+    if (A.type == JYHIP_T_F32)
+        load_query<float, T::KC, STEP>(static_cast<const float*>(A.q.data) + qbase, hd, on, x);
+    else if (A.type == JYHIP_T_F16)
+        load_query<_Float16, T::KC, STEP>(static_cast<const _Float16*>(A.q.data) + qbase, hd, on, x);
+    else
+        load_query<__bf16, T::KC, STEP>(static_cast<const __bf16*>(A.q.data) + qbase, hd, on, x);
+    if (c0 >= n && split != 0) return;
 
     Loader<PT, NC> ld;
-    ld.k = static_cast<const char*>(P.k);
-    ld.v = static_cast<const char*>(P.v);
+    const int64_t first = (int64_t)kvh * P.page_size;  // this head's first position in page 0
+    ld.k = static_cast<const char*>(P.k) + first * (hd * ES);
+    ld.v = static_cast<const char*>(P.v) + first * (hd * ES);
+    ld.ks = PT == JYHIP_T_I8 ? P.k_scale + first : nullptr;
+    ld.vs = PT == JYHIP_T_I8 ? P.v_scale + first : nullptr;
     ld.head_stride = (int64_t)nkv * P.page_size;
     ld.num_pages = P.num_pages;
     ld.ps = P.page_size;
     ld.hd = hd;
-    const int64_t first = (int64_t)kvh * P.page_size;  // this head's first position in page 0
-    ld.k += first * (hd * ES);
-    ld.v += first * (hd * ES);
-    ld.ks = PT == JYHIP_T_I8 ? P.k_scale + first : nullptr;
-    ld.vs = PT == JYHIP_T_I8 ? P.v_scale + first : nullptr;
 #pragma unroll
     for (int c = 0; c < T::KC; c++) {
         int d = c * 4 * STEP + (lane >> 4) * STEP;
@@ -522,30 +540,45 @@ __global__ __launch_bounds__(256) void paged_attend_kernel(AttnKernelArgs K) {
         if (d >= hd) d = 0;  // (outputs past the head's end are not stored)
         ld.voff = (unsigned)(((lane >> 4) * 4 * hd + d) * ES);
     }
-
-    State<PT, NC> st;
+    const int end = min(n, c0 + K.plan.chunk);
     const int ntiles = end > c0 ? (end - c0 + 31) / 32 : 0;
-    const int* table = A.M.tables + (int64_t)b * A.M.stride;
-    // 64 page ids at a time: lane 2i + g holds the page of group g of the wave's i-th tile
-    int ids = -1;
-    auto fetch_ids = [&](int t0) {
-        const int key = c0 + (t0 + 4 * (lane >> 1)) * 32 + 16 * (lane & 1);
-        ids = key < end ? table[key >> K.ps_log2] : -1;
-    };
-    auto load = [&](T& t, int i, int tl) {
+    const int cnt = (ntiles - wave + 3) / 4;  // (not positive for a wave without any)
+    auto load = [&](T& t, int i) {
         const int p0 = __builtin_amdgcn_readlane(ids, 2 * i), p1 = __builtin_amdgcn_readlane(ids, 2 * i + 1);
-        ld.load(t, p0, p1, c0 + tl * 32, end);
+        ld.load(t, p0, p1, c0 + (wave + 4 * i) * 32, end);
     };
-    for (int t0 = wave; t0 < ntiles; t0 += 128) {
-        fetch_ids(t0);
-        const int cnt = min(32, (ntiles - t0 + 3) / 4);
-        T cur, nxt;
-        load(cur, 0, t0);
-        for (int i = 0; i < cnt; i++) {
-            if (i + 1 < cnt) load(nxt, i + 1, t0 + 4 * (i + 1));
-            st.add(q, qf, cur);
-            cur = nxt;
+    T t0, t1;
+    if (cnt > 0) load(t0, 0);
+    if (cnt > 1) load(t1, 1);
+
+    // the query as operands, while the first positions are on their way
+    Q q;
+    float qf;
+    {
+        float amax = 0.0f;
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < T::KC * STEP; i++) {
+            amax = fmaxf(amax, fabsf(x[i]));
+            bad |= !(fabsf(x[i]) <= 3.402823466e38f);
         }
+        amax = head_max(amax);
+        bad = head_max(bad ? 1.0f : 0.0f) > 0.0f;
+        if (bad) {
+#pragma unroll
+            for (int i = 0; i < T::KC * STEP; i++) x[i] = 0.0f;
+            amax = 0.0f;
+        }
+        q.load(x, amax);
+        qf = bad ? __builtin_nanf("") : q.factor(amax) * (A.scale * kLog2e);
+    }
+    State<PT, NC> st;
+    for (int i = 0; i < cnt; i += 2) {
+        st.add(q, qf, t0);
+        if (i + 1 >= cnt) break;
+        if (i + 2 < cnt) load(t0, i + 2);
+        st.add(q, qf, t1);
+        if (i + 3 < cnt) load(t1, i + 3);
     }
 
     // join the waves
@@ -561,22 +594,29 @@ __global__ __launch_bounds__(256) void paged_attend_kernel(AttnKernelArgs K) {
         sl[wave][g] = st.l;
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < heads * hd; e += 256) {
-        const int r = e / hd, d = e - r * hd;
-        const float mx = fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r]));
-        float sum = 0.0f, acc = 0.0f;
+    const int quads = hd / 4;
+    for (int e = threadIdx.x; e < heads * quads; e += 256) {
+        const int r = e / quads, d = 4 * (e - r * quads);
+        float m[4], f[4], sum = 0.0f, mx = kNone;
+        f4_t acc = {};
 #pragma unroll
         for (int w = 0; w < 4; w++) {
-            const float f = State<PT, NC>::exp2_hw(sm[w][r] - mx);
-            sum += f * sl[w][r];
-            acc += f * so[w][r][d];
+            m[w] = sm[w][r];
+            mx = fmaxf(mx, m[w]);
+        }
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            f[w] = State<PT, NC>::exp2_hw(m[w] - mx);
+            sum += f[w] * sl[w][r];
+            const f4_t o = *reinterpret_cast<const f4_t*>(&so[w][r][d]);
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[i] += f[w] * o[i];
         }
         const int64_t row = (int64_t)b * A.nh + h0 + r;
         if (K.plan.splits == 1) {
-            store_io(A.out.data, b * A.out.row_stride + (h0 + r) * A.out.head_stride + d, A.type,
-                     sum == 0.0f ? 0.0f : acc / sum);
+            store_out(A, b, h0 + r, d, acc, sum);
         } else {
-            K.part_o[(row * K.plan.splits + split) * hd + d] = acc;
+            *reinterpret_cast<f4_t*>(K.part_o + (row * K.plan.splits + split) * hd + d) = acc;
             if (d == 0) K.part_ml[row * K.plan.splits + split] = float2{mx, sum};
         }
     }
@@ -584,72 +624,85 @@ __global__ __launch_bounds__(256) void paged_attend_kernel(AttnKernelArgs K) {
 }
 
 // One workgroup per (sequence, query head): the chunks' outputs weighted by 2^(m - max m) over the
-// sum of their weighted sums, in the chunks' order.  hd / 4 threads read one chunk's output, the
-// others the next ones'.
-__global__ __launch_bounds__(256) void paged_join_kernel(AttnKernelArgs K) {
+// sum of their weighted sums.  hd / 4 threads read one chunk's output, the others the next ones',
+// each with a running maximum of its own (so the first outputs are read before the sequence's
+// length is known), joined through LDS in a fixed order.
+template <int NT>
+__global__ __launch_bounds__(NT) void paged_join_kernel(AttnKernelArgs K) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    __shared__ float4 so[256];
-    __shared__ float ss[256];
+    __shared__ f4_t so[NT];
+    __shared__ float sm[NT], ss[NT];
     const PagedAttn& A = K.A;
     const int row = blockIdx.x, b = row / A.nh, h = row % A.nh, hd = A.P.head_dim;
-    const int n = min(A.lens[b], A.cap);
-    const int live = max(1, (max(n, 0) + K.plan.chunk - 1) / K.plan.chunk);
     const int splits = K.plan.splits;
-    const float2* ml = K.part_ml + (int64_t)row * splits;
-    const float* po = K.part_o + (int64_t)row * splits * hd;
-    float mx = kNone;
-    for (int i = threadIdx.x & 63; i < live; i += 64) mx = fmaxf(mx, ml[i].x);
-    mx = head_max(mx);
-    mx = fmaxf(mx, dpp_f<0xB1>(mx));
-    mx = fmaxf(mx, dpp_f<0x4E>(mx));
-    mx = fmaxf(mx, dpp_f<0x124>(mx));
-    mx = fmaxf(mx, dpp_f<0x128>(mx));
-    const int quads = hd / 4, groups = 256 / quads;
+    const int quads = hd / 4, groups = NT / quads;
     const int gi = threadIdx.x / quads, d4 = threadIdx.x % quads;
-    float4 acc = {0, 0, 0, 0};
-    float sum = 0.0f;
-    if (gi < groups) {
-#pragma unroll 4
-        for (int i = gi; i < live; i += groups) {
-            const float2 x = ml[i];
-            const float f = __builtin_amdgcn_exp2f(x.x - mx);
-            const float4 o = *reinterpret_cast<const float4*>(po + (int64_t)i * hd + 4 * d4);
-            sum += f * x.y;
-            acc.x += f * o.x;
-            acc.y += f * o.y;
-            acc.z += f * o.z;
-            acc.w += f * o.w;
-        }
-    }
-    so[threadIdx.x] = acc;
-    ss[threadIdx.x] = sum;
-    __syncthreads();
-    if (gi == 0) {
-        for (int w = 1; w < groups; w++) {
-            const float4 o = so[w * quads + d4];
-            sum += ss[w * quads + d4];
-            acc.x += o.x;
-            acc.y += o.y;
-            acc.z += o.z;
-            acc.w += o.w;
-        }
-        const int64_t at = b * A.out.row_stride + h * A.out.head_stride + 4 * d4;
-        const float v[4] = {acc.x, acc.y, acc.z, acc.w};
+    const float2* ml = K.part_ml + (int64_t)row * splits;
+    const float* po = K.part_o + (int64_t)row * splits * hd + 4 * d4;
+    float2 x[4];
+    f4_t o[4];
+    auto read = [&](int i) {  // chunks i, i + groups, ...: those that are live are told apart in use
 #pragma unroll
-        for (int i = 0; i < 4; i++) store_io(A.out.data, at + i, A.type, sum == 0.0f ? 0.0f : v[i] / sum);
+        for (int j = 0; j < 4; j++) {
+            const int at = min(i + j * groups, splits - 1);
+            x[j] = ml[at];
+            o[j] = *reinterpret_cast<const f4_t*>(po + (int64_t)at * hd);
+        }
+    };
+    read(gi);
+    const int n = min(A.lens[b], A.cap);
+    const int live = gi < groups ? max(1, (max(n, 0) + K.plan.chunk - 1) / K.plan.chunk) : 0;
+    f4_t acc = {};
+    float sum = 0.0f, m = kNone;
+    auto add = [&](float mo, float so1, const f4_t& oo) {  // one more part into (m, sum, acc)
+        const float mn = fmaxf(m, mo);
+        const float a = __builtin_amdgcn_exp2f(m - mn), f = __builtin_amdgcn_exp2f(mo - mn);
+        m = mn;
+        sum = sum * a + f * so1;
+#pragma unroll
+        for (int c = 0; c < 4; c++) acc[c] = acc[c] * a + f * oo[c];
+    };
+    for (int i = gi; i < live; i += 4 * groups) {
+        if (i != gi) read(i);
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (i + j * groups < live) add(x[j].x, x[j].y, o[j]);
     }
+    // two rounds: every eighth group's threads take their seven neighbours', then the first group's
+    // take those
+    for (int step = 1; step < groups; step *= 8) {
+        so[threadIdx.x] = acc;
+        sm[threadIdx.x] = m;
+        ss[threadIdx.x] = sum;
+        __syncthreads();
+        if (gi % (8 * step) == 0)
+            for (int w = gi + step; w < min(gi + 8 * step, groups); w += step)
+                add(sm[w * quads + d4], ss[w * quads + d4], so[w * quads + d4]);
+        __syncthreads();
+    }
+    if (gi == 0) store_out(A, b, h, 4 * d4, acc, sum);
 #endif
 }
 
-template <int PT>
+template <int PT, bool WIDE>
 void launch_nc(const AttnKernelArgs& K, unsigned grid, hipStream_t st) {
     const int hd = K.A.P.head_dim;
     if (hd <= 64)
-        paged_attend_kernel<PT, 1><<<grid, 256, 0, st>>>(K);
+        paged_attend_kernel<PT, 1, WIDE><<<grid, 256, 0, st>>>(K);
     else if (hd <= 128)
-        paged_attend_kernel<PT, 2><<<grid, 256, 0, st>>>(K);
+        paged_attend_kernel<PT, 2, WIDE><<<grid, 256, 0, st>>>(K);
     else
-        paged_attend_kernel<PT, 4><<<grid, 256, 0, st>>>(K);
+        paged_attend_kernel<PT, 4, WIDE><<<grid, 256, 0, st>>>(K);
+}
+
+// WIDE: a query that one 16-bit operand cannot hold (fp32, and fp16 against bf16 keys); the int8
+// form's digits hold any
+template <int PT>
+void launch_wide(const AttnKernelArgs& K, unsigned grid, hipStream_t st) {
+    if (PT == JYHIP_T_I8 || K.A.type == JYHIP_T_F32 || (PT == JYHIP_T_BF16 && K.A.type == JYHIP_T_F16))
+        launch_nc<PT, true>(K, grid, st);
+    else if constexpr (PT != JYHIP_T_I8)
+        launch_nc<PT, false>(K, grid, st);
 }
 
 }  // namespace
@@ -674,12 +727,19 @@ void launch_paged_attend(const PagedAttn& A, hipStream_t st) {
     K.part_ml = reinterpret_cast<float2*>(A.part + (size_t)A.M.nseq * A.nh * K.plan.splits * A.P.head_dim);
     const unsigned grid = (unsigned)((int64_t)A.M.nseq * A.P.num_kv_heads * K.plan.tiles * K.plan.splits);
     if (A.P.type == JYHIP_T_I8)
-        launch_nc<JYHIP_T_I8>(K, grid, st);
+        launch_wide<JYHIP_T_I8>(K, grid, st);
     else if (A.P.type == JYHIP_T_F16)
-        launch_nc<JYHIP_T_F16>(K, grid, st);
+        launch_wide<JYHIP_T_F16>(K, grid, st);
     else
-        launch_nc<JYHIP_T_BF16>(K, grid, st);
-    if (K.plan.splits > 1) paged_join_kernel<<<(unsigned)(A.M.nseq * A.nh), 256, 0, st>>>(K);
+        launch_wide<JYHIP_T_BF16>(K, grid, st);
+    if (K.plan.splits > 1) {
+        // four chunks a thread are read at once: more threads where those are not all
+        const unsigned rows = (unsigned)(A.M.nseq * A.nh);
+        if (K.plan.splits * (A.P.head_dim / 4) <= 4 * 256)
+            paged_join_kernel<256><<<rows, 256, 0, st>>>(K);
+        else
+            paged_join_kernel<1024><<<rows, 1024, 0, st>>>(K);
+    }
 }
 
 }  // namespace jy
