@@ -14,7 +14,7 @@
 //   1  the largest logit, and the maxima of 1024 parts of the row: the k-th largest of those is at
 //      most the k-th largest logit, so it bounds the top-k candidates from below
 //   2  top-k: the candidates into a list; else the masses of blocks of 2048 tokens, or with top-p a
-//      histogram of mass over the distance to M (39 bins per factor of two)
+//      histogram of mass over the distance to M (32 bins per factor of two)
 //   3  top-p: the masses of the blocks above the bin that the border lies in, that bin's tokens
 //      into the list
 //   4  one workgroup per row: the border among the list's tokens, then the block and the token in
@@ -40,7 +40,9 @@ constexpr int LIST = 8192;          // tokens of a row's list
 constexpr int BLOCK = 2048;         // tokens per partial mass
 constexpr int STRIPES = 1024;       // parts whose maxima bound the k-th largest logit
 constexpr int MAX_SEGS = 64;
-constexpr double BINS_PER_OCTAVE = 39.0;  // masses below 2^-52 round to nothing: 52 * 39 < BINS
+constexpr int STEPS = 512;          // table entries per factor of two of mass
+constexpr int PER_BIN = 16;         // of them in a histogram bin: masses under 2^-52 are none, 53 * 512 / 16 < BINS
+constexpr int STAGE = 1024;         // list entries a workgroup collects before it takes places for them
 
 enum { ROW_GREEDY, ROW_TOPK, ROW_MASS, ROW_NUCLEUS, ROW_ALONE };
 
@@ -117,54 +119,113 @@ __device__ __forceinline__ Set set_of(const SampleArgs& A, int row) {
 
 __device__ constexpr u64 kExp2[32] = JY_EXP2_TABLE;
 
-// masses of a row's logits.  2^y = 2^(j/32) 2^r, |r| <= 1/64: the table entry (2^(j/32) less j << 47
-// in its bits, so adding j << 47 gives any j) times a polynomial of degree 5 (the Taylor terms of
-// 2^r; the rest is under 2.3e-15).
+// Masses of a row's logits, e 2^s.  With y = 512 (x - M) log2 e / T = k + r, k whole and |r| <= 1/2:
+// 2^(k/512) from a table of 512 (2^s in it) and the exponent, times the Taylor terms of 2^(r/512) up
+// to r^3 (the rest is under 9e-15).
 struct Masses {
-    float M;
-    double c;        // log2 e / T
+    float M, low;    // low: the logit whose mass is far under 2^-52, standing for all below it and NaN
+    double c;        // 512 log2 e / T
     double unit;     // 2^s
-    u64 unit_bits;   // s << 52
-    const u64* tab;
-    __device__ __forceinline__ void set(float top, float T, int vocab, const u64* table) {
+    const u64* tab;  // [STEPS]
+    // false: the largest logit is infinite or T so large that no such logit is finite (then c is 0
+    // or M infinite, and only pick_alone() takes the row)
+    __device__ __forceinline__ bool set(float top, float T, int vocab, const u64* table) {
         M = top;
-        c = 1.4426950408889634074 / (double)T;
+        c = 512.0 * 1.4426950408889634074 / (double)T;
+        low = (float)((double)M - 64.0 * 512.0 / c);
         int s = 51;
         while (s > 40 && (1ll << (62 - s)) < vocab) s--;
-        unit_bits = (u64)s << 52;
         unit = (double)(1ull << s);
         tab = table;
+        return M < __builtin_inff() && low > -3.4e38f;
     }
-    // log2 of the mass; NaN or under -64 where there is none
-    __device__ __forceinline__ double y(float l) const { return l == M ? 0.0 : ((double)l - (double)M) * c; }
-    // the mass times 2^s
-    __device__ __forceinline__ double scaled(double y) const {
-        if (!(y > -64.0)) return 0.0;
+    // entry i of the table: 2^(i/512) 2^s, from 2^(j/32) (its bits less j << 47, so adding any
+    // j << 47 gives 2^(j/32)) and the Taylor terms of 2^r, |r| <= 1/64, up to r^5 (the rest is
+    // under 2.3e-15)
+    __device__ __forceinline__ void fill(u64* table) const {
+        for (int i = threadIdx.x; i < STEPS; i += blockDim.x) table[i] = __builtin_bit_cast(u64, unit * exp2_slow(i / 512.0));
+    }
+    static __device__ __forceinline__ double exp2_slow(double y) {
         const double shift = 0x1.8p+52;
         double kd = __builtin_fma(y, 32.0, shift);
         const u64 ki = __builtin_bit_cast(u64, kd);
         kd -= shift;
         const double r = __builtin_fma(kd, -0.03125, y);
-        const double t = __builtin_bit_cast(double, tab[ki & 31u] + (ki << 47) + unit_bits);
         double q = __builtin_fma(r, 0.0013333558146428443, 0.0096181291076284772);
         q = __builtin_fma(q, r, 0.055504108664821580);
         q = __builtin_fma(q, r, 0.24022650695910071);
         q = __builtin_fma(q, r, 0.69314718055994531);
         q = __builtin_fma(q, r, 1.0);
-        return q * t;
+        return q * __builtin_bit_cast(double, kExp2[ki & 31u] + (ki << 47));
     }
+    struct At {
+        double r;
+        int k;  // <= 0
+        __device__ __forceinline__ int bin() const { return (unsigned)-k / PER_BIN; }
+    };
+    // l within [low, M], NaN as low
+    __device__ __forceinline__ float clamp(float l) const {
+#if defined(__HIP_DEVICE_COMPILE__)
+        return __builtin_amdgcn_fmed3f(l, low, M);
+#else
+        return l;
+#endif
+    }
+    __device__ __forceinline__ At at(float l) const {
+        const double y = ((double)clamp(l) - (double)M) * c;
+        const double shift = 0x1.8p+52;
+        const double kd = y + shift;
+        return At{y - (kd - shift), (int)(uint32_t)__builtin_bit_cast(u64, kd)};
+    }
+    __device__ __forceinline__ double scaled(const At& a) const {
+        constexpr double L = 0.69314718055994531 / 512.0;
+        double q = __builtin_fma(a.r, L * L * L / 6.0, L * L / 2.0);
+        q = __builtin_fma(q, a.r, L);
+        q = __builtin_fma(q, a.r, 1.0);
+        const u64 t = tab[a.k & (STEPS - 1)] + ((u64)(uint32_t)((a.k >> 9) << 20) << 32);
+        return q * __builtin_bit_cast(double, t);
+    }
+    __device__ __forceinline__ double scaled(float l) const { return scaled(at(l)); }
     // the nearest whole number of a scaled mass (under 2^52)
     static __device__ __forceinline__ u64 whole(double scaled) {
         return __builtin_bit_cast(u64, scaled + 0x1p+52) & 0xfffffffffffffull;
     }
-    __device__ __forceinline__ u64 mass(float l) const { return whole(scaled(y(l))); }
-    static __device__ __forceinline__ int bin(double y) { return (int)(y * -BINS_PER_OCTAVE); }
+    __device__ __forceinline__ u64 mass(float l) const { return whole(scaled(l)); }
+    // the same for any M and T
+    __device__ __forceinline__ double scaled_any(float l) const {
+        if (l == M) return unit;
+        if (!(l > -__builtin_inff()) || M == __builtin_inff()) return 0.0;
+        const double y = ((double)l - (double)M) * (c / 512.0);
+        return y > -64.0 ? unit * exp2_slow(y) : 0.0;
+    }
+    __device__ __forceinline__ u64 mass_any(float l) const { return whole(scaled_any(l)); }
 };
 
 // the sum of v over the wave, in every lane (whole numbers: any order)
-__device__ __forceinline__ u64 wave_sum(u64 v) {
-    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
+template <int CTRL>
+__device__ __forceinline__ u64 dpp_u64(u64 v) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, 0xf, 0xf, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, 0xf, 0xf, false);
+    return (u64)hi << 32 | lo;
+#else
     return v;
+#endif
+}
+__device__ __forceinline__ u64 lane_u64(u64 v, int lane) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+#else
+    return v;
+#endif
+}
+__device__ __forceinline__ u64 wave_sum(u64 v) {
+    v += dpp_u64<0xB1>(v);
+    v += dpp_u64<0x4E>(v);
+    v += dpp_u64<0x124>(v);
+    v += dpp_u64<0x128>(v);  // every lane: its row of 16's sum
+    return lane_u64(v, 0) + lane_u64(v, 16) + lane_u64(v, 32) + lane_u64(v, 48);
 }
 
 // VL consecutive logits from index i (those at or past `end` as NaN, which has no mass)
@@ -224,16 +285,52 @@ __device__ __forceinline__ void row_top(const RowWs& w, int segs, float& top, in
     }
 }
 
-// n of the wave's lanes add a list entry each
-__device__ __forceinline__ void append(const RowWs& w, bool mine, u64 entry) {
-    const u64 who = __ballot(mine);
-    if (!who) return;
-    const int lane = threadIdx.x & 63, lead = __builtin_ctzll(who);
-    uint32_t at = 0;
-    if (lane == lead) at = atomicAdd(w.count, (uint32_t)__popcll(who));
-    at = __shfl(at, lead) + __popcll(who & ((1ull << lane) - 1));
-    if (mine && at < LIST) w.list[at] = entry;
-}
+// list entries of a workgroup: collected in LDS (one atomic on the row's counter for all of them),
+// the ones that find it full go to the list by themselves
+struct Stage {
+    u64 entry[STAGE];
+    uint32_t n, at;
+    __device__ __forceinline__ void clear() {
+        if (threadIdx.x == 0) n = 0;
+    }
+    // those of a lane's N entries that are marked, from any of a wave's lanes: one place for each
+    template <int N, class F>
+    __device__ __forceinline__ void add(const RowWs& w, const bool (&mine)[N], F&& of) {
+        u64 who[N];
+        int total = 0;
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+            who[e] = __ballot(mine[e]);
+            total += __popcll(who[e]);
+        }
+        if (!total) return;
+        const u64 below = (1ull << (threadIdx.x & 63)) - 1;
+        uint32_t i = 0;
+        if ((threadIdx.x & 63) == 0) i = atomicAdd(&n, (uint32_t)total);
+        i = __builtin_amdgcn_readfirstlane(i);
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+            if (mine[e]) {
+                const uint32_t j = i + __popcll(who[e] & below);
+                if (j < STAGE) {
+                    entry[j] = of(e);
+                } else {
+                    const uint32_t g = atomicAdd(w.count, 1u);
+                    if (g < LIST) w.list[g] = of(e);
+                }
+            }
+            i += __popcll(who[e]);
+        }
+    }
+    __device__ __forceinline__ void flush(const RowWs& w) {
+        __syncthreads();
+        const uint32_t m = min(n, (uint32_t)STAGE);
+        if (threadIdx.x == 0 && m) at = atomicAdd(w.count, m);
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < m; i += NP)
+            if (at + i < LIST) w.list[at + i] = entry[i];
+    }
+};
 
 // ---- 1: the parts' largest logits
 template <class E>
@@ -246,9 +343,6 @@ __global__ __launch_bounds__(NP) void sample_top_kernel(SampleArgs A, SamplePlan
     const RowWs w = row_ws(A, P, row);
     const Set s = set_of(A, row);
     const int i0 = seg * P.seg_len, i1 = min(i0 + P.seg_len, A.vocab);
-    if (s.mode == ROW_NUCLEUS)
-        for (int i = seg * NP + threadIdx.x; i < BINS; i += P.segs * NP) w.hist[i] = 0;
-    if (seg == 0 && threadIdx.x == 0) *w.count = 0;
     // each thread two maxima (even and odd elements): 1024 parts of the segment
     float top[2] = {-__builtin_inff(), -__builtin_inff()};
     int at = -1;
@@ -260,6 +354,9 @@ __global__ __launch_bounds__(NP) void sample_top_kernel(SampleArgs A, SamplePlan
             top[e & 1] = fmaxf(top[e & 1], l[e]);
         }
     });
+    if (s.mode == ROW_NUCLEUS)
+        for (int i = seg * NP + threadIdx.x; i < BINS; i += P.segs * NP) w.hist[i] = 0;
+    if (seg == 0 && threadIdx.x == 0) *w.count = 0;
     if (s.mode == ROW_TOPK) {
         part[threadIdx.x] = top[0];
         part[NP + threadIdx.x] = top[1];
@@ -297,31 +394,46 @@ __global__ __launch_bounds__(NP) void sample_top_kernel(SampleArgs A, SamplePlan
     }
 }
 
-// a lower bound of the k-th largest of the row's stripe maxima, as a key: its leading 20 bits, found
-// bit by bit, the rest zero; one wave, 16 maxima a lane
-__device__ uint32_t stripe_bound(const RowWs& w, int k) {
-    const int lane = threadIdx.x & 63;
+// A lower bound of the k-th largest of the row's stripe maxima, as a key: its leading 21 bits, the
+// rest zero.  Every wave holds all maxima, 16 a lane, and counts those at or above one of seven
+// thresholds: three bits a round.
+struct Bound {
+    int n[2][8];
+};
+__device__ uint32_t stripe_bound(Bound& S, const RowWs& w, int k) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint32_t key[STRIPES / 64];
 #pragma unroll
     for (int j = 0; j < STRIPES / 64; j++) key[j] = key_of(w.stripe[j * 64 + lane]);
     uint32_t bound = 0;
-    for (int bit = 31; bit >= 12; bit--) {
-        const uint32_t t = bound | 1u << bit;
+    for (int round = 0; round < 7; round++) {
+        const int shift = 29 - 3 * round;
+        const uint32_t t = bound | (uint32_t)wave << shift;
         int n = 0;
 #pragma unroll
         for (int j = 0; j < STRIPES / 64; j++) n += __popcll(__ballot(key[j] >= t));
-        if (n >= k) bound = t;
+        if (lane == 0) S.n[round & 1][wave] = n;
+        __syncthreads();
+        int best = 0;
+        for (int v = 1; v < 8; v++)
+            if (S.n[round & 1][v] >= k) best = v;
+        bound |= (uint32_t)best << shift;
     }
     return bound;
 }
+static_assert(NP / 64 == 8, "a wave for each value of three bits");
 
 // ---- 2: top-k candidates, masses or the histogram
 template <class E>
 __global__ __launch_bounds__(NP) void sample_mass_kernel(SampleArgs A, SamplePlan P) {
     constexpr int VL = Logits<E>::VL;
-    __shared__ u64 hist[BINS];
-    __shared__ u64 tab[32];
-    __shared__ uint32_t bound;
+    __shared__ union {
+        u64 hist[BINS];
+        Stage stage;
+    } U;
+    __shared__ u64 tab[STEPS];
+    __shared__ Bound bound;
+    u64* const hist = U.hist;
     const int row = blockIdx.x / P.segs, seg = blockIdx.x % P.segs;
     const Set s = set_of(A, row);
     if (s.mode == ROW_GREEDY || s.mode == ROW_ALONE) return;
@@ -329,45 +441,38 @@ __global__ __launch_bounds__(NP) void sample_mass_kernel(SampleArgs A, SamplePla
     const int i0 = seg * P.seg_len, i1 = min(i0 + P.seg_len, A.vocab);
     const Logits<E> x = row_logits<E>(A, row);
     if (s.mode == ROW_TOPK) {
-        if (threadIdx.x < 64) {
-            const uint32_t b = stripe_bound(w, s.k);
-            if (threadIdx.x == 0) bound = b;
-        }
-        __syncthreads();
-        const uint32_t b = max(bound, 0x00800000u);  // (the key after -infinity's)
+        U.stage.clear();
+        const uint32_t b = max(stripe_bound(bound, w, s.k), 0x00800000u);  // (the key after -infinity's); has barriers
         each<E>(x, i0, i1, [&](const float (&l)[VL], int i) {
-            bool any = false;
+            bool mine[VL];
             uint32_t k[VL];
 #pragma unroll
             for (int e = 0; e < VL; e++) {
-                k[e] = i + e < i1 ? key_of(l[e]) : 0;
-                any |= i + e < i1 && k[e] >= b;
+                k[e] = key_of(l[e]);  // (past the end NaN, whose key is under any bound)
+                mine[e] = k[e] >= b;
             }
-            if (__any(any)) {
-#pragma unroll
-                for (int e = 0; e < VL; e++) append(w, i + e < i1 && k[e] >= b, (u64)k[e] << 32 | (uint32_t)~(i + e));
-            }
+            U.stage.add(w, mine, [&](int e) { return (u64)k[e] << 32 | (uint32_t)~(i + e); });
         });
+        U.stage.flush(w);
         return;
     }
     float top;
     int at;
     row_top(w, P.segs, top, at);
-    if (at < 0) return;
+    Masses m;
+    if (at < 0 || !m.set(top, s.T, A.vocab, tab)) return;
     const bool bins = s.mode == ROW_NUCLEUS;
     const int nb = bins ? BINS : (i1 - i0 + BLOCK - 1) / BLOCK;
     for (int i = threadIdx.x; i < nb; i += NP) hist[i] = 0;
-    if (threadIdx.x < 32) tab[threadIdx.x] = kExp2[threadIdx.x];
+    m.fill(tab);
     __syncthreads();
-    Masses m;
-    m.set(top, s.T, A.vocab, tab);
     if (bins) {
         each<E>(x, i0, i1, [&](const float (&l)[VL], int) {
 #pragma unroll
             for (int e = 0; e < VL; e++) {
-                const double y = m.y(l[e]);
+                const Masses::At y = m.at(l[e]);
                 const u64 q = Masses::whole(m.scaled(y));
-                if (q) atomicAdd(&hist[Masses::bin(y)], q);
+                if (q) atomicAdd(&hist[y.bin()], q);
             }
         });
         __syncthreads();
@@ -379,7 +484,7 @@ __global__ __launch_bounds__(NP) void sample_mass_kernel(SampleArgs A, SamplePla
             u64 q = 0;
 #pragma unroll
             for (int e = 0; e < VL; e++) {
-                const double v = m.scaled(m.y(l[e]));
+                const double v = m.scaled(l[e]);
                 q += v >= least ? Masses::whole(v) : 0;
             }
             q = wave_sum(q);
@@ -458,7 +563,8 @@ template <class E>
 __global__ __launch_bounds__(NP) void sample_border_kernel(SampleArgs A, SamplePlan P) {
     constexpr int VL = Logits<E>::VL;
     __shared__ u64 block[SAMPLE_MAX_VOCAB / BLOCK];
-    __shared__ u64 tab[32];
+    __shared__ u64 tab[STEPS];
+    __shared__ Stage stage;
     __shared__ Scan<NP> scan;
     __shared__ int found;
     __shared__ u64 found_above;
@@ -469,40 +575,36 @@ __global__ __launch_bounds__(NP) void sample_border_kernel(SampleArgs A, SampleP
     float top;
     int at;
     row_top(w, P.segs, top, at);
-    if (at < 0) return;
+    Masses m;
+    if (at < 0 || !m.set(top, s.T, A.vocab, tab)) return;
     const int i0 = seg * P.seg_len, i1 = min(i0 + P.seg_len, A.vocab);
     const int nb = max(0, (i1 - i0 + BLOCK - 1) / BLOCK);
     for (int i = threadIdx.x; i < nb; i += NP) block[i] = 0;
-    if (threadIdx.x < 32) tab[threadIdx.x] = kExp2[threadIdx.x];
+    m.fill(tab);
+    stage.clear();
     const BorderBin b = border_bin<NP>(w.hist, s.p, scan, &found, &found_above);  // (with barriers)
-    Masses m;
-    m.set(top, s.T, A.vocab, tab);
     const double least = s.min_e * m.unit;
     const Logits<E> x = row_logits<E>(A, row);
     each<E>(x, i0, i1, [&](const float (&l)[VL], int i) {
         u64 q = 0;
-        bool any = false;
-        int bin[VL];
+        bool mine[VL];
 #pragma unroll
         for (int e = 0; e < VL; e++) {
-            const double y = m.y(l[e]);
-            bin[e] = y > -52.5 ? Masses::bin(y) : BINS;
-            if (bin[e] < b.bin) {
+            const Masses::At y = m.at(l[e]);
+            const int bin = y.bin();
+            if (bin < b.bin) {
                 const double v = m.scaled(y);
                 q += v >= least ? Masses::whole(v) : 0;
             }
-            any |= bin[e] == b.bin;
+            mine[e] = bin == b.bin;
         }
         if (__any(q != 0)) {
             q = wave_sum(q);
             if ((threadIdx.x & 63) == 0) atomicAdd(&block[(i - i0) / BLOCK], q);
         }
-        if (__any(any)) {
-#pragma unroll
-            for (int e = 0; e < VL; e++) append(w, bin[e] == b.bin, (u64)key_of(l[e]) << 32 | (uint32_t)~(i + e));
-        }
+        stage.add(w, mine, [&](int e) { return (u64)key_of(l[e]) << 32 | (uint32_t)~(i + e); });
     });
-    __syncthreads();
+    stage.flush(w);  // (with barriers)
     for (int i = threadIdx.x; i < nb; i += NP) w.block[i0 / BLOCK + i] = block[i];
 }
 
@@ -522,8 +624,7 @@ struct RowShared {
     u64 list[LIST];
     Scan<NT> scan;
     u64 part[NT / 64];
-    u64 tab[32];
-    u64 picked;
+    u64 tab[STEPS];
     uint32_t tpart[NT / 64];
     u64 above;
     uint32_t bin, left;
@@ -579,14 +680,13 @@ __device__ void choose(RowShared& S, bool by_mass, u64 above, u64 want) {
     __syncthreads();
 }
 
-// the border at key `key`, whose tokens S.left are, S.above before them
-__device__ Border border_at(RowShared& S, const Masses& m, uint32_t key, bool by_mass, u64 want) {
+// the border at key `key`, whose tokens S.left are, each of mass `one`, S.above before them
+__device__ Border border_at(RowShared& S, u64 one, uint32_t key, bool by_mass, u64 want) {
     Border r;
     r.key = key;
     const u64 left = S.left;
     u64 ties;
     if (by_mass) {
-        const u64 one = m.mass(logit_of(key));  // (equal logits have equal masses)
         ties = S.above >= want ? 0 : one ? (want - S.above + one - 1) / one : left;
     } else {
         ties = want - S.above;
@@ -622,7 +722,7 @@ __device__ Border descend(RowShared& S, const Row& R, const Masses& m, bool by_m
             const uint32_t b = mask - ((k >> shift) & mask);
             atomicAdd(&S.count[b], 1u);
             if (by_mass) {
-                const u64 q = m.mass(l);
+                const u64 q = m.mass_any(l);
                 if (q) atomicAdd(&S.sum[b], q);
             }
         }
@@ -631,12 +731,12 @@ __device__ Border descend(RowShared& S, const Row& R, const Masses& m, bool by_m
         prefix = (step ? prefix << nb : 0) | (mask - S.bin);
         above = S.above;
     }
-    return border_at(S, m, prefix, by_mass, want);
+    return border_at(S, prefix ? m.mass_any(logit_of(prefix)) : 0, prefix, by_mass, want);
 }
 
-// the same border by mass among the n tokens of the list (all that lie in the border's bin), with
-// `above` before them: the keys' range divided by up to 2048 until one key is left
-__device__ Border descend_list(RowShared& S, const Masses& m, int n, u64 above, u64 want) {
+// the same border among the n tokens of the list, with `above` before them: the keys' range divided by
+// up to 2048 until one key is left
+__device__ Border descend_list(RowShared& S, const Masses& m, int n, bool by_mass, u64 above, u64 want) {
     uint32_t lo = 0xffffffffu, hi = 0;
     for (int i = threadIdx.x; i < n; i += NT) {
         const uint32_t k = (uint32_t)(S.list[i] >> 32);
@@ -671,14 +771,14 @@ __device__ Border descend_list(RowShared& S, const Masses& m, int n, u64 above, 
             if (k < lo || k > hi) continue;
             const uint32_t b = (hi - k) >> shift;
             atomicAdd(&S.count[b], 1u);
-            const u64 q = m.mass(logit_of(k));
+            const u64 q = by_mass ? m.mass(logit_of(k)) : 0;
             if (q) atomicAdd(&S.sum[b], q);
         }
         __syncthreads();
-        choose(S, true, above, want);
+        choose(S, by_mass, above, want);
         above = S.above;
         const uint32_t top = hi - (S.bin << shift);
-        if (shift == 0) return border_at(S, m, top, true, want);
+        if (shift == 0) return border_at(S, m.mass(logit_of(top)), top, by_mass, want);
         const uint32_t low = top - ((1u << shift) - 1);
         lo = low > lo && low <= top ? low : lo;
         hi = top;
@@ -728,7 +828,7 @@ __device__ Kept walk(const Row& R, const Masses& m, const Border& B, double leas
         const u64 tm = __ballot(tie);
         const uint32_t rank = r.ties + __popcll(tm & ((1ull << lane) - 1));
         r.ties += __popcll(tm);
-        const double v = m.scaled(m.y(l));
+        const double v = m.scaled_any(l);
         u64 q = 0;
         if (j < i1 && (k > B.key || (tie && rank < B.ties)) && v >= least) q = Masses::whole(v);
         if (find) {
@@ -767,10 +867,10 @@ __device__ int pick_alone(RowShared& S, const Row& R, const Masses& m, const Set
         for (int i = threadIdx.x; i < R.V; i += NT) {
             const float l = R.at(i);
             const uint32_t k = key_of(l);
-            if (k > B.key || (k == B.key && B.ties == ALL)) z += m.mass(l);
+            if (k > B.key || (k == B.key && B.ties == ALL)) z += m.mass_any(l);
         }
         z = block_sum(S, z);
-        if (B.ties != ALL) z += B.ties * (B.key ? m.mass(logit_of(B.key)) : 0);
+        if (B.ties != ALL) z += B.ties * (B.key ? m.mass_any(logit_of(B.key)) : 0);
         const u64 want = (u64)ceil((s.p > 0.0f ? (double)s.p : 0.0) * (double)z);
         const Border C = descend(S, R, m, true, want);
         if (C.key > B.key || (C.key == B.key && C.ties < B.ties)) B = C;
@@ -808,44 +908,21 @@ __device__ int pick_alone(RowShared& S, const Row& R, const Masses& m, const Set
     return S.found;
 }
 
-// top-k: the n candidates in S.list
-__device__ int pick_topk(RowShared& S, const Masses& m, const Set& s, int n, float u) {
-    // more candidates than threads: the k-th largest, bit by bit, and those from it on
-    if (n > NT) {
-        u64 t = 0;
-        for (int bit = 63; bit >= 0; bit--) {
-            const u64 c = t | 1ull << bit;
-            u64 cnt = 0;
-            for (int i = threadIdx.x; i < n; i += NT) cnt += S.list[i] >= c;
-            if (block_sum(S, cnt) >= (u64)s.k) t = c;
-        }
-        u64 mine[LIST / NT];
-#pragma unroll
-        for (int j = 0; j < LIST / NT; j++) {
-            const int i = j * NT + threadIdx.x;
-            mine[j] = i < n ? S.list[i] : 0;
-        }
-        __syncthreads();
-        if (threadIdx.x == 0) S.left = 0;
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < LIST / NT; j++)
-            if (mine[j] >= t && mine[j]) S.list[atomicAdd(&S.left, 1u)] = mine[j];
-        __syncthreads();
-        n = S.left;  // (k: the entries differ in their indices)
-    }
-    // each candidate's place in the order
+// top-k, few candidates: the n in S.list, a thread each, every one compared with every other
+constexpr int FEW = 256;
+__device__ int pick_few(RowShared& S, const Masses& m, const Set& s, int n, float u) {
     const int me = threadIdx.x;
     const u64 entry = me < n ? S.list[me] : 0;
     int rank = 0;
     if (me < n)
+#pragma unroll 8
         for (int i = 0; i < n; i++) rank += S.list[i] > entry;
     __syncthreads();
     if (me < n) S.list[rank] = entry;
     __syncthreads();
     n = min(n, s.k);
     const u64 mine = me < n ? S.list[me] : 0;
-    const double v = me < n ? m.scaled(m.y(logit_of((uint32_t)(mine >> 32)))) : 0.0;
+    const double v = me < n ? m.scaled(logit_of((uint32_t)(mine >> 32))) : 0.0;
     const u64 q = Masses::whole(v);
     u64 z;
     const u64 before = S.scan.before(q, z);
@@ -854,20 +931,78 @@ __device__ int pick_topk(RowShared& S, const Masses& m, const Set& s, int n, flo
     keep = (keep && v >= s.min_e * m.unit) || me == 0;
     const u64 kept = keep ? q : 0;
     const uint32_t idx = ~(uint32_t)mine;
-    S.scan.before(kept, z);
-    const u64 target = target_of(u, z);
-    // the running sum up to each kept token's index
     S.sum[me] = kept;
     S.count[me] = idx;
     if (me == 0) S.found = 0x7fffffff;
-    __syncthreads();
+    S.scan.before(kept, z);  // (with barriers)
+    const u64 target = target_of(u, z);
+    // the running sum up to each kept token's index
     if (kept) {
         u64 run = 0;
+#pragma unroll 8
         for (int i = 0; i < n; i++) run += S.count[i] <= idx ? S.sum[i] : 0;
         if (run > target) atomicMin(&S.found, (int)idx);
     }
     __syncthreads();
     return S.found;
+}
+
+// top-k, many candidates: the border among the n in S.list, then the token by histograms over the
+// indices' blocks and within the block
+__device__ int pick_list(RowShared& S, const Masses& m, const Set& s, int n, float u) {
+    const double least = s.min_e * m.unit;
+    Border B;
+    if (n > s.k) B = descend_list(S, m, n, false, 0, (u64)s.k);
+    uint32_t cut = last_tie(S, B, n);
+    auto kept = [&](u64 e) {
+        const uint32_t k = (uint32_t)(e >> 32);
+        return k > B.key || (k == B.key && ~(uint32_t)e <= cut);
+    };
+    if (s.p < 1.0f) {
+        u64 z = 0;
+        for (int i = threadIdx.x; i < n; i += NT)
+            if (kept(S.list[i])) z += m.mass(logit_of((uint32_t)(S.list[i] >> 32)));
+        z = block_sum(S, z);
+        const u64 want = (u64)ceil((s.p > 0.0f ? (double)s.p : 0.0) * (double)z);
+        const Border C = descend_list(S, m, n, true, 0, want);
+        if (C.key > B.key || (C.key == B.key && C.ties < B.ties)) {
+            B = C;
+            cut = last_tie(S, B, n);
+        }
+    }
+    u64 target = 0, above = 0;
+    uint32_t block = 0;
+    for (int step = 0; step < 2; step++) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < BINS; i += NT) S.sum[i] = 0;
+        __syncthreads();
+        for (int i = threadIdx.x; i < n; i += NT) {
+            const u64 e = S.list[i];
+            const uint32_t at = ~(uint32_t)e;
+            if (!kept(e) || (step && at / BLOCK != block)) continue;
+            const double v = m.scaled(logit_of((uint32_t)(e >> 32)));
+            const u64 q = v >= least ? Masses::whole(v) : 0;
+            if (q) atomicAdd(&S.sum[step ? at % BLOCK : at / BLOCK], q);
+        }
+        __syncthreads();
+        u64 v[2], z;
+        const int b0 = threadIdx.x * 2;
+        for (int j = 0; j < 2; j++) v[j] = S.sum[b0 + j];
+        u64 run = above + S.scan.before(v[0] + v[1], z);
+        if (step == 0) target = target_of(u, z);
+        for (int j = 0; j < 2; j++) {
+            if (run <= target && run + v[j] > target) {
+                S.bin = b0 + j;
+                S.above = run;
+            }
+            run += v[j];
+        }
+        __syncthreads();
+        if (step) break;
+        block = S.bin;
+        above = S.above;
+    }
+    return (int)(block * BLOCK + S.bin);
 }
 
 // no top-k: the blocks' masses are in the workspace (with top-p those above the border's bin, whose
@@ -879,7 +1014,7 @@ __device__ int pick_blocks(RowShared& S, const Row& R, const Masses& m, const Se
     uint32_t cut = ALL;
     if (s.mode == ROW_NUCLEUS) {
         const BorderBin b = border_bin<NT>(w.hist, s.p, S.scan, &S.found, &S.above);
-        B = descend_list(S, m, n, b.above, b.want);
+        B = descend_list(S, m, n, true, b.above, b.want);
         cut = last_tie(S, B, n);
     }
     __syncthreads();
@@ -890,7 +1025,7 @@ __device__ int pick_blocks(RowShared& S, const Row& R, const Masses& m, const Se
         for (int i = threadIdx.x; i < n; i += NT) {
             const uint32_t k = (uint32_t)(S.list[i] >> 32), i1 = ~(uint32_t)S.list[i];
             if (k < B.key || (k == B.key && i1 > cut)) continue;
-            const double v = m.scaled(m.y(logit_of(k)));
+            const double v = m.scaled(logit_of(k));
             const u64 q = v >= least ? Masses::whole(v) : 0;
             if (q) atomicAdd(&S.sum[i1 / BLOCK], q);
         }
@@ -917,7 +1052,7 @@ __device__ int pick_blocks(RowShared& S, const Row& R, const Masses& m, const Se
     for (int j = 0; j < 2; j++) {
         const float l = i + j < R.V ? R.at(i + j) : __builtin_nanf("");
         const uint32_t k = key_of(l);
-        const double v = m.scaled(m.y(l));
+        const double v = m.scaled(l);
         const bool keep = k > B.key || (k == B.key && (uint32_t)(i + j) <= cut);
         q[j] = keep && v >= least ? Masses::whole(v) : 0;
     }
@@ -944,23 +1079,23 @@ __global__ __launch_bounds__(NT) void sample_pick_kernel(SampleArgs A, SamplePla
         if (threadIdx.x == 0) A.ids[row] = at;
         return;
     }
-    if (threadIdx.x < 32) S.tab[threadIdx.x] = kExp2[threadIdx.x];
+    Masses m;
+    const bool plain = m.set(top, s.T, A.vocab, S.tab);
+    m.fill(S.tab);
     const int n = s.mode == ROW_TOPK || s.mode == ROW_NUCLEUS ? (int)min(*w.count, (uint32_t)LIST + 1) : 0;
     if (n <= LIST)
         for (int i = threadIdx.x; i < n; i += NT) S.list[i] = w.list[i];
     __syncthreads();
-    Masses m;
-    m.set(top, s.T, A.vocab, S.tab);
     Row R;
     R.x = static_cast<const char*>(A.logits) + row * A.row_stride * (A.type == JYHIP_T_F32 ? 4 : 2);
     R.type = A.type;
     R.V = A.vocab;
     const float u = A.u[row];
     int id;
-    if (s.mode == ROW_ALONE || n > LIST)
+    if (s.mode == ROW_ALONE || n > LIST || !plain)
         id = pick_alone(S, R, m, s, u);
     else if (s.mode == ROW_TOPK)
-        id = pick_topk(S, m, s, n, u);
+        id = n <= FEW ? pick_few(S, m, s, n, u) : pick_list(S, m, s, n, u);
     else
         id = pick_blocks(S, R, m, s, w, P.blocks, n, u);
     if (threadIdx.x == 0) A.ids[row] = id;
