@@ -70,8 +70,7 @@ struct RowWs {
     u64* hist;      // [BINS]
     u64* list;      // [LIST] key << 32 | ~index
     u64* block;     // [blocks]
-    float* seg_max; // [MAX_SEGS]
-    int* seg_arg;   // [MAX_SEGS]
+    u64* seg_top;   // [MAX_SEGS] the segment's first token in the order, as a list entry; 0: none
     float* stripe;  // [STRIPES]
     uint32_t* count;
 };
@@ -81,9 +80,8 @@ __device__ __forceinline__ RowWs row_ws(const SampleArgs& A, const SamplePlan& P
     w.hist = reinterpret_cast<u64*>(p);
     w.list = w.hist + BINS;
     w.block = w.list + LIST;
-    w.seg_max = reinterpret_cast<float*>(w.block + P.blocks);
-    w.seg_arg = reinterpret_cast<int*>(w.seg_max + MAX_SEGS);
-    w.stripe = reinterpret_cast<float*>(w.seg_arg + MAX_SEGS);
+    w.seg_top = w.block + P.blocks;
+    w.stripe = reinterpret_cast<float*>(w.seg_top + MAX_SEGS);
     w.count = reinterpret_cast<uint32_t*>(w.stripe + STRIPES);
     return w;
 }
@@ -177,28 +175,25 @@ struct Masses {
         const double kd = y + shift;
         return At{y - (kd - shift), (int)(uint32_t)__builtin_bit_cast(u64, kd)};
     }
-    __device__ __forceinline__ double scaled(const At& a) const {
+    // the mass, rounded to a whole number by adding it to 2^52 (it is under that)
+    __device__ __forceinline__ u64 mass(const At& a) const {
         constexpr double L = 0.69314718055994531 / 512.0;
         double q = __builtin_fma(a.r, L * L * L / 6.0, L * L / 2.0);
         q = __builtin_fma(q, a.r, L);
         q = __builtin_fma(q, a.r, 1.0);
         const u64 t = tab[a.k & (STEPS - 1)] + ((u64)(uint32_t)((a.k >> 9) << 20) << 32);
-        return q * __builtin_bit_cast(double, t);
+        return __builtin_bit_cast(u64, __builtin_fma(q, __builtin_bit_cast(double, t), 0x1p+52)) & 0xfffffffffffffull;
     }
-    __device__ __forceinline__ double scaled(float l) const { return scaled(at(l)); }
-    // the nearest whole number of a scaled mass (under 2^52)
-    static __device__ __forceinline__ u64 whole(double scaled) {
-        return __builtin_bit_cast(u64, scaled + 0x1p+52) & 0xfffffffffffffull;
-    }
-    __device__ __forceinline__ u64 mass(float l) const { return whole(scaled(l)); }
+    __device__ __forceinline__ u64 mass(float l) const { return mass(at(l)); }
+    // min-p's least mass
+    __device__ __forceinline__ u64 least(const Set& s) const { return (u64)__builtin_rint(s.min_e * unit); }
     // the same for any M and T
-    __device__ __forceinline__ double scaled_any(float l) const {
-        if (l == M) return unit;
-        if (!(l > -__builtin_inff()) || M == __builtin_inff()) return 0.0;
+    __device__ __forceinline__ u64 mass_any(float l) const {
+        if (l == M) return (u64)unit;
+        if (!(l > -__builtin_inff()) || M == __builtin_inff()) return 0;
         const double y = ((double)l - (double)M) * (c / 512.0);
-        return y > -64.0 ? unit * exp2_slow(y) : 0.0;
+        return y > -64.0 ? (u64)__builtin_rint(unit * exp2_slow(y)) : 0;
     }
-    __device__ __forceinline__ u64 mass_any(float l) const { return whole(scaled_any(l)); }
 };
 
 // the sum of v over the wave, in every lane (whole numbers: any order)
@@ -228,6 +223,15 @@ __device__ __forceinline__ u64 wave_sum(u64 v) {
     return lane_u64(v, 0) + lane_u64(v, 16) + lane_u64(v, 32) + lane_u64(v, 48);
 }
 
+// the largest of v over the wave, in every lane
+__device__ __forceinline__ u64 wave_max(u64 v) {
+    v = max(v, dpp_u64<0xB1>(v));
+    v = max(v, dpp_u64<0x4E>(v));
+    v = max(v, dpp_u64<0x124>(v));
+    v = max(v, dpp_u64<0x128>(v));
+    return max(max(lane_u64(v, 0), lane_u64(v, 16)), max(lane_u64(v, 32), lane_u64(v, 48)));
+}
+
 // VL consecutive logits from index i (those at or past `end` as NaN, which has no mass)
 template <class E>
 struct Logits {
@@ -255,35 +259,44 @@ __device__ __forceinline__ Logits<E> row_logits(const SampleArgs& A, int row) {
 }
 
 // f(l, i) for the workgroup's VL logits at a time of [i0, i1), all lanes of a wave together; the next
-// ones are read before f takes the present ones
+// ones are read before f takes the present ones.  The first ones: first(), for a caller with other
+// work before.
+template <class E>
+struct First {
+    float l[Logits<E>::VL];
+};
+template <class E>
+__device__ __forceinline__ First<E> first(const Logits<E>& x, int i0, int i1) {
+    First<E> a;
+    x.load(i0 + (int)threadIdx.x * Logits<E>::VL, i1, a.l);
+    return a;
+}
+template <class E, class F>
+__device__ __forceinline__ void each(const Logits<E>& x, First<E> a, int i0, int i1, F&& f) {
+    constexpr int VL = Logits<E>::VL, STEP = NP * VL;
+    First<E> b;
+    int i = i0 + (int)threadIdx.x * VL;
+    for (int base = i0; base < i1; base += STEP, i += STEP) {
+        if (base + STEP < i1) x.load(i + STEP, i1, b.l);
+        f(a.l, i);
+        a = b;
+    }
+}
 template <class E, class F>
 __device__ __forceinline__ void each(const Logits<E>& x, int i0, int i1, F&& f) {
-    constexpr int VL = Logits<E>::VL, STEP = NP * VL;
-    float a[VL], b[VL];
-    int i = i0 + (int)threadIdx.x * VL;
-    x.load(i, i1, a);
-    for (int base = i0; base < i1; base += STEP, i += STEP) {
-        if (base + STEP < i1) x.load(i + STEP, i1, b);
-        f(a, i);
-#pragma unroll
-        for (int e = 0; e < VL; e++) a[e] = b[e];
-    }
+    each(x, first(x, i0, i1), i0, i1, f);
 }
 
-// the row's largest logit and its lowest index (-1: none), from its parts; every wave by itself
-__device__ __forceinline__ void row_top(const RowWs& w, int segs, float& top, int& at) {
+// a token in the order: falling logits, equal ones by index
+__device__ __forceinline__ u64 entry_of(uint32_t key, int i) { return (u64)key << 32 | (uint32_t)~i; }
+constexpr uint32_t LEAST_KEY = 0x00800000u;  // after -infinity's
+
+// the row's first token from its parts' (0: none above -infinity); every wave by itself
+__device__ __forceinline__ u64 row_top(const RowWs& w, int segs) {
     const int lane = threadIdx.x & 63;
-    top = lane < segs ? w.seg_max[lane] : -__builtin_inff();
-    at = lane < segs ? w.seg_arg[lane] : -1;
-    for (int d = 32; d; d >>= 1) {
-        const float ot = __shfl_xor(top, d);
-        const int oa = __shfl_xor(at, d);
-        if (ot > top || (ot == top && oa >= 0 && (at < 0 || oa < at))) {
-            top = ot;
-            at = oa;
-        }
-    }
+    return wave_max(lane < segs ? w.seg_top[lane] : 0);
 }
+__device__ __forceinline__ float top_logit(u64 top) { return logit_of((uint32_t)(top >> 32)); }
 
 // list entries of a workgroup: collected in LDS (one atomic on the row's counter for all of them),
 // the ones that find it full go to the list by themselves
@@ -337,60 +350,42 @@ template <class E>
 __global__ __launch_bounds__(NP) void sample_top_kernel(SampleArgs A, SamplePlan P) {
     constexpr int VL = Logits<E>::VL;
     __shared__ float part[2 * NP];
-    __shared__ int arg[NP / 64];
+    __shared__ u64 first[NP / 64];
     const int row = blockIdx.x / P.segs, seg = blockIdx.x % P.segs;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const RowWs w = row_ws(A, P, row);
     const Set s = set_of(A, row);
     const int i0 = seg * P.seg_len, i1 = min(i0 + P.seg_len, A.vocab);
     // each thread two maxima (even and odd elements): 1024 parts of the segment
     float top[2] = {-__builtin_inff(), -__builtin_inff()};
     int at = -1;
-    const Logits<E> x = row_logits<E>(A, row);
-    each<E>(x, i0, i1, [&](const float (&l)[VL], int i) {
+    each(row_logits<E>(A, row), i0, i1, [&](const float (&l)[VL], int i) {
 #pragma unroll
         for (int e = 0; e < VL; e++) {
             if (l[e] > fmaxf(top[0], top[1])) at = i + e;
             top[e & 1] = fmaxf(top[e & 1], l[e]);
         }
     });
+    const u64 mine = wave_max(at < 0 ? 0 : entry_of(key_of(fmaxf(top[0], top[1])), at));
+    if ((threadIdx.x & 63) == 0) first[threadIdx.x >> 6] = mine;
+    part[threadIdx.x] = top[0];
+    part[NP + threadIdx.x] = top[1];
+    __syncthreads();
     if (s.mode == ROW_NUCLEUS)
         for (int i = seg * NP + threadIdx.x; i < BINS; i += P.segs * NP) w.hist[i] = 0;
-    if (seg == 0 && threadIdx.x == 0) *w.count = 0;
     if (s.mode == ROW_TOPK) {
-        part[threadIdx.x] = top[0];
-        part[NP + threadIdx.x] = top[1];
-        __syncthreads();
-        const int mine = STRIPES / P.segs;
-        for (int r = threadIdx.x; r < mine; r += NP) {
+        const int n = STRIPES / P.segs;
+        for (int r = threadIdx.x; r < n; r += NP) {
             float m = part[r];
-            for (int j = r + mine; j < 2 * NP; j += mine) m = fmaxf(m, part[j]);
-            w.stripe[seg * mine + r] = m;
-        }
-        __syncthreads();
-    }
-    float m = fmaxf(top[0], top[1]);
-    for (int d = 32; d; d >>= 1) {
-        const float om = __shfl_xor(m, d);
-        const int oa = __shfl_xor(at, d);
-        if (om > m || (om == m && oa >= 0 && (at < 0 || oa < at))) {
-            m = om;
-            at = oa;
+            for (int j = r + n; j < 2 * NP; j += n) m = fmaxf(m, part[j]);
+            w.stripe[seg * n + r] = m;
         }
     }
-    if (lane == 0) {
-        part[wave] = m;
-        arg[wave] = at;
-    }
-    __syncthreads();
     if (threadIdx.x == 0) {
-        for (int v = 1; v < NP / 64; v++)
-            if (part[v] > m || (part[v] == m && arg[v] >= 0 && (at < 0 || arg[v] < at))) {
-                m = part[v];
-                at = arg[v];
-            }
-        w.seg_max[seg] = m;
-        w.seg_arg[seg] = at;
+        u64 t = first[0];
+#pragma unroll
+        for (int v = 1; v < NP / 64; v++) t = max(t, first[v]);
+        w.seg_top[seg] = t;
+        if (seg == 0) *w.count = 0;
     }
 }
 
@@ -440,10 +435,11 @@ __global__ __launch_bounds__(NP) void sample_mass_kernel(SampleArgs A, SamplePla
     const RowWs w = row_ws(A, P, row);
     const int i0 = seg * P.seg_len, i1 = min(i0 + P.seg_len, A.vocab);
     const Logits<E> x = row_logits<E>(A, row);
+    const First<E> f = first(x, i0, i1);
     if (s.mode == ROW_TOPK) {
         U.stage.clear();
-        const uint32_t b = max(stripe_bound(bound, w, s.k), 0x00800000u);  // (the key after -infinity's); has barriers
-        each<E>(x, i0, i1, [&](const float (&l)[VL], int i) {
+        const uint32_t b = max(stripe_bound(bound, w, s.k), LEAST_KEY);  // (with barriers)
+        each(x, f, i0, i1, [&](const float (&l)[VL], int i) {
             bool mine[VL];
             uint32_t k[VL];
 #pragma unroll
@@ -451,27 +447,25 @@ __global__ __launch_bounds__(NP) void sample_mass_kernel(SampleArgs A, SamplePla
                 k[e] = key_of(l[e]);  // (past the end NaN, whose key is under any bound)
                 mine[e] = k[e] >= b;
             }
-            U.stage.add(w, mine, [&](int e) { return (u64)k[e] << 32 | (uint32_t)~(i + e); });
+            U.stage.add(w, mine, [&](int e) { return entry_of(k[e], i + e); });
         });
         U.stage.flush(w);
         return;
     }
-    float top;
-    int at;
-    row_top(w, P.segs, top, at);
+    const u64 top = row_top(w, P.segs);
     Masses m;
-    if (at < 0 || !m.set(top, s.T, A.vocab, tab)) return;
+    if (!top || !m.set(top_logit(top), s.T, A.vocab, tab)) return;
     const bool bins = s.mode == ROW_NUCLEUS;
     const int nb = bins ? BINS : (i1 - i0 + BLOCK - 1) / BLOCK;
     for (int i = threadIdx.x; i < nb; i += NP) hist[i] = 0;
     m.fill(tab);
     __syncthreads();
     if (bins) {
-        each<E>(x, i0, i1, [&](const float (&l)[VL], int) {
+        each(x, f, i0, i1, [&](const float (&l)[VL], int) {
 #pragma unroll
             for (int e = 0; e < VL; e++) {
                 const Masses::At y = m.at(l[e]);
-                const u64 q = Masses::whole(m.scaled(y));
+                const u64 q = m.mass(y);
                 if (q) atomicAdd(&hist[y.bin()], q);
             }
         });
@@ -479,13 +473,13 @@ __global__ __launch_bounds__(NP) void sample_mass_kernel(SampleArgs A, SamplePla
         for (int i = threadIdx.x; i < BINS; i += NP)
             if (hist[i]) atomicAdd(&w.hist[i], hist[i]);
     } else {
-        const double least = s.min_e * m.unit;
-        each<E>(x, i0, i1, [&](const float (&l)[VL], int i) {
+        const u64 least = m.least(s);
+        each(x, f, i0, i1, [&](const float (&l)[VL], int i) {
             u64 q = 0;
 #pragma unroll
             for (int e = 0; e < VL; e++) {
-                const double v = m.scaled(l[e]);
-                q += v >= least ? Masses::whole(v) : 0;
+                const u64 v = m.mass(l[e]);
+                q += v >= least ? v : 0;
             }
             q = wave_sum(q);
             if ((threadIdx.x & 63) == 0 && q) atomicAdd(&hist[(i - i0) / BLOCK], q);
@@ -495,66 +489,69 @@ __global__ __launch_bounds__(NP) void sample_mass_kernel(SampleArgs A, SamplePla
     }
 }
 
-// running sums over a workgroup of N threads
+// the running sum of v over the wave's lanes up to and with this one
+__device__ __forceinline__ u64 wave_scan(u64 v) {
+    const int lane = threadIdx.x & 63;
+    // within rows of 16 (row_shr:n brings zeros in from the left)
+    v += dpp_u64<0x111>(v);
+    v += dpp_u64<0x112>(v);
+    v += dpp_u64<0x114>(v);
+    v += dpp_u64<0x118>(v);
+    const u64 r0 = lane_u64(v, 15), r1 = r0 + lane_u64(v, 31), r2 = r1 + lane_u64(v, 47);
+    return v + (lane < 16 ? 0 : lane < 32 ? r0 : lane < 48 ? r1 : r2);
+}
+
+// Running sums over a workgroup of N threads, one barrier each: the waves' sums go to the two halves of
+// `part` in turn, and a half is written again only after the barrier of the call between.
 template <int N>
 struct Scan {
-    u64 part[N / 64];
-    // (the sum before this thread, the total)
-    __device__ __forceinline__ u64 before(u64 v, u64& total) {
+    u64 part[2][N / 64];
+    // (the sum before this thread, the total); `turn` is the caller's, 0 at first
+    __device__ __forceinline__ u64 before(int& turn, u64 v, u64& total) {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        u64 run = v;
-        for (int d = 1; d < 64; d <<= 1) {
-            const u64 o = __shfl_up(run, d);
-            if (lane >= d) run += o;
-        }
+        const u64 run = wave_scan(v);
+        u64* const p = part[turn];
+        turn ^= 1;
+        if (lane == 63) p[wave] = run;
         __syncthreads();
-        if (lane == 63) part[wave] = run;
-        __syncthreads();
-        u64 a = 0;
-        total = 0;
-        for (int i = 0; i < N / 64; i++) {
-            if (i < wave) a += part[i];
-            total += part[i];
-        }
-        return a + run - v;
+        const u64 w = wave_scan(lane < N / 64 ? p[lane] : 0);
+        total = lane_u64(w, N / 64 - 1);
+        const u64 mine = __shfl(w, wave) - lane_u64(run, 63);
+        return mine + run - v;
     }
 };
 
 // The bin that the last kept token lies in: the last one, from the top, with mass in it and less than
-// `want` = ceil(p total) above; `above` that mass, `total` all of it.  All threads return the same.
+// `want` = ceil(p total) above; `above` that mass.  All threads return the same.
 struct BorderBin {
     int bin;
     u64 above, want;
 };
+struct BorderFound {
+    int bin;
+    u64 above;
+};
 template <int N>
-__device__ BorderBin border_bin(const u64* hist, float p, Scan<N>& scan, int* found, u64* found_above) {
+__device__ BorderBin border_bin(const u64 (&h)[BINS / N], float p, Scan<N>& scan, int& turn, BorderFound& found) {
     constexpr int PER = BINS / N;
-    u64 h[PER], sum = 0, total;
+    u64 sum = 0, total;
 #pragma unroll
-    for (int j = 0; j < PER; j++) {
-        h[j] = hist[threadIdx.x * PER + j];
-        sum += h[j];
-    }
-    if (threadIdx.x == 0) *found = -1;
-    u64 run = scan.before(sum, total);
+    for (int j = 0; j < PER; j++) sum += h[j];
+    u64 run = scan.before(turn, sum, total);
     BorderBin b;
     b.want = (u64)ceil((p > 0.0f ? (double)p : 0.0) * (double)total);
-    int mine = -1;
-    u64 mine_above = 0;
 #pragma unroll
     for (int j = 0; j < PER; j++) {
-        if (h[j] && (run < b.want || run == 0)) {  // (run == 0: the first token is always kept)
-            mine = threadIdx.x * PER + j;
-            mine_above = run;
+        // (run == 0: the first token is always kept)
+        if (h[j] && (run < b.want || run == 0) && run + h[j] >= b.want) {
+            found.bin = threadIdx.x * PER + j;
+            found.above = run;
         }
         run += h[j];
     }
-    if (mine >= 0) atomicMax(found, mine);
     __syncthreads();
-    if (mine >= 0 && *found == mine) *found_above = mine_above;
-    __syncthreads();
-    b.bin = *found;
-    b.above = *found_above;
+    b.bin = found.bin;
+    b.above = found.above;
     return b;
 }
 
@@ -566,26 +563,28 @@ __global__ __launch_bounds__(NP) void sample_border_kernel(SampleArgs A, SampleP
     __shared__ u64 tab[STEPS];
     __shared__ Stage stage;
     __shared__ Scan<NP> scan;
-    __shared__ int found;
-    __shared__ u64 found_above;
+    __shared__ BorderFound found;
     const int row = blockIdx.x / P.segs, seg = blockIdx.x % P.segs;
     const Set s = set_of(A, row);
     if (s.mode != ROW_NUCLEUS) return;
     const RowWs w = row_ws(A, P, row);
-    float top;
-    int at;
-    row_top(w, P.segs, top, at);
+    const u64 top = row_top(w, P.segs);
     Masses m;
-    if (at < 0 || !m.set(top, s.T, A.vocab, tab)) return;
+    if (!top || !m.set(top_logit(top), s.T, A.vocab, tab)) return;
     const int i0 = seg * P.seg_len, i1 = min(i0 + P.seg_len, A.vocab);
     const int nb = max(0, (i1 - i0 + BLOCK - 1) / BLOCK);
     for (int i = threadIdx.x; i < nb; i += NP) block[i] = 0;
+    const Logits<E> x = row_logits<E>(A, row);
+    const First<E> f = first(x, i0, i1);
     m.fill(tab);
     stage.clear();
-    const BorderBin b = border_bin<NP>(w.hist, s.p, scan, &found, &found_above);  // (with barriers)
-    const double least = s.min_e * m.unit;
-    const Logits<E> x = row_logits<E>(A, row);
-    each<E>(x, i0, i1, [&](const float (&l)[VL], int i) {
+    u64 h[BINS / NP];
+#pragma unroll
+    for (int j = 0; j < BINS / NP; j++) h[j] = w.hist[threadIdx.x * (BINS / NP) + j];
+    int turn = 0;
+    const BorderBin b = border_bin<NP>(h, s.p, scan, turn, found);  // (with barriers)
+    const u64 least = m.least(s);
+    each(x, f, i0, i1, [&](const float (&l)[VL], int i) {
         u64 q = 0;
         bool mine[VL];
 #pragma unroll
@@ -593,8 +592,8 @@ __global__ __launch_bounds__(NP) void sample_border_kernel(SampleArgs A, SampleP
             const Masses::At y = m.at(l[e]);
             const int bin = y.bin();
             if (bin < b.bin) {
-                const double v = m.scaled(y);
-                q += v >= least ? Masses::whole(v) : 0;
+                const u64 v = m.mass(y);
+                q += v >= least ? v : 0;
             }
             mine[e] = bin == b.bin;
         }
@@ -602,7 +601,7 @@ __global__ __launch_bounds__(NP) void sample_border_kernel(SampleArgs A, SampleP
             q = wave_sum(q);
             if ((threadIdx.x & 63) == 0) atomicAdd(&block[(i - i0) / BLOCK], q);
         }
-        stage.add(w, mine, [&](int e) { return (u64)key_of(l[e]) << 32 | (uint32_t)~(i + e); });
+        stage.add(w, mine, [&](int e) { return entry_of(key_of(l[e]), i + e); });
     });
     stage.flush(w);  // (with barriers)
     for (int i = threadIdx.x; i < nb; i += NP) w.block[i0 / BLOCK + i] = block[i];
@@ -618,10 +617,12 @@ struct Border {
     uint32_t ties = ALL;
 };
 
+constexpr int WAYS = NT;            // bins of one step of a descent in kernel 4, one a thread
 struct RowShared {
-    uint32_t count[BINS];
-    u64 sum[BINS];
+    uint32_t count[WAYS];           // zero between steps
+    u64 sum[WAYS];                  // zero between steps
     u64 list[LIST];
+    u64 block[SAMPLE_MAX_VOCAB / BLOCK];
     Scan<NT> scan;
     u64 part[NT / 64];
     u64 tab[STEPS];
@@ -629,6 +630,7 @@ struct RowShared {
     u64 above;
     uint32_t bin, left;
     int found;
+    BorderFound border;
 };
 
 struct Row {
@@ -652,30 +654,21 @@ __device__ __forceinline__ u64 block_sum(RowShared& S, u64 v) {
     return v;
 }
 
-// One step of a descent: of the bins in S (bin 0 the highest keys), the last one with a token in it and
-// less than `want` above it, `above` lying above the first.  Leaves bin, above and the bin's count.
-__device__ void choose(RowShared& S, bool by_mass, u64 above, u64 want) {
-    u64 v[2], total;
-    const int b0 = threadIdx.x * 2;
-    for (int j = 0; j < 2; j++) v[j] = by_mass ? S.sum[b0 + j] : S.count[b0 + j];
-    u64 run = above + S.scan.before(v[0] + v[1], total);
-    if (threadIdx.x == 0) S.found = -1;
+// One step of a descent: of the bins in S (bin 0 the first in the order), the last one with a token in it
+// and less than `want` above it, `above` lying above the first; it is the one that reaches `want`.
+// Leaves the bin, what lies above it and its count; the bins are zero again.
+__device__ __forceinline__ void choose(RowShared& S, int& turn, bool by_mass, u64 above, u64 want) {
     __syncthreads();
-    int mine = -1;
-    u64 mine_above = 0;
-    for (int j = 0; j < 2; j++) {
-        if (S.count[b0 + j] && (run < want || run == 0)) {
-            mine = b0 + j;
-            mine_above = run;
-        }
-        run += v[j];
-    }
-    if (mine >= 0) atomicMax(&S.found, mine);
-    __syncthreads();
-    if (mine >= 0 && S.found == mine) {
-        S.bin = mine;
-        S.above = mine_above;
-        S.left = S.count[mine];
+    const uint32_t n = S.count[threadIdx.x];
+    const u64 v = by_mass ? S.sum[threadIdx.x] : n;
+    S.count[threadIdx.x] = 0;
+    S.sum[threadIdx.x] = 0;
+    u64 total;
+    const u64 run = above + S.scan.before(turn, v, total);
+    if (n && (run < want || run == 0) && run + v >= want) {
+        S.bin = threadIdx.x;
+        S.above = run;
+        S.left = n;
     }
     __syncthreads();
 }
@@ -693,28 +686,18 @@ __device__ Border border_at(RowShared& S, u64 one, uint32_t key, bool by_mass, u
     }
     r.ties = ties < left ? (uint32_t)ties : ALL;
     if (r.ties == 0) r.ties = 1;  // (want == 0: the first token is kept all the same)
-    __syncthreads();
     return r;
 }
 
 // The border of the `want` first tokens in the order (by_mass: of the tokens before which less
 // than `want` of mass lies; ties share what is left), by a radix descent over the whole row's keys,
-// 11, 11 and 10 bits at a time
-__device__ Border descend(RowShared& S, const Row& R, const Masses& m, bool by_mass, u64 want) {
+// 10 bits at a time
+__device__ Border descend(RowShared& S, int& turn, const Row& R, const Masses& m, bool by_mass, u64 want) {
     uint32_t prefix = 0;
     u64 above = 0;
-    const int bits[3] = {11, 11, 10};
-    int shift = 32;
-    for (int step = 0; step < 3; step++) {
-        const int nb = bits[step];
+    for (int shift = 22, step = 0; step < 4; step++) {
+        const int nb = step < 3 ? 10 : 2;
         const uint32_t mask = (1u << nb) - 1;
-        shift -= nb;
-        __syncthreads();
-        for (int i = threadIdx.x; i < BINS; i += NT) {
-            S.count[i] = 0;
-            S.sum[i] = 0;
-        }
-        __syncthreads();
         for (int i = threadIdx.x; i < R.V; i += NT) {
             const float l = R.at(i);
             const uint32_t k = key_of(l);
@@ -726,56 +709,52 @@ __device__ Border descend(RowShared& S, const Row& R, const Masses& m, bool by_m
                 if (q) atomicAdd(&S.sum[b], q);
             }
         }
-        __syncthreads();
-        choose(S, by_mass, above, want);
+        choose(S, turn, by_mass, above, want);
         prefix = (step ? prefix << nb : 0) | (mask - S.bin);
         above = S.above;
+        shift -= step < 2 ? 10 : 2;
     }
     return border_at(S, prefix ? m.mass_any(logit_of(prefix)) : 0, prefix, by_mass, want);
 }
 
-// the same border among the n tokens of the list, with `above` before them: the keys' range divided by
-// up to 2048 until one key is left
-__device__ Border descend_list(RowShared& S, const Masses& m, int n, bool by_mass, u64 above, u64 want) {
-    uint32_t lo = 0xffffffffu, hi = 0;
-    for (int i = threadIdx.x; i < n; i += NT) {
-        const uint32_t k = (uint32_t)(S.list[i] >> 32);
-        lo = min(lo, k);
-        hi = max(hi, k);
+// The same border among the n tokens of the list, with `above` before them: the keys' range divided by
+// up to 1024 until one key is left.  A thread has at most PER of them.
+template <int PER>
+__device__ Border descend_list(RowShared& S, int& turn, const Masses& m, int n, bool by_mass, u64 above, u64 want) {
+    uint32_t key[PER], lo = 0xffffffffu, hi = 0;
+    u64 q[PER];
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+        const int i = j * NT + threadIdx.x;
+        key[j] = i < n ? (uint32_t)(S.list[i] >> 32) : 0;
+        q[j] = by_mass && key[j] ? m.mass(logit_of(key[j])) : 0;
+        if (key[j]) {
+            lo = min(lo, key[j]);
+            hi = max(hi, key[j]);
+        }
     }
-    for (int d = 32; d; d >>= 1) {
-        lo = min(lo, (uint32_t)__shfl_xor((int)lo, d));
-        hi = max(hi, (uint32_t)__shfl_xor((int)hi, d));
-    }
-    __syncthreads();
+    const u64 far = wave_max((u64)hi << 32), near = wave_max((u64)(uint32_t)~lo);
     if ((threadIdx.x & 63) == 0) {
-        S.tpart[threadIdx.x >> 6] = lo;
-        S.part[threadIdx.x >> 6] = hi;
+        S.tpart[threadIdx.x >> 6] = ~(uint32_t)near;
+        S.part[threadIdx.x >> 6] = far >> 32;
     }
     __syncthreads();
+#pragma unroll
     for (int w = 0; w < NT / 64; w++) {
         lo = min(lo, S.tpart[w]);
         hi = max(hi, (uint32_t)S.part[w]);
     }
     for (;;) {
         int shift = 0;  // keys per bin, as a power of two
-        while (((hi - lo) >> shift) >= BINS) shift++;
-        __syncthreads();
-        for (int i = threadIdx.x; i < BINS; i += NT) {
-            S.count[i] = 0;
-            S.sum[i] = 0;
-        }
-        __syncthreads();
-        for (int i = threadIdx.x; i < n; i += NT) {
-            const uint32_t k = (uint32_t)(S.list[i] >> 32);
-            if (k < lo || k > hi) continue;
-            const uint32_t b = (hi - k) >> shift;
-            atomicAdd(&S.count[b], 1u);
-            const u64 q = by_mass ? m.mass(logit_of(k)) : 0;
-            if (q) atomicAdd(&S.sum[b], q);
-        }
-        __syncthreads();
-        choose(S, by_mass, above, want);
+        while (((hi - lo) >> shift) >= WAYS) shift++;
+#pragma unroll
+        for (int j = 0; j < PER; j++)
+            if (key[j] && key[j] >= lo && key[j] <= hi) {
+                const uint32_t b = (hi - key[j]) >> shift;
+                atomicAdd(&S.count[b], 1u);
+                if (q[j]) atomicAdd(&S.sum[b], q[j]);
+            }
+        choose(S, turn, by_mass, above, want);
         above = S.above;
         const uint32_t top = hi - (S.bin << shift);
         if (shift == 0) return border_at(S, m.mass(logit_of(top)), top, by_mass, want);
@@ -785,28 +764,29 @@ __device__ Border descend_list(RowShared& S, const Masses& m, int n, bool by_mas
     }
 }
 
-// the index of the last tie that B keeps among the list's n tokens (those at B's key): the block of
-// 2048 indices that it lies in, then the index
-__device__ uint32_t last_tie(RowShared& S, const Border& B, int n) {
+// the index of the last tie that B keeps among the list's n tokens (those at B's key): 10 bits of
+// it at a time
+template <int PER>
+__device__ uint32_t last_tie(RowShared& S, int& turn, const Border& B, int n) {
     if (B.ties == ALL) return ALL;
-    uint32_t block = 0;
+    uint32_t prefix = 0;
     u64 above = 0;
-    for (int step = 0; step < 2; step++) {
-        __syncthreads();
-        for (int i = threadIdx.x; i < BINS; i += NT) S.count[i] = 0;
-        __syncthreads();
-        for (int i = threadIdx.x; i < n; i += NT) {
+    static_assert(SAMPLE_MAX_VOCAB == 1 << 22, "22 bits of index");
+    for (int shift = 12, step = 0; step < 3; step++) {
+        const int nb = step < 2 ? 10 : 2;
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+            const int i = j * NT + threadIdx.x;
+            if (i >= n || (uint32_t)(S.list[i] >> 32) != B.key) continue;
             const uint32_t at = ~(uint32_t)S.list[i];
-            if ((uint32_t)(S.list[i] >> 32) == B.key && (step == 0 || at / BLOCK == block))
-                atomicAdd(&S.count[step ? at % BLOCK : at / BLOCK], 1u);
+            if (step == 0 || at >> (shift + nb) == prefix) atomicAdd(&S.count[(at >> shift) & ((1u << nb) - 1)], 1u);
         }
-        __syncthreads();
-        choose(S, false, above, B.ties);
-        if (step) return block * BLOCK + S.bin;
-        block = S.bin;
+        choose(S, turn, false, above, B.ties);
+        prefix = prefix << nb | S.bin;
         above = S.above;
+        shift -= step == 0 ? 10 : 2;
     }
-    return 0;  // (not reached)
+    return prefix;
 }
 
 // the kept mass of tokens with indices in [i0, i1), per wave in steps of 64, `ties` the ties before
@@ -816,7 +796,7 @@ struct Kept {
     uint32_t ties;
     int at;
 };
-__device__ Kept walk(const Row& R, const Masses& m, const Border& B, double least, int i0, int i1, uint32_t ties,
+__device__ Kept walk(const Row& R, const Masses& m, const Border& B, u64 least, int i0, int i1, uint32_t ties,
                      bool find, u64 target) {
     const int lane = threadIdx.x & 63;
     Kept r{0, ties, -1};
@@ -828,9 +808,8 @@ __device__ Kept walk(const Row& R, const Masses& m, const Border& B, double leas
         const u64 tm = __ballot(tie);
         const uint32_t rank = r.ties + __popcll(tm & ((1ull << lane) - 1));
         r.ties += __popcll(tm);
-        const double v = m.scaled_any(l);
-        u64 q = 0;
-        if (j < i1 && (k > B.key || (tie && rank < B.ties)) && v >= least) q = Masses::whole(v);
+        const u64 v = m.mass_any(l);
+        const u64 q = j < i1 && (k > B.key || (tie && rank < B.ties)) && v >= least ? v : 0;
         if (find) {
             u64 run = q;
             for (int d = 1; d < 64; d <<= 1) {
@@ -857,11 +836,11 @@ __device__ __forceinline__ u64 target_of(float u, u64 total) {
 }
 
 // the whole row by this workgroup
-__device__ int pick_alone(RowShared& S, const Row& R, const Masses& m, const Set& s, float u) {
+__device__ int pick_alone(RowShared& S, int& turn, const Row& R, const Masses& m, const Set& s, float u) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const double least = s.min_e * m.unit;
+    const u64 least = m.least(s);
     Border B;
-    if (s.k > 0 && s.k < R.V) B = descend(S, R, m, false, (u64)s.k);
+    if (s.k > 0 && s.k < R.V) B = descend(S, turn, R, m, false, (u64)s.k);
     if (s.p < 1.0f) {
         u64 z = 0;
         for (int i = threadIdx.x; i < R.V; i += NT) {
@@ -872,7 +851,7 @@ __device__ int pick_alone(RowShared& S, const Row& R, const Masses& m, const Set
         z = block_sum(S, z);
         if (B.ties != ALL) z += B.ties * (B.key ? m.mass_any(logit_of(B.key)) : 0);
         const u64 want = (u64)ceil((s.p > 0.0f ? (double)s.p : 0.0) * (double)z);
-        const Border C = descend(S, R, m, true, want);
+        const Border C = descend(S, turn, R, m, true, want);
         if (C.key > B.key || (C.key == B.key && C.ties < B.ties)) B = C;
     }
     // the kept mass of each wave's run of indices, then the run and the index in it
@@ -910,132 +889,134 @@ __device__ int pick_alone(RowShared& S, const Row& R, const Masses& m, const Set
 
 // top-k, few candidates: the n in S.list, a thread each, every one compared with every other
 constexpr int FEW = 256;
-__device__ int pick_few(RowShared& S, const Masses& m, const Set& s, int n, float u) {
+__device__ int pick_few(RowShared& S, int& turn, const Masses& m, const Set& s, int n, float u) {
     const int me = threadIdx.x;
     const u64 entry = me < n ? S.list[me] : 0;
     int rank = 0;
     if (me < n)
 #pragma unroll 8
         for (int i = 0; i < n; i++) rank += S.list[i] > entry;
-    __syncthreads();
-    if (me < n) S.list[rank] = entry;
+    if (me < n) S.block[rank] = entry;
+    if (me == 0) S.found = 0x7fffffff;
     __syncthreads();
     n = min(n, s.k);
-    const u64 mine = me < n ? S.list[me] : 0;
-    const double v = me < n ? m.scaled(logit_of((uint32_t)(mine >> 32))) : 0.0;
-    const u64 q = Masses::whole(v);
-    u64 z;
-    const u64 before = S.scan.before(q, z);
+    const u64 mine = me < n ? S.block[me] : 0;
+    const u64 q = me < n ? m.mass(logit_of((uint32_t)(mine >> 32))) : 0;
     bool keep = me < n;
-    if (s.p < 1.0f) keep &= before < (u64)ceil((s.p > 0.0f ? (double)s.p : 0.0) * (double)z);
-    keep = (keep && v >= s.min_e * m.unit) || me == 0;
+    u64 z;
+    if (s.p < 1.0f) {
+        const u64 before = S.scan.before(turn, q, z);
+        keep &= before < (u64)ceil((s.p > 0.0f ? (double)s.p : 0.0) * (double)z);
+    }
+    keep = (keep && q >= m.least(s)) || me == 0;
     const u64 kept = keep ? q : 0;
     const uint32_t idx = ~(uint32_t)mine;
-    S.sum[me] = kept;
-    S.count[me] = idx;
-    if (me == 0) S.found = 0x7fffffff;
-    S.scan.before(kept, z);  // (with barriers)
+    if (me < FEW) {
+        S.list[me] = kept;
+        S.count[me] = idx;
+    }
+    S.scan.before(turn, kept, z);  // (with a barrier)
     const u64 target = target_of(u, z);
     // the running sum up to each kept token's index
     if (kept) {
         u64 run = 0;
 #pragma unroll 8
-        for (int i = 0; i < n; i++) run += S.count[i] <= idx ? S.sum[i] : 0;
+        for (int i = 0; i < n; i++) run += S.count[i] <= idx ? S.list[i] : 0;
         if (run > target) atomicMin(&S.found, (int)idx);
     }
     __syncthreads();
     return S.found;
 }
+static_assert(FEW <= WAYS && FEW <= LIST && FEW <= SAMPLE_MAX_VOCAB / BLOCK, "one place for each");
 
-// top-k, many candidates: the border among the n in S.list, then the token by histograms over the
-// indices' blocks and within the block
-__device__ int pick_list(RowShared& S, const Masses& m, const Set& s, int n, float u) {
-    const double least = s.min_e * m.unit;
-    Border B;
-    if (n > s.k) B = descend_list(S, m, n, false, 0, (u64)s.k);
-    uint32_t cut = last_tie(S, B, n);
-    auto kept = [&](u64 e) {
-        const uint32_t k = (uint32_t)(e >> 32);
-        return k > B.key || (k == B.key && ~(uint32_t)e <= cut);
-    };
+// top-k, many candidates: the k first of the n in S.list, the border of top-p among them, then the token
+// by its index, 10 bits at a time
+__device__ int pick_list(RowShared& S, int& turn, const Masses& m, const Set& s, int n, float u) {
+    constexpr int PER = LIST / NT;
+    if (n > s.k) {
+        const Border B = descend_list<PER>(S, turn, m, n, false, 0, (u64)s.k);
+        const uint32_t cut = last_tie<PER>(S, turn, B, n);
+        u64 mine[PER];
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+            const int i = j * NT + threadIdx.x;
+            mine[j] = i < n ? S.list[i] : 0;
+        }
+        __syncthreads();  // (everyone has read the list and S.left)
+        if (threadIdx.x == 0) S.left = 0;
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+            const uint32_t k = (uint32_t)(mine[j] >> 32);
+            if (k > B.key || (k == B.key && ~(uint32_t)mine[j] <= cut)) S.list[atomicAdd(&S.left, 1u)] = mine[j];
+        }
+        __syncthreads();
+        n = S.left;
+    }
+    static_assert(STRIPES <= NT, "at most one of the k a thread");
+    const u64 e = (int)threadIdx.x < n ? S.list[threadIdx.x] : 0;
+    const uint32_t key = (uint32_t)(e >> 32), at = ~(uint32_t)e;
+    const u64 q = e ? m.mass(logit_of(key)) : 0;
+    bool kept = q && q >= m.least(s);
+    u64 z;
     if (s.p < 1.0f) {
-        u64 z = 0;
-        for (int i = threadIdx.x; i < n; i += NT)
-            if (kept(S.list[i])) z += m.mass(logit_of((uint32_t)(S.list[i] >> 32)));
-        z = block_sum(S, z);
+        S.scan.before(turn, q, z);
         const u64 want = (u64)ceil((s.p > 0.0f ? (double)s.p : 0.0) * (double)z);
-        const Border C = descend_list(S, m, n, true, 0, want);
-        if (C.key > B.key || (C.key == B.key && C.ties < B.ties)) {
-            B = C;
-            cut = last_tie(S, B, n);
-        }
+        const Border B = descend_list<1>(S, turn, m, n, true, 0, want);
+        const uint32_t cut = last_tie<1>(S, turn, B, n);
+        kept = kept && (key > B.key || (key == B.key && at <= cut));
     }
-    u64 target = 0, above = 0;
-    uint32_t block = 0;
-    for (int step = 0; step < 2; step++) {
-        __syncthreads();
-        for (int i = threadIdx.x; i < BINS; i += NT) S.sum[i] = 0;
-        __syncthreads();
-        for (int i = threadIdx.x; i < n; i += NT) {
-            const u64 e = S.list[i];
-            const uint32_t at = ~(uint32_t)e;
-            if (!kept(e) || (step && at / BLOCK != block)) continue;
-            const double v = m.scaled(logit_of((uint32_t)(e >> 32)));
-            const u64 q = v >= least ? Masses::whole(v) : 0;
-            if (q) atomicAdd(&S.sum[step ? at % BLOCK : at / BLOCK], q);
+    S.scan.before(turn, kept ? q : 0, z);
+    const u64 target = target_of(u, z);
+    u64 above = 0;
+    uint32_t prefix = 0;
+    for (int shift = 12, step = 0; step < 3; step++) {
+        const int nb = step < 2 ? 10 : 2;
+        if (kept && (step == 0 || at >> (shift + nb) == prefix)) {
+            const uint32_t b = (at >> shift) & ((1u << nb) - 1);
+            atomicAdd(&S.count[b], 1u);
+            atomicAdd(&S.sum[b], q);
         }
-        __syncthreads();
-        u64 v[2], z;
-        const int b0 = threadIdx.x * 2;
-        for (int j = 0; j < 2; j++) v[j] = S.sum[b0 + j];
-        u64 run = above + S.scan.before(v[0] + v[1], z);
-        if (step == 0) target = target_of(u, z);
-        for (int j = 0; j < 2; j++) {
-            if (run <= target && run + v[j] > target) {
-                S.bin = b0 + j;
-                S.above = run;
-            }
-            run += v[j];
-        }
-        __syncthreads();
-        if (step) break;
-        block = S.bin;
+        choose(S, turn, true, above, target + 1);  // (the first bin whose running sum exceeds the target)
+        prefix = prefix << nb | S.bin;
         above = S.above;
+        shift -= step == 0 ? 10 : 2;
     }
-    return (int)(block * BLOCK + S.bin);
+    return (int)prefix;
 }
 
 // no top-k: the blocks' masses are in the workspace (with top-p those above the border's bin, whose
-// tokens are the n in S.list)
-__device__ int pick_blocks(RowShared& S, const Row& R, const Masses& m, const Set& s, const RowWs& w, int blocks, int n,
-                           float u) {
-    const double least = s.min_e * m.unit;
+// tokens are the n in S.list; h: this thread's bins)
+__device__ int pick_blocks(RowShared& S, int& turn, const Row& R, const Masses& m, const Set& s, const RowWs& w,
+                           int blocks, int n, const u64 (&h)[BINS / NT], float u) {
+    constexpr int PER = LIST / NT;
+    const u64 least = m.least(s);
     Border B;
     uint32_t cut = ALL;
+    for (int i = threadIdx.x; i < blocks; i += NT) S.block[i] = w.block[i];
     if (s.mode == ROW_NUCLEUS) {
-        const BorderBin b = border_bin<NT>(w.hist, s.p, S.scan, &S.found, &S.above);
-        B = descend_list(S, m, n, true, b.above, b.want);
-        cut = last_tie(S, B, n);
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < blocks; i += NT) S.sum[i] = w.block[i];
-    __syncthreads();
-    // the border's tokens
-    if (s.mode == ROW_NUCLEUS) {
-        for (int i = threadIdx.x; i < n; i += NT) {
-            const uint32_t k = (uint32_t)(S.list[i] >> 32), i1 = ~(uint32_t)S.list[i];
-            if (k < B.key || (k == B.key && i1 > cut)) continue;
-            const double v = m.scaled(logit_of(k));
-            const u64 q = v >= least ? Masses::whole(v) : 0;
-            if (q) atomicAdd(&S.sum[i1 / BLOCK], q);
+        const BorderBin b = border_bin<NT>(h, s.p, S.scan, turn, S.border);
+        if (n <= NT) {
+            B = descend_list<1>(S, turn, m, n, true, b.above, b.want);
+            cut = last_tie<1>(S, turn, B, n);
+        } else {
+            B = descend_list<PER>(S, turn, m, n, true, b.above, b.want);
+            cut = last_tie<PER>(S, turn, B, n);
         }
-        __syncthreads();
+        // the border's tokens
+        for (int i = threadIdx.x; i < n; i += NT) {
+            const uint32_t k = (uint32_t)(S.list[i] >> 32), at = ~(uint32_t)S.list[i];
+            if (k < B.key || (k == B.key && at > cut)) continue;
+            const u64 q = m.mass(logit_of(k));
+            if (q && q >= least) atomicAdd(&S.block[at / BLOCK], q);
+        }
     }
-    static_assert(SAMPLE_MAX_VOCAB / BLOCK <= 2 * NT && BINS >= 2 * NT, "two blocks a thread");
+    __syncthreads();
+    static_assert(SAMPLE_MAX_VOCAB / BLOCK <= 2 * NT, "two blocks a thread");
     u64 v[2], z;
     const int b0 = threadIdx.x * 2;
-    for (int j = 0; j < 2; j++) v[j] = b0 + j < blocks ? S.sum[b0 + j] : 0;
-    u64 run = S.scan.before(v[0] + v[1], z);
+    for (int j = 0; j < 2; j++) v[j] = b0 + j < blocks ? S.block[b0 + j] : 0;
+    u64 run = S.scan.before(turn, v[0] + v[1], z);
     const u64 target = target_of(u, z);
     for (int j = 0; j < 2; j++) {
         if (run <= target && run + v[j] > target) {
@@ -1045,20 +1026,17 @@ __device__ int pick_blocks(RowShared& S, const Row& R, const Masses& m, const Se
         run += v[j];
     }
     __syncthreads();
-    const int i0 = (int)S.bin * BLOCK;
+    const int i = (int)S.bin * BLOCK + threadIdx.x * 2;
     const u64 left = target - S.above;
-    const int i = i0 + threadIdx.x * 2;
-    u64 q[2], total;
+    u64 q[2];
     for (int j = 0; j < 2; j++) {
         const float l = i + j < R.V ? R.at(i + j) : __builtin_nanf("");
         const uint32_t k = key_of(l);
-        const double v = m.scaled(l);
+        const u64 q1 = m.mass(l);
         const bool keep = k > B.key || (k == B.key && (uint32_t)(i + j) <= cut);
-        q[j] = keep && v >= least ? Masses::whole(v) : 0;
+        q[j] = keep && q1 >= least ? q1 : 0;
     }
-    run = S.scan.before(q[0] + q[1], total);
-    if (threadIdx.x == 0) S.found = -1;
-    __syncthreads();
+    run = S.scan.before(turn, q[0] + q[1], z);
     for (int j = 0; j < 2; j++) {
         if (run <= left && run + q[j] > left) S.found = i + j;
         run += q[j];
@@ -1071,33 +1049,42 @@ __global__ __launch_bounds__(NT) void sample_pick_kernel(SampleArgs A, SamplePla
     __shared__ RowShared S;
     const int row = blockIdx.x;
     const RowWs w = row_ws(A, P, row);
+    // (read with the rest, before it is known how many there are and whether they are needed)
+    const u64 e0 = w.list[threadIdx.x];
+    u64 h[BINS / NT];
+#pragma unroll
+    for (int j = 0; j < BINS / NT; j++) h[j] = w.hist[threadIdx.x * (BINS / NT) + j];
+    const uint32_t count = *w.count;
+    const float u = A.u[row];
+    const u64 top = row_top(w, P.segs);
     const Set s = set_of(A, row);
-    float top;
-    int at;
-    row_top(w, P.segs, top, at);
-    if (s.mode == ROW_GREEDY || at < 0) {
-        if (threadIdx.x == 0) A.ids[row] = at;
+    if (s.mode == ROW_GREEDY || !top) {
+        if (threadIdx.x == 0) A.ids[row] = top ? (int)~(uint32_t)top : -1;
         return;
     }
     Masses m;
-    const bool plain = m.set(top, s.T, A.vocab, S.tab);
+    const bool plain = m.set(top_logit(top), s.T, A.vocab, S.tab);
     m.fill(S.tab);
-    const int n = s.mode == ROW_TOPK || s.mode == ROW_NUCLEUS ? (int)min(*w.count, (uint32_t)LIST + 1) : 0;
-    if (n <= LIST)
-        for (int i = threadIdx.x; i < n; i += NT) S.list[i] = w.list[i];
+    S.count[threadIdx.x] = 0;
+    S.sum[threadIdx.x] = 0;
+    int turn = 0;
+    const int n = s.mode == ROW_TOPK || s.mode == ROW_NUCLEUS ? (int)min(count, (uint32_t)LIST + 1) : 0;
+    if (n <= LIST) {
+        if ((int)threadIdx.x < n) S.list[threadIdx.x] = e0;
+        for (int i = NT + threadIdx.x; i < n; i += NT) S.list[i] = w.list[i];
+    }
     __syncthreads();
     Row R;
     R.x = static_cast<const char*>(A.logits) + row * A.row_stride * (A.type == JYHIP_T_F32 ? 4 : 2);
     R.type = A.type;
     R.V = A.vocab;
-    const float u = A.u[row];
     int id;
     if (s.mode == ROW_ALONE || n > LIST || !plain)
-        id = pick_alone(S, R, m, s, u);
+        id = pick_alone(S, turn, R, m, s, u);
     else if (s.mode == ROW_TOPK)
-        id = n <= FEW ? pick_few(S, m, s, n, u) : pick_list(S, m, s, n, u);
+        id = n <= FEW ? pick_few(S, turn, m, s, n, u) : pick_list(S, turn, m, s, n, u);
     else
-        id = pick_blocks(S, R, m, s, w, P.blocks, n, u);
+        id = pick_blocks(S, turn, R, m, s, w, P.blocks, n, h, u);
     if (threadIdx.x == 0) A.ids[row] = id;
 }
 
