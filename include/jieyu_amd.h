@@ -335,6 +335,29 @@ JYHIP_API int jyhip_sample(const void* logits, int type, int rows, int vocab, lo
                            int* ids, void* workspace, size_t workspace_bytes, int device, void* stream);
 JYHIP_API size_t jyhip_sample_workspace(int rows, int vocab);
 
+/* One pass of a model over `rows` tokens of several sequences whose keys and values lie in pages: row r
+ * is position pos[r] of sequence seq[r] (seq NULL: of sequence r).  X and out: host [rows][hidden], the
+ * tokens' embeddings and their final-normed hidden states, as in jyhip_forward_cached_to (out may be X).
+ * pages: one pool per layer of the model (pages[0 .. num_layers)), all of one shape, on the model's
+ * device, its heads the model's.  tables, seq and pos are HOST arrays here ([num_seqs][table_stride],
+ * [rows], [rows]).  Each layer writes the rows' keys and values into the pages, then every row attends
+ * over positions 0 .. pos[r] of its sequence, so several new positions of one sequence may come in one
+ * call (a prompt) as long as the earlier ones are in the pages or in the call.
+ * Refused before anything is enqueued: positions outside the RoPE table or the page table, page ids
+ * outside the pool among those that a row attends over, two rows with the same slot.
+ * The products are the model's (its mode's); the attention is jyhip_pages_attend's, which does not
+ * round the query to int8 as the reference's does.  Waits for the model's stream; work on other streams
+ * that the pages depend on has to be done before. */
+JYHIP_API int jyhip_forward_paged(jyhip_model* model, const jyhip_pages* pages, const float* X, float* out, int rows,
+                                  const int* tables, int num_seqs, int table_stride, const int* seq, const int* pos);
+
+/* jyhip_session_step for a sampled session, the tokens drawn on the device by jyhip_sample with the
+ * session's temperature, these filters (top_k <= 0, top_p >= 1, min_p <= 0: off) and the given numbers
+ * u (host, n of them in [0, 1), one per step): the logits do not leave the device.  Returns how many
+ * tokens were produced.  Refuses a greedy session (temperature <= 0) and one with a repetition
+ * penalty.  The session's first token came from jyhip_session_begin. */
+JYHIP_API int jyhip_session_step_sampled(jyhip_session* s, int n, int top_k, float top_p, float min_p, const float* u);
+
 #ifdef __cplusplus
 }
 #endif

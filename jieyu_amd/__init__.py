@@ -83,6 +83,8 @@ def lib():
     _proto(L, "jyhip_session_graph_info", I, P, I, P)
     _proto(L, "jyhip_session_resume", P, P, P, P, I, P, I, I, I, F, F)
     _proto(L, "jyhip_session_step", I, P, I)
+    _proto(L, "jyhip_session_step_sampled", I, P, I, I, F, F, P)
+    _proto(L, "jyhip_forward_paged", I, P, P, P, P, I, P, I, I, P, P)
     _proto(L, "jyhip_session_remaining", I, P)
     _proto(L, "jyhip_session_len", I, P)
     _proto(L, "jyhip_session_ids", I, P, P, I)
@@ -218,6 +220,33 @@ class GpuModel:
         _check(self._lib.jyhip_forward_cached_noalloc(self.h, kv.h, _ptr(X), X.shape[0], start_pos))
         return X
 
+    def forward_paged(self, pool, X, tables, pos, seq=None):
+        """One pass over tokens of several sequences whose keys and values lie in `pool` (a PagePool with
+        a layer for each of the model's): X [rows][hidden] float32, row r the token at position pos[r]
+        of sequence seq[r] (without seq: of sequence r), tables int32 [sequences][pages].  X, tables, pos
+        and seq are host arrays; returns the final-normed states (new array).  Waits for torch's
+        current stream of the pool's device first."""
+        import torch
+
+        from .batch import _Pages
+        if pool.layers < self.num_layers:
+            raise JyError("forward_paged: the pool has fewer layers than the model")
+        X = np.ascontiguousarray(X, np.float32)
+        if X.ndim != 2 or X.shape[1] != self.hidden:
+            raise JyError(f"forward_paged: X must be [rows][{self.hidden}]")
+        rows = X.shape[0]
+        tables = np.ascontiguousarray(tables, np.int32)
+        pos = np.ascontiguousarray(pos, np.int32)
+        seq = None if seq is None else np.ascontiguousarray(seq, np.int32)
+        if tables.ndim != 2 or pos.shape != (rows,) or (seq is not None and seq.shape != (rows,)):
+            raise JyError("forward_paged: tables are [sequences][pages], pos and seq one for each row")
+        out = np.empty(X.shape, np.float32)
+        torch.cuda.current_stream(pool.device).synchronize()
+        pages = (_Pages * pool.layers)(*pool._layers)
+        _check(self._lib.jyhip_forward_paged(self.h, pages, _ptr(X), _ptr(out), rows, _ptr(tables), tables.shape[0],
+                                             tables.shape[1], _ptr(seq), _ptr(pos)))
+        return out
+
     def generate(self, prompt, max_new, max_seq=None, temperature=0.0, repetition_penalty=1.0, eos=None,
                  kv=None, callback=None, want_logits=False):
         """generate(): returns (ids up to the returned length, Stats[, last logits])."""
@@ -274,6 +303,12 @@ class Session:
 
     def step(self, n):
         return _check(self._lib.jyhip_session_step(self.h, n))
+
+    def step_sampled(self, u, top_k=0, top_p=1.0, min_p=0.0):
+        """len(u) more tokens, drawn on the device with the session's temperature, these filters and the
+        numbers u in [0, 1); returns how many were produced."""
+        u = np.ascontiguousarray(u, np.float32).reshape(-1)
+        return _check(self._lib.jyhip_session_step_sampled(self.h, len(u), top_k, top_p, min_p, _ptr(u)))
 
     @property
     def remaining(self):

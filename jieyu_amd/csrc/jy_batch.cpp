@@ -14,33 +14,7 @@
 
 using namespace jy;
 
-namespace {
-
-// the caller's device, put back when the call ends
-class OnDevice {
-public:
-    OnDevice(int device, hipStream_t st) {
-        CK(hipGetDevice(&was_));
-        int on = device;
-        if (st) CK(hipStreamGetDevice(st, &on));
-        if (on != device) fail("the stream is on another device than the buffers");
-        if (was_ != device) {
-            CK(hipSetDevice(device));
-            set_ = true;
-        }
-    }
-    ~OnDevice() {
-        if (set_) (void)hipSetDevice(was_);
-    }
-    OnDevice(const OnDevice&) = delete;
-    OnDevice& operator=(const OnDevice&) = delete;
-
-private:
-    int was_ = 0;
-    bool set_ = false;
-};
-
-void check_pages(const jyhip_pages* p) {
+void jy::check_pages(const jyhip_pages* p) {
     if (!p) fail("pages is NULL");
     if (p->type != JYHIP_T_I8 && p->type != JYHIP_T_F16 && p->type != JYHIP_T_BF16)
         fail("pages: the type must be int8, fp16 or bf16");
@@ -59,6 +33,8 @@ void check_pages(const jyhip_pages* p) {
         fail("pages: 16-bit pages have no scales");
     }
 }
+
+namespace {
 
 void check_tables(const jyhip_page_tables* t) {
     if (!t || !t->tables) fail("NULL page tables");

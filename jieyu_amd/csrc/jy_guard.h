@@ -21,6 +21,30 @@ inline void ck(hipError_t e, const char* what) {
     if (e != hipSuccess) fail(std::string(what) + ": " + hipGetErrorString(e));
 }
 
+// `device` current for a call (the caller's is put back when it ends); a stream of another is refused
+class OnDevice {
+public:
+    OnDevice(int device, hipStream_t st) {
+        ck(hipGetDevice(&was_), "hipGetDevice");
+        int on = device;
+        if (st) ck(hipStreamGetDevice(st, &on), "hipStreamGetDevice");
+        if (on != device) fail("the stream is on another device than the buffers");
+        if (was_ != device) {
+            ck(hipSetDevice(device), "hipSetDevice");
+            set_ = true;
+        }
+    }
+    ~OnDevice() {
+        if (set_) (void)hipSetDevice(was_);
+    }
+    OnDevice(const OnDevice&) = delete;
+    OnDevice& operator=(const OnDevice&) = delete;
+
+private:
+    int was_ = 0;
+    bool set_ = false;
+};
+
 template <class F>
 auto guarded(F&& f, decltype(f()) bad) -> decltype(f()) {
     try {

@@ -8,6 +8,9 @@
 
 namespace jy {
 
+// throws jy::Error where the kernels cannot run on these pages
+void check_pages(const jyhip_pages* p);
+
 // which position each row is, and where it lies (jyhip_page_tables with the rows' indices)
 struct PageMap {
     const int* tables = nullptr;
@@ -20,6 +23,11 @@ void launch_paged_write(const jyhip_pages& P, const PageMap& M, int rows, const 
                         const jyhip_vectors& v, int type, hipStream_t st);
 void launch_paged_read(const jyhip_pages& P, const PageMap& M, int rows, const jyhip_vectors& k,
                        const jyhip_vectors& v, int type, hipStream_t st);
+
+// RoPE on the q and k heads of every row of qkv ([rows][width], q then k first) in place, row r at
+// position pos[r], the rotated pairs in rope_pack's order; head_dim a multiple of 16
+void launch_rope_rows(float* qkv, int rows, int width, const int* pos, int heads, int hd, const float* cos_t,
+                      const float* sin_t, hipStream_t st);
 
 struct PagedAttn {
     jyhip_pages P;

@@ -112,6 +112,28 @@ __global__ __launch_bounds__(256) void paged_read_kernel(Moved A) {
     store_n<E, DL, VEC>(static_cast<E*>(dst.data) + it.row * dst.row_stride + it.head * dst.head_stride + d0, x);
 }
 
+// a thread takes 8 pairs, which is as far as the rotation moves them
+__global__ __launch_bounds__(256) void rope_rows_kernel(float* qkv, int rows, int width, const int* pos, int heads, int hd,
+                                                        const float* cos_t, const float* sin_t) {
+    const int half = hd / 2, groups = half / 8;
+    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (id >= (int64_t)rows * heads * groups) return;
+    const int g = (int)(id % groups), head = (int)(id / groups % heads);
+    const int64_t row = id / groups / heads;
+    float* const x = qkv + row * width + head * hd + g * 16;
+    const size_t t = (size_t)pos[row] * half + g * 8;
+    float v[16], y[16];
+    load_n<float, 16, true>(x, v);
+#pragma unroll
+    for (int o = 0; o < 8; o++) {
+        const float c = cos_t[t + o], s = sin_t[t + o];
+        const int d = o == 2 || o == 3 ? o + 2 : o == 4 || o == 5 ? o - 2 : o;
+        y[2 * d] = __builtin_fmaf(v[2 * o], c, -(v[2 * o + 1] * s));
+        y[2 * d + 1] = __builtin_fmaf(v[2 * o], s, v[2 * o + 1] * c);
+    }
+    store_n<float, 16, true>(x, y);
+}
+
 // whether every vector starts at a multiple of 16 bytes
 bool aligned(const jyhip_vectors& x, int type) {
     const long long e = type == JYHIP_T_F32 ? 4 : 2;
@@ -168,6 +190,12 @@ void launch_moved(const jyhip_pages& P, const PageMap& M, int rows, const jyhip_
 }
 
 }  // namespace
+
+void launch_rope_rows(float* qkv, int rows, int width, const int* pos, int heads, int hd, const float* cos_t,
+                      const float* sin_t, hipStream_t st) {
+    const int64_t n = (int64_t)rows * heads * (hd / 16);
+    rope_rows_kernel<<<(unsigned)((n + 255) / 256), 256, 0, st>>>(qkv, rows, width, pos, heads, hd, cos_t, sin_t);
+}
 
 void launch_paged_write(const jyhip_pages& P, const PageMap& M, int rows, const jyhip_vectors& k,
                         const jyhip_vectors& v, int type, hipStream_t st) {

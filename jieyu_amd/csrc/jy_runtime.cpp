@@ -7,6 +7,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <climits>
 #include <chrono>
 #include <cmath>
 #include <cstdio>
@@ -17,6 +18,8 @@
 #include "jieyu_amd.h"
 #include "jy_guard.h"
 #include "jy_kernels.h"
+#include "jy_paged.h"
+#include "jy_sample.h"
 #include "jy_stage.h"
 
 using namespace jy;
@@ -150,6 +153,10 @@ struct jyhip_model {
     size_t pk_flag_bytes = 0;
     int* pk_err = nullptr;         // set by the kernel when a barrier wait gave up
     size_t pk_lds = 0;
+    int* paged_idx = nullptr;  // jyhip_forward_paged's tables and rows, and its attention's parts
+    size_t paged_idx_n = 0;
+    float* paged_part = nullptr;
+    size_t paged_part_n = 0;
     HostStage stage;  // forward calls' rows in and out (while it has no ring: plain copies)
     std::vector<void*> owned;
 };
@@ -777,6 +784,8 @@ void release(jyhip_model* m) {
                     (void*)w.q8, (void*)w.qsc, (void*)w.scores, (void*)w.part, (void*)w.ah, (void*)w.al,
                     (void*)w.aus, (void*)w.kp})
         dfree(p);
+    dfree(m->paged_idx);
+    dfree(m->paged_part);
     m->stage.release();
     if (m->stream) (void)hipStreamDestroy(m->stream);
     delete m;
@@ -952,8 +961,15 @@ void run_decode_layers(jyhip_model* m, Workspace& w, const KVDev& kv, const int*
 
 // the prompt (seq > 1): the generic m > 1 matmul path (matmul_q.h:145-161) as tiled
 // GEMMs, RoPE + K/V packing of every row before attention.
+// With `paged` the rows are positions of several sequences whose cache lies in pages (kv and
+// start_pos unused).
+struct PagedRows {
+    const jyhip_pages* pages = nullptr;  // [L]
+    PageMap map;                         // the rows' sequences and positions
+    PagedAttn att;                       // each row with its sequence's table and its own length
+};
 void run_prefill_layers(jyhip_model* m, Workspace& w, const KVDev& kv, int seq, int start_pos,
-                        float* layer_out_host, int max_keys) {
+                        float* layer_out_host, int max_keys, PagedRows* paged = nullptr) {
     hipStream_t st = m->stream;
     const bool q8 = m->wtype == JY_Q8_0, mixed = m->wtype == WT_MIXED;
     const int H = m->H, NQ = m->qd + 2 * m->kvd, F = m->F;
@@ -1027,16 +1043,23 @@ void run_prefill_layers(jyhip_model* m, Workspace& w, const KVDev& kv, int seq, 
             launch_gemm(D.w[1], seq, w.xn, w.qkv + qd, NQ, D.bqkv ? D.bqkv + qd : nullptr, qkv_epi, st);
             launch_gemm(D.w[2], seq, w.xn, w.qkv + qd + kvd, NQ, D.bqkv ? D.bqkv + qd + kvd : nullptr, qkv_epi, st);
         } else if (mf) {
-            pending_qkv = norm_gemm_q8(D.mqkv, D.rms1, w.qkv, D.qkv.rows, D.bqkv, qkv_epi, true);
+            pending_qkv = norm_gemm_q8(D.mqkv, D.rms1, w.qkv, D.qkv.rows, D.bqkv, qkv_epi, !paged);
         } else if (q8) {
             gemm_q8(D.qkv, D.mqkv, w.xn, w.qkv, D.bqkv, qkv_epi);
         } else {
             launch_gemm_f32(D.f_qkv, H, NQ, seq, w.xn, w.qkv, D.bqkv, qkv_epi, st);
         }
-        launch_rope_pack(w.qkv, seq, start_pos, nullptr, m->nh, m->nkv, m->hd, m->cos_t, m->sin_t, kv, l, w.q8,
-                         w.qsc, st, w.kp, pending_qkv, pending_qkv > 1 ? D.bqkv : nullptr);
+        if (!paged)
+            launch_rope_pack(w.qkv, seq, start_pos, nullptr, m->nh, m->nkv, m->hd, m->cos_t, m->sin_t, kv, l, w.q8,
+                             w.qsc, st, w.kp, pending_qkv, pending_qkv > 1 ? D.bqkv : nullptr);
         at.layer = l;
-        if (split_rows) {
+        if (paged) {
+            launch_rope_rows(w.qkv, seq, NQ, paged->map.pos, m->nh + m->nkv, m->hd, m->cos_t, m->sin_t, st);
+            const jyhip_vectors k{w.qkv + m->qd, NQ, m->hd}, v{w.qkv + m->qd + m->kvd, NQ, m->hd};
+            launch_paged_write(paged->pages[l], paged->map, seq, k, v, JYHIP_T_F32, st);
+            paged->att.P = paged->pages[l];
+            launch_paged_attend(paged->att, st);
+        } else if (split_rows) {
             at.row0 = 0;
             at.nrows = seq;
             launch_attention_prefill_split(at, st);
@@ -1343,10 +1366,13 @@ struct Session {
     int decoded = 0;
     std::vector<float> hlog;
     float* logits_out = nullptr;
+    unsigned char* draw = nullptr;  // step_sampled's settings, random numbers and sampling workspace
+    size_t draw_n = 0;
 
     ~Session() {
         for (hipGraphExec_t e : exec)
             if (e) (void)hipGraphExecDestroy(e);
+        dfree(draw);
         if (m && m->owner == this) m->owner = nullptr;
         for (hipEvent_t e : ev)
             if (e) (void)hipEventDestroy(e);
@@ -1504,10 +1530,8 @@ struct Session {
     // the graph for a step over a sequence of `length` tokens (it attends `length` keys)
     hipGraphExec_t graph_for(int length) const { return exec[length <= short_keys(m) ? 1 : 0]; }
 
-    // up to n more tokens; returns how many were produced
-    int step(int n) {
-        n = std::min(n, remaining());
-        if (n <= 0) return 0;
+    // the graphs for n steps from here, captured (again) where needed
+    void ready(int n) {
         if (m->owner != this)
             fail("session: a later generation has started on this model; this one can no longer step");
         // a graph captured before the workspace was replaced (a longer prompt or chunk
@@ -1523,6 +1547,13 @@ struct Session {
         if (len + n - 1 > short_keys(m) && !exec[0]) capture(0);
         check_buffers(0);
         check_buffers(1);
+    }
+
+    // up to n more tokens; returns how many were produced
+    int step(int n) {
+        n = std::min(n, remaining());
+        if (n <= 0) return 0;
+        ready(n);
         hipStream_t st = m->stream;
         CK(hipEventRecord(ev[2], st));
         int made = 0;
@@ -1540,6 +1571,77 @@ struct Session {
         CK(hipEventRecord(ev[3], st));
         CK(hipStreamSynchronize(st));
         check_persist(m);
+        float ms = 0.0f;
+        CK(hipEventElapsedTime(&ms, ev[2], ev[3]));
+        decode_ms += ms;
+        decoded += made;
+        return made;
+    }
+
+    // step() with the tokens drawn on the device from the given numbers
+    int step_sampled(int n, int top_k, float top_p, float min_p, const float* u) {
+        if (greedy) fail("step_sampled: the session is greedy (temperature <= 0)");
+        if (rp != 1.0f) fail("step_sampled: the session has a repetition penalty");
+        n = std::min(n, remaining());
+        if (n <= 0) return 0;
+        if (!u) fail("step_sampled: u is NULL");
+        if (m->V > SAMPLE_MAX_VOCAB) fail("step_sampled: the vocabulary is too large");
+        ready(n);
+        hipStream_t st = m->stream;
+        // [settings: temperature, top_k, top_p, min_p][u][workspace]
+        const size_t head = (16 + sizeof(float) * (size_t)n + 255) / 256 * 256;
+        const size_t need = head + sample_workspace_bytes(1, m->V);
+        if (draw_n < need) {
+            dfree(draw);
+            draw = nullptr;
+            draw_n = 0;
+            draw = dalloc<uint8_t>(need, false);
+            draw_n = need;
+        }
+        std::vector<unsigned char> h(16 + sizeof(float) * (size_t)n);
+        memcpy(&h[0], &temperature, 4);
+        memcpy(&h[4], &top_k, 4);
+        memcpy(&h[8], &top_p, 4);
+        memcpy(&h[12], &min_p, 4);
+        memcpy(&h[16], u, sizeof(float) * (size_t)n);
+        CK(hipMemcpyAsync(draw, h.data(), h.size(), hipMemcpyHostToDevice, st));
+        SampleArgs A;
+        A.logits = m->logits;
+        A.row_stride = m->V;
+        A.type = JYHIP_T_F32;
+        A.rows = 1;
+        A.vocab = m->V;
+        A.temperature = reinterpret_cast<const float*>(draw);
+        A.top_k = reinterpret_cast<const int*>(draw + 4);
+        A.top_p = reinterpret_cast<const float*>(draw + 8);
+        A.min_p = reinterpret_cast<const float*>(draw + 12);
+        A.ws = draw + head;
+        const int from = len;
+        CK(hipEventRecord(ev[2], st));
+        int made = 0;
+        for (; made < n && !stopped; made++) {
+            CK(hipGraphLaunch(graph_for(from + made), st));
+            A.u = reinterpret_cast<const float*>(draw + 16) + made;
+            A.ids = m->ids + from + made;
+            launch_sample(A, st);
+            launch_advance(m->ids, m->state, from + made, st);
+            CK(hipGetLastError());
+            if (cb || neos > 0) accept(fetch_last());
+        }
+        if (!cb && neos == 0) {
+            CK(hipMemcpyAsync(ids.data() + from, m->ids + from, sizeof(int) * made, hipMemcpyDeviceToHost, st));
+            len += made;
+        }
+        CK(hipEventRecord(ev[3], st));
+        CK(hipStreamSynchronize(st));
+        check_persist(m);
+        if (logits_out) CK(hipMemcpy(logits_out, m->logits, sizeof(float) * m->V, hipMemcpyDeviceToHost));
+        int state[3];
+        CK(hipMemcpy(state, m->state, sizeof(state), hipMemcpyDeviceToHost));
+        if (state[2]) {
+            stopped = true;
+            fail("step_sampled: a step's logits hold no number to pick from");
+        }
         float ms = 0.0f;
         CK(hipEventElapsedTime(&ms, ev[2], ev[3]));
         decode_ms += ms;
@@ -1627,6 +1729,100 @@ int forward_impl(jyhip_model* m, jyhip_kv* kv, const float* X, float* out, int s
     rows_out(m, w, out, seq, true);
     check_persist(m);
     kv->current_len = start_pos + seq;
+    return 0;
+}
+
+int forward_paged(jyhip_model* m, const jyhip_pages* pages, const float* X, float* out, int rows, const int* tables,
+                  int num_seqs, int table_stride, const int* seq, const int* pos) {
+    if (!pages || !X || !out) fail("forward_paged: NULL pages, X or out");
+    if (!tables || !pos) fail("forward_paged: NULL tables or pos");
+    if (rows <= 0) fail("forward_paged: rows must be positive");
+    if (num_seqs < 1 || table_stride < 1) fail("forward_paged: num_seqs and table_stride must be positive");
+    if (!seq && rows > num_seqs) fail("forward_paged: without seq there is one row per sequence: more rows than sequences");
+    for (int l = 0; l < m->L; l++) {
+        check_pages(&pages[l]);
+        if (pages[l].num_kv_heads != m->nkv || pages[l].head_dim != m->hd)
+            fail("forward_paged: the pages' heads are not the model's");
+        if (pages[l].device != m->device) fail("forward_paged: the pages are on another device than the model");
+        if (pages[l].num_pages != pages[0].num_pages || pages[l].page_size != pages[0].page_size)
+            fail("forward_paged: the layers' pools differ in shape");
+    }
+    const int ps = pages[0].page_size;
+    // [tables of the sequences][seq][pos][pos + 1][each row's table]
+    const size_t nt = (size_t)num_seqs * table_stride, rt = (size_t)rows * table_stride;
+    std::vector<int> h;
+    h.reserve(nt + 3 * (size_t)rows + rt);
+    h.assign(tables, tables + nt);
+    std::vector<int64_t> slots(rows);
+    int max_len = 0;
+    for (int r = 0; r < rows; r++) {
+        const int s = seq ? seq[r] : r;
+        if (s < 0 || s >= num_seqs) fail("forward_paged: row " + std::to_string(r) + "'s sequence is out of range");
+        if (pos[r] < 0 || pos[r] >= m->max_seq) fail("forward_paged: a position outside the RoPE table");
+        if (pos[r] / ps >= table_stride) fail("forward_paged: a position past the page table");
+        max_len = std::max(max_len, pos[r] + 1);
+        const int* t = tables + (size_t)s * table_stride;
+        for (int i = 0; i <= pos[r] / ps; i++)
+            if (t[i] < 0 || t[i] >= pages[0].num_pages)
+                fail("forward_paged: sequence " + std::to_string(s) + " has no page for a position that it attends over");
+        slots[r] = (int64_t)t[pos[r] / ps] * ps + pos[r] % ps;
+        h.push_back(s);
+    }
+    std::sort(slots.begin(), slots.end());
+    if (std::adjacent_find(slots.begin(), slots.end()) != slots.end())
+        fail("forward_paged: two rows are written to the same slot");
+    for (int r = 0; r < rows; r++) h.push_back(pos[r]);
+    for (int r = 0; r < rows; r++) h.push_back(pos[r] + 1);
+    for (int r = 0; r < rows; r++) {
+        const int* t = tables + (size_t)(seq ? seq[r] : r) * table_stride;
+        h.insert(h.end(), t, t + table_stride);
+    }
+    if (paged_attend_blocks(pages[0], rows, m->nh, max_len) >= (1 << 24) ||
+        (int64_t)rows * m->nkv > INT_MAX)
+        fail("forward_paged: too many rows for one call");
+    const OnDevice on(m->device, nullptr);
+    ensure_ws(m, rows);
+    const size_t part = paged_attend_part_floats(pages[0], rows, m->nh, max_len);
+    if (m->paged_idx_n < h.size()) {
+        dfree(m->paged_idx);
+        m->paged_idx = nullptr;
+        m->paged_idx_n = 0;
+        m->paged_idx = dalloc<int>(h.size(), false);
+        m->paged_idx_n = h.size();
+    }
+    if (m->paged_part_n < part) {
+        dfree(m->paged_part);
+        m->paged_part = nullptr;
+        m->paged_part_n = 0;
+        m->paged_part = dalloc<float>(part, false);
+        m->paged_part_n = part;
+    }
+    hipStream_t st = m->stream;
+    CK(hipMemcpyAsync(m->paged_idx, h.data(), h.size() * sizeof(int), hipMemcpyHostToDevice, st));
+    Workspace& w = m->ws;
+    PagedRows p;
+    p.pages = pages;
+    const int* d = m->paged_idx;
+    p.map.tables = d;
+    p.map.nseq = num_seqs;
+    p.map.stride = table_stride;
+    p.map.seq = d + nt;
+    p.map.pos = d + nt + rows;
+    PagedAttn& a = p.att;
+    a.M.tables = d + nt + 3 * (size_t)rows;
+    a.M.nseq = rows;
+    a.M.stride = table_stride;
+    a.lens = d + nt + 2 * (size_t)rows;
+    a.max_len = a.cap = max_len;
+    a.nh = m->nh;
+    a.scale = 1.0f / sqrtf((float)m->hd);
+    a.q = jyhip_vectors{w.qkv, m->qd + 2 * m->kvd, m->hd};
+    a.out = jyhip_vectors{w.att, m->qd, m->hd};
+    a.type = JYHIP_T_F32;
+    a.part = m->paged_part;
+    rows_in(m, w, X, rows, true);
+    run_prefill_layers(m, w, KVDev{}, rows, 0, nullptr, std::max(4, max_len), &p);
+    rows_out(m, w, out, rows, true);
     return 0;
 }
 
@@ -1891,6 +2087,14 @@ JYHIP_API int jyhip_forward_cached_noalloc(jyhip_model* m, jyhip_kv* kv, float* 
     }, -1);
 }
 
+JYHIP_API int jyhip_forward_paged(jyhip_model* m, const jyhip_pages* pages, const float* X, float* out, int rows,
+                                  const int* tables, int num_seqs, int table_stride, const int* seq, const int* pos) {
+    return guarded([&]() {
+        if (!m) fail("model is NULL");
+        return forward_paged(m, pages, X, out, rows, tables, num_seqs, table_stride, seq, pos);
+    }, -1);
+}
+
 JYHIP_API int jyhip_generate(jyhip_model* m, jyhip_kv* kv, const int* prompt_ids, int prompt_len, const int* eos_ids,
                              int num_eos, int max_seq, int max_new, float temperature, float repetition_penalty,
                              int* out_ids, jyhip_token_cb cb, void* cb_ud, float* logits_out, jyhip_stats* stats) {
@@ -1944,6 +2148,16 @@ JYHIP_API int jyhip_session_step(jyhip_session* h, int n) {
         if (!h) fail("session is NULL");
         if (!h->active || n <= 0) return 0;
         const int made = h->s.step(n);
+        h->s.finish();
+        return made;
+    }, -1);
+}
+
+JYHIP_API int jyhip_session_step_sampled(jyhip_session* h, int n, int top_k, float top_p, float min_p, const float* u) {
+    return guarded([&]() {
+        if (!h) fail("session is NULL");
+        if (!h->active || n <= 0) return 0;
+        const int made = h->s.step_sampled(n, top_k, top_p, min_p, u);
         h->s.finish();
         return made;
     }, -1);

@@ -25,5 +25,8 @@ struct SampleArgs {
 };
 size_t sample_workspace_bytes(int rows, int vocab);
 void launch_sample(const SampleArgs& A, hipStream_t st);
+// a generation's device state after the token ids[at]: state[0] = at + 1, state[1] (stopped) = 0; where
+// there was none to pick (-1), id 0 stands for it and state[2] is set
+void launch_advance(int* ids, int* state, int at, hipStream_t st);
 
 }  // namespace jy

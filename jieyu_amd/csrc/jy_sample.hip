@@ -1088,6 +1088,15 @@ __global__ __launch_bounds__(NT) void sample_pick_kernel(SampleArgs A, SamplePla
     if (threadIdx.x == 0) A.ids[row] = id;
 }
 
+__global__ void advance_kernel(int* ids, int* state, int at) {
+    if (ids[at] < 0) {
+        ids[at] = 0;
+        state[2] = 1;
+    }
+    state[0] = at + 1;
+    state[1] = 0;
+}
+
 template <class E>
 void launch_type(const SampleArgs& A, const SamplePlan& P, hipStream_t st) {
     const unsigned grid = (unsigned)(A.rows * P.segs);
@@ -1110,5 +1119,7 @@ void launch_sample(const SampleArgs& A, hipStream_t st) {
     else
         launch_type<__bf16>(A, P, st);
 }
+
+void launch_advance(int* ids, int* state, int at, hipStream_t st) { advance_kernel<<<1, 1, 0, st>>>(ids, state, at); }
 
 }  // namespace jy
