@@ -38,10 +38,13 @@ class _Bound:
     def __init__(self):
         import torch
         L = lib()
-        self.torch = torch
+        self.torch, self.int32 = torch, torch.int32
         self.io = {torch.float32: T_F32, torch.float16: T_F16, torch.bfloat16: T_BF16}
         self.pool = {torch.int8: T_I8, torch.float16: T_F16, torch.bfloat16: T_BF16}
-        self.stream = torch.cuda.current_stream
+        # the address of the current stream of device i (without torch.cuda.Stream's object around it,
+        # where this torch has that)
+        self.stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda i: torch.cuda.current_stream(i).cuda_stream)
 
         def proto(name, res, *args):
             fn = getattr(L, name)
@@ -73,7 +76,7 @@ def _failed(b):
 
 def _indices(b, t, n, device, name):
     """The address of n int32 values."""
-    if t.dtype is not b.torch.int32 or t.dim() != 1 or t.shape[0] != n or t.device != device or not t.is_contiguous():
+    if t.dtype is not b.int32 or t.shape != (n,) or t.device != device or not t.is_contiguous():
         raise JyError(f"{name}: {n} contiguous int32 values on {device} are needed")
     return t.data_ptr()
 
@@ -129,30 +132,31 @@ class PagePool:
         return self._layers[layer]
 
     def _tables(self, t):
-        if t.dtype is not self._b.torch.int32 or t.dim() != 2 or t.device != self.device or not t.is_contiguous():
+        shape = t.shape
+        if t.dtype is not self._b.int32 or len(shape) != 2 or t.device != self.device or not t.is_contiguous():
             raise JyError(f"tables: a contiguous int32 tensor [sequences][pages] on {self.device} is needed")
-        return _Tables(t.data_ptr(), t.shape[0], t.shape[1])
+        return _Tables(t.data_ptr(), *shape)
 
-    def _vectors(self, t, rows, heads, dtype, name):
-        if (t.dim() != 3 or t.shape[0] != rows or t.shape[1] != heads or t.shape[2] != self.hd or t.dtype is not dtype or
-                t.device != self.device):
-            raise JyError(f"{name}: a {dtype} tensor of {(rows, heads, self.hd)} on {self.device} is needed")
-        s = t.stride()
-        if s[2] != 1:
+    def _vectors(self, t, shape, dtype, name):
+        if t.shape != shape or t.dtype is not dtype or t.device != self.device:
+            raise JyError(f"{name}: a {dtype} tensor of {shape} on {self.device} is needed")
+        row, head, one = t.stride()
+        if one != 1:
             raise JyError(f"{name}: a vector's elements must lie side by side")
-        return _Vectors(t.data_ptr(), s[0], s[1])
+        return _Vectors(t.data_ptr(), row, head)
 
     def _move(self, fn, layer, k, v, tables, pos, seq):
-        b, rows = self._b, k.shape[0]
-        code = b.io.get(k.dtype)
-        if code is None:
-            raise JyError("k and v: float32, float16 or bfloat16")
+        b, device, dtype, shape = self._b, self.device, k.dtype, k.shape
+        code = b.io.get(dtype)
+        if code is None or len(shape) != 3:
+            raise JyError("k and v: float32, float16 or bfloat16 [rows][kv heads][head size]")
+        rows = shape[0]
+        shape = (rows, self.nkv, self.hd)
         pages = self._layer(layer)
-        K = self._vectors(k, rows, self.nkv, k.dtype, "k")
-        V = self._vectors(v, rows, self.nkv, k.dtype, "v")
-        at = None if seq is None else _indices(b, seq, rows, self.device, "seq")
-        p = _indices(b, pos, rows, self.device, "pos")
-        if rows and fn(pages, self._tables(tables), rows, at, p, K, V, code, b.stream(self.device).cuda_stream) != 0:
+        K, V = self._vectors(k, shape, dtype, "k"), self._vectors(v, shape, dtype, "v")
+        at = None if seq is None else _indices(b, seq, rows, device, "seq")
+        p = _indices(b, pos, rows, device, "pos")
+        if rows and fn(pages, self._tables(tables), rows, at, p, K, V, code, b.stream(device.index)) != 0:
             _failed(b)
 
     def write(self, layer, k, v, tables, pos, seq=None):
@@ -177,14 +181,14 @@ class PagePool:
         lens, sizes the launch: a longer one is cut to it.  scale: 1 / sqrt(head size) unless given."""
         b = self._b
         pages, T = self._layer(layer), self._tables(tables)
-        batch, heads = q.shape[0], q.shape[1]
         code = b.io.get(q.dtype)
-        if code is None:
-            raise JyError("q: float32, float16 or bfloat16")
+        if code is None or q.dim() != 3:
+            raise JyError("q: float32, float16 or bfloat16 [sequences][heads][head size]")
+        batch, heads, _ = q.shape
         if out is None:
             out = q.new_empty((batch, heads, self.hd))
-        Q = self._vectors(q, batch, heads, q.dtype, "q")
-        O = self._vectors(out, batch, heads, q.dtype, "out")
+        shape = (batch, heads, self.hd)
+        Q, O = self._vectors(q, shape, q.dtype, "q"), self._vectors(out, shape, q.dtype, "out")
         n = _indices(b, lens, batch, self.device, "lens")
         if T.num_seqs != batch:
             raise JyError("attend: one query row for each sequence of the tables")
@@ -193,7 +197,7 @@ class PagePool:
         need = b.attend_workspace(pages, batch, heads, max_len)
         ws = q.new_empty(need, dtype=b.torch.uint8) if need else None
         if b.attend(pages, T, n, max_len, heads, 1.0 / math.sqrt(self.hd) if scale is None else scale, Q, O, code,
-                    ws.data_ptr() if need else None, need, b.stream(self.device).cuda_stream) != 0:
+                    ws.data_ptr() if need else None, need, b.stream(self.device.index)) != 0:
             _failed(b)
         return out
 
@@ -202,7 +206,7 @@ def _settings(b, t, rows, device, dtype, name):
     """The address of one setting per row (None: off)."""
     if t is None:
         return None
-    if t.dtype is not dtype or t.dim() != 1 or t.shape[0] != rows or t.device != device or not t.is_contiguous():
+    if t.dtype is not dtype or t.shape != (rows,) or t.device != device or not t.is_contiguous():
         raise JyError(f"sample: {name} must be {rows} contiguous {dtype} values on {device}")
     return t.data_ptr()
 
@@ -232,7 +236,7 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, out=
     need = b.sample_workspace(rows, vocab)
     ws = logits.new_empty(need, dtype=torch.uint8) if need else None
     if b.sample(logits.data_ptr(), code, rows, vocab, logits.stride(0), *args, ws.data_ptr() if need else None, need,
-                dev.index, b.stream(dev).cuda_stream) != 0:
+                dev.index, b.stream(dev.index)) != 0:
         _failed(b)
     return out
 
