@@ -2,7 +2,9 @@
 //
 // A vector (one row's key or value of one head, head_dim elements) belongs to 16 lanes, DL
 // consecutive elements each, so its absolute maximum takes four DPP moves within a row of
-// lanes and its bytes leave as one contiguous run.  Both kernels move each byte once.
+// lanes and its bytes leave as one contiguous run.  The lanes take the key and the value of a head
+// together: one look-up of the slot, two vectors in flight.  Every byte moves once; small calls are
+// bound by the launch and the look-up's chain (position, page id), large ones by memory.
 #include <hip/hip_runtime.h>
 
 #include "jy_device.h"
@@ -15,48 +17,30 @@ namespace {
 struct Moved {
     jyhip_pages P;
     PageMap M;
-    int rows;
+    int rows, ps_log2;
     jyhip_vectors k, v;
 };
 
-// the vector of this group of 16 lanes: (row, K or V, head), heads fastest; false past the end
+// the vectors of this group of 16 lanes: (row, head), heads fastest; false past the end
 struct Item {
-    int row, which, head;
+    int row, head;
 };
 __device__ __forceinline__ bool item_of(const Moved& A, Item& it) {
-    const int64_t i = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-    const int nkv = A.P.num_kv_heads;
-    if (i >= (int64_t)A.rows * 2 * nkv) return false;
-    it.head = (int)(i % nkv);
-    const int64_t r = i / nkv;
-    it.which = (int)(r & 1);
-    it.row = (int)(r >> 1);
-    return true;
+    const unsigned i = blockIdx.x * 16 + (threadIdx.x >> 4), nkv = A.P.num_kv_heads;
+    it.row = (int)(i / nkv);
+    it.head = (int)(i - it.row * nkv);
+    return it.row < A.rows;
 }
 
-template <int PT, int T, int DL, bool VEC>
-__global__ __launch_bounds__(256) void paged_write_kernel(Moved A) {
-    typedef elem_t<PT> PE;
-    typedef elem_t<T> E;
-    Item it;
-    if (!item_of(A, it)) return;
-    const jyhip_pages& P = A.P;
-    const int lane = threadIdx.x & 15;
-    const int d0 = lane * DL;
-    const bool on = d0 < P.head_dim;
-    const jyhip_vectors& src = it.which ? A.v : A.k;
-    float x[DL];
-    if (on) {
-        load_n<E, DL, VEC>(static_cast<const E*>(src.data) + it.row * src.row_stride + it.head * src.head_stride + d0, x);
-    } else {
-#pragma unroll
-        for (int i = 0; i < DL; i++) x[i] = 0.0f;
-    }
-    const int64_t slot = slot_of(A.M, P.num_pages, P.page_size, A.M.seq ? A.M.seq[it.row] : it.row, A.M.pos[it.row]);
-    if (slot < 0) return;
-    const int64_t page = slot / P.page_size;
-    const int64_t vec = (page * P.num_kv_heads + it.head) * P.page_size + slot % P.page_size;
-    PE* dst = static_cast<PE*>(it.which ? P.v : P.k) + vec * P.head_dim + d0;
+// where the item's vectors lie in the pool (-1: they do not exist)
+__device__ __forceinline__ int64_t vector_of(const Moved& A, const Item& it) {
+    const int64_t slot = slot_of(A.M, A.P.num_pages, A.ps_log2, A.M.seq ? A.M.seq[it.row] : it.row, A.M.pos[it.row]);
+    if (slot < 0) return -1;
+    return (((slot >> A.ps_log2) * A.P.num_kv_heads + it.head) << A.ps_log2) + (slot & ((1 << A.ps_log2) - 1));
+}
+
+template <class PE, int PT, int DL>
+__device__ __forceinline__ void hold(PE* dst, float* scale, const float (&x)[DL], bool on) {
     if constexpr (PT == JYHIP_T_I8) {
         float a = 0.0f;
         bool bad = false;
@@ -79,10 +63,33 @@ __global__ __launch_bounds__(256) void paged_write_kernel(Moved A) {
             typedef int words __attribute__((ext_vector_type(DL / 4)));
             *reinterpret_cast<words*>(dst) = __builtin_bit_cast(words, q);
         }
-        if (lane == 0) (it.which ? P.v_scale : P.k_scale)[vec] = bad ? __builtin_nanf("") : quant_scale(a);
+        if ((threadIdx.x & 15) == 0) *scale = bad ? __builtin_nanf("") : quant_scale(a);
     } else if (on) {
         store_n<PE, DL, true>(dst, x);
     }
+}
+
+template <int PT, int T, int DL, bool VEC>
+__global__ __launch_bounds__(256) void paged_write_kernel(Moved A) {
+    typedef elem_t<PT> PE;
+    typedef elem_t<T> E;
+    Item it;
+    if (!item_of(A, it)) return;
+    const jyhip_pages& P = A.P;
+    const int d0 = (threadIdx.x & 15) * DL;
+    const bool on = d0 < P.head_dim;
+    float k[DL], v[DL];
+    if (on) {
+        load_n<E, DL, VEC>(static_cast<const E*>(A.k.data) + it.row * A.k.row_stride + it.head * A.k.head_stride + d0, k);
+        load_n<E, DL, VEC>(static_cast<const E*>(A.v.data) + it.row * A.v.row_stride + it.head * A.v.head_stride + d0, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < DL; i++) k[i] = v[i] = 0.0f;
+    }
+    const int64_t vec = vector_of(A, it);
+    if (vec < 0) return;
+    hold<PE, PT, DL>(static_cast<PE*>(P.k) + vec * P.head_dim + d0, P.k_scale + vec, k, on);
+    hold<PE, PT, DL>(static_cast<PE*>(P.v) + vec * P.head_dim + d0, P.v_scale + vec, v, on);
 }
 
 template <int PT, int T, int DL, bool VEC>
@@ -94,22 +101,25 @@ __global__ __launch_bounds__(256) void paged_read_kernel(Moved A) {
     const jyhip_pages& P = A.P;
     const int d0 = (threadIdx.x & 15) * DL;
     if (d0 >= P.head_dim) return;
-    const int64_t slot = slot_of(A.M, P.num_pages, P.page_size, A.M.seq ? A.M.seq[it.row] : it.row, A.M.pos[it.row]);
-    float x[DL];
-#pragma unroll
-    for (int i = 0; i < DL; i++) x[i] = 0.0f;
-    if (slot >= 0) {
-        const int64_t page = slot / P.page_size;
-        const int64_t vec = (page * P.num_kv_heads + it.head) * P.page_size + slot % P.page_size;
-        load_n<PE, DL, true>(static_cast<const PE*>(it.which ? P.v : P.k) + vec * P.head_dim + d0, x);
+    const int64_t vec = vector_of(A, it);
+    float k[DL], v[DL];
+    if (vec >= 0) {
+        load_n<PE, DL, true>(static_cast<const PE*>(P.k) + vec * P.head_dim + d0, k);
+        load_n<PE, DL, true>(static_cast<const PE*>(P.v) + vec * P.head_dim + d0, v);
         if constexpr (PT == JYHIP_T_I8) {
-            const float s = (it.which ? P.v_scale : P.k_scale)[vec];
+            const float ks = P.k_scale[vec], vs = P.v_scale[vec];
 #pragma unroll
-            for (int i = 0; i < DL; i++) x[i] *= s;
+            for (int i = 0; i < DL; i++) {
+                k[i] *= ks;
+                v[i] *= vs;
+            }
         }
+    } else {
+#pragma unroll
+        for (int i = 0; i < DL; i++) k[i] = v[i] = 0.0f;
     }
-    const jyhip_vectors& dst = it.which ? A.v : A.k;
-    store_n<E, DL, VEC>(static_cast<E*>(dst.data) + it.row * dst.row_stride + it.head * dst.head_stride + d0, x);
+    store_n<E, DL, VEC>(static_cast<E*>(A.k.data) + it.row * A.k.row_stride + it.head * A.k.head_stride + d0, k);
+    store_n<E, DL, VEC>(static_cast<E*>(A.v.data) + it.row * A.v.row_stride + it.head * A.v.head_stride + d0, v);
 }
 
 // a thread takes 8 pairs, which is as far as the rotation moves them
@@ -178,9 +188,9 @@ void launch_io(const Moved& A, int type, bool vec, unsigned grid, hipStream_t st
 template <bool WRITE>
 void launch_moved(const jyhip_pages& P, const PageMap& M, int rows, const jyhip_vectors& k, const jyhip_vectors& v,
                   int type, hipStream_t st) {
-    const Moved A{P, M, rows, k, v};
+    const Moved A{P, M, rows, __builtin_ctz(P.page_size), k, v};
     const bool vec = aligned(k, type) && aligned(v, type);
-    const unsigned grid = (unsigned)(((int64_t)rows * 2 * P.num_kv_heads + 15) / 16);
+    const unsigned grid = (unsigned)(((int64_t)rows * P.num_kv_heads + 15) / 16);
     if (P.type == JYHIP_T_I8)
         launch_io<WRITE, JYHIP_T_I8>(A, type, vec, grid, st);
     else if (P.type == JYHIP_T_F16)

@@ -69,14 +69,15 @@ __device__ __forceinline__ void store_n(E* p, const float (&x)[N]) {
     }
 }
 
-// the slot of (sequence, position) as an index over [num_pages][page_size], -1 where there is none
-__device__ __forceinline__ int64_t slot_of(const PageMap& M, int num_pages, int page_size, int seq, int pos) {
+// the slot of (sequence, position) as an index over [num_pages][page_size], -1 where there is none;
+// page_size = 1 << ps_log2
+__device__ __forceinline__ int64_t slot_of(const PageMap& M, int num_pages, int ps_log2, int seq, int pos) {
     if (seq < 0 || seq >= M.nseq || pos < 0) return -1;
-    const int at = pos / page_size;
+    const int at = pos >> ps_log2;
     if (at >= M.stride) return -1;
     const int page = M.tables[(int64_t)seq * M.stride + at];
     if (page < 0 || page >= num_pages) return -1;
-    return (int64_t)page * page_size + pos % page_size;
+    return ((int64_t)page << ps_log2) + (pos & ((1 << ps_log2) - 1));
 }
 
 }  // namespace jy
