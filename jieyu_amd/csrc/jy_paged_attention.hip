@@ -182,7 +182,8 @@ struct Query<JYHIP_T_I8, KC, WIDE> {
             for (int p = 0; p < 3; p++) d[p] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[c], q[c][p], d[p], 0, 0, 0);
 #pragma unroll
         for (int i = 0; i < 4; i++)
-            s[i] = __builtin_fmaf((float)d[2][i], 65536.0f, __builtin_fmaf((float)d[1][i], 256.0f, (float)d[0][i]));
+            // (|d| <= 128 * 128 * 256 = 2^22, so the lower two digits add up in 31 bits)
+            s[i] = __builtin_fmaf((float)d[2][i], 65536.0f, (float)(d[1][i] * 256 + d[0][i]));
     }
 };
 
@@ -267,53 +268,62 @@ struct Tile {
     int live[2];  // positions of each group that exist: the first ones
 };
 
+// Loads of 16 positions go through a buffer resource over just those that exist: the ones that do not
+// (past the sequence's end, in a hole) read as zeros and are not fetched.
 template <int PT, int NC>
 struct Loader {
     typedef Tile<PT, NC> T;
     static constexpr int ES = T::ES, DL = 4 * NC;
-    const char *k, *v;
+    const char *k, *v;       // this head's first position in page 0
     const float *ks, *vs;
-    unsigned koff[T::KC], voff;
-    int64_t head_stride;     // positions between pages of one head: nkv * page_size
-    int num_pages, ps, hd;
+    unsigned koff[T::KC], voff[4];
+    int64_t page_rows;       // positions (of all heads) per page
+    int num_pages, ps, row_bytes;
 
     __device__ __forceinline__ void load(T& t, int page0, int page1, int key0, int n) const {
+#if defined(__HIP_DEVICE_COMPILE__)
 #pragma unroll
         for (int g = 0; g < 2; g++) {
-            int page = g ? page1 : page0;
-            const int at = key0 + 16 * g;
+            const int page = g ? page1 : page0, at = key0 + 16 * g;
             const bool here = (unsigned)page < (unsigned)num_pages;
-            t.live[g] = here ? min(max(n - at, 0), 16) : 0;
-            if (!here) page = 0;
-            // (positions past the sequence's end are in the page all the same; they are masked)
-            const int64_t row = page * head_stride + (at & (ps - 1));
-            const char* kr = k + row * (hd * ES);
-            const char* vr = v + row * (hd * ES);
+            t.live[g] = __builtin_amdgcn_readfirstlane(here ? min(max(n - at, 0), 16) : 0);
+            const int64_t row = (here ? page * page_rows : 0) + (at & (ps - 1));
+            const auto kr = buffer(k + row * row_bytes, t.live[g] * row_bytes);
+            const auto vr = buffer(v + row * row_bytes, t.live[g] * row_bytes);
 #pragma unroll
-            for (int c = 0; c < T::KC; c++) t.k[g][c] = *reinterpret_cast<const i4_t*>(kr + koff[c]);
+            for (int c = 0; c < T::KC; c++)
+                t.k[g][c] = __builtin_bit_cast(i4_t, __builtin_amdgcn_raw_buffer_load_b128(kr, koff[c], 0, 0));
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const char* p = vr + voff + (unsigned)(j * hd * ES);
-                typedef uint32_t words __attribute__((ext_vector_type(T::VW < 4 ? T::VW : 4)));
-                constexpr int PER = T::VW < 4 ? T::VW : 4;
+                uint32_t* const d = t.v[g * 4 + j];
+                if constexpr (T::VW == 1) {
+                    d[0] = __builtin_amdgcn_raw_buffer_load_b32(vr, voff[j], 0, 0);
+                } else if constexpr (T::VW == 2) {
+                    const i2_t x = __builtin_bit_cast(i2_t, __builtin_amdgcn_raw_buffer_load_b64(vr, voff[j], 0, 0));
+                    d[0] = x[0];
+                    d[1] = x[1];
+                } else {
 #pragma unroll
-                for (int w = 0; w < T::VW / PER; w++) {
-                    if constexpr (PER == 1) {
-                        t.v[g * 4 + j][w] = reinterpret_cast<const uint32_t*>(p)[w];
-                    } else {
-                        const words x = reinterpret_cast<const words*>(p)[w];
+                    for (int w = 0; w < T::VW; w += 4) {
+                        const i4_t x = __builtin_bit_cast(i4_t, __builtin_amdgcn_raw_buffer_load_b128(vr, voff[j] + 4 * w, 0, 0));
 #pragma unroll
-                        for (int i = 0; i < PER; i++) t.v[g * 4 + j][w * PER + i] = x[i];
+                        for (int i = 0; i < 4; i++) d[w + i] = x[i];
                     }
                 }
             }
             if constexpr (PT == JYHIP_T_I8) {
-                const int64_t sr = row + ((threadIdx.x & 63) >> 4) * 4;
-                t.ks[g] = *reinterpret_cast<const f4_t*>(ks + sr);
-                t.vs[g] = *reinterpret_cast<const f4_t*>(vs + sr);
+                const unsigned o = ((threadIdx.x & 63) >> 4) * 16;
+                t.ks[g] = __builtin_bit_cast(f4_t, __builtin_amdgcn_raw_buffer_load_b128(buffer(ks + row, t.live[g] * 4), o, 0, 0));
+                t.vs[g] = __builtin_bit_cast(f4_t, __builtin_amdgcn_raw_buffer_load_b128(buffer(vs + row, t.live[g] * 4), o, 0, 0));
             }
         }
+#endif
     }
+#if defined(__HIP_DEVICE_COMPILE__)
+    static __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer(const void* p, int bytes) {
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, bytes, 0x00020000);
+    }
+#endif
 };
 
 // One head group's state in a wave: output tiles (lane: head l & 15, dim (4 (l >> 4) + i) DL + t),
@@ -323,7 +333,7 @@ struct State {
     static constexpr int DL = 4 * NC;
     f4_t o[DL] = {};
     float m = kNone, l = 0.0f;
-    float vref = 0.0f, vinv = 0.0f;  // int8: o counts in units of vref / 2^15 / 512
+    float vref = 0.0f, vinv = 0.0f;  // int8: o counts in units of vref / 2^15 * 512; vinv = 2^15 / vref
 
     template <class Q>
     __device__ __forceinline__ void add(const Q& q, float qf, Tile<PT, NC>& t) {
@@ -338,20 +348,13 @@ struct State {
                 if constexpr (PT == JYHIP_T_I8) s[g][i] *= t.ks[g][i];
             }
         }
-        if (t.live[0] + t.live[1] < 32) {  // what does not exist: weight 0, whatever its slot holds
+        if (t.live[0] + t.live[1] < 32) {  // no weight for what does not exist (its value and scale are 0)
+            asm volatile("");              // (a branch: as selects this would cost every tile)
 #pragma unroll
             for (int g = 0; g < 2; g++)
 #pragma unroll
                 for (int i = 0; i < 4; i++)
-                    if (kg + i >= t.live[g]) {
-                        s[g][i] = -__builtin_inff();
-                        if constexpr (PT == JYHIP_T_I8) {
-                            t.vs[g][i] = 0.0f;
-                        } else {
-#pragma unroll
-                            for (int w = 0; w < Tile<PT, NC>::VW; w++) t.v[g * 4 + i][w] = 0;
-                        }
-                    }
+                    if (kg + i >= t.live[g]) s[g][i] = -__builtin_inff();
         }
         float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
                           fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
@@ -375,8 +378,8 @@ struct State {
                     // the power of two over vtop, within [2^-120, 2^126]
                     const int e = min(max((int)(__builtin_bit_cast(uint32_t, vtop) >> 23) - 126, -120), 126);
                     const float next = __builtin_ldexpf(1.0f, e);
-                    vinv = __builtin_ldexpf(1.0f, -e);
-                    a *= vref * vinv;
+                    vinv = __builtin_ldexpf(1.0f, 15 - e);
+                    a *= vref * __builtin_ldexpf(1.0f, -e);
                     vref = next;
                 }
             }
@@ -394,7 +397,7 @@ struct State {
                 const float w = exp2_hw(s[g][i] - m);
                 sum += w;
                 if constexpr (PT == JYHIP_T_I8)
-                    p[g * 4 + i] = w * (t.vs[g][i] * vinv) * 32768.0f;
+                    p[g * 4 + i] = w * (t.vs[g][i] * vinv);
                 else if constexpr (PT == JYHIP_T_F16)
                     p[g * 4 + i] = w * 32768.0f;
                 else
@@ -425,7 +428,8 @@ struct State {
 #pragma unroll
             for (int j = 0; j < 8; j += 2) {
                 const auto a = __builtin_amdgcn_cvt_pkrtz(p[j], p[j + 1]);
-                const auto b = __builtin_amdgcn_cvt_pkrtz(p[j] - (float)a[0], p[j + 1] - (float)a[1]);
+                const auto b = __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)a[0], -1.0f, p[j]),
+                                                          __builtin_fmaf((float)a[1], -1.0f, p[j + 1]));
                 hi[j] = (_Float16)a[0];
                 hi[j + 1] = (_Float16)a[1];
                 lo[j] = (_Float16)b[0];
@@ -507,7 +511,7 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void paged_attend_kernel(Attn
         const int at = (c0 + (wave + 4 * (lane >> 1)) * 32 + 16 * (lane & 1)) >> K.ps_log2;
         if (at < A.M.stride) ids = A.M.tables[(int64_t)b * A.M.stride + at];
     }
-    const int n = min(A.lens[b], A.cap);
+    const int n = __builtin_amdgcn_readfirstlane(min(A.lens[b], A.cap));
     const bool on = (lane & 15) < heads;
     const int64_t qbase = b * A.q.row_stride + (h0 + (on ? lane & 15 : 0)) * A.q.head_stride;
     float x[T::KC * STEP];
@@ -525,10 +529,10 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void paged_attend_kernel(Attn
     ld.v = static_cast<const char*>(P.v) + first * (hd * ES);
     ld.ks = PT == JYHIP_T_I8 ? P.k_scale + first : nullptr;
     ld.vs = PT == JYHIP_T_I8 ? P.v_scale + first : nullptr;
-    ld.head_stride = (int64_t)nkv * P.page_size;
+    ld.page_rows = (int64_t)nkv * P.page_size;
     ld.num_pages = P.num_pages;
     ld.ps = P.page_size;
-    ld.hd = hd;
+    ld.row_bytes = hd * ES;
 #pragma unroll
     for (int c = 0; c < T::KC; c++) {
         int d = c * 4 * STEP + (lane >> 4) * STEP;
@@ -538,7 +542,8 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void paged_attend_kernel(Attn
     {
         int d = (lane & 15) * DL;
         if (d >= hd) d = 0;  // (outputs past the head's end are not stored)
-        ld.voff = (unsigned)(((lane >> 4) * 4 * hd + d) * ES);
+#pragma unroll
+        for (int j = 0; j < 4; j++) ld.voff[j] = (unsigned)((((lane >> 4) * 4 + j) * hd + d) * ES);
     }
     const int end = min(n, c0 + K.plan.chunk);
     const int ntiles = end > c0 ? (end - c0 + 31) / 32 : 0;
