@@ -40,8 +40,9 @@ constexpr int LIST = 8192;          // tokens of a row's list
 constexpr int BLOCK = 2048;         // tokens per partial mass
 constexpr int STRIPES = 1024;       // parts whose maxima bound the k-th largest logit
 constexpr int MAX_SEGS = 64;
-constexpr int STEPS = 512;          // table entries per factor of two of mass
-constexpr int PER_BIN = 16;         // of them in a histogram bin: masses under 2^-52 are none, 53 * 512 / 16 < BINS
+constexpr int SEG_BLOCKS = 512;     // blocks of a segment at most
+constexpr int STEPS = 32;           // table entries, and histogram bins, per factor of two of mass: masses
+                                    // under 2^-52 are none, and 53 * 32 < BINS
 constexpr int STAGE = 1024;         // list entries a workgroup collects before it takes places for them
 
 enum { ROW_GREEDY, ROW_TOPK, ROW_MASS, ROW_NUCLEUS, ROW_ALONE };
@@ -58,7 +59,9 @@ SamplePlan plan_of(int rows, int vocab) {
     p.blocks = (vocab + BLOCK - 1) / BLOCK;
     // about 1024 workgroups, none of less than a block
     p.segs = 1;
-    while (p.segs < MAX_SEGS && (int64_t)rows * p.segs * 2 <= 1024 && p.segs * 2 <= p.blocks) p.segs *= 2;
+    while (p.segs < MAX_SEGS && (((int64_t)rows * p.segs * 2 <= 1024 && p.segs * 2 <= p.blocks) ||
+                                 (p.blocks + p.segs - 1) / p.segs > SEG_BLOCKS))
+        p.segs *= 2;
     p.seg_len = (p.blocks + p.segs - 1) / p.segs * BLOCK;
     const size_t n = (size_t)BINS * 8 + (size_t)LIST * 8 + (size_t)p.blocks * 8 + MAX_SEGS * 8 + STRIPES * 4 + 16;
     p.row_bytes = (n + 255) / 256 * 256;
@@ -117,49 +120,46 @@ __device__ __forceinline__ Set set_of(const SampleArgs& A, int row) {
 
 __device__ constexpr u64 kExp2[32] = JY_EXP2_TABLE;
 
-// Masses of a row's logits, e 2^s.  With y = 512 (x - M) log2 e / T = k + r, k whole and |r| <= 1/2:
-// 2^(k/512) from a table of 512 (2^s in it) and the exponent, times the Taylor terms of 2^(r/512) up
-// to r^3 (the rest is under 9e-15).
+// Masses of a row's logits, e 2^s.  With y = 32 (x - M) log2 e / T = k + r, k whole and |r| <= 1/2:
+// 2^(k/32) from a table of 32 (2^s in it) and the exponent, times the Taylor terms of 2^(r/32) up to r^5
+// (the rest is under 2.3e-15).  32 entries are one for each pair of LDS banks: lanes that want
+// different ones do not wait for each other (512 and a cubic measured 9 % slower).
 struct Masses {
     float M, low;    // low: the logit whose mass is far under 2^-52, standing for all below it and NaN
-    double c;        // 512 log2 e / T
+    double c;        // 32 log2 e / T
     double unit;     // 2^s
     const u64* tab;  // [STEPS]
     // false: the largest logit is infinite or T so large that no such logit is finite (then c is 0
     // or M infinite, and only pick_alone() takes the row)
     __device__ __forceinline__ bool set(float top, float T, int vocab, const u64* table) {
         M = top;
-        c = 512.0 * 1.4426950408889634074 / (double)T;
-        low = (float)((double)M - 64.0 * 512.0 / c);
+        c = STEPS * 1.4426950408889634074 / (double)T;
+        low = (float)((double)M - 64.0 * STEPS / c);
         int s = 51;
         while (s > 40 && (1ll << (62 - s)) < vocab) s--;
         unit = (double)(1ull << s);
         tab = table;
         return M < __builtin_inff() && low > -3.4e38f;
     }
-    // entry i of the table: 2^(i/512) 2^s, from 2^(j/32) (its bits less j << 47, so adding any
-    // j << 47 gives 2^(j/32)) and the Taylor terms of 2^r, |r| <= 1/64, up to r^5 (the rest is
-    // under 2.3e-15)
+    // (kExp2's entry j is 2^(j/32) less j << 47 in its bits)
     __device__ __forceinline__ void fill(u64* table) const {
-        for (int i = threadIdx.x; i < STEPS; i += blockDim.x) table[i] = __builtin_bit_cast(u64, unit * exp2_slow(i / 512.0));
+        if (threadIdx.x < STEPS)
+            table[threadIdx.x] = __builtin_bit_cast(
+                u64, unit * __builtin_bit_cast(double, kExp2[threadIdx.x] + ((u64)threadIdx.x << 47)));
     }
-    static __device__ __forceinline__ double exp2_slow(double y) {
-        const double shift = 0x1.8p+52;
-        double kd = __builtin_fma(y, 32.0, shift);
-        const u64 ki = __builtin_bit_cast(u64, kd);
-        kd -= shift;
-        const double r = __builtin_fma(kd, -0.03125, y);
-        double q = __builtin_fma(r, 0.0013333558146428443, 0.0096181291076284772);
-        q = __builtin_fma(q, r, 0.055504108664821580);
-        q = __builtin_fma(q, r, 0.24022650695910071);
-        q = __builtin_fma(q, r, 0.69314718055994531);
-        q = __builtin_fma(q, r, 1.0);
-        return q * __builtin_bit_cast(double, kExp2[ki & 31u] + (ki << 47));
+    // 2^(r/32)
+    static __device__ __forceinline__ double near(double r) {
+        constexpr double L = 0.69314718055994531 / STEPS;
+        double q = __builtin_fma(r, L * L * L * L * L / 120.0, L * L * L * L / 24.0);
+        q = __builtin_fma(q, r, L * L * L / 6.0);
+        q = __builtin_fma(q, r, L * L / 2.0);
+        q = __builtin_fma(q, r, L);
+        return __builtin_fma(q, r, 1.0);
     }
     struct At {
         double r;
         int k;  // <= 0
-        __device__ __forceinline__ int bin() const { return (unsigned)-k / PER_BIN; }
+        __device__ __forceinline__ int bin() const { return -k; }
     };
     // l within [low, M], NaN as low
     __device__ __forceinline__ float clamp(float l) const {
@@ -177,22 +177,25 @@ struct Masses {
     }
     // the mass, rounded to a whole number by adding it to 2^52 (it is under that)
     __device__ __forceinline__ u64 mass(const At& a) const {
-        constexpr double L = 0.69314718055994531 / 512.0;
-        double q = __builtin_fma(a.r, L * L * L / 6.0, L * L / 2.0);
-        q = __builtin_fma(q, a.r, L);
-        q = __builtin_fma(q, a.r, 1.0);
-        const u64 t = tab[a.k & (STEPS - 1)] + ((u64)(uint32_t)((a.k >> 9) << 20) << 32);
-        return __builtin_bit_cast(u64, __builtin_fma(q, __builtin_bit_cast(double, t), 0x1p+52)) & 0xfffffffffffffull;
+        const u64 t = tab[a.k & (STEPS - 1)] + ((u64)(uint32_t)((a.k >> 5) << 20) << 32);
+        return __builtin_bit_cast(u64, __builtin_fma(near(a.r), __builtin_bit_cast(double, t), 0x1p+52)) & 0xfffffffffffffull;
     }
     __device__ __forceinline__ u64 mass(float l) const { return mass(at(l)); }
     // min-p's least mass
     __device__ __forceinline__ u64 least(const Set& s) const { return (u64)__builtin_rint(s.min_e * unit); }
+    // a logit at or under the least one of a bin
+    __device__ __forceinline__ float under(int bin) const {
+        const double l = (double)M - (bin + 1.0) / c;
+        return (float)(l - fabs(l) * 0x1p-20 - 0x1p-120);
+    }
     // the same for any M and T
     __device__ __forceinline__ u64 mass_any(float l) const {
         if (l == M) return (u64)unit;
         if (!(l > -__builtin_inff()) || M == __builtin_inff()) return 0;
-        const double y = ((double)l - (double)M) * (c / 512.0);
-        return y > -64.0 ? (u64)__builtin_rint(unit * exp2_slow(y)) : 0;
+        const double y = ((double)l - (double)M) * c, k = __builtin_rint(y);
+        if (!(y > -64.0 * STEPS)) return 0;
+        const u64 t = tab[(int)k & (STEPS - 1)] + ((u64)(uint32_t)(((int)k >> 5) << 20) << 32);
+        return (u64)__builtin_rint(near(y - k) * __builtin_bit_cast(double, t));
     }
 };
 
@@ -349,7 +352,6 @@ struct Stage {
 template <class E>
 __global__ __launch_bounds__(NP) void sample_top_kernel(SampleArgs A, SamplePlan P) {
     constexpr int VL = Logits<E>::VL;
-    __shared__ float part[2 * NP];
     __shared__ u64 first[NP / 64];
     const int row = blockIdx.x / P.segs, seg = blockIdx.x % P.segs;
     const RowWs w = row_ws(A, P, row);
@@ -367,19 +369,27 @@ __global__ __launch_bounds__(NP) void sample_top_kernel(SampleArgs A, SamplePlan
     });
     const u64 mine = wave_max(at < 0 ? 0 : entry_of(key_of(fmaxf(top[0], top[1])), at));
     if ((threadIdx.x & 63) == 0) first[threadIdx.x >> 6] = mine;
-    part[threadIdx.x] = top[0];
-    part[NP + threadIdx.x] = top[1];
+    if (s.mode == ROW_TOPK) {
+        // the segment's share of the row's 1024 maxima, each over 1024 / n of these
+        const int n = STRIPES / P.segs;
+        if (n == 2 * NP) {
+            w.stripe[seg * n + threadIdx.x] = top[0];
+            w.stripe[seg * n + NP + threadIdx.x] = top[1];
+        } else {
+            float m = fmaxf(top[0], top[1]);
+            if (n < NP) m = fmaxf(m, dpp_f<0xB1>(m));       // 2 lanes
+            if (n < NP / 2) m = fmaxf(m, dpp_f<0x4E>(m));   // 4
+            if (n < NP / 4) m = fmaxf(m, dpp_f<0x141>(m));  // 8: the half row mirrored
+            if (n < NP / 8) m = fmaxf(m, dpp_f<0x140>(m));  // 16: the row mirrored
+            if (n < NP / 16) m = fmaxf(m, __shfl_xor(m, 16));
+            const int lanes = NP / n;
+            if (threadIdx.x % lanes == 0) w.stripe[seg * n + threadIdx.x / lanes] = m;
+        }
+        static_assert(STRIPES == 2 * NP && STRIPES / MAX_SEGS >= NP / 32, "groups of up to 32 lanes");
+    }
     __syncthreads();
     if (s.mode == ROW_NUCLEUS)
         for (int i = seg * NP + threadIdx.x; i < BINS; i += P.segs * NP) w.hist[i] = 0;
-    if (s.mode == ROW_TOPK) {
-        const int n = STRIPES / P.segs;
-        for (int r = threadIdx.x; r < n; r += NP) {
-            float m = part[r];
-            for (int j = r + n; j < 2 * NP; j += n) m = fmaxf(m, part[j]);
-            w.stripe[seg * n + r] = m;
-        }
-    }
     if (threadIdx.x == 0) {
         u64 t = first[0];
 #pragma unroll
@@ -420,7 +430,7 @@ static_assert(NP / 64 == 8, "a wave for each value of three bits");
 
 // ---- 2: top-k candidates, masses or the histogram
 template <class E>
-__global__ __launch_bounds__(NP) void sample_mass_kernel(SampleArgs A, SamplePlan P) {
+__global__ __launch_bounds__(NP, 8) void sample_mass_kernel(SampleArgs A, SamplePlan P) {
     constexpr int VL = Logits<E>::VL;
     __shared__ union {
         u64 hist[BINS];
@@ -557,11 +567,12 @@ __device__ BorderBin border_bin(const u64 (&h)[BINS / N], float p, Scan<N>& scan
 
 // ---- 3: top-p: the masses above the border's bin, its tokens into the list
 template <class E>
-__global__ __launch_bounds__(NP) void sample_border_kernel(SampleArgs A, SamplePlan P) {
-    constexpr int VL = Logits<E>::VL;
-    __shared__ u64 block[SAMPLE_MAX_VOCAB / BLOCK];
+__global__ __launch_bounds__(NP, 8) void sample_border_kernel(SampleArgs A, SamplePlan P) {
+    constexpr int VL = Logits<E>::VL, HALF = 4;  // elements packed at a time
+    __shared__ u64 block[SEG_BLOCKS];
     __shared__ u64 tab[STEPS];
     __shared__ Stage stage;
+    __shared__ uint2 mine[NP / 64][64 * (HALF + 1)];
     __shared__ Scan<NP> scan;
     __shared__ BorderFound found;
     const int row = blockIdx.x / P.segs, seg = blockIdx.x % P.segs;
@@ -584,24 +595,41 @@ __global__ __launch_bounds__(NP) void sample_border_kernel(SampleArgs A, SampleP
     int turn = 0;
     const BorderBin b = border_bin<NP>(h, s.p, scan, turn, found);  // (with barriers)
     const u64 least = m.least(s);
+    // Most tokens lie below the border.  Each wave packs those that may not, then takes them 64 at a
+    // time: with a nucleus of 9 % of the tokens the masses of all lanes' every token cost 1.7 times as much.
+    const float floor = m.under(b.bin);
+    const int lane = threadIdx.x & 63;
+    uint2* const pack = mine[threadIdx.x >> 6];
     each(x, f, i0, i1, [&](const float (&l)[VL], int i) {
+        int n = 0;
         u64 q = 0;
-        bool mine[VL];
+        auto take = [&](bool have, int j) {
+            const uint2 t = pack[have ? j : 0];
+            const float tl = __builtin_bit_cast(float, t.x);
+            const Masses::At y = m.at(tl);
+            const u64 v = m.mass(y);
+            q += have && y.bin() < b.bin && v >= least ? v : 0;
+            const bool edge[1] = {have && y.bin() == b.bin};
+            stage.add(w, edge, [&](int) { return entry_of(key_of(tl), (int)t.y); });
+        };
 #pragma unroll
-        for (int e = 0; e < VL; e++) {
-            const Masses::At y = m.at(l[e]);
-            const int bin = y.bin();
-            if (bin < b.bin) {
-                const u64 v = m.mass(y);
-                q += v >= least ? v : 0;
+        for (int h = 0; h < VL; h += HALF) {
+#pragma unroll
+            for (int e = h; e < h + HALF; e++) {
+                const bool in = l[e] >= floor;
+                const u64 who = __ballot(in);
+                if (in) pack[n + __popcll(who & ((1ull << lane) - 1))] = uint2{__builtin_bit_cast(uint32_t, l[e]), (uint32_t)(i + e)};
+                n += __popcll(who);
             }
-            mine[e] = bin == b.bin;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            for (; n >= 64; n -= 64) take(true, n - 64 + lane);
         }
+        if (n) take(lane < n, lane);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         if (__any(q != 0)) {
             q = wave_sum(q);
-            if ((threadIdx.x & 63) == 0) atomicAdd(&block[(i - i0) / BLOCK], q);
+            if (lane == 0) atomicAdd(&block[(i - i0) / BLOCK], q);
         }
-        stage.add(w, mine, [&](int e) { return entry_of(key_of(l[e]), i + e); });
     });
     stage.flush(w);  // (with barriers)
     for (int i = threadIdx.x; i < nb; i += NP) w.block[i0 / BLOCK + i] = block[i];
@@ -617,7 +645,8 @@ struct Border {
     uint32_t ties = ALL;
 };
 
-constexpr int WAYS = NT;            // bins of one step of a descent in kernel 4, one a thread
+constexpr int WAY_BITS = 12;         // bits of key or index that one step of a descent in kernel 4 settles
+constexpr int WAYS = 1 << WAY_BITS;
 struct RowShared {
     uint32_t count[WAYS];           // zero between steps
     u64 sum[WAYS];                  // zero between steps
@@ -658,17 +687,27 @@ __device__ __forceinline__ u64 block_sum(RowShared& S, u64 v) {
 // and less than `want` above it, `above` lying above the first; it is the one that reaches `want`.
 // Leaves the bin, what lies above it and its count; the bins are zero again.
 __device__ __forceinline__ void choose(RowShared& S, int& turn, bool by_mass, u64 above, u64 want) {
+    constexpr int PER = WAYS / NT;
     __syncthreads();
-    const uint32_t n = S.count[threadIdx.x];
-    const u64 v = by_mass ? S.sum[threadIdx.x] : n;
-    S.count[threadIdx.x] = 0;
-    S.sum[threadIdx.x] = 0;
-    u64 total;
-    const u64 run = above + S.scan.before(turn, v, total);
-    if (n && (run < want || run == 0) && run + v >= want) {
-        S.bin = threadIdx.x;
-        S.above = run;
-        S.left = n;
+    uint32_t n[PER];
+    u64 v[PER], sum = 0, total;
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+        n[j] = S.count[threadIdx.x * PER + j];
+        v[j] = by_mass ? S.sum[threadIdx.x * PER + j] : n[j];
+        sum += v[j];
+        S.count[threadIdx.x * PER + j] = 0;
+        S.sum[threadIdx.x * PER + j] = 0;
+    }
+    u64 run = above + S.scan.before(turn, sum, total);
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+        if (n[j] && (run < want || run == 0) && run + v[j] >= want) {
+            S.bin = threadIdx.x * PER + j;
+            S.above = run;
+            S.left = n[j];
+        }
+        run += v[j];
     }
     __syncthreads();
 }
@@ -691,13 +730,13 @@ __device__ Border border_at(RowShared& S, u64 one, uint32_t key, bool by_mass, u
 
 // The border of the `want` first tokens in the order (by_mass: of the tokens before which less
 // than `want` of mass lies; ties share what is left), by a radix descent over the whole row's keys,
-// 10 bits at a time
+// 12 bits at a time
 __device__ Border descend(RowShared& S, int& turn, const Row& R, const Masses& m, bool by_mass, u64 want) {
     uint32_t prefix = 0;
     u64 above = 0;
-    for (int shift = 22, step = 0; step < 4; step++) {
-        const int nb = step < 3 ? 10 : 2;
+    for (int shift = 32 - WAY_BITS, nb = WAY_BITS; nb; shift -= nb) {
         const uint32_t mask = (1u << nb) - 1;
+        const bool step = shift + nb < 32;
         for (int i = threadIdx.x; i < R.V; i += NT) {
             const float l = R.at(i);
             const uint32_t k = key_of(l);
@@ -712,13 +751,13 @@ __device__ Border descend(RowShared& S, int& turn, const Row& R, const Masses& m
         choose(S, turn, by_mass, above, want);
         prefix = (step ? prefix << nb : 0) | (mask - S.bin);
         above = S.above;
-        shift -= step < 2 ? 10 : 2;
+        nb = min(nb, shift);
     }
     return border_at(S, prefix ? m.mass_any(logit_of(prefix)) : 0, prefix, by_mass, want);
 }
 
 // The same border among the n tokens of the list, with `above` before them: the keys' range divided by
-// up to 1024 until one key is left.  A thread has at most PER of them.
+// up to 4096 until one key is left.  A thread has at most PER of them.
 template <int PER>
 __device__ Border descend_list(RowShared& S, int& turn, const Masses& m, int n, bool by_mass, u64 above, u64 want) {
     uint32_t key[PER], lo = 0xffffffffu, hi = 0;
@@ -764,29 +803,29 @@ __device__ Border descend_list(RowShared& S, int& turn, const Masses& m, int n, 
     }
 }
 
-// the index of the last tie that B keeps among the list's n tokens (those at B's key): 10 bits of
-// it at a time
+// the index of the last tie that B keeps among the list's n tokens (those at B's key)
+constexpr int INDEX_BITS = 22;
+static_assert(SAMPLE_MAX_VOCAB == 1 << INDEX_BITS && INDEX_BITS <= 2 * WAY_BITS, "two steps over an index");
+constexpr int LOW_BITS = INDEX_BITS - WAY_BITS;
 template <int PER>
 __device__ uint32_t last_tie(RowShared& S, int& turn, const Border& B, int n) {
     if (B.ties == ALL) return ALL;
-    uint32_t prefix = 0;
+    uint32_t high = 0;
     u64 above = 0;
-    static_assert(SAMPLE_MAX_VOCAB == 1 << 22, "22 bits of index");
-    for (int shift = 12, step = 0; step < 3; step++) {
-        const int nb = step < 2 ? 10 : 2;
+    for (int step = 0; step < 2; step++) {
 #pragma unroll
         for (int j = 0; j < PER; j++) {
             const int i = j * NT + threadIdx.x;
             if (i >= n || (uint32_t)(S.list[i] >> 32) != B.key) continue;
             const uint32_t at = ~(uint32_t)S.list[i];
-            if (step == 0 || at >> (shift + nb) == prefix) atomicAdd(&S.count[(at >> shift) & ((1u << nb) - 1)], 1u);
+            if (step == 0 || at >> LOW_BITS == high) atomicAdd(&S.count[step ? at & ((1u << LOW_BITS) - 1) : at >> LOW_BITS], 1u);
         }
         choose(S, turn, false, above, B.ties);
-        prefix = prefix << nb | S.bin;
+        if (step) break;
+        high = S.bin;
         above = S.above;
-        shift -= step == 0 ? 10 : 2;
     }
-    return prefix;
+    return high << LOW_BITS | S.bin;
 }
 
 // the kept mass of tokens with indices in [i0, i1), per wave in steps of 64, `ties` the ties before
@@ -930,7 +969,7 @@ __device__ int pick_few(RowShared& S, int& turn, const Masses& m, const Set& s, 
 static_assert(FEW <= WAYS && FEW <= LIST && FEW <= SAMPLE_MAX_VOCAB / BLOCK, "one place for each");
 
 // top-k, many candidates: the k first of the n in S.list, the border of top-p among them, then the token
-// by its index, 10 bits at a time
+// by its index, in two steps
 __device__ int pick_list(RowShared& S, int& turn, const Masses& m, const Set& s, int n, float u) {
     constexpr int PER = LIST / NT;
     if (n > s.k) {
@@ -969,20 +1008,19 @@ __device__ int pick_list(RowShared& S, int& turn, const Masses& m, const Set& s,
     S.scan.before(turn, kept ? q : 0, z);
     const u64 target = target_of(u, z);
     u64 above = 0;
-    uint32_t prefix = 0;
-    for (int shift = 12, step = 0; step < 3; step++) {
-        const int nb = step < 2 ? 10 : 2;
-        if (kept && (step == 0 || at >> (shift + nb) == prefix)) {
-            const uint32_t b = (at >> shift) & ((1u << nb) - 1);
+    uint32_t high = 0;
+    for (int step = 0; step < 2; step++) {
+        if (kept && (step == 0 || at >> LOW_BITS == high)) {
+            const uint32_t b = step ? at & ((1u << LOW_BITS) - 1) : at >> LOW_BITS;
             atomicAdd(&S.count[b], 1u);
             atomicAdd(&S.sum[b], q);
         }
         choose(S, turn, true, above, target + 1);  // (the first bin whose running sum exceeds the target)
-        prefix = prefix << nb | S.bin;
+        if (step) break;
+        high = S.bin;
         above = S.above;
-        shift -= step == 0 ? 10 : 2;
     }
-    return (int)prefix;
+    return (int)(high << LOW_BITS | S.bin);
 }
 
 // no top-k: the blocks' masses are in the workspace (with top-p those above the border's bin, whose
@@ -1065,8 +1103,10 @@ __global__ __launch_bounds__(NT) void sample_pick_kernel(SampleArgs A, SamplePla
     Masses m;
     const bool plain = m.set(top_logit(top), s.T, A.vocab, S.tab);
     m.fill(S.tab);
-    S.count[threadIdx.x] = 0;
-    S.sum[threadIdx.x] = 0;
+    for (int i = threadIdx.x; i < WAYS; i += NT) {
+        S.count[i] = 0;
+        S.sum[i] = 0;
+    }
     int turn = 0;
     const int n = s.mode == ROW_TOPK || s.mode == ROW_NUCLEUS ? (int)min(count, (uint32_t)LIST + 1) : 0;
     if (n <= LIST) {
