@@ -41,8 +41,9 @@ constexpr int BLOCK = 2048;         // tokens per partial mass
 constexpr int STRIPES = 1024;       // parts whose maxima bound the k-th largest logit
 constexpr int MAX_SEGS = 64;
 constexpr int SEG_BLOCKS = 512;     // blocks of a segment at most
-constexpr int STEPS = 32;           // table entries, and histogram bins, per factor of two of mass: masses
-                                    // under 2^-52 are none, and 53 * 32 < BINS
+constexpr int STEP_BITS = 9;
+constexpr int STEPS = 1 << STEP_BITS;  // table entries per factor of two of mass
+constexpr int PER_BIN = 16;         // of them in a histogram bin: masses under 2^-52 are none, 53 * 512 / 16 < BINS
 constexpr int STAGE = 1024;         // list entries a workgroup collects before it takes places for them
 
 enum { ROW_GREEDY, ROW_TOPK, ROW_MASS, ROW_NUCLEUS, ROW_ALONE };
@@ -120,13 +121,13 @@ __device__ __forceinline__ Set set_of(const SampleArgs& A, int row) {
 
 __device__ constexpr u64 kExp2[32] = JY_EXP2_TABLE;
 
-// Masses of a row's logits, e 2^s.  With y = 32 (x - M) log2 e / T = k + r, k whole and |r| <= 1/2:
-// 2^(k/32) from a table of 32 (2^s in it) and the exponent, times the Taylor terms of 2^(r/32) up to r^5
-// (the rest is under 2.3e-15).  32 entries are one for each pair of LDS banks: lanes that want
-// different ones do not wait for each other (512 and a cubic measured 9 % slower).
+// Masses of a row's logits, e 2^s.  With y = 512 (x - M) log2 e / T = k + r, k whole and |r| <= 1/2:
+// 2^(k/512) from a table of 512 (2^s in it) and the exponent, times the Taylor terms of 2^(r/512) up to
+// r^3 (the rest is under 9e-15).  The fp64 operations bound the passes that weigh every token, so
+// few of them: a table of 32 and two more terms measured 41 us against 38 over 256 x 152064.
 struct Masses {
     float M, low;    // low: the logit whose mass is far under 2^-52, standing for all below it and NaN
-    double c;        // 32 log2 e / T
+    double c;        // 512 log2 e / T
     double unit;     // 2^s
     const u64* tab;  // [STEPS]
     // false: the largest logit is infinite or T so large that no such logit is finite (then c is 0
@@ -141,25 +142,33 @@ struct Masses {
         tab = table;
         return M < __builtin_inff() && low > -3.4e38f;
     }
-    // (kExp2's entry j is 2^(j/32) less j << 47 in its bits)
+    // entry i: 2^(i/512) 2^s, from 2^(j/32) (kExp2's entry is that less j << 47 in its bits) and the
+    // Taylor terms of 2^(f/32), 0 <= f < 1, up to f^6 (the rest is under 5e-16)
     __device__ __forceinline__ void fill(u64* table) const {
-        if (threadIdx.x < STEPS)
-            table[threadIdx.x] = __builtin_bit_cast(
-                u64, unit * __builtin_bit_cast(double, kExp2[threadIdx.x] + ((u64)threadIdx.x << 47)));
+        constexpr double L = 0.69314718055994531 / 32;
+        for (int i = threadIdx.x; i < STEPS; i += blockDim.x) {
+            const int j = i * 32 / STEPS;
+            const double f = (i * 32 % STEPS) * (1.0 / STEPS);
+            double q = __builtin_fma(f, L * L * L * L * L * L / 720.0, L * L * L * L * L / 120.0);
+            q = __builtin_fma(q, f, L * L * L * L / 24.0);
+            q = __builtin_fma(q, f, L * L * L / 6.0);
+            q = __builtin_fma(q, f, L * L / 2.0);
+            q = __builtin_fma(q, f, L);
+            q = __builtin_fma(q, f, 1.0);
+            table[i] = __builtin_bit_cast(u64, unit * (q * __builtin_bit_cast(double, kExp2[j] + ((u64)j << 47))));
+        }
     }
-    // 2^(r/32)
+    // 2^(r/512)
     static __device__ __forceinline__ double near(double r) {
         constexpr double L = 0.69314718055994531 / STEPS;
-        double q = __builtin_fma(r, L * L * L * L * L / 120.0, L * L * L * L / 24.0);
-        q = __builtin_fma(q, r, L * L * L / 6.0);
-        q = __builtin_fma(q, r, L * L / 2.0);
+        double q = __builtin_fma(r, L * L * L / 6.0, L * L / 2.0);
         q = __builtin_fma(q, r, L);
         return __builtin_fma(q, r, 1.0);
     }
     struct At {
         double r;
         int k;  // <= 0
-        __device__ __forceinline__ int bin() const { return -k; }
+        __device__ __forceinline__ int bin() const { return (unsigned)-k / PER_BIN; }
     };
     // l within [low, M], NaN as low
     __device__ __forceinline__ float clamp(float l) const {
@@ -177,7 +186,7 @@ struct Masses {
     }
     // the mass, rounded to a whole number by adding it to 2^52 (it is under that)
     __device__ __forceinline__ u64 mass(const At& a) const {
-        const u64 t = tab[a.k & (STEPS - 1)] + ((u64)(uint32_t)((a.k >> 5) << 20) << 32);
+        const u64 t = tab[a.k & (STEPS - 1)] + ((u64)(uint32_t)((a.k >> STEP_BITS) << 20) << 32);
         return __builtin_bit_cast(u64, __builtin_fma(near(a.r), __builtin_bit_cast(double, t), 0x1p+52)) & 0xfffffffffffffull;
     }
     __device__ __forceinline__ u64 mass(float l) const { return mass(at(l)); }
@@ -185,7 +194,7 @@ struct Masses {
     __device__ __forceinline__ u64 least(const Set& s) const { return (u64)__builtin_rint(s.min_e * unit); }
     // a logit at or under the least one of a bin
     __device__ __forceinline__ float under(int bin) const {
-        const double l = (double)M - (bin + 1.0) / c;
+        const double l = (double)M - (bin + 1.0) * PER_BIN / c;
         return (float)(l - fabs(l) * 0x1p-20 - 0x1p-120);
     }
     // the same for any M and T
@@ -194,7 +203,7 @@ struct Masses {
         if (!(l > -__builtin_inff()) || M == __builtin_inff()) return 0;
         const double y = ((double)l - (double)M) * c, k = __builtin_rint(y);
         if (!(y > -64.0 * STEPS)) return 0;
-        const u64 t = tab[(int)k & (STEPS - 1)] + ((u64)(uint32_t)(((int)k >> 5) << 20) << 32);
+        const u64 t = tab[(int)k & (STEPS - 1)] + ((u64)(uint32_t)(((int)k >> STEP_BITS) << 20) << 32);
         return (u64)__builtin_rint(near(y - k) * __builtin_bit_cast(double, t));
     }
 };
@@ -645,7 +654,7 @@ struct Border {
     uint32_t ties = ALL;
 };
 
-constexpr int WAY_BITS = 12;         // bits of key or index that one step of a descent in kernel 4 settles
+constexpr int WAY_BITS = 11;         // bits of key or index that one step of a descent in kernel 4 settles
 constexpr int WAYS = 1 << WAY_BITS;
 struct RowShared {
     uint32_t count[WAYS];           // zero between steps
