@@ -414,7 +414,7 @@ __global__ __launch_bounds__(NP) void sample_top_kernel(SampleArgs A, SamplePlan
 struct Bound {
     int n[2][8];
 };
-__device__ uint32_t stripe_bound(Bound& S, const RowWs& w, int k) {
+__device__ __forceinline__ uint32_t stripe_bound(Bound& S, const RowWs& w, int k) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     uint32_t key[STRIPES / 64];
 #pragma unroll
@@ -520,28 +520,38 @@ __device__ __forceinline__ u64 wave_scan(u64 v) {
     return v + (lane < 16 ? 0 : lane < 32 ? r0 : lane < 48 ? r1 : r2);
 }
 
-// Running sums over a workgroup of N threads, one barrier each: the waves' sums go to the two halves of
-// `part` in turn, and a half is written again only after the barrier of the call between.
-template <int N>
+// Running sums over the first WT threads of a workgroup, one wave on each SIMD of the CU: the sums'
+// instructions are what a step costs, and sixteen waves would issue them four times over.  One barrier
+// (for all threads) each: the waves' sums go to the two halves of `part` in turn, and a half is
+// written again only after the barrier of the call between.
+constexpr int WT = 256;
 struct Scan {
-    u64 part[2][N / 64];
-    // (the sum before this thread, the total); `turn` is the caller's, 0 at first
+    u64 part[2][WT / 64];
+    // (the sum before this one of the WT threads; the total, in every thread); `turn` is the caller's, 0 at
+    // first
     __device__ __forceinline__ u64 before(int& turn, u64 v, u64& total) {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        const u64 run = wave_scan(v);
+        const int wave = threadIdx.x >> 6;
         u64* const p = part[turn];
         turn ^= 1;
-        if (lane == 63) p[wave] = run;
+        u64 run = 0;
+        if (threadIdx.x < WT) {
+            run = wave_scan(v);
+            if ((threadIdx.x & 63) == 63) p[wave] = run;
+        }
         __syncthreads();
-        const u64 w = wave_scan(lane < N / 64 ? p[lane] : 0);
-        total = lane_u64(w, N / 64 - 1);
-        const u64 mine = __shfl(w, wave) - lane_u64(run, 63);
-        return mine + run - v;
+        u64 a = 0;
+        total = 0;
+#pragma unroll
+        for (int w = 0; w < WT / 64; w++) {
+            if (w == wave) a = total;
+            total += p[w];
+        }
+        return a + run - v;
     }
 };
 
 // The bin that the last kept token lies in: the last one, from the top, with mass in it and less than
-// `want` = ceil(p total) above; `above` that mass.  All threads return the same.
+// `want` = ceil(p total) above; `above` that mass.  h: a worker's bins.  All threads return the same.
 struct BorderBin {
     int bin;
     u64 above, want;
@@ -550,24 +560,31 @@ struct BorderFound {
     int bin;
     u64 above;
 };
-template <int N>
-__device__ BorderBin border_bin(const u64 (&h)[BINS / N], float p, Scan<N>& scan, int& turn, BorderFound& found) {
-    constexpr int PER = BINS / N;
-    u64 sum = 0, total;
+constexpr int BINS_EACH = BINS / WT;
+__device__ __forceinline__ void load_bins(const u64* hist, u64 (&h)[BINS_EACH]) {
+    if (threadIdx.x < WT)
 #pragma unroll
-    for (int j = 0; j < PER; j++) sum += h[j];
+        for (int j = 0; j < BINS_EACH; j++) h[j] = hist[threadIdx.x * BINS_EACH + j];
+}
+__device__ __forceinline__ BorderBin border_bin(const u64 (&h)[BINS_EACH], float p, Scan& scan, int& turn, BorderFound& found) {
+    const bool worker = threadIdx.x < WT;
+    u64 sum = 0, total;
+    if (worker)
+#pragma unroll
+        for (int j = 0; j < BINS_EACH; j++) sum += h[j];
     u64 run = scan.before(turn, sum, total);
     BorderBin b;
     b.want = (u64)ceil((p > 0.0f ? (double)p : 0.0) * (double)total);
+    if (worker && (run < b.want || run == 0) && run + sum >= b.want && sum)
 #pragma unroll
-    for (int j = 0; j < PER; j++) {
-        // (run == 0: the first token is always kept)
-        if (h[j] && (run < b.want || run == 0) && run + h[j] >= b.want) {
-            found.bin = threadIdx.x * PER + j;
-            found.above = run;
+        for (int j = 0; j < BINS_EACH; j++) {
+            // (run == 0: the first token is always kept)
+            if (h[j] && (run < b.want || run == 0) && run + h[j] >= b.want) {
+                found.bin = threadIdx.x * BINS_EACH + j;
+                found.above = run;
+            }
+            run += h[j];
         }
-        run += h[j];
-    }
     __syncthreads();
     b.bin = found.bin;
     b.above = found.above;
@@ -582,7 +599,7 @@ __global__ __launch_bounds__(NP, 8) void sample_border_kernel(SampleArgs A, Samp
     __shared__ u64 tab[STEPS];
     __shared__ Stage stage;
     __shared__ uint2 mine[NP / 64][64 * (HALF + 1)];
-    __shared__ Scan<NP> scan;
+    __shared__ Scan scan;
     __shared__ BorderFound found;
     const int row = blockIdx.x / P.segs, seg = blockIdx.x % P.segs;
     const Set s = set_of(A, row);
@@ -598,11 +615,10 @@ __global__ __launch_bounds__(NP, 8) void sample_border_kernel(SampleArgs A, Samp
     const First<E> f = first(x, i0, i1);
     m.fill(tab);
     stage.clear();
-    u64 h[BINS / NP];
-#pragma unroll
-    for (int j = 0; j < BINS / NP; j++) h[j] = w.hist[threadIdx.x * (BINS / NP) + j];
+    u64 h[BINS_EACH];
+    load_bins(w.hist, h);
     int turn = 0;
-    const BorderBin b = border_bin<NP>(h, s.p, scan, turn, found);  // (with barriers)
+    const BorderBin b = border_bin(h, s.p, scan, turn, found);  // (with barriers)
     const u64 least = m.least(s);
     // Most tokens lie below the border.  Each wave packs those that may not, then takes them 64 at a
     // time: with a nucleus of 9 % of the tokens the masses of all lanes' every token cost 1.7 times as much.
@@ -656,15 +672,19 @@ struct Border {
 
 constexpr int WAY_BITS = 11;         // bits of key or index that one step of a descent in kernel 4 settles
 constexpr int WAYS = 1 << WAY_BITS;
+constexpr int WAYS_EACH = WAYS / WT;
+// where a bin lies: a worker takes consecutive ones, but the workers' first ones lie side by side, then
+// their second ones (consecutive ones side by side would put 64 lanes on four banks)
+__device__ __forceinline__ uint32_t place(uint32_t bin) { return (bin & (WAYS_EACH - 1)) * WT + bin / WAYS_EACH; }
 struct RowShared {
-    uint32_t count[WAYS];           // zero between steps
-    u64 sum[WAYS];                  // zero between steps
+    uint32_t count[WAYS];           // at place(bin); zero between steps
+    u64 sum[WAYS];                  // the same
     u64 list[LIST];
     u64 block[SAMPLE_MAX_VOCAB / BLOCK];
-    Scan<NT> scan;
+    Scan scan;
     u64 part[NT / 64];
     u64 tab[STEPS];
-    uint32_t tpart[NT / 64];
+    uint32_t tpart[NT / 64], lo_part[NT / 64], hi_part[NT / 64];
     u64 above;
     uint32_t bin, left;
     int found;
@@ -696,33 +716,37 @@ __device__ __forceinline__ u64 block_sum(RowShared& S, u64 v) {
 // and less than `want` above it, `above` lying above the first; it is the one that reaches `want`.
 // Leaves the bin, what lies above it and its count; the bins are zero again.
 __device__ __forceinline__ void choose(RowShared& S, int& turn, bool by_mass, u64 above, u64 want) {
-    constexpr int PER = WAYS / NT;
+    constexpr int PER = WAYS_EACH;
+    const bool worker = threadIdx.x < WT;
     __syncthreads();
     uint32_t n[PER];
     u64 v[PER], sum = 0, total;
+    if (worker)
 #pragma unroll
-    for (int j = 0; j < PER; j++) {
-        n[j] = S.count[threadIdx.x * PER + j];
-        v[j] = by_mass ? S.sum[threadIdx.x * PER + j] : n[j];
-        sum += v[j];
-        S.count[threadIdx.x * PER + j] = 0;
-        S.sum[threadIdx.x * PER + j] = 0;
-    }
-    u64 run = above + S.scan.before(turn, sum, total);
-#pragma unroll
-    for (int j = 0; j < PER; j++) {
-        if (n[j] && (run < want || run == 0) && run + v[j] >= want) {
-            S.bin = threadIdx.x * PER + j;
-            S.above = run;
-            S.left = n[j];
+        for (int j = 0; j < PER; j++) {
+            const int b = j * WT + threadIdx.x;
+            n[j] = S.count[b];
+            v[j] = by_mass ? S.sum[b] : n[j];
+            sum += v[j];
+            S.count[b] = 0;
+            if (by_mass) S.sum[b] = 0;
         }
-        run += v[j];
-    }
+    u64 run = above + S.scan.before(turn, sum, total);
+    if (worker && (run < want || run == 0) && run + sum >= want)
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+            if (n[j] && (run < want || run == 0) && run + v[j] >= want) {
+                S.bin = threadIdx.x * PER + j;
+                S.above = run;
+                S.left = n[j];
+            }
+            run += v[j];
+        }
     __syncthreads();
 }
 
 // the border at key `key`, whose tokens S.left are, each of mass `one`, S.above before them
-__device__ Border border_at(RowShared& S, u64 one, uint32_t key, bool by_mass, u64 want) {
+__device__ __forceinline__ Border border_at(RowShared& S, u64 one, uint32_t key, bool by_mass, u64 want) {
     Border r;
     r.key = key;
     const u64 left = S.left;
@@ -740,7 +764,7 @@ __device__ Border border_at(RowShared& S, u64 one, uint32_t key, bool by_mass, u
 // The border of the `want` first tokens in the order (by_mass: of the tokens before which less
 // than `want` of mass lies; ties share what is left), by a radix descent over the whole row's keys,
 // 12 bits at a time
-__device__ Border descend(RowShared& S, int& turn, const Row& R, const Masses& m, bool by_mass, u64 want) {
+__device__ __forceinline__ Border descend(RowShared& S, int& turn, const Row& R, const Masses& m, bool by_mass, u64 want) {
     uint32_t prefix = 0;
     u64 above = 0;
     for (int shift = 32 - WAY_BITS, nb = WAY_BITS; nb; shift -= nb) {
@@ -750,7 +774,7 @@ __device__ Border descend(RowShared& S, int& turn, const Row& R, const Masses& m
             const float l = R.at(i);
             const uint32_t k = key_of(l);
             if (step && (k >> (shift + nb)) != prefix) continue;
-            const uint32_t b = mask - ((k >> shift) & mask);
+            const uint32_t b = place(mask - ((k >> shift) & mask));
             atomicAdd(&S.count[b], 1u);
             if (by_mass) {
                 const u64 q = m.mass_any(l);
@@ -768,7 +792,7 @@ __device__ Border descend(RowShared& S, int& turn, const Row& R, const Masses& m
 // The same border among the n tokens of the list, with `above` before them: the keys' range divided by
 // up to 4096 until one key is left.  A thread has at most PER of them.
 template <int PER>
-__device__ Border descend_list(RowShared& S, int& turn, const Masses& m, int n, bool by_mass, u64 above, u64 want) {
+__device__ __forceinline__ Border descend_list(RowShared& S, int& turn, const Masses& m, int n, bool by_mass, u64 above, u64 want) {
     uint32_t key[PER], lo = 0xffffffffu, hi = 0;
     u64 q[PER];
 #pragma unroll
@@ -783,14 +807,14 @@ __device__ Border descend_list(RowShared& S, int& turn, const Masses& m, int n, 
     }
     const u64 far = wave_max((u64)hi << 32), near = wave_max((u64)(uint32_t)~lo);
     if ((threadIdx.x & 63) == 0) {
-        S.tpart[threadIdx.x >> 6] = ~(uint32_t)near;
-        S.part[threadIdx.x >> 6] = far >> 32;
+        S.lo_part[threadIdx.x >> 6] = ~(uint32_t)near;
+        S.hi_part[threadIdx.x >> 6] = (uint32_t)(far >> 32);
     }
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < NT / 64; w++) {
-        lo = min(lo, S.tpart[w]);
-        hi = max(hi, (uint32_t)S.part[w]);
+        lo = min(lo, S.lo_part[w]);
+        hi = max(hi, S.hi_part[w]);
     }
     for (;;) {
         int shift = 0;  // keys per bin, as a power of two
@@ -798,7 +822,7 @@ __device__ Border descend_list(RowShared& S, int& turn, const Masses& m, int n, 
 #pragma unroll
         for (int j = 0; j < PER; j++)
             if (key[j] && key[j] >= lo && key[j] <= hi) {
-                const uint32_t b = (hi - key[j]) >> shift;
+                const uint32_t b = place((hi - key[j]) >> shift);
                 atomicAdd(&S.count[b], 1u);
                 if (q[j]) atomicAdd(&S.sum[b], q[j]);
             }
@@ -817,7 +841,7 @@ constexpr int INDEX_BITS = 22;
 static_assert(SAMPLE_MAX_VOCAB == 1 << INDEX_BITS && INDEX_BITS <= 2 * WAY_BITS, "two steps over an index");
 constexpr int LOW_BITS = INDEX_BITS - WAY_BITS;
 template <int PER>
-__device__ uint32_t last_tie(RowShared& S, int& turn, const Border& B, int n) {
+__device__ __forceinline__ uint32_t last_tie(RowShared& S, int& turn, const Border& B, int n) {
     if (B.ties == ALL) return ALL;
     uint32_t high = 0;
     u64 above = 0;
@@ -827,7 +851,7 @@ __device__ uint32_t last_tie(RowShared& S, int& turn, const Border& B, int n) {
             const int i = j * NT + threadIdx.x;
             if (i >= n || (uint32_t)(S.list[i] >> 32) != B.key) continue;
             const uint32_t at = ~(uint32_t)S.list[i];
-            if (step == 0 || at >> LOW_BITS == high) atomicAdd(&S.count[step ? at & ((1u << LOW_BITS) - 1) : at >> LOW_BITS], 1u);
+            if (step == 0 || at >> LOW_BITS == high) atomicAdd(&S.count[place(step ? at & ((1u << LOW_BITS) - 1) : at >> LOW_BITS)], 1u);
         }
         choose(S, turn, false, above, B.ties);
         if (step) break;
@@ -844,7 +868,7 @@ struct Kept {
     uint32_t ties;
     int at;
 };
-__device__ Kept walk(const Row& R, const Masses& m, const Border& B, u64 least, int i0, int i1, uint32_t ties,
+__device__ __forceinline__ Kept walk(const Row& R, const Masses& m, const Border& B, u64 least, int i0, int i1, uint32_t ties,
                      bool find, u64 target) {
     const int lane = threadIdx.x & 63;
     Kept r{0, ties, -1};
@@ -884,7 +908,7 @@ __device__ __forceinline__ u64 target_of(float u, u64 total) {
 }
 
 // the whole row by this workgroup
-__device__ int pick_alone(RowShared& S, int& turn, const Row& R, const Masses& m, const Set& s, float u) {
+__device__ __forceinline__ int pick_alone(RowShared& S, int& turn, const Row& R, const Masses& m, const Set& s, float u) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const u64 least = m.least(s);
     Border B;
@@ -936,8 +960,8 @@ __device__ int pick_alone(RowShared& S, int& turn, const Row& R, const Masses& m
 }
 
 // top-k, few candidates: the n in S.list, a thread each, every one compared with every other
-constexpr int FEW = 256;
-__device__ int pick_few(RowShared& S, int& turn, const Masses& m, const Set& s, int n, float u) {
+constexpr int FEW = WT;
+__device__ __forceinline__ int pick_few(RowShared& S, int& turn, const Masses& m, const Set& s, int n, float u) {
     const int me = threadIdx.x;
     const u64 entry = me < n ? S.list[me] : 0;
     int rank = 0;
@@ -979,7 +1003,7 @@ static_assert(FEW <= WAYS && FEW <= LIST && FEW <= SAMPLE_MAX_VOCAB / BLOCK, "on
 
 // top-k, many candidates: the k first of the n in S.list, the border of top-p among them, then the token
 // by its index, in two steps
-__device__ int pick_list(RowShared& S, int& turn, const Masses& m, const Set& s, int n, float u) {
+__device__ __forceinline__ int pick_list(RowShared& S, int& turn, const Masses& m, const Set& s, int n, float u) {
     constexpr int PER = LIST / NT;
     if (n > s.k) {
         const Border B = descend_list<PER>(S, turn, m, n, false, 0, (u64)s.k);
@@ -1006,21 +1030,19 @@ __device__ int pick_list(RowShared& S, int& turn, const Masses& m, const Set& s,
     const uint32_t key = (uint32_t)(e >> 32), at = ~(uint32_t)e;
     const u64 q = e ? m.mass(logit_of(key)) : 0;
     bool kept = q && q >= m.least(s);
-    u64 z;
     if (s.p < 1.0f) {
-        S.scan.before(turn, q, z);
+        const u64 z = block_sum(S, q);
         const u64 want = (u64)ceil((s.p > 0.0f ? (double)s.p : 0.0) * (double)z);
         const Border B = descend_list<1>(S, turn, m, n, true, 0, want);
         const uint32_t cut = last_tie<1>(S, turn, B, n);
         kept = kept && (key > B.key || (key == B.key && at <= cut));
     }
-    S.scan.before(turn, kept ? q : 0, z);
-    const u64 target = target_of(u, z);
+    const u64 target = target_of(u, block_sum(S, kept ? q : 0));
     u64 above = 0;
     uint32_t high = 0;
     for (int step = 0; step < 2; step++) {
         if (kept && (step == 0 || at >> LOW_BITS == high)) {
-            const uint32_t b = step ? at & ((1u << LOW_BITS) - 1) : at >> LOW_BITS;
+            const uint32_t b = place(step ? at & ((1u << LOW_BITS) - 1) : at >> LOW_BITS);
             atomicAdd(&S.count[b], 1u);
             atomicAdd(&S.sum[b], q);
         }
@@ -1034,15 +1056,15 @@ __device__ int pick_list(RowShared& S, int& turn, const Masses& m, const Set& s,
 
 // no top-k: the blocks' masses are in the workspace (with top-p those above the border's bin, whose
 // tokens are the n in S.list; h: this thread's bins)
-__device__ int pick_blocks(RowShared& S, int& turn, const Row& R, const Masses& m, const Set& s, const RowWs& w,
-                           int blocks, int n, const u64 (&h)[BINS / NT], float u) {
+__device__ __forceinline__ int pick_blocks(RowShared& S, int& turn, const Row& R, const Masses& m, const Set& s, const RowWs& w,
+                           int blocks, int n, const u64 (&h)[BINS_EACH], float u) {
     constexpr int PER = LIST / NT;
     const u64 least = m.least(s);
     Border B;
     uint32_t cut = ALL;
     for (int i = threadIdx.x; i < blocks; i += NT) S.block[i] = w.block[i];
     if (s.mode == ROW_NUCLEUS) {
-        const BorderBin b = border_bin<NT>(h, s.p, S.scan, turn, S.border);
+        const BorderBin b = border_bin(h, s.p, S.scan, turn, S.border);
         if (n <= NT) {
             B = descend_list<1>(S, turn, m, n, true, b.above, b.want);
             cut = last_tie<1>(S, turn, B, n);
@@ -1059,20 +1081,29 @@ __device__ int pick_blocks(RowShared& S, int& turn, const Row& R, const Masses& 
         }
     }
     __syncthreads();
-    static_assert(SAMPLE_MAX_VOCAB / BLOCK <= 2 * NT, "two blocks a thread");
-    u64 v[2], z;
-    const int b0 = threadIdx.x * 2;
-    for (int j = 0; j < 2; j++) v[j] = b0 + j < blocks ? S.block[b0 + j] : 0;
-    u64 run = S.scan.before(turn, v[0] + v[1], z);
-    const u64 target = target_of(u, z);
-    for (int j = 0; j < 2; j++) {
-        if (run <= target && run + v[j] > target) {
-            S.bin = b0 + j;
-            S.above = run;
+    constexpr int EACH = SAMPLE_MAX_VOCAB / BLOCK / WT;  // blocks a worker
+    u64 v[EACH], sum = 0, z;
+    const int b0 = threadIdx.x * EACH;
+    if (threadIdx.x < WT)
+#pragma unroll
+        for (int j = 0; j < EACH; j++) {
+            v[j] = b0 + j < blocks ? S.block[b0 + j] : 0;
+            sum += v[j];
         }
-        run += v[j];
-    }
+    u64 run = S.scan.before(turn, sum, z);
+    const u64 target = target_of(u, z);
+    if (threadIdx.x < WT && run <= target && run + sum > target)
+#pragma unroll
+        for (int j = 0; j < EACH; j++) {
+            if (run <= target && run + v[j] > target) {
+                S.bin = b0 + j;
+                S.above = run;
+            }
+            run += v[j];
+        }
     __syncthreads();
+    // the block's tokens, two a thread; the wave whose sum reaches the target looks closer
+    static_assert(BLOCK == 2 * NT, "two tokens a thread");
     const int i = (int)S.bin * BLOCK + threadIdx.x * 2;
     const u64 left = target - S.above;
     u64 q[2];
@@ -1083,10 +1114,17 @@ __device__ int pick_blocks(RowShared& S, int& turn, const Row& R, const Masses& 
         const bool keep = k > B.key || (k == B.key && (uint32_t)(i + j) <= cut);
         q[j] = keep && q1 >= least ? q1 : 0;
     }
-    run = S.scan.before(turn, q[0] + q[1], z);
-    for (int j = 0; j < 2; j++) {
-        if (run <= left && run + q[j] > left) S.found = i + j;
-        run += q[j];
+    const u64 mine = wave_sum(q[0] + q[1]);
+    if ((threadIdx.x & 63) == 0) S.part[threadIdx.x >> 6] = mine;
+    __syncthreads();
+    run = 0;
+    for (int w = 0; w < (int)(threadIdx.x >> 6); w++) run += S.part[w];
+    if (run <= left && run + mine > left) {
+        run += wave_scan(q[0] + q[1]) - q[0] - q[1];
+        for (int j = 0; j < 2; j++) {
+            if (run <= left && run + q[j] > left) S.found = i + j;
+            run += q[j];
+        }
     }
     __syncthreads();
     return S.found;
@@ -1098,9 +1136,8 @@ __global__ __launch_bounds__(NT) void sample_pick_kernel(SampleArgs A, SamplePla
     const RowWs w = row_ws(A, P, row);
     // (read with the rest, before it is known how many there are and whether they are needed)
     const u64 e0 = w.list[threadIdx.x];
-    u64 h[BINS / NT];
-#pragma unroll
-    for (int j = 0; j < BINS / NT; j++) h[j] = w.hist[threadIdx.x * (BINS / NT) + j];
+    u64 h[BINS_EACH];
+    load_bins(w.hist, h);
     const uint32_t count = *w.count;
     const float u = A.u[row];
     const u64 top = row_top(w, P.segs);
