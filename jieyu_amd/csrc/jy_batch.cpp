@@ -3,7 +3,6 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
-#include <climits>
 #include <cmath>
 #include <string>
 
@@ -63,7 +62,8 @@ bool check_moved(const jyhip_pages* p, const jyhip_page_tables* t, int rows, con
     if (!seq && rows > t->num_seqs) fail("without seq there is one row per sequence: more rows than sequences");
     check_vectors(k, type, "k");
     check_vectors(v, type, "v");
-    if ((int64_t)rows * p->num_kv_heads > (int64_t)INT_MAX) fail("rows x heads is too large for one call");
+    // 16 threads a (row, head), under 2^32 threads a launch
+    if ((int64_t)rows * p->num_kv_heads >= 1 << 28) fail("rows x heads is too large for one call");
     return true;
 }
 
@@ -161,7 +161,7 @@ JYHIP_API int jyhip_sample(const void* logits, int type, int rows, int vocab, lo
         if (rows < 0) fail("rows must not be negative");
         if (rows == 0) return 0;
         if (vocab < 1 || vocab > SAMPLE_MAX_VOCAB) fail("sample: vocab must be between 1 and 2^22");
-        if (rows >= 1 << 21) fail("sample: too many rows for one call");
+        if (rows >= 1 << 20) fail("sample: too many rows for one call");
         if (!logits || !u || !ids) fail("sample: NULL logits, u or ids");
         if ((uintptr_t)logits % (type == JYHIP_T_F32 ? 4 : 2)) fail("sample: logits are not aligned to their elements");
         if (row_stride < 0) fail("sample: a negative row stride");

@@ -42,7 +42,7 @@ struct PagedAttn {
     float* part = nullptr;       // paged_attend_part_floats() floats
 };
 size_t paged_attend_part_floats(const jyhip_pages& P, int nseq, int nh, int max_len);
-// workgroups of the larger of its launches (256 threads each)
+// workgroups of 256 threads of the larger of its launches
 int64_t paged_attend_blocks(const jyhip_pages& P, int nseq, int nh, int max_len);
 void launch_paged_attend(const PagedAttn& A, hipStream_t st);
 

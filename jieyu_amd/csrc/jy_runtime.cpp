@@ -1778,7 +1778,7 @@ int forward_paged(jyhip_model* m, const jyhip_pages* pages, const float* X, floa
         h.insert(h.end(), t, t + table_stride);
     }
     if (paged_attend_blocks(pages[0], rows, m->nh, max_len) >= (1 << 24) ||
-        (int64_t)rows * m->nkv > INT_MAX)
+        (int64_t)rows * m->nkv >= 1 << 28)
         fail("forward_paged: too many rows for one call");
     const OnDevice on(m->device, nullptr);
     ensure_ws(m, rows);
