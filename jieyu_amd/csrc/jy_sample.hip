@@ -135,7 +135,12 @@ struct Masses {
     __device__ __forceinline__ bool set(float top, float T, int vocab, const u64* table) {
         M = top;
         c = STEPS * 1.4426950408889634074 / (double)T;
-        low = (float)((double)M - 64.0 * STEPS / c);
+        // the largest logit 64 factors of two under M.  Where T is so small next to M that this is the
+        // float before M, none lies between: a c of twice that keeps y within a whole number's bits.
+        const double far = (double)M - 64.0 * STEPS / c;
+        low = (float)far;
+        if ((double)low > far || low == M) low = logit_of(key_of(low) - 1);
+        if (key_of(low) + 1 == key_of(M)) c = fmin(c, 128.0 * STEPS / ((double)M - (double)low));
         int s = 51;
         while (s > 40 && (1ll << (62 - s)) < vocab) s--;
         unit = (double)(1ull << s);

@@ -143,6 +143,18 @@ def test_masked_logits(jy, V, io):
     assert run(jy, x, u, SETTINGS) == [V // 2] * n
 
 
+@pytest.mark.parametrize("centre", [0.0, 20.0, -20.0, 1e4, -1e8, 1e30, -1e30])
+def test_temperatures_far_under_the_logits_spacing(jy, centre):
+    """next to a large logit the float before it is many temperatures away: it has no mass"""
+    Ts = [1.0, 1e-3, 1e-5, 3e-7, 1e-7, 3e-8, 1e-8, 1e-10, 1e-20, 1e-37, 1e-42]
+    for V in (500, 20000):
+        settings = [(torch.tensor(T).item(), k, p, m) for T in Ts
+                    for k, p, m in ((0, 1.0, 0.0), (0, 1.0, 0.1), (40, 1.0, 0.0), (300, 0.9, 0.0), (0, 0.9, 0.0), (2000, 0.99, 0.0))]
+        x, u = logits(len(settings), V, 5, "f32")
+        x = (centre + x * max(1.0, abs(centre) * 1e-6)).float()
+        check(jy, x, u, settings)
+
+
 def test_positive_infinity(jy):
     x, u = logits(len(SETTINGS), 3000, 4, "f32")
     x[:, 100] = x[:, 2000] = math.inf
