@@ -305,8 +305,8 @@ JYHIP_API int jyhip_pages_read(const jyhip_pages* pages, const jyhip_page_tables
  * `tables`: out[s][h] = sum_j softmax_j(scale q[s][h] . k_j) v_j, head h reading kv head
  * h / (num_heads / num_kv_heads).  q and out are of `type` (JYHIP_T_F32, _F16, _BF16); scores,
  * softmax and sums are held in fp32.  A sequence without any position (lens[s] <= 0, only holes)
- * gives zeros.  max_len is an upper bound of lens known on the host: it sizes the launch, and a
- * longer lens[s] is cut to it.  The workspace needs jyhip_pages_attend_workspace() bytes, aligned
+ * gives zeros.  max_len, at most 2^30, is an upper bound of lens known on the host: it sizes the launch,
+ * and a longer lens[s] is cut to it.  The workspace needs jyhip_pages_attend_workspace() bytes, aligned
  * to 16. */
 JYHIP_API int jyhip_pages_attend(const jyhip_pages* pages, const jyhip_page_tables* tables, const int* lens,
                                  int max_len, int num_heads, float scale, const jyhip_vectors* q,

@@ -192,6 +192,8 @@ class PagePool:
         n = _indices(b, lens, batch, self.device, "lens")
         if T.num_seqs != batch:
             raise JyError("attend: one query row for each sequence of the tables")
+        if not 0 <= max_len <= 1 << 30:
+            raise JyError("attend: max_len must be between 0 and 2^30")
         if not batch:
             return out
         need = b.attend_workspace(pages, batch, heads, max_len)

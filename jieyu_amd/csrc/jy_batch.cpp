@@ -35,6 +35,8 @@ void jy::check_pages(const jyhip_pages* p) {
 
 namespace {
 
+constexpr int MAX_LEN = 1 << 30;  // (a position plus a chunk is an int in the kernels)
+
 void check_tables(const jyhip_page_tables* t) {
     if (!t || !t->tables) fail("NULL page tables");
     if (t->num_seqs < 1 || t->table_stride < 1) fail("page tables: num_seqs and table_stride must be positive");
@@ -105,7 +107,7 @@ JYHIP_API int jyhip_pages_read(const jyhip_pages* pages, const jyhip_page_tables
 }
 
 JYHIP_API size_t jyhip_pages_attend_workspace(const jyhip_pages* pages, int num_seqs, int num_heads, int max_len) {
-    if (!pages || num_seqs < 1 || num_heads < 1 || pages->num_kv_heads < 1 || max_len < 1) return 0;
+    if (!pages || num_seqs < 1 || num_heads < 1 || pages->num_kv_heads < 1 || max_len < 1 || max_len > MAX_LEN) return 0;
     return paged_attend_part_floats(*pages, num_seqs, num_heads, max_len) * sizeof(float);
 }
 
@@ -118,7 +120,7 @@ JYHIP_API int jyhip_pages_attend(const jyhip_pages* pages, const jyhip_page_tabl
         check_tables(tables);
         check_type(type);
         if (!lens) fail("lens is NULL");
-        if (max_len < 0) fail("max_len must not be negative");
+        if (max_len < 0 || max_len > MAX_LEN) fail("max_len must be between 0 and 2^30");
         if (num_heads < 1 || num_heads % pages->num_kv_heads)
             fail("the query heads must be a multiple of the key/value heads");
         if (!std::isfinite(scale)) fail("scale must be finite");

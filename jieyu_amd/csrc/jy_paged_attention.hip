@@ -41,7 +41,7 @@ namespace {
 typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
 typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
 
-constexpr float kNone = -3.0e38f;       // the running maximum before any score
+constexpr float kNone = -3.402823466e38f;  // the running maximum before any score: at most any finite one
 constexpr int kMaxChunk = 4096;          // 64 groups of 16 positions per wave: one lane holds each one's page
 constexpr float kLog2e = 1.4426950408889634f;
 

@@ -267,6 +267,31 @@ def test_attend_peaked(jy, pool):
     check(c.attend(zero.to(DEV)), *attention64(zero, c.k, c.v, 1.0))  # a mean of the values
 
 
+@pytest.mark.parametrize("n", [2, 40, 3000])
+def test_attend_scores_near_the_types_lowest(jy, n):
+    """finite scores down to fp32's lowest value have weight: equal ones the same"""
+    k = torch.zeros((1, (n + 255) // 256, 1, 256, 64), dtype=torch.bfloat16)
+    v = torch.randn(k.shape, generator=gen(3)).to(torch.bfloat16)
+    k[..., 0] = 2.0**63
+    q = torch.zeros((1, 3, 64))
+    q[..., 0] = torch.tensor([-1.3 * 2.0**64, -1.0, 0.0])
+    pool = jy.PagePool(k.to(DEV), v.to(DEV))
+    tables = torch.arange(k.shape[1], dtype=torch.int32, device=DEV)[None]
+    got = pool.attend(0, q.to(DEV), tables, torch.tensor([n], dtype=torch.int32, device=DEV), n, scale=1.0)
+    x = v[0, :, 0].reshape(-1, 64)[:n].double()
+    # equal weights of exactly 1: the sums' n steps of fp32, one division
+    room = (n + 1) * 2.0**-24 * x.abs().mean(0)
+    assert ((got[0].double().cpu() - x.mean(0)).abs() <= room).all()
+
+
+def test_attend_max_len_is_checked(jy):
+    c = Cache(jy, [5], 1, 64, 16, "i8")
+    q = torch.zeros((1, 1, 64), device=DEV)
+    for n in (-1, (1 << 30) + 1, 1 << 32):
+        with pytest.raises(jy.JyError, match="max_len"):
+            c.attend(q, max_len=n)
+
+
 def test_attend_nan_and_infinity_reach_their_own_rows_only(jy):
     c = Cache(jy, [40, 40, 40], 2, 64, 16, "i8", seed=13)
     q = torch.randn((3, 4, 64), generator=gen(3))

@@ -89,6 +89,13 @@ def test_bad_attention(b, over, text):
     assert text in error(b)
 
 
+def test_lengths_whose_chunks_pass_an_int(b):
+    for n in ((1 << 30) + 1, (1 << 31) - 1):
+        assert attend(b, max_len=n) == -1 and "2^30" in error(b)
+        assert b.attend_workspace(pages(), 1, 4, n) == 0
+    assert 0 < b.attend_workspace(pages(), 1, 4, 1 << 30) < 1 << 32
+
+
 def test_null_structs(b):
     none = C.POINTER(B._Pages)()
     assert b.write(none, tables(), 1, None, 0x1000, vectors(), vectors(), B.T_F32, None) == -1
