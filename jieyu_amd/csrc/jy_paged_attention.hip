@@ -758,8 +758,8 @@ void launch_paged_attend(const PagedAttn& A, hipStream_t st) {
     else
         launch_wide<JYHIP_T_BF16>(K, grid, st);
     if (K.plan.splits > 1) {
-        // 32 sequences of 32 heads in 16 chunks: both kernels 18.5 us with a workgroup a row, 17.5 us
-        // with a thread for four dims.  Longer splits: four chunks a thread are read at once, so
+        // 32 sequences of up to 1500 positions, 32 heads of 128, 3 chunks: both kernels 18.5 us with a
+        // workgroup a row, 17.5 us with a thread for four dims.  Longer splits: four chunks a thread are read at once, so
         // more threads where those are not all (one sequence of 32000, 14 heads of 64: 11.6 us
         // with 256 threads, 13.2 us with 1024).
         const int quads = A.P.head_dim / 4;

@@ -21,6 +21,13 @@
 //      it
 // A row whose candidates do not fit the list (k > 1024, or thousands of equal logits at the border)
 // is done by its workgroup in kernel 4 alone, by a radix descent over the logits' bits.
+//
+// Time of the kernels (1, 2, 3, 4), us: one row of 151936, fp32, k = 50: 3.8, 6.2, 1.7, 7.9: the launches
+// and each kernel's chain of loads and barriers.  64 rows of 128256, fp32, all kinds of settings: 8.9,
+// 13.8, 9.9, 21.1, the last for k = 1000: ten steps of a descent, a barrier or two and two waits for LDS
+// each.  256 rows of 152064, bf16, top-p 0.9: 17, 32, 33, 16: the first is memory's time (4.5 TB/s);
+// the next two have that and 10 us of start and end, which no other workgroup's work covers as all
+// are resident at once (with half of them at a time it was more).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -119,12 +126,10 @@ __device__ __forceinline__ Set set_of(const SampleArgs& A, int row) {
     return s;
 }
 
-__device__ constexpr u64 kExp2[32] = JY_EXP2_TABLE;
-
 // Masses of a row's logits, e 2^s.  With y = 512 (x - M) log2 e / T = k + r, k whole and |r| <= 1/2:
 // 2^(k/512) from a table of 512 (2^s in it) and the exponent, times the Taylor terms of 2^(r/512) up to
 // r^3 (the rest is under 9e-15).  The fp64 operations bound the passes that weigh every token, so
-// few of them: a table of 32 and two more terms measured 41 us against 38 over 256 x 152064.
+// few of them: with a table of 32 and two more terms kernel 2 took 41 us over 256 x 152064, 38 us so.
 struct Masses {
     float M, low;    // low: the logit whose mass is far under 2^-52, standing for all below it and NaN
     double c;        // 512 log2 e / T
@@ -147,20 +152,15 @@ struct Masses {
         tab = table;
         return M < __builtin_inff() && low > -3.4e38f;
     }
-    // entry i: 2^(i/512) 2^s, from 2^(j/32) (kExp2's entry is that less j << 47 in its bits) and the
-    // Taylor terms of 2^(f/32), 0 <= f < 1, up to f^6 (the rest is under 5e-16)
+    // entry i: 2^(i/512) 2^s, as the square root of two times the Taylor terms of e^x up to x^12, x = ln 2
+    // (i/512 - 1/2) (the rest is under 2e-16)
     __device__ __forceinline__ void fill(u64* table) const {
-        constexpr double L = 0.69314718055994531 / 32;
         for (int i = threadIdx.x; i < STEPS; i += blockDim.x) {
-            const int j = i * 32 / STEPS;
-            const double f = (i * 32 % STEPS) * (1.0 / STEPS);
-            double q = __builtin_fma(f, L * L * L * L * L * L / 720.0, L * L * L * L * L / 120.0);
-            q = __builtin_fma(q, f, L * L * L * L / 24.0);
-            q = __builtin_fma(q, f, L * L * L / 6.0);
-            q = __builtin_fma(q, f, L * L / 2.0);
-            q = __builtin_fma(q, f, L);
-            q = __builtin_fma(q, f, 1.0);
-            table[i] = __builtin_bit_cast(u64, unit * (q * __builtin_bit_cast(double, kExp2[j] + ((u64)j << 47))));
+            const double x = (i - STEPS / 2) * (0.69314718055994531 / STEPS);
+            double q = 1.0;
+#pragma unroll
+            for (int n = 12; n > 0; n--) q = __builtin_fma(q, x * (1.0 / n), 1.0);
+            table[i] = __builtin_bit_cast(u64, unit * 1.4142135623730951 * q);
         }
     }
     // 2^(r/512)
@@ -442,6 +442,27 @@ __device__ __forceinline__ uint32_t stripe_bound(Bound& S, const RowWs& w, int k
 }
 static_assert(NP / 64 == 8, "a wave for each value of three bits");
 
+// bf16 logits have few values: a workgroup counts its tokens by value and weighs each value once
+// (256 x 152064: 38 us with every token weighed, 32 us so).
+// A cell for every magnitude of the upper 16 powers of two of those with mass, either sign; the tokens
+// nearer to zero are weighed one by one.
+constexpr int SIDE = 16 << 7;
+struct Cells {
+    int base;  // the least magnitude with a cell (a bf16's bits)
+    __device__ __forceinline__ Cells(const Masses& m) {
+        const uint32_t low = __builtin_bit_cast(uint32_t, m.low) & 0x7fffffffu, M = __builtin_bit_cast(uint32_t, m.M) & 0x7fffffffu;
+        base = max((int)(max(M, low + 0xffffu) >> 16) - (SIDE - 1), 0);
+    }
+    // the cell of l, SIDE or more: none
+    __device__ __forceinline__ uint32_t magnitude(float l) const {
+        return (__builtin_bit_cast(uint32_t, l) >> 16 & 0x7fffu) - (uint32_t)base;
+    }
+    static __device__ __forceinline__ uint32_t side(float l) { return __builtin_bit_cast(uint32_t, l) >> 31 ? SIDE : 0; }
+    __device__ __forceinline__ float logit(int cell) const {
+        return __builtin_bit_cast(float, (uint32_t)(base + cell % SIDE) << 16 | (cell >= SIDE ? 0x80000000u : 0));
+    }
+};
+
 // ---- 2: top-k candidates, masses or the histogram
 template <class E>
 __global__ __launch_bounds__(NP, 8) void sample_mass_kernel(SampleArgs A, SamplePlan P) {
@@ -452,6 +473,8 @@ __global__ __launch_bounds__(NP, 8) void sample_mass_kernel(SampleArgs A, Sample
     } U;
     __shared__ u64 tab[STEPS];
     __shared__ Bound bound;
+    constexpr bool BF16 = __is_same(E, __bf16);
+    __shared__ uint32_t cell[BF16 ? 2 * SIDE + 64 : 1];  // (64: for the tokens without a cell)
     u64* const hist = U.hist;
     const int row = blockIdx.x / P.segs, seg = blockIdx.x % P.segs;
     const Set s = set_of(A, row);
@@ -483,8 +506,43 @@ __global__ __launch_bounds__(NP, 8) void sample_mass_kernel(SampleArgs A, Sample
     const int nb = bins ? BINS : (i1 - i0 + BLOCK - 1) / BLOCK;
     for (int i = threadIdx.x; i < nb; i += NP) hist[i] = 0;
     m.fill(tab);
+    // where the cells are fewer than the tokens
+    const bool counted = BF16 && bins && P.seg_len > 2 * SIDE;
+    if (counted)
+        for (int i = threadIdx.x; i < 2 * SIDE; i += NP) cell[i] = 0;
     __syncthreads();
-    if (bins) {
+    if (counted) {
+        const Cells cells(m);
+        const uint32_t none = 2 * SIDE + (threadIdx.x & 63);
+        each(x, f, i0, i1, [&](const float (&l)[VL], int) {
+            bool far = false;
+#pragma unroll
+            for (int e = 0; e < VL; e++) {
+                const uint32_t c = cells.magnitude(l[e]);
+                atomicAdd(&cell[c < SIDE ? c + Cells::side(l[e]) : none], 1u);
+                far |= c >= SIDE && l[e] > m.low;
+            }
+            if (__any(far)) {
+#pragma unroll
+                for (int e = 0; e < VL; e++) {
+                    const Masses::At y = m.at(l[e]);
+                    const u64 q = m.mass(y);
+                    if (q && cells.magnitude(l[e]) >= SIDE) atomicAdd(&hist[y.bin()], q);
+                }
+            }
+        });
+        __syncthreads();
+        for (int i = threadIdx.x; i < 2 * SIDE; i += NP) {
+            const uint32_t n = cell[i];
+            if (!n) continue;
+            const Masses::At y = m.at(cells.logit(i));
+            const u64 q = m.mass(y);
+            if (q) atomicAdd(&hist[y.bin()], n * q);
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < BINS; i += NP)
+            if (hist[i]) atomicAdd(&w.hist[i], hist[i]);
+    } else if (bins) {
         each(x, f, i0, i1, [&](const float (&l)[VL], int) {
 #pragma unroll
             for (int e = 0; e < VL; e++) {
@@ -597,19 +655,26 @@ __device__ __forceinline__ BorderBin border_bin(const u64 (&h)[BINS_EACH], float
 }
 
 // ---- 3: top-p: the masses above the border's bin, its tokens into the list
+constexpr int VALUES = 2048;  // values of 16-bit logits from the largest down that a table holds
+constexpr u64 EDGE = 1ull << 63;
 template <class E>
 __global__ __launch_bounds__(NP, 8) void sample_border_kernel(SampleArgs A, SamplePlan P) {
     constexpr int VL = Logits<E>::VL, HALF = 4;  // elements packed at a time
     __shared__ u64 block[SEG_BLOCKS];
     __shared__ u64 tab[STEPS];
     __shared__ Stage stage;
-    __shared__ uint2 mine[NP / 64][64 * (HALF + 1)];
+    __shared__ union {
+        uint2 mine[NP / 64][64 * (HALF + 1)];
+        u64 value[VALUES + 1];
+    } U;
     __shared__ Scan scan;
     __shared__ BorderFound found;
     const int row = blockIdx.x / P.segs, seg = blockIdx.x % P.segs;
     const Set s = set_of(A, row);
     if (s.mode != ROW_NUCLEUS) return;
     const RowWs w = row_ws(A, P, row);
+    u64 h[BINS_EACH];
+    load_bins(w.hist, h);
     const u64 top = row_top(w, P.segs);
     Masses m;
     if (!top || !m.set(top_logit(top), s.T, A.vocab, tab)) return;
@@ -620,16 +685,53 @@ __global__ __launch_bounds__(NP, 8) void sample_border_kernel(SampleArgs A, Samp
     const First<E> f = first(x, i0, i1);
     m.fill(tab);
     stage.clear();
-    u64 h[BINS_EACH];
-    load_bins(w.hist, h);
     int turn = 0;
     const BorderBin b = border_bin(h, s.p, scan, turn, found);  // (with barriers)
     const u64 least = m.least(s);
-    // Most tokens lie below the border.  Each wave packs those that may not, then takes them 64 at a
-    // time: with a nucleus of 9 % of the tokens the masses of all lanes' every token cost 1.7 times as much.
     const float floor = m.under(b.bin);
     const int lane = threadIdx.x & 63;
-    uint2* const pack = mine[threadIdx.x >> 6];
+    if constexpr (sizeof(E) == 2) {
+        // 16-bit logits have few values above the border: their masses from a table, by the distance to
+        // the largest one in steps of a value (EDGE for those of the border's bin).  256 x 152064 in
+        // bf16: 33 us, 37 us as below.
+        constexpr int SHIFT = __is_same(E, __bf16) ? 16 : 13;
+        const uint32_t at_M = __builtin_bit_cast(uint32_t, m.M), at_floor = __builtin_bit_cast(uint32_t, floor);
+        const uint32_t flip = at_M >> 31 ? 0u : ~0u;  // (of one sign they grow apart upwards or downwards)
+        const uint32_t values = (((at_floor ^ flip) - (at_M ^ flip)) >> SHIFT) + 1;
+        if ((at_M ^ at_floor) >> 31 == 0 && values <= VALUES) {
+            for (uint32_t i = threadIdx.x; i <= values; i += NP) {
+                const Masses::At y = m.at(__builtin_bit_cast(float, at_M + (at_M >> 31 ? i << SHIFT : -(i << SHIFT))));
+                const u64 v = m.mass(y);
+                U.value[i] = i == values || y.bin() > b.bin ? 0 : y.bin() == b.bin ? EDGE : v >= least ? v : 0;
+            }
+            __syncthreads();
+            each(x, f, i0, i1, [&](const float (&l)[VL], int i) {
+                u64 v[VL], q = 0;
+#pragma unroll
+                for (int e = 0; e < VL; e++) {
+                    const uint32_t far = ((__builtin_bit_cast(uint32_t, l[e]) ^ flip) - (at_M ^ flip)) >> SHIFT;
+                    v[e] = U.value[l[e] >= floor ? far : values];
+                    q += v[e];
+                }
+#pragma unroll
+                for (int e = 0; e < VL; e++) {
+                    const bool edge[1] = {(v[e] & EDGE) != 0};
+                    stage.add(w, edge, [&](int) { return entry_of(key_of(l[e]), i + e); });
+                }
+                q &= EDGE - 1;  // (an even or odd number of EDGEs, and masses under 2^55)
+                if (__any(q != 0)) {
+                    q = wave_sum(q);
+                    if (lane == 0) atomicAdd(&block[(i - i0) / BLOCK], q);
+                }
+            });
+            stage.flush(w);  // (with barriers)
+            for (int i = threadIdx.x; i < nb; i += NP) w.block[i0 / BLOCK + i] = block[i];
+            return;
+        }
+    }
+    // Most tokens lie below the border.  Each wave packs those that may not, then takes them 64 at a
+    // time: with a nucleus of 9 % of the tokens the masses of all lanes' every token cost 1.7 times as much.
+    uint2* const pack = U.mine[threadIdx.x >> 6];
     each(x, f, i0, i1, [&](const float (&l)[VL], int i) {
         int n = 0;
         u64 q = 0;

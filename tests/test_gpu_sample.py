@@ -155,6 +155,21 @@ def test_temperatures_far_under_the_logits_spacing(jy, centre):
         check(jy, x, u, settings)
 
 
+@pytest.mark.parametrize("io", ["bf16", "f16"])
+@pytest.mark.parametrize("centre,spread", [(0.0, 3.0), (0.0, 1e-3), (20.0, 3.0), (-20.0, 3.0), (-3.0, 3.0), (8.0, 0.01), (0.0, 30.0), (-1e4, 900.0)])
+def test_long_rows_of_16_bit_logits(jy, io, centre, spread):
+    """few values, met many times, of one sign or both; half of one row masked, another mostly zeros"""
+    V = 152064
+    settings = [(torch.tensor(T).item(), 0, torch.tensor(p).item(), m) for T in (0.3, 1.0, 5.0, 50.0)
+                for p, m in ((0.5, 0.0), (0.9, 0.0), (0.99, 0.0), (0.9, 0.02), (1e-4, 0.0))]
+    x, u = logits(len(settings), V, 9, io, spread=spread)
+    x = (centre + x.float()).to(IO[io])
+    x[1::5, ::2] = -math.inf
+    x[2::5, 3:] = torch.where(x[2::5, 3:].float().abs() < 2.5 * spread, torch.zeros_like(x[2::5, 3:]), x[2::5, 3:])
+    x[3::5, 1::3] = math.nan
+    check(jy, x, u, settings)
+
+
 def test_positive_infinity(jy):
     x, u = logits(len(SETTINGS), 3000, 4, "f32")
     x[:, 100] = x[:, 2000] = math.inf
