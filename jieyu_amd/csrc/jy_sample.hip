@@ -22,12 +22,13 @@
 // A row whose candidates do not fit the list (k > 1024, or thousands of equal logits at the border)
 // is done by its workgroup in kernel 4 alone, by a radix descent over the logits' bits.
 //
-// Time of the kernels (1, 2, 3, 4), us: one row of 151936, fp32, k = 50: 3.8, 6.2, 1.7, 7.9: the launches
+// Time of the kernels (1, 2, 3, 4), us: one row of 151936, fp32, k = 50: 3.8, 6.2, 1.7, 6.2: the launches
 // and each kernel's chain of loads and barriers.  64 rows of 128256, fp32, all kinds of settings: 8.9,
-// 13.8, 9.9, 21.1, the last for k = 1000: ten steps of a descent, a barrier or two and two waits for LDS
-// each.  256 rows of 152064, bf16, top-p 0.9: 17, 32, 33, 16: the first is memory's time (4.5 TB/s);
-// the next two have that and 10 us of start and end, which no other workgroup's work covers as all
-// are resident at once (with half of them at a time it was more).
+// 13.8, 9.9, 17.2, the last for k = 1000: a step of a descent and an ordering for each border, two steps
+// for the token, each some barriers and waits for LDS.  256 rows of 152064, bf16, top-p 0.9: 17, 32,
+// 33, 16: the first is memory's time (4.5 TB/s); the next two have that and 10 us of start and end,
+// which no other workgroup's work covers as all are resident at once (with half of them at a time it
+// was more).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -780,20 +781,24 @@ struct Border {
 constexpr int WAY_BITS = 11;         // bits of key or index that one step of a descent in kernel 4 settles
 constexpr int WAYS = 1 << WAY_BITS;
 constexpr int WAYS_EACH = WAYS / WT;
+constexpr int FEW = WT;              // tokens that are put in order by comparing each with each
+constexpr int FEWER = 128;           // of several keys, where another step (1.3 us) may leave less (256: 2 us)
+constexpr int BATCH = 4;             // of them at a time: one wait for LDS
 // where a bin lies: a worker takes consecutive ones, but the workers' first ones lie side by side, then
 // their second ones (consecutive ones side by side would put 64 lanes on four banks)
 __device__ __forceinline__ uint32_t place(uint32_t bin) { return (bin & (WAYS_EACH - 1)) * WT + bin / WAYS_EACH; }
 struct RowShared {
     uint32_t count[WAYS];           // at place(bin); zero between steps
     u64 sum[WAYS];                  // the same
-    u64 list[LIST];
+    u64 list[LIST + BATCH];         // zeros behind the last entry
+    u64 few[2][FEW + BATCH];
     u64 block[SAMPLE_MAX_VOCAB / BLOCK];
     Scan scan;
     u64 part[NT / 64];
     u64 tab[STEPS];
     uint32_t tpart[NT / 64], lo_part[NT / 64], hi_part[NT / 64];
-    u64 above;
-    uint32_t bin, left;
+    u64 above, edge;
+    uint32_t bin, left, few_n;
     int found;
     BorderFound border;
 };
@@ -817,6 +822,19 @@ __device__ __forceinline__ u64 block_sum(RowShared& S, u64 v) {
     v = 0;
     for (int w = 0; w < NT / 64; w++) v += S.part[w];
     return v;
+}
+
+// how many of the n entries of a list are greater (zeros behind them up to a multiple of BATCH)
+__device__ __forceinline__ int rank_of(const u64* list, int n, u64 entry) {
+    int rank = 0;
+    for (int i = 0; i < n; i += BATCH) {
+        u64 x[BATCH];
+#pragma unroll
+        for (int j = 0; j < BATCH; j++) x[j] = list[i + j];
+#pragma unroll
+        for (int j = 0; j < BATCH; j++) rank += x[j] > entry;
+    }
+    return rank;
 }
 
 // One step of a descent: of the bins in S (bin 0 the first in the order), the last one with a token in it
@@ -849,6 +867,7 @@ __device__ __forceinline__ void choose(RowShared& S, int& turn, bool by_mass, u6
             }
             run += v[j];
         }
+    if (threadIdx.x == 0) S.few_n = 0;
     __syncthreads();
 }
 
@@ -870,7 +889,7 @@ __device__ __forceinline__ Border border_at(RowShared& S, u64 one, uint32_t key,
 
 // The border of the `want` first tokens in the order (by_mass: of the tokens before which less
 // than `want` of mass lies; ties share what is left), by a radix descent over the whole row's keys,
-// 12 bits at a time
+// 11 bits at a time
 __device__ __forceinline__ Border descend(RowShared& S, int& turn, const Row& R, const Masses& m, bool by_mass, u64 want) {
     uint32_t prefix = 0;
     u64 above = 0;
@@ -896,10 +915,63 @@ __device__ __forceinline__ Border descend(RowShared& S, int& turn, const Row& R,
     return border_at(S, prefix ? m.mass_any(logit_of(prefix)) : 0, prefix, by_mass, want);
 }
 
-// The same border among the n tokens of the list, with `above` before them: the keys' range divided by
-// up to 4096 until one key is left.  A thread has at most PER of them.
+// The index of the last tie that B keeps among the list's n tokens (those at B's key)
+constexpr int INDEX_BITS = 22;
+static_assert(SAMPLE_MAX_VOCAB == 1 << INDEX_BITS && INDEX_BITS <= 2 * WAY_BITS, "two steps over an index");
+constexpr int LOW_BITS = INDEX_BITS - WAY_BITS;
 template <int PER>
-__device__ __forceinline__ Border descend_list(RowShared& S, int& turn, const Masses& m, int n, bool by_mass, u64 above, u64 want) {
+__device__ __forceinline__ uint32_t last_tie(RowShared& S, int& turn, const Border& B, int n) {
+    if (B.ties == ALL) return ALL;
+    uint32_t high = 0;
+    u64 above = 0;
+    for (int step = 0; step < 2; step++) {
+#pragma unroll
+        for (int j = 0; j < PER; j++) {
+            const int i = j * NT + threadIdx.x;
+            if (i >= n || (uint32_t)(S.list[i] >> 32) != B.key) continue;
+            const uint32_t at = ~(uint32_t)S.list[i];
+            if (step == 0 || at >> LOW_BITS == high) atomicAdd(&S.count[place(step ? at & ((1u << LOW_BITS) - 1) : at >> LOW_BITS)], 1u);
+        }
+        choose(S, turn, false, above, B.ties);
+        if (step) break;
+        high = S.bin;
+        above = S.above;
+    }
+    return high << LOW_BITS | S.bin;
+}
+
+// The last kept one of the n entries in `list` (FEW at most, zeros behind them), `above` before them
+__device__ __forceinline__ u64 last_of_few(RowShared& S, int& turn, const Masses& m, const u64* list, int n, bool by_mass,
+                                           u64 above, u64 want) {
+    const int me = threadIdx.x;
+    if (me < FEW) {
+        const u64 entry = me < n ? list[me] : 0;
+        const int rank = rank_of(list, n, entry);
+        if (me < n) S.few[1][rank] = entry;
+    }
+    __syncthreads();
+    const u64 mine = me < n ? S.few[1][me] : 0;
+    if (by_mass) {
+        const u64 q = me < n ? m.mass(logit_of((uint32_t)(mine >> 32))) : 0;
+        u64 total;
+        const u64 before = above + S.scan.before(turn, q, total);
+        if (me < n && (me == 0 || before < want) && (me + 1 == n || before + q >= want)) S.edge = mine;
+    } else if (me < n && above + me + 1 == want) {
+        S.edge = mine;
+    }
+    __syncthreads();
+    return S.edge;
+}
+
+// The last kept one of the n tokens of the list, of which the first `want` are kept (by_mass: those
+// before which less than `want` of mass lies), with `above` before them: the keys' range is divided
+// by up to 2048 until few tokens are left, or one key.  A thread has at most PER of them.  ORDER: few
+// are put in order.  (For the border of top-p alone it costs registers and saves nothing: its tokens of
+// 16-bit logits have one or two keys.)
+template <int PER, bool ORDER>
+__device__ __forceinline__ u64 last_kept(RowShared& S, int& turn, const Masses& m, int n, bool by_mass, u64 above, u64 want) {
+    if constexpr (ORDER)
+        if (n <= FEWER) return last_of_few(S, turn, m, S.list, n, by_mass, above, want);
     uint32_t key[PER], lo = 0xffffffffu, hi = 0;
     u64 q[PER];
 #pragma unroll
@@ -935,37 +1007,24 @@ __device__ __forceinline__ Border descend_list(RowShared& S, int& turn, const Ma
             }
         choose(S, turn, by_mass, above, want);
         above = S.above;
-        const uint32_t top = hi - (S.bin << shift);
-        if (shift == 0) return border_at(S, m.mass(logit_of(top)), top, by_mass, want);
-        const uint32_t low = top - ((1u << shift) - 1);
+        const uint32_t top = hi - (S.bin << shift), low = top - ((1u << shift) - 1);
         lo = low > lo && low <= top ? low : lo;
         hi = top;
-    }
-}
-
-// the index of the last tie that B keeps among the list's n tokens (those at B's key)
-constexpr int INDEX_BITS = 22;
-static_assert(SAMPLE_MAX_VOCAB == 1 << INDEX_BITS && INDEX_BITS <= 2 * WAY_BITS, "two steps over an index");
-constexpr int LOW_BITS = INDEX_BITS - WAY_BITS;
-template <int PER>
-__device__ __forceinline__ uint32_t last_tie(RowShared& S, int& turn, const Border& B, int n) {
-    if (B.ties == ALL) return ALL;
-    uint32_t high = 0;
-    u64 above = 0;
-    for (int step = 0; step < 2; step++) {
+        const int left = (int)S.left;
+        if constexpr (ORDER)
+            if (left <= (shift ? FEWER : FEW)) {
 #pragma unroll
-        for (int j = 0; j < PER; j++) {
-            const int i = j * NT + threadIdx.x;
-            if (i >= n || (uint32_t)(S.list[i] >> 32) != B.key) continue;
-            const uint32_t at = ~(uint32_t)S.list[i];
-            if (step == 0 || at >> LOW_BITS == high) atomicAdd(&S.count[place(step ? at & ((1u << LOW_BITS) - 1) : at >> LOW_BITS)], 1u);
+                for (int j = 0; j < PER; j++)
+                    if (key[j] && key[j] >= lo && key[j] <= hi) S.few[0][atomicAdd(&S.few_n, 1u)] = S.list[j * NT + threadIdx.x];
+                if (threadIdx.x < BATCH) S.few[0][left + threadIdx.x] = 0;
+                __syncthreads();
+                return last_of_few(S, turn, m, S.few[0], left, by_mass, above, want);
+            }
+        if (shift == 0) {
+            const Border B = border_at(S, m.mass(logit_of(top)), top, by_mass, want);
+            return (u64)B.key << 32 | ~last_tie<PER>(S, turn, B, n);
         }
-        choose(S, turn, false, above, B.ties);
-        if (step) break;
-        high = S.bin;
-        above = S.above;
     }
-    return high << LOW_BITS | S.bin;
 }
 
 // the kept mass of tokens with indices in [i0, i1), per wave in steps of 64, `ties` the ties before
@@ -1067,15 +1126,13 @@ __device__ __forceinline__ int pick_alone(RowShared& S, int& turn, const Row& R,
 }
 
 // top-k, few candidates: the n in S.list, a thread each, every one compared with every other
-constexpr int FEW = WT;
 __device__ __forceinline__ int pick_few(RowShared& S, int& turn, const Masses& m, const Set& s, int n, float u) {
     const int me = threadIdx.x;
-    const u64 entry = me < n ? S.list[me] : 0;
-    int rank = 0;
-    if (me < n)
-#pragma unroll 8
-        for (int i = 0; i < n; i++) rank += S.list[i] > entry;
-    if (me < n) S.block[rank] = entry;
+    if (me < FEW) {
+        const u64 entry = me < n ? S.list[me] : 0;
+        const int rank = rank_of(S.list, n, entry);
+        if (me < n) S.block[rank] = entry;
+    }
     if (me == 0) S.found = 0x7fffffff;
     __syncthreads();
     n = min(n, s.k);
@@ -1096,12 +1153,21 @@ __device__ __forceinline__ int pick_few(RowShared& S, int& turn, const Masses& m
     }
     S.scan.before(turn, kept, z);  // (with a barrier)
     const u64 target = target_of(u, z);
-    // the running sum up to each kept token's index
-    if (kept) {
+    // the running sum up to each kept token's index (of all FEW places those without a token are zero)
+    if (me < FEW) {
         u64 run = 0;
-#pragma unroll 8
-        for (int i = 0; i < n; i++) run += S.count[i] <= idx ? S.list[i] : 0;
-        if (run > target) atomicMin(&S.found, (int)idx);
+        for (int i = 0; i < n; i += BATCH) {
+            u64 v[BATCH];
+            uint32_t at[BATCH];
+#pragma unroll
+            for (int j = 0; j < BATCH; j++) {
+                v[j] = S.list[i + j];
+                at[j] = S.count[i + j];
+            }
+#pragma unroll
+            for (int j = 0; j < BATCH; j++) run += at[j] <= idx ? v[j] : 0;
+        }
+        if (kept && run > target) atomicMin(&S.found, (int)idx);
     }
     __syncthreads();
     return S.found;
@@ -1113,8 +1179,7 @@ static_assert(FEW <= WAYS && FEW <= LIST && FEW <= SAMPLE_MAX_VOCAB / BLOCK, "on
 __device__ __forceinline__ int pick_list(RowShared& S, int& turn, const Masses& m, const Set& s, int n, float u) {
     constexpr int PER = LIST / NT;
     if (n > s.k) {
-        const Border B = descend_list<PER>(S, turn, m, n, false, 0, (u64)s.k);
-        const uint32_t cut = last_tie<PER>(S, turn, B, n);
+        const u64 last = last_kept<PER, true>(S, turn, m, n, false, 0, (u64)s.k);
         u64 mine[PER];
 #pragma unroll
         for (int j = 0; j < PER; j++) {
@@ -1125,12 +1190,11 @@ __device__ __forceinline__ int pick_list(RowShared& S, int& turn, const Masses& 
         if (threadIdx.x == 0) S.left = 0;
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < PER; j++) {
-            const uint32_t k = (uint32_t)(mine[j] >> 32);
-            if (k > B.key || (k == B.key && ~(uint32_t)mine[j] <= cut)) S.list[atomicAdd(&S.left, 1u)] = mine[j];
-        }
+        for (int j = 0; j < PER; j++)
+            if (mine[j] >= last) S.list[atomicAdd(&S.left, 1u)] = mine[j];
         __syncthreads();
         n = S.left;
+        if (threadIdx.x < BATCH) S.list[n + threadIdx.x] = 0;  // (read after the next barrier)
     }
     static_assert(STRIPES <= NT, "at most one of the k a thread");
     const u64 e = (int)threadIdx.x < n ? S.list[threadIdx.x] : 0;
@@ -1140,9 +1204,8 @@ __device__ __forceinline__ int pick_list(RowShared& S, int& turn, const Masses& 
     if (s.p < 1.0f) {
         const u64 z = block_sum(S, q);
         const u64 want = (u64)ceil((s.p > 0.0f ? (double)s.p : 0.0) * (double)z);
-        const Border B = descend_list<1>(S, turn, m, n, true, 0, want);
-        const uint32_t cut = last_tie<1>(S, turn, B, n);
-        kept = kept && (key > B.key || (key == B.key && at <= cut));
+        const u64 last = last_kept<1, true>(S, turn, m, n, true, 0, want);  // (by all threads)
+        kept = kept && e >= last;
     }
     const u64 target = target_of(u, block_sum(S, kept ? q : 0));
     u64 above = 0;
@@ -1167,24 +1230,18 @@ __device__ __forceinline__ int pick_blocks(RowShared& S, int& turn, const Row& R
                            int blocks, int n, const u64 (&h)[BINS_EACH], float u) {
     constexpr int PER = LIST / NT;
     const u64 least = m.least(s);
-    Border B;
-    uint32_t cut = ALL;
+    u64 last = 0;
     for (int i = threadIdx.x; i < blocks; i += NT) S.block[i] = w.block[i];
     if (s.mode == ROW_NUCLEUS) {
         const BorderBin b = border_bin(h, s.p, S.scan, turn, S.border);
-        if (n <= NT) {
-            B = descend_list<1>(S, turn, m, n, true, b.above, b.want);
-            cut = last_tie<1>(S, turn, B, n);
-        } else {
-            B = descend_list<PER>(S, turn, m, n, true, b.above, b.want);
-            cut = last_tie<PER>(S, turn, B, n);
-        }
+        last = n <= NT ? last_kept<1, false>(S, turn, m, n, true, b.above, b.want)
+                       : last_kept<PER, false>(S, turn, m, n, true, b.above, b.want);
         // the border's tokens
         for (int i = threadIdx.x; i < n; i += NT) {
-            const uint32_t k = (uint32_t)(S.list[i] >> 32), at = ~(uint32_t)S.list[i];
-            if (k < B.key || (k == B.key && at > cut)) continue;
-            const u64 q = m.mass(logit_of(k));
-            if (q && q >= least) atomicAdd(&S.block[at / BLOCK], q);
+            const u64 e = S.list[i];
+            if (e < last) continue;
+            const u64 q = m.mass(logit_of((uint32_t)(e >> 32)));
+            if (q && q >= least) atomicAdd(&S.block[~(uint32_t)e / BLOCK], q);
         }
     }
     __syncthreads();
@@ -1216,10 +1273,8 @@ __device__ __forceinline__ int pick_blocks(RowShared& S, int& turn, const Row& R
     u64 q[2];
     for (int j = 0; j < 2; j++) {
         const float l = i + j < R.V ? R.at(i + j) : __builtin_nanf("");
-        const uint32_t k = key_of(l);
         const u64 q1 = m.mass(l);
-        const bool keep = k > B.key || (k == B.key && (uint32_t)(i + j) <= cut);
-        q[j] = keep && q1 >= least ? q1 : 0;
+        q[j] = entry_of(key_of(l), i + j) >= last && q1 >= least ? q1 : 0;
     }
     const u64 mine = wave_sum(q[0] + q[1]);
     if ((threadIdx.x & 63) == 0) S.part[threadIdx.x >> 6] = mine;
@@ -1265,6 +1320,7 @@ __global__ __launch_bounds__(NT) void sample_pick_kernel(SampleArgs A, SamplePla
     if (n <= LIST) {
         if ((int)threadIdx.x < n) S.list[threadIdx.x] = e0;
         for (int i = NT + threadIdx.x; i < n; i += NT) S.list[i] = w.list[i];
+        if (threadIdx.x < BATCH) S.list[n + threadIdx.x] = 0;
     }
     __syncthreads();
     Row R;

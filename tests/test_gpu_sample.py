@@ -112,6 +112,16 @@ def test_ties(jy, io, step):
         check(jy, x, u, SETTINGS)
 
 
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+@pytest.mark.parametrize("step", [0.003, 0.03, 0.1, 0.3, 1.0])
+def test_large_top_k_with_ties_at_the_border(jy, io, step):
+    """the borders of top-k and of top-p within it among one, few and hundreds of equal logits"""
+    settings = [(T, k, p, 0.0) for T in (1.0, 4.0) for k in (127, 257, 300, 500, 1000, 1024) for p in (1.0, 0.9375, 0.5)]
+    for V in (1500, 30000):
+        x, u = logits(len(settings), V, 11, io, step=step)
+        check(jy, x, u, settings)
+
+
 def test_all_equal(jy):
     for V in (1, 64, 9001, 152064):
         check(jy, torch.zeros(len(SETTINGS), V), torch.rand(len(SETTINGS)), SETTINGS)
