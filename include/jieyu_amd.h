@@ -354,7 +354,8 @@ JYHIP_API int jyhip_forward_paged(jyhip_model* model, const jyhip_pages* pages, 
 /* jyhip_session_step for a sampled session, the tokens drawn on the device by jyhip_sample with the
  * session's temperature, these filters (top_k <= 0, top_p >= 1, min_p <= 0: off) and the given numbers
  * u (host, n of them in [0, 1), one per step): the logits do not leave the device.  Returns how many
- * tokens were produced.  Refuses a greedy session (temperature <= 0) and one with a repetition
+ * tokens were produced; -1, and the session ends, where a step's logits hold nothing but NaN and
+ * -infinity.  Refuses a greedy session (temperature <= 0) and one with a repetition
  * penalty.  The session's first token came from jyhip_session_begin. */
 JYHIP_API int jyhip_session_step_sampled(jyhip_session* s, int n, int top_k, float top_p, float min_p, const float* u);
 

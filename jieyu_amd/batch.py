@@ -2,7 +2,8 @@
 tensors in device memory: a paged key/value cache, attention over it, and sampling.
 
 Everything runs on torch's current stream of the tensors' device and nothing waits for it, so
-calls can be recorded into a graph.  Workspaces come from torch's allocator, call by call.
+calls can be recorded into a graph.  Workspaces come from torch's allocator, call by call.  There are
+no gradients: what comes out is not connected to what went in.
 """
 import ctypes as C
 import math

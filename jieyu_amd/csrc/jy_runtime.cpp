@@ -1578,6 +1578,13 @@ struct Session {
         return made;
     }
 
+    // whether a step of step_sampled() had nothing to pick from
+    bool drew_none() {
+        int v = 0;
+        CK(hipMemcpy(&v, m->state + 2, sizeof(int), hipMemcpyDeviceToHost));
+        return v != 0;
+    }
+
     // step() with the tokens drawn on the device from the given numbers
     int step_sampled(int n, int top_k, float top_p, float min_p, const float* u) {
         if (greedy) fail("step_sampled: the session is greedy (temperature <= 0)");
@@ -1626,22 +1633,23 @@ struct Session {
             launch_sample(A, st);
             launch_advance(m->ids, m->state, from + made, st);
             CK(hipGetLastError());
-            if (cb || neos > 0) accept(fetch_last());
+            if (cb || neos > 0) {
+                const int id = fetch_last();
+                if (drew_none()) break;
+                accept(id);
+            }
         }
-        if (!cb && neos == 0) {
+        if (!cb && neos == 0)
             CK(hipMemcpyAsync(ids.data() + from, m->ids + from, sizeof(int) * made, hipMemcpyDeviceToHost, st));
-            len += made;
-        }
         CK(hipEventRecord(ev[3], st));
         CK(hipStreamSynchronize(st));
         check_persist(m);
         if (logits_out) CK(hipMemcpy(logits_out, m->logits, sizeof(float) * m->V, hipMemcpyDeviceToHost));
-        int state[3];
-        CK(hipMemcpy(state, m->state, sizeof(state), hipMemcpyDeviceToHost));
-        if (state[2]) {
+        if (drew_none()) {  // (without a callback or an end token the call's tokens are not taken over)
             stopped = true;
             fail("step_sampled: a step's logits hold no number to pick from");
         }
+        if (!cb && neos == 0) len += made;
         float ms = 0.0f;
         CK(hipEventElapsedTime(&ms, ev[2], ev[3]));
         decode_ms += ms;

@@ -269,6 +269,25 @@ def test_sampled_steps_stop_and_refuse(jy):
     g.close()
 
 
+@pytest.mark.parametrize("eos", [None, [298]])
+def test_sampled_steps_without_any_number(jy, eos):
+    """a step whose logits are all NaN ends the session with an error, and gives no token"""
+    m = build(spec(QM.JY_F32))
+    np.asarray(m["lm"][1])[:] = np.nan
+    d, keep = QM.desc_of(m)
+    g = jy.GpuModel(d, 64)
+    prompt = QM.prompt_of(m, 6)
+    s = g.session(prompt, 9, temperature=1.0, eos=eos)
+    n, ids = len(s), s.ids().tolist()
+    if s.remaining:  # (the first token is the host's)
+        with pytest.raises(jy.JyError, match="no number"):
+            s.step_sampled(np.full(4, 0.5, np.float32), top_k=5)
+    assert s.remaining == 0 and len(s) == n and s.ids().tolist() == ids
+    assert s.step_sampled([0.5]) == 0
+    s.close()
+    g.close()
+
+
 def test_batched_loop_from_pages_to_tokens(jy):
     """the operators as a server uses them: a pass of all sequences, logits, a token for each by its own
     settings, the next pass; the run is the same twice, and a sequence alone draws the same tokens"""
