@@ -269,6 +269,34 @@ def test_sampled_steps_stop_and_refuse(jy):
     g.close()
 
 
+@pytest.mark.parametrize("wtype,mode", [(QM.JY_F32, 0), (QM.JY_Q8_0, 0), (QM.JY_Q8_0, 7)])
+def test_a_first_pass_of_one_row_and_passes_between_a_sessions_steps(jy, wtype, mode):
+    """a new model's first call is one row; a session whose workspace a longer pass replaces goes on
+    with the tokens it would have drawn"""
+    m = build(spec(wtype))
+    d, keep = QM.desc_of(m)
+    rng = np.random.default_rng(4)
+    X = rng.standard_normal((40, 256)).astype(np.float32)
+    u = rng.random(12).astype(np.float32)
+    prompt = QM.prompt_of(m, 6)
+    runs = []
+    for between in (False, True):
+        g = jy.GpuModel(d, 64)
+        g.mode = mode
+        p = jy.PagePool.empty(2, 6, 16, 2, 64, device=DEV)
+        tables = np.array([[4, 2, 0], [1, 5, 3]], np.int32)
+        near(g.forward_paged(p, X[:1], tables, [0]), Reference(m, "i8").token(0, 0, X[0])[None])
+        s = g.session(prompt, 13, temperature=1.0)
+        for i in range(0, 12, 4):
+            if between:
+                g.forward_paged(p, X[:13 + i], tables, np.arange(13 + i), np.ones(13 + i, np.int32))
+            assert s.step_sampled(u[i:i + 4], top_p=0.9) == 4
+        runs.append(s.ids().tolist())
+        s.close()
+        g.close()
+    assert runs[0] == runs[1]
+
+
 @pytest.mark.parametrize("eos", [None, [298]])
 def test_sampled_steps_without_any_number(jy, eos):
     """a step whose logits are all NaN ends the session with an error, and gives no token"""
