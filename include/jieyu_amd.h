@@ -292,7 +292,8 @@ typedef struct jyhip_vectors {
  * positions: row r is position pos[r] of sequence seq[r] (seq NULL: of sequence r).  A row whose
  * sequence or position does not exist (negative, past the table, a hole) is skipped: so the idle
  * rows of a padded batch have position -1.  The rows of one call are different positions; where
- * two name the same slot, that slot's contents are unspecified. */
+ * two name the same slot, that slot's contents are unspecified.  rows x num_kv_heads is less than
+ * 2^28. */
 JYHIP_API int jyhip_pages_write(const jyhip_pages* pages, const jyhip_page_tables* tables, int rows, const int* seq,
                                 const int* pos, const jyhip_vectors* k, const jyhip_vectors* v, int type,
                                 void* stream);
@@ -329,7 +330,7 @@ JYHIP_API size_t jyhip_pages_attend_workspace(const jyhip_pages* pages, int num_
  * A logit that is NaN or -infinity is never picked; a row of nothing else gives -1.  With +infinity
  * among the logits, those alone have mass.  Each of temperature, top_k, top_p and min_p may be
  * NULL: 1, off, off, off.  u outside [0, 1) counts as the nearest value in it, NaN as 0.  vocab is
- * at most 2^22.  The workspace needs jyhip_sample_workspace() bytes, aligned to 16. */
+ * at most 2^22, rows less than 2^20.  The workspace needs jyhip_sample_workspace() bytes, aligned to 16. */
 JYHIP_API int jyhip_sample(const void* logits, int type, int rows, int vocab, long long row_stride, const float* u,
                            const float* temperature, const int* top_k, const float* top_p, const float* min_p,
                            int* ids, void* workspace, size_t workspace_bytes, int device, void* stream);

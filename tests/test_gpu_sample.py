@@ -122,6 +122,26 @@ def test_large_top_k_with_ties_at_the_border(jy, io, step):
         check(jy, x, u, settings)
 
 
+@pytest.mark.parametrize("io,rows", [("f32", 2), ("bf16", 2), ("bf16", 600), ("f16", 70)])
+def test_the_longest_rows(jy, io, rows):
+    """2^22 logits, by 64 workgroups a row and by as few as there may be"""
+    V = 1 << 22
+    g = torch.Generator(device=DEV)
+    g.manual_seed(rows)
+    x = torch.empty((rows, V), dtype=IO[io], device=DEV).normal_(0.0, 3.0, generator=g)
+    u = torch.rand(rows, generator=g, device=DEV)
+    settings = [(1.0, 0, 0.9375, 0.0), (0.75, 50, 1.0, 0.0), (1.0, 0, 1.0, 0.0), (1.5, 0, 1.0, 0.03125), (0.5, 1000, 0.5, 0.0), (1.0, 5000, 0.875, 0.0)]
+    at = sorted({0, rows - 1})
+    for i in range(0, len(settings), len(at)):
+        mine = [settings[(r + i) % len(settings)] for r in range(rows)]
+        T, k, p, m = (list(c) for c in zip(*mine))
+        f = lambda v, t=torch.float32: torch.tensor(v, dtype=t, device=DEV)  # noqa: E731
+        got = jy.sample(x, u, f(T), f(k, torch.int32), f(p), f(m)).cpu()
+        for r in at:
+            want = pick64(x[r].cpu(), float(u[r]), *mine[r])
+            assert int(got[r]) in want, f"row {r}, settings {mine[r]}: {int(got[r])}, not {want}"
+
+
 def test_all_equal(jy):
     for V in (1, 64, 9001, 152064):
         check(jy, torch.zeros(len(SETTINGS), V), torch.rand(len(SETTINGS)), SETTINGS)
