@@ -308,7 +308,7 @@ JYHIP_API int jyhip_pages_read(const jyhip_pages* pages, const jyhip_page_tables
  * softmax and sums are held in fp32.  A sequence without any position (lens[s] <= 0, only holes)
  * gives zeros.  max_len, at most 2^30, is an upper bound of lens known on the host: it sizes the launch,
  * and a longer lens[s] is cut to it.  The workspace needs jyhip_pages_attend_workspace() bytes, aligned
- * to 16. */
+ * to 16 (0 bytes, too, for arguments that jyhip_pages_attend refuses). */
 JYHIP_API int jyhip_pages_attend(const jyhip_pages* pages, const jyhip_page_tables* tables, const int* lens,
                                  int max_len, int num_heads, float scale, const jyhip_vectors* q,
                                  const jyhip_vectors* out, int type, void* workspace, size_t workspace_bytes,

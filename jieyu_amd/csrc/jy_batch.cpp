@@ -108,6 +108,7 @@ JYHIP_API int jyhip_pages_read(const jyhip_pages* pages, const jyhip_page_tables
 
 JYHIP_API size_t jyhip_pages_attend_workspace(const jyhip_pages* pages, int num_seqs, int num_heads, int max_len) {
     if (!pages || num_seqs < 1 || num_heads < 1 || pages->num_kv_heads < 1 || max_len < 1 || max_len > MAX_LEN) return 0;
+    if (num_heads % pages->num_kv_heads || pages->head_dim < 16 || pages->head_dim > 256) return 0;
     return paged_attend_part_floats(*pages, num_seqs, num_heads, max_len) * sizeof(float);
 }
 

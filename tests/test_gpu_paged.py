@@ -508,3 +508,12 @@ def test_on_other_streams(jy):
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(x, want[i]) for x in got[i])
+
+
+@pytest.mark.parametrize("max_len", [40, 3000])
+def test_attend_refuses_heads_at_any_length(jy, max_len):
+    """query heads that are no multiple of the key/value heads, fewer of them among those"""
+    c = Cache(jy, [40], 4, 64, 16, "i8", seed=33)
+    for heads in (1, 2, 3, 6):
+        with pytest.raises(jy.JyError, match="multiple"):
+            c.attend(torch.zeros((1, heads, 64), device=DEV), max_len=max_len)

@@ -110,3 +110,15 @@ def test_pool_wants_device_tensors():
     x = torch.zeros((1, 2, 2, 16, 64), dtype=torch.int8)
     with pytest.raises(jieyu_amd.JyError, match="device tensors"):
         jieyu_amd.PagePool(x, x, torch.zeros(1, 2, 2, 16), torch.zeros(1, 2, 2, 16))
+
+
+@pytest.mark.parametrize("nkv,heads", [(4, 2), (4, 1), (8, 7), (4, 6), (3, 2)])
+@pytest.mark.parametrize("max_len", [1, 1000, 1025, 2000, 1 << 30])
+def test_workspace_of_heads_that_are_refused(b, nkv, heads, max_len):
+    """fewer query heads than key/value heads, or no multiple of them: no workspace at any length, and
+    attend says why"""
+    p = pages(num_kv_heads=nkv)
+    assert b.attend_workspace(p, 1, heads, max_len) == 0
+    assert attend(b, p=p, heads=heads, max_len=max_len, ws=None, bytes=0) == -1 and "multiple" in error(b)
+    for hd in (0, -16, 272):
+        assert b.attend_workspace(pages(head_dim=hd), 1, 4, max_len) == 0
