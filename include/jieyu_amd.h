@@ -292,8 +292,8 @@ typedef struct jyhip_vectors {
  * positions: row r is position pos[r] of sequence seq[r] (seq NULL: of sequence r).  A row whose
  * sequence or position does not exist (negative, past the table, a hole) is skipped: so the idle
  * rows of a padded batch have position -1.  The rows of one call are different positions; where
- * two name the same slot, that slot's contents are unspecified.  rows x num_kv_heads is less than
- * 2^28. */
+ * two name the same slot, that slot's contents are unspecified.  rows x num_kv_heads is at most
+ * 2^28 - 16. */
 JYHIP_API int jyhip_pages_write(const jyhip_pages* pages, const jyhip_page_tables* tables, int rows, const int* seq,
                                 const int* pos, const jyhip_vectors* k, const jyhip_vectors* v, int type,
                                 void* stream);

@@ -33,6 +33,11 @@ void jy::check_pages(const jyhip_pages* p) {
     }
 }
 
+void jy::check_moved_size(int rows, int num_kv_heads) {
+    // 16 threads a (row, head) in workgroups of 256, and a launch has less than 2^32 threads
+    if ((int64_t)rows * num_kv_heads > (1 << 28) - 16) fail("rows x heads is too large for one call");
+}
+
 namespace {
 
 constexpr int MAX_LEN = 1 << 30;  // (a position plus a chunk is an int in the kernels)
@@ -64,8 +69,7 @@ bool check_moved(const jyhip_pages* p, const jyhip_page_tables* t, int rows, con
     if (!seq && rows > t->num_seqs) fail("without seq there is one row per sequence: more rows than sequences");
     check_vectors(k, type, "k");
     check_vectors(v, type, "v");
-    // 16 threads a (row, head), under 2^32 threads a launch
-    if ((int64_t)rows * p->num_kv_heads >= 1 << 28) fail("rows x heads is too large for one call");
+    check_moved_size(rows, p->num_kv_heads);
     return true;
 }
 

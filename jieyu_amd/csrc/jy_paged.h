@@ -10,6 +10,8 @@ namespace jy {
 
 // throws jy::Error where the kernels cannot run on these pages
 void check_pages(const jyhip_pages* p);
+// throws jy::Error where rows x heads is more than one launch of launch_paged_write / _read takes
+void check_moved_size(int rows, int num_kv_heads);
 
 // which position each row is, and where it lies (jyhip_page_tables with the rows' indices)
 struct PageMap {

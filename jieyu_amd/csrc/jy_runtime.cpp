@@ -1785,9 +1785,8 @@ int forward_paged(jyhip_model* m, const jyhip_pages* pages, const float* X, floa
         const int* t = tables + (size_t)(seq ? seq[r] : r) * table_stride;
         h.insert(h.end(), t, t + table_stride);
     }
-    if (paged_attend_blocks(pages[0], rows, m->nh, max_len) >= (1 << 24) ||
-        (int64_t)rows * m->nkv >= 1 << 28)
-        fail("forward_paged: too many rows for one call");
+    if (paged_attend_blocks(pages[0], rows, m->nh, max_len) >= (1 << 24)) fail("forward_paged: too many rows for one call");
+    check_moved_size(rows, m->nkv);
     const OnDevice on(m->device, nullptr);
     ensure_ws(m, rows);
     const size_t part = paged_attend_part_floats(pages[0], rows, m->nh, max_len);

@@ -122,3 +122,11 @@ def test_workspace_of_heads_that_are_refused(b, nkv, heads, max_len):
     assert attend(b, p=p, heads=heads, max_len=max_len, ws=None, bytes=0) == -1 and "multiple" in error(b)
     for hd in (0, -16, 272):
         assert b.attend_workspace(pages(head_dim=hd), 1, 4, max_len) == 0
+
+
+@pytest.mark.parametrize("fn", ["write", "read"])
+@pytest.mark.parametrize("nkv,rows", [(1, (1 << 28) - 15), (1, 1 << 28), (2, (1 << 27) - 7), (8, (1 << 25) - 1), (3, 89478481)])
+def test_rows_past_one_launch(b, fn, nkv, rows):
+    """more than 2^28 - 16 rows x heads, 16 threads each, would be 2^32 threads"""
+    assert move(b, fn, p=pages(num_kv_heads=nkv), rows=rows, seq=0x70000) == -1
+    assert "too large" in error(b)
