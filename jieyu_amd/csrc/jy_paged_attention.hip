@@ -380,8 +380,8 @@ struct State {
             if constexpr (PT == JYHIP_T_I8) {
                 vtop = head_max(vtop);
                 if (vtop > vref) {  // (the same in every lane)
-                    // the power of two over vtop, within [2^-120, 2^126]
-                    const int e = min(max((int)(__builtin_bit_cast(uint32_t, vtop) >> 23) - 126, -120), 126);
+                    // the power of two over vtop, within [2^-112, 2^126] (2^15 over it has to be finite)
+                    const int e = min(max((int)(__builtin_bit_cast(uint32_t, vtop) >> 23) - 126, -112), 126);
                     const float next = __builtin_ldexpf(1.0f, e);
                     vinv = __builtin_ldexpf(1.0f, 15 - e);
                     a *= vref * __builtin_ldexpf(1.0f, -e);

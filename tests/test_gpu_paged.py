@@ -517,3 +517,20 @@ def test_attend_refuses_heads_at_any_length(jy, max_len):
     for heads in (1, 2, 3, 6):
         with pytest.raises(jy.JyError, match="multiple"):
             c.attend(torch.zeros((1, heads, 64), device=DEV), max_len=max_len)
+
+
+@pytest.mark.parametrize("size", [1e-33, 1e-34, 1e-36])
+def test_attend_value_scales_down_to_the_smallest(jy, size):
+    """value scales of any size, those far under 2^-112 among them.  There a weight times its scale counts
+    in steps of 2^-24 2^-127 (the smallest half, times the largest power of two that fp32 holds) instead of
+    2^-39 of the largest: each of the n products is off by at most that times a byte of 127, over a sum of
+    weights of at least 1; and fp32's own steps down there are 2^-149, once per product and for the output."""
+    c = Cache(jy, [100], 1, 64, 16, "i8", seed=11)
+    vs = c.vs * size
+    pool = jy.PagePool(c.pool.k, c.pool.v, c.pool.k_scale, vs.to(DEV))
+    at = c.tables[0].long()
+    v = (c.vq.double() * vs.double()[..., None])[c.layer, at].permute(1, 0, 2, 3).reshape(1, -1, 64)[:, :100].permute(1, 0, 2)
+    q = torch.randn((1, 4, 64), generator=gen(3))
+    got = pool.attend(c.layer, q.to(DEV), c.dtables, c.dlens, 100)
+    want, bound = attention64(q, c.k, [v], 0.125)
+    check(got, want, bound + 100 * 127 * 2.0**-151 + 101 * 2.0**-149)
