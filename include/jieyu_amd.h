@@ -305,10 +305,10 @@ JYHIP_API int jyhip_pages_read(const jyhip_pages* pages, const jyhip_page_tables
 /* Attention of one query row per sequence over the first lens[s] positions of every sequence s of
  * `tables`: out[s][h] = sum_j softmax_j(scale q[s][h] . k_j) v_j, head h reading kv head
  * h / (num_heads / num_kv_heads).  q and out are of `type` (JYHIP_T_F32, _F16, _BF16); scores,
- * softmax and sums are held in fp32.  A sequence without any position (lens[s] <= 0, only holes)
- * gives zeros.  max_len, at most 2^30, is an upper bound of lens known on the host: it sizes the launch,
- * and a longer lens[s] is cut to it.  The workspace needs jyhip_pages_attend_workspace() bytes, aligned
- * to 16 (0 bytes, too, for arguments that jyhip_pages_attend refuses). */
+ * softmax and sums are held in fp32 (against int8 keys a query vector under 2^-104 counts as zeros).  A
+ * sequence without any position (lens[s] <= 0, only holes) gives zeros.  max_len, at most 2^30, is an upper
+ * bound of lens known on the host: it sizes the launch, and a longer lens[s] is cut to it.  The workspace
+ * needs jyhip_pages_attend_workspace() bytes, aligned to 16 (0 for arguments that are refused). */
 JYHIP_API int jyhip_pages_attend(const jyhip_pages* pages, const jyhip_page_tables* tables, const int* lens,
                                  int max_len, int num_heads, float scale, const jyhip_vectors* q,
                                  const jyhip_vectors* out, int type, void* workspace, size_t workspace_bytes,

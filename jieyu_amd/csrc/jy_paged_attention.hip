@@ -163,7 +163,8 @@ template <int KC, bool WIDE>
 struct Query<JYHIP_T_I8, KC, WIDE> {
     i4_t q[KC][3];
     __device__ __forceinline__ void load(const float* x, float amax) {  // x: KC x 16 elements of this lane
-        const float inv = amax > 0.0f ? 8323072.0f / amax : 0.0f;       // 127 * 65536
+        // 127 * 65536 over the largest, which is finite from 2^-104 on; a smaller query counts as zeros
+        const float inv = amax >= 0x1p-104f ? 8323072.0f / amax : 0.0f;
 #pragma unroll
         for (int c = 0; c < KC; c++) {
             uint32_t w[3][4] = {};

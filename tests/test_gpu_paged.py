@@ -534,3 +534,16 @@ def test_attend_value_scales_down_to_the_smallest(jy, size):
     got = pool.attend(c.layer, q.to(DEV), c.dtables, c.dlens, 100)
     want, bound = attention64(q, c.k, [v], 0.125)
     check(got, want, bound + 100 * 127 * 2.0**-151 + 101 * 2.0**-149)
+
+
+@pytest.mark.parametrize("size", [1e-30, 1e-31, 1e-33, 1e-38, 1e-42])
+def test_attend_queries_down_to_the_smallest(jy, size):
+    """a query under 2^-104 against int8 keys counts as zeros, however large the keys (the row is a mean);
+    above that it does not"""
+    c = Cache(jy, [100], 1, 64, 16, "i8", seed=11)
+    pool = jy.PagePool(c.pool.k, c.pool.v, (c.ks * 2.0**100).to(DEV), c.pool.v_scale)
+    q = torch.randn((1, 4, 64), generator=gen(3)) * size
+    got = pool.attend(c.layer, q.to(DEV), c.dtables, c.dlens, 100)
+    if q.abs().max() < 2.0**-104:
+        q.zero_()
+    check(got, *attention64(q, [x * 2.0**100 for x in c.k], c.v, 0.125))
