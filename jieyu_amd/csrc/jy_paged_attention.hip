@@ -275,7 +275,10 @@ struct Tile {
 };
 
 // Loads of 16 positions go through a buffer resource over just those that exist: the ones that do not
-// (past the sequence's end, in a hole) read as zeros and are not fetched.
+// (past the sequence's end, in a hole) read as zeros and are not fetched.  So do the lanes past the
+// head's end, at an offset behind any resource: another dim's key in their place, against a query of
+// zero, would make NaN of an infinity.
+constexpr unsigned kNowhere = 1u << 30;
 template <int PT, int NC>
 struct Loader {
     typedef Tile<PT, NC> T;
@@ -541,15 +544,13 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void paged_attend_kernel(Attn
     ld.row_bytes = hd * ES;
 #pragma unroll
     for (int c = 0; c < T::KC; c++) {
-        int d = c * 4 * STEP + (lane >> 4) * STEP;
-        if (d >= hd) d = 0;  // (past the head's end the query is zero)
-        ld.koff[c] = (unsigned)(((lane & 15) * hd + d) * ES);
+        const int d = c * 4 * STEP + (lane >> 4) * STEP;
+        ld.koff[c] = d < hd ? (unsigned)(((lane & 15) * hd + d) * ES) : kNowhere;
     }
     {
-        int d = (lane & 15) * DL;
-        if (d >= hd) d = 0;  // (outputs past the head's end are not stored)
+        const int d = (lane & 15) * DL;  // (outputs past the head's end are not stored)
 #pragma unroll
-        for (int j = 0; j < 4; j++) ld.voff[j] = (unsigned)((((lane >> 4) * 4 + j) * hd + d) * ES);
+        for (int j = 0; j < 4; j++) ld.voff[j] = d < hd ? (unsigned)((((lane >> 4) * 4 + j) * hd + d) * ES) : kNowhere;
     }
     const int end = min(n, c0 + K.plan.chunk);
     const int ntiles = end > c0 ? (end - c0 + 31) / 32 : 0;

@@ -547,3 +547,22 @@ def test_attend_queries_down_to_the_smallest(jy, size):
     if q.abs().max() < 2.0**-104:
         q.zero_()
     check(got, *attention64(q, [x * 2.0**100 for x in c.k], c.v, 0.125))
+
+
+# ---------------------------------------------------------------- infinities in 16-bit pools
+
+@pytest.mark.parametrize("hd", [16, 32, 48, 80, 96, 112, 144, 192, 240])
+@pytest.mark.parametrize("pool", ["f16", "bf16"])
+def test_attend_infinite_keys_of_any_head_size(jy, pool, hd):
+    """a key's infinity in any of its dims, against the query's sign: that position has no weight, and the
+    row is the others'"""
+    n = 60
+    c = Cache(jy, [n], 1, hd, 16, pool, seed=43, layers=1, layer=0)
+    q = torch.ones((1, 2, hd), dtype=POOL[pool])
+    live = torch.ones(n, dtype=torch.bool)
+    for p in range(0, n, 3):
+        c.pool.k[0, int(c.tables[0, p // 16]), 0, p % 16, (p // 3 * 5) % hd] = -math.inf
+        live[p] = False
+    got = c.attend(q.to(DEV))
+    # (a weight of 0 and what stands beside it add nothing: the bound is the others')
+    check(got, *attention64(q, [c.k[0][live]], [c.v[0][live]], 1 / math.sqrt(hd)))
