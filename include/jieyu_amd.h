@@ -308,7 +308,14 @@ JYHIP_API int jyhip_pages_read(const jyhip_pages* pages, const jyhip_page_tables
  * softmax and sums are held in fp32 (against int8 keys a query vector under 2^-104 counts as zeros).  A
  * sequence without any position (lens[s] <= 0, only holes) gives zeros.  max_len, at most 2^30, is an upper
  * bound of lens known on the host: it sizes the launch, and a longer lens[s] is cut to it.  The workspace
- * needs jyhip_pages_attend_workspace() bytes, aligned to 16 (0 for arguments that are refused). */
+ * needs jyhip_pages_attend_workspace() bytes, aligned to 16 (0 for arguments that are refused).
+ *
+ * What is not finite: a query vector with an infinity or a NaN gives NaN.  A score of -infinity has no
+ * weight (a row of nothing else gives zeros), one of +infinity or NaN makes its row NaN, and a value that is
+ * not finite is so in its dim of every row that reads it, NaN where its weight is 0.  There a query's
+ * element under 2^-39 of its vector's largest and a weight under 2^-39 of its row's largest may count as
+ * 0.  Int8 scales are finite or NaN.  Scores of 2^127 and more, and sums of weights (the largest 1) times
+ * values past fp32's range, are infinite. */
 JYHIP_API int jyhip_pages_attend(const jyhip_pages* pages, const jyhip_page_tables* tables, const int* lens,
                                  int max_len, int num_heads, float scale, const jyhip_vectors* q,
                                  const jyhip_vectors* out, int type, void* workspace, size_t workspace_bytes,

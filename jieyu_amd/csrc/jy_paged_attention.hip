@@ -13,7 +13,8 @@
 //        heads as the columns.  int8 keys stay int8: the query is split into three base-256
 //        digits relative to its largest element (23 bits), each digit's dot an exact int32 on
 //        mfma_i32_16x16x64_i8.  fp16 keys take the query as two fp16 parts, bf16 keys as three
-//        bf16 parts, accumulated in fp32.
+//        bf16 parts, accumulated in fp32; so split that an infinite key gives the score that the
+//        whole query would.
 //   p.v  o^T = V^T p^T: the weights come out of the first product in the very layout the second
 //        takes as its B operand (lane: head l & 15, keys 4 (l >> 4) + i of two 16-key groups), so
 //        they change no lane.  V is read row by row, lane l holding DL consecutive dims from
@@ -22,7 +23,7 @@
 //        (their bytes read as subnormal halves, one packed fma gives (u - 128) / 512); a weight
 //        times its value scale is carried as two fp16 parts (21 bits, relative to the running
 //        maximum and to a power of two over the value scales seen), for bf16 values as three
-//        bf16 parts.
+//        bf16 parts, none of them 0 beside a first one that is not: 0 times an infinite value is NaN.
 //
 // A workgroup's four waves take the tiles of one chunk of a sequence in turn and join through
 // LDS; chunks are joined by a second kernel where there is more than one.
@@ -153,6 +154,17 @@ __device__ __forceinline__ float bf16_cut(float a) {
     return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, a) & 0xffff0000u);
 }
 
+// the smaller / larger of two pairs of 16-bit numbers: of halves or bf16 that are not negative, too.
+// The second and third parts of a weight are at least the type's smallest number wherever the first is not
+// 0, so that an infinite value times them is that infinity and not NaN.
+typedef unsigned short s2_t __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t min16(uint32_t a, uint32_t b) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(s2_t, a), __builtin_bit_cast(s2_t, b)));
+}
+__device__ __forceinline__ uint32_t max16(uint32_t a, uint32_t b) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(s2_t, a), __builtin_bit_cast(s2_t, b)));
+}
+
 // The query of 16 heads as B operands of q.k, and the factor that turns their products into
 // scores.  Without WIDE one 16-bit operand holds the query (fp16 or bf16 ones against fp16 keys:
 // scaled, they lose only what lies 2^-40 below the largest element; bf16 ones against bf16 keys).
@@ -214,15 +226,22 @@ struct Query<JYHIP_T_F16, KC, WIDE> {
             }
     }
     static __device__ __forceinline__ float factor(float amax) { return __builtin_ldexpf(1.0f, -exponent(amax)); }
+    // An infinite key: the first parts' product says which infinity (or NaN), the second ones', of any sign or
+    // 0, have no say.
     __device__ __forceinline__ void dot(const i4_t (&k)[KC], float (&s)[4]) const {
-        f4_t d = {};
+#if defined(__HIP_DEVICE_COMPILE__)
+        f4_t d[PARTS] = {};
 #pragma unroll
         for (int p = PARTS - 1; p >= 0; p--)
 #pragma unroll
             for (int c = 0; c < KC; c++)
-                d = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, k[c]), q[c][p], d, 0, 0, 0);
+                d[p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, k[c]), q[c][p], d[p], 0, 0, 0);
 #pragma unroll
-        for (int i = 0; i < 4; i++) s[i] = d[i];
+        for (int i = 0; i < 4; i++) {
+            s[i] = d[0][i];
+            if constexpr (WIDE) s[i] += __builtin_amdgcn_fmed3f(d[1][i], -3.402823466e38f, 3.402823466e38f);
+        }
+#endif
     }
 };
 
@@ -243,6 +262,11 @@ struct Query<JYHIP_T_BF16, KC, WIDE> {
                     a -= bf16_cut(a);
                     b -= bf16_cut(b);
                 }
+                // parts of one sign, none of them 0 where the first is not: an infinite key times 0 would be NaN
+                const uint32_t sign = w[0][e >> 1] & 0x80008000u;
+                const uint32_t least = min16(w[0][e >> 1] & 0x7fff7fffu, 0x00800080u) | sign;
+#pragma unroll
+                for (int p = 1; p < PARTS; p++) w[p][e >> 1] = max16(w[p][e >> 1] | sign, least);
             }
 #pragma unroll
             for (int p = 0; p < PARTS; p++) q[c][p] = __builtin_bit_cast(b8_t, u4_t{w[p][0], w[p][1], w[p][2], w[p][3]});
@@ -422,6 +446,7 @@ struct State {
                     w[c][j >> 1] = bf16_pair(p[j], p[j + 1]);
                     p[j] -= bf16_cut(p[j]);
                     p[j + 1] -= bf16_cut(p[j + 1]);
+                    if (c) w[c][j >> 1] = max16(w[c][j >> 1], min16(w[0][j >> 1], 0x00800080u));
                 }
             b8_t pb[3];
 #pragma unroll
@@ -441,8 +466,15 @@ struct State {
                                                           __builtin_fmaf((float)a[1], -1.0f, p[j + 1]));
                 hi[j] = (_Float16)a[0];
                 hi[j + 1] = (_Float16)a[1];
-                lo[j] = (_Float16)b[0];
-                lo[j + 1] = (_Float16)b[1];
+                if constexpr (PT == JYHIP_T_F16) {
+                    const uint32_t c = max16(__builtin_bit_cast(uint32_t, b), min16(__builtin_bit_cast(uint32_t, a), 0x00010001u));
+                    const h2_t d = __builtin_bit_cast(h2_t, c);
+                    lo[j] = d.x;
+                    lo[j + 1] = d.y;
+                } else {
+                    lo[j] = (_Float16)b[0];
+                    lo[j + 1] = (_Float16)b[1];
+                }
             }
 #pragma unroll
             for (int d = 0; d < DL; d++) {
@@ -545,7 +577,9 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void paged_attend_kernel(Attn
 #pragma unroll
     for (int c = 0; c < T::KC; c++) {
         const int d = c * 4 * STEP + (lane >> 4) * STEP;
-        ld.koff[c] = d < hd ? (unsigned)(((lane & 15) * hd + d) * ES) : kNowhere;
+        // (the first half is inside any head of this form: one register and offsets in the loads)
+        const bool in = (NC > 1 && (c + 1) * 4 * STEP <= 32 * NC) || d < hd;
+        ld.koff[c] = in ? (unsigned)(((lane & 15) * hd + d) * ES) : kNowhere;
     }
     {
         const int d = (lane & 15) * DL;  // (outputs past the head's end are not stored)

@@ -566,3 +566,98 @@ def test_attend_infinite_keys_of_any_head_size(jy, pool, hd):
     got = c.attend(q.to(DEV))
     # (a weight of 0 and what stands beside it add nothing: the bound is the others')
     check(got, *attention64(q, [c.k[0][live]], [c.v[0][live]], 1 / math.sqrt(hd)))
+
+
+def attention_of_infinities(q, k, v, scale):
+    """(out, bound) of one sequence's definition in 64 bits with infinities among keys and values:
+    a score of -infinity has no weight (all of them: zeros), one of +infinity or NaN makes its row NaN,
+    a value that is not finite its dim of the rows whose head reads it.  (No position here has both.)"""
+    nh, hd = q.shape
+    per = nh // k.shape[1]
+    out, bound = torch.empty(nh, hd, dtype=torch.float64), torch.zeros(nh, hd, dtype=torch.float64)
+    for h in range(nh):
+        kk, vv = k[:, h // per], v[:, h // per]
+        s = (kk * q[h].double()).sum(-1) * scale
+        live = s != -math.inf
+        if not torch.isfinite(s[live]).all():
+            out[h] = math.nan
+            continue
+        if not live.any():
+            out[h] = 0.0
+            continue
+        kk, vv = kk[live][:, None], vv[live][:, None]
+        a, b = attention64(q[None, h:h + 1], [kk], [torch.nan_to_num(vv, nan=0.0, posinf=0.0, neginf=0.0)], scale)
+        inf = torch.where(torch.isfinite(vv), torch.zeros_like(vv), vv).sum((0, 1))  # (opposite ones: NaN)
+        out[h], bound[h] = a[0, 0] + inf, b[0, 0]
+    return out, bound
+
+
+def check_infinities(got, want, bound):
+    got = got.double().cpu()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    inf = torch.isinf(want)
+    assert torch.equal(torch.isinf(got), inf) and torch.equal(got[inf], want[inf])
+    return ~(torch.isnan(want) | inf)
+
+
+@pytest.mark.parametrize("n", [40, 700, 3000])
+@pytest.mark.parametrize("hd", [64, 80, 112, 128, 256])
+@pytest.mark.parametrize("io", list(IO))
+@pytest.mark.parametrize("pool", ["f16", "bf16"])
+def test_attend_infinities_in_16_bit_pages(jy, pool, io, hd, n):
+    """infinite keys and values, as fp32 rows past a 16-bit type's range are held, whatever the query's type
+    and the head size: whole numbers as queries, which need no second part"""
+    c = Cache(jy, [n, 33, 20], 2, hd, 16, pool, seed=40, layers=1, layer=0, outliers=False)
+    g = gen(41)
+    q = torch.randint(1, 4, (3, 4, hd), generator=g).float() * (torch.randint(0, 2, (3, 4, hd), generator=g) * 2 - 1)
+    q[:, 2:] += torch.rand((3, 2, hd), generator=g) * 0.9  # (and others)
+    q = q.to(IO[io])
+
+    def put(which, b, p, head, d, x):
+        getattr(c.pool, which)[0, int(c.tables[b, p // 16]), head, p % 16, d] = x
+        getattr(c, which)[b][p, head, d] = x
+
+    # a key against the sign of head 0's query, so the position has no weight there
+    for p, d in ((0, 0), (1, hd - 1), (17, 5), (n - 1, hd // 2)):
+        put("k", 0, p, 0, d, -math.inf * float(torch.sign(q[0, 0, d].float())))
+        q[0, 1, d] = q[0, 0, d]
+    # values: one dim of each sign, one with both
+    for p, d, x in ((3, 0, math.inf), (n - 2, 9, -math.inf), (5, hd - 1, math.inf), (30, hd - 1, -math.inf)):
+        put("v", 0, p, 0, d, x)
+    # a key along the query of head 2 (kv head 1): its row is NaN; head 3 by its own sign
+    put("k", 0, 6, 1, 2, math.inf * float(torch.sign(q[0, 2, 2].float())))
+    # an infinity that meets a zero, and a held NaN
+    q[1, 0, 7] = 0.0
+    put("k", 1, 4, 0, 7, math.inf)
+    put("v", 1, 32, 1, 3, math.nan)
+    # every score -infinity: zeros
+    for p in range(20):
+        put("k", 2, p, 0, 1, -math.inf)
+    q[2, :2, 1] = 1.0
+    scale = 0.25 / math.sqrt(hd)
+    got = c.attend(q.to(DEV), scale=scale)
+    want, bound = (torch.stack(x) for x in zip(*[attention_of_infinities(q[b], c.k[b], c.v[b], scale) for b in range(3)]))
+    ok = check_infinities(got, want, bound)
+    zero = torch.zeros((), dtype=torch.float64)
+    check(torch.where(ok.to(DEV), got, zero.to(got.dtype).to(DEV)), torch.where(ok, want, zero), bound)
+    assert not got[2, :2].any() and torch.isfinite(got[2, 2:]).all()
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+def test_rows_past_fp16s_range_from_write_to_attention(jy, io):
+    """written to an fp16 pool they are held as infinities, and attention takes them as such"""
+    c = Cache(jy, [40], 1, 80, 16, "f16", seed=42, layers=1, layer=0)
+    k, v = torch.randn((1, 1, 80), generator=gen(1)), torch.randn((1, 1, 80), generator=gen(2))
+    k[0, 0, 3], v[0, 0, 70] = -1e5, 7e4
+    pos = torch.tensor([21], dtype=torch.int32, device=DEV)
+    c.pool.write(0, k.to(IO[io]).to(DEV), v.to(IO[io]).to(DEV), c.dtables, pos)
+    c.k[0][21], c.v[0][21] = held(k.to(IO[io]), "f16")[0], held(v.to(IO[io]), "f16")[0]
+    assert c.k[0][21, 0, 3] == -math.inf and c.v[0][21, 0, 70] == math.inf
+    q = torch.ones((1, 2, 80)).to(IO[io])
+    q[0, 1, 3] = -1.0
+    got = c.attend(q.to(DEV), scale=0.05)
+    # head 0's score there is -infinity: its weight, 0, times the infinite value is NaN, the rest is finite
+    want, bound = attention_of_infinities(q[0], c.k[0], c.v[0], 0.05)
+    want[0, 70] = math.nan
+    check_infinities(got[0], want, bound)
+    assert torch.isnan(got[0, 1]).all() and torch.isfinite(got[0, 0, :70]).all()
