@@ -345,3 +345,47 @@ def test_batched_loop_from_pages_to_tokens(jy):
     assert np.array_equal(a, run([0, 1, 2]))
     assert (a >= 0).all() and (a < 300).all()
     g.close()
+
+
+@pytest.mark.parametrize("wtype,mode", [(QM.JY_F32, 0), (QM.JY_Q8_0, 0), (QM.JY_Q8_0, 7)])
+def test_a_sequence_of_a_batch_and_alone(jy, wtype, mode):
+    """each sequence of a batched loop run by itself, fed the batch's tokens: the same states (to the
+    products' rounding, which may go by the number of rows), and the batch's token is among those that
+    its own state and settings allow; so no row reads another's table, settings or random number"""
+    m = build(spec(wtype))
+    d, keep = QM.desc_of(m)
+    g = jy.GpuModel(d, 64)
+    g.mode = mode
+    rng = np.random.default_rng(6)
+    E = rng.standard_normal((300, 256)).astype(np.float32)
+    W = (rng.standard_normal((256, 300)) / 8).astype(np.float32)
+    head = torch.from_numpy(W).to(DEV)
+    T, P, mp, top_k = [0.0, 0.9, 1.2], [0.5, 0.95, 1.0], [0.0, 0.05, 0.0], [0, 30, 0]
+    settings = [torch.tensor(v, device=DEV) for v in (T, P, mp)]
+    ks = torch.tensor(top_k, dtype=torch.int32, device=DEV)
+    prompts = [[5, 6, 7, 8, 9], [10], [11, 12, 13]]
+    n = [len(p) for p in prompts]
+    tables = np.array([[7, 2, 5], [1, 9, 0], [8, 4, 3]], np.int32)
+    p = jy.PagePool.empty(2, 10, 16, 2, 64, device=DEV)
+    seq = [s for s in range(3) for _ in range(n[s])]
+    h = g.forward_paged(p, E[sum(prompts, [])], tables, [i for s in range(3) for i in range(n[s])], seq)[np.cumsum(n) - 1]
+    states, tokens, us = [], [], []
+    for t in range(14):
+        u = rng.random(3).astype(np.float32)
+        tok = jy.sample(torch.from_numpy(h).to(DEV) @ head, torch.from_numpy(u).to(DEV), settings[0], ks, *settings[1:]).cpu().numpy()
+        states.append(h), tokens.append(tok), us.append(u)
+        h = g.forward_paged(p, E[tok], tables, [a + t for a in n])
+    for s in range(3):
+        p = jy.PagePool.empty(2, 3, 16, 2, 64, device=DEV)
+        table = np.array([[1, 2, 0]], np.int32)
+        h = g.forward_paged(p, E[prompts[s]], table, np.arange(n[s]), np.zeros(n[s], np.int32))[-1:]
+        for t in range(14):
+            near(h, states[t][s:s + 1])
+            logits = (h[0].astype(np.float64) @ W).astype(np.float32)
+            tok = int(tokens[t][s])
+            if T[s] > 0:
+                assert tok in allowed(logits, float(us[t][s]), T[s], top_k[s], P[s], mp[s], 2e-3), (s, t)
+            else:
+                assert logits[tok] >= logits.max() - 2 * TOL * np.abs(logits).max(), (s, t)
+            h = g.forward_paged(p, E[[tok]], table, [n[s] + t])
+    g.close()
