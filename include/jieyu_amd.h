@@ -307,7 +307,8 @@ JYHIP_API int jyhip_pages_read(const jyhip_pages* pages, const jyhip_page_tables
  * h / (num_heads / num_kv_heads).  q and out are of `type` (JYHIP_T_F32, _F16, _BF16); scores,
  * softmax and sums are held in fp32 (against int8 keys a query vector under 2^-104 counts as zeros).  A
  * sequence without any position (lens[s] <= 0, only holes) gives zeros.  max_len, at most 2^30, is an upper
- * bound of lens known on the host: it sizes the launch, and a longer lens[s] is cut to it.  The workspace
+ * bound of lens known on the host: it sizes the launch, and a longer lens[s] is cut to it; a loose one costs
+ * some time, as it sizes the pieces that the sequences are taken in, too.  The workspace
  * needs jyhip_pages_attend_workspace() bytes, aligned to 16 (0 for arguments that are refused).
  *
  * What is not finite: a query vector with an infinity or a NaN gives NaN.  A score of -infinity has no
@@ -336,8 +337,9 @@ JYHIP_API size_t jyhip_pages_attend_workspace(const jyhip_pages* pages, int num_
  * at most 2^-40 of the largest mass), so a row's id does not depend on the order of additions.
  * A logit that is NaN or -infinity is never picked; a row of nothing else gives -1.  With +infinity
  * among the logits, those alone have mass.  Each of temperature, top_k, top_p and min_p may be
- * NULL: 1, off, off, off.  u outside [0, 1) counts as the nearest value in it, NaN as 0.  vocab is
- * at most 2^22, rows less than 2^20.  The workspace needs jyhip_sample_workspace() bytes, aligned to 16. */
+ * NULL: 1, off, off, off.  A NaN temperature counts as 0, a NaN top_p or min_p is off.  u outside [0, 1) counts
+ * as the nearest value in it, NaN as 0.  A row with a top_k from 1024 on (and below vocab) takes about ten
+ * times as long as others.  vocab is at most 2^22, rows less than 2^20.  The workspace needs jyhip_sample_workspace() bytes, aligned to 16. */
 JYHIP_API int jyhip_sample(const void* logits, int type, int rows, int vocab, long long row_stride, const float* u,
                            const float* temperature, const int* top_k, const float* top_p, const float* min_p,
                            int* ids, void* workspace, size_t workspace_bytes, int device, void* stream);
@@ -350,7 +352,8 @@ JYHIP_API size_t jyhip_sample_workspace(int rows, int vocab);
  * device, its heads the model's.  tables, seq and pos are HOST arrays here ([num_seqs][table_stride],
  * [rows], [rows]).  Each layer writes the rows' keys and values into the pages, then every row attends
  * over positions 0 .. pos[r] of its sequence, so several new positions of one sequence may come in one
- * call (a prompt) as long as the earlier ones are in the pages or in the call.
+ * call (a prompt) as long as the earlier ones are in the pages or in the call; each row reads its positions
+ * by itself, so a long prompt takes a time that grows with its square.
  * Refused before anything is enqueued: positions outside the RoPE table or the page table, page ids
  * outside the pool among those that a row attends over, two rows with the same slot.
  * The products are the model's (its mode's); the attention is jyhip_pages_attend's, which does not

@@ -5,9 +5,9 @@
 // lanes and its bytes leave as one contiguous run.  The lanes take the key and the value of a head
 // together: one look-up of the slot, two vectors in flight.  Every byte moves once; small calls are
 // bound by the launch and the look-up's chain (position, page id), large ones by memory:
-//   1 row of 2 heads of 64, fp32 to int8          2.7 us written, 2.1 read
-//   256 rows of 8 heads of 128, bf16 to int8      4.6 and 3.2
-//   8191 rows of the same (51 MB each way)        18.0 (2.8 TB/s) and 11.3 (4.5 TB/s)
+//   1 row of 2 heads of 64, fp32 to int8          2.6 us written, 1.9 read
+//   256 rows of 8 heads of 128, bf16 to int8      4.5 and 3.1
+//   8191 rows of the same (51 MB each way)        17.4 (2.9 TB/s) and 11.3 (4.5 TB/s)
 //   32770 rows of 4 heads of 128 read (101 MB)    20 (5.1 TB/s, some of it the infinity cache's)
 // Sixteen rows of one head a workgroup, so that a page's vectors leave side by side, measured 17.3 and
 // 11.1 us for the 8191 rows, but 3.2 and 2.5 for one: heads stay fastest.

@@ -28,10 +28,13 @@
 // A workgroup's four waves take the tiles of one chunk of a sequence in turn and join through
 // LDS; chunks are joined by a second kernel where there is more than one.
 //
-// 64 sequences of 200 to 8190 positions, 32 / 8 heads of 128, bf16 (591 MB): 112 to 133 us, 4.4 to 5.3 TB/s,
-// and 4.8 of join.  One of 32769, 28 / 4 heads, int8 (34.6 MB): 12.8 us, of them 5 for the bytes (a wave
-// per SIMD), and 5.3 of join.  32 of 1 to 1500, int8: 15 us, the chain of the longest chunk, and 3.9.  One of
-// 61 positions, 14 / 2 heads of 64: 4.8 us, the start, one step and the end.
+// 64 sequences of 200 to 8190 positions, 32 / 8 heads of 128, bf16 (591 MB): 112 to 160 us from launch to
+// launch, half of them within 136 (4.3 TB/s), and 4.8 of join.  One of 32769, 28 / 4 heads, int8 (34.6 MB):
+// 12.6 us, of them 5 for the bytes (a wave per SIMD), and 5.2 of join.  32 of 1 to 1500, int8: 14.2 us, the
+// chain of the longest chunk, and 3.9.  One of 61 positions, 14 / 2 heads of 64: 4.7 us, the start, one step
+// and the end.  fp32 queries cost more than 16-bit ones against 16-bit pools, in products and in registers
+// (some spilled from head size 128 on): 48 of 200 to 6000, 32 / 8 heads of 128, both kernels 128 us
+// against 89 in bf16, 102 against 89 in fp16.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

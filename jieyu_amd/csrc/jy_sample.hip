@@ -19,16 +19,18 @@
 //      into the list
 //   4  one workgroup per row: the border among the list's tokens, then the block and the token in
 //      it
-// A row whose candidates do not fit the list (k > 1024, or thousands of equal logits at the border)
-// is done by its workgroup in kernel 4 alone, by a radix descent over the logits' bits.
+// A row whose candidates do not fit the list (k > 1024, thousands of equal logits at the border, and many a
+// row with k = 1024, whose bound is the least of the parts' maxima) is done by its workgroup in kernel 4
+// alone, by a radix descent over the logits' bits: 64 rows of 128256, fp32, all passes: k = 50 30 us,
+// 500 40, 1000 43, 1024 490, 2000 580; one row 20, 28, 30, 420 and 410.
 //
-// Time of the kernels (1, 2, 3, 4), us: one row of 151936, fp32, k = 50: 3.8, 6.2, 1.7, 6.2: the launches
-// and each kernel's chain of loads and barriers.  64 rows of 128256, fp32, all kinds of settings: 8.9,
-// 13.8, 9.9, 17.2, the last for k = 1000: a step of a descent and an ordering for each border, two steps
+// Time of the kernels (1, 2, 3, 4), us: one row of 151936, fp32, k = 50: 3.8, 6.4, 1.7, 6.2: the launches
+// and each kernel's chain of loads and barriers.  64 rows of 128256, fp32, all kinds of settings: 8.5,
+// 14.5, 9.8, 17.1, the last for k = 1000: a step of a descent and an ordering for each border, two steps
 // for the token, each some barriers and waits for LDS.  256 rows of 152064, bf16, top-p 0.9: 17, 32,
-// 33, 16: the first is memory's time (4.5 TB/s); the next two have that and 10 us of start and end,
-// which no other workgroup's work covers as all are resident at once (with half of them at a time it
-// was more).
+// 33, 16: the first is memory's time (4.7 TB/s); the next two have that and 15 us more, their start
+// (the table, the cells or the border's bin) and end, which no other workgroup's work covers as all are
+// resident at once (with half of them at a time it was more).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
