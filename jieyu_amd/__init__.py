@@ -119,6 +119,16 @@ def _ptr(a):
     return None if a is None else a.ctypes.data_as(P)
 
 
+def _int32s(a, name):
+    """a as contiguous int32; refuses values that int32 does not hold, rather than wrapping or cutting them."""
+    a = np.asarray(a)
+    with np.errstate(invalid="ignore"):
+        out = np.ascontiguousarray(a, np.int32)
+    if a.dtype != np.int32 and not np.array_equal(out, a):
+        raise JyError(f"{name}: whole numbers that fit in 32 bits are needed")
+    return out
+
+
 def device_count():
     return lib().jyhip_device_count()
 
@@ -235,9 +245,8 @@ class GpuModel:
         if X.ndim != 2 or X.shape[1] != self.hidden:
             raise JyError(f"forward_paged: X must be [rows][{self.hidden}]")
         rows = X.shape[0]
-        tables = np.ascontiguousarray(tables, np.int32)
-        pos = np.ascontiguousarray(pos, np.int32)
-        seq = None if seq is None else np.ascontiguousarray(seq, np.int32)
+        tables, pos = _int32s(tables, "tables"), _int32s(pos, "pos")
+        seq = None if seq is None else _int32s(seq, "seq")
         if tables.ndim != 2 or pos.shape != (rows,) or (seq is not None and seq.shape != (rows,)):
             raise JyError("forward_paged: tables are [sequences][pages], pos and seq one for each row")
         out = np.empty(X.shape, np.float32)

@@ -130,3 +130,33 @@ def test_rows_past_one_launch(b, fn, nkv, rows):
     """more than 2^28 - 16 rows x heads, 16 threads each, would be 2^32 threads"""
     assert move(b, fn, p=pages(num_kv_heads=nkv), rows=rows, seq=0x70000) == -1
     assert "too large" in error(b)
+
+
+def paged_pass(**over):
+    """GpuModel.forward_paged of a model and a pool that only have their shapes: what it refuses before it
+    comes to a device."""
+    np = pytest.importorskip("numpy")
+    g = jieyu_amd.GpuModel.__new__(jieyu_amd.GpuModel)
+    g.h, g.num_layers, g.hidden = None, 1, 8
+    pool = type("Pool", (), dict(layers=1, device=None, _layers=[]))()
+    d = dict(tables=[[0, 1], [2, 3]], pos=[3, 4], seq=[0, 1])
+    d.update(over)
+    return g.forward_paged(pool, np.zeros((2, 8), np.float32), d["tables"], d["pos"], d["seq"])
+
+
+@pytest.mark.parametrize("name,value", [("pos", [3, 1 << 32]), ("pos", [3.5, 4.0]), ("pos", [3, float("nan")]), ("seq", [0, (1 << 32) + 1]),
+                                        ("tables", [[0, 1], [2, -(1 << 31) - 1]]), ("tables", [[0, 1e20]] * 2)])
+@pytest.mark.parametrize("as_array", [False, True])
+def test_indices_that_would_wrap_around(name, value, as_array):
+    """an index of 64 bits is not cut to its lower 32, a fraction not to a whole number"""
+    np = pytest.importorskip("numpy")
+    with pytest.raises(jieyu_amd.JyError, match=name + ": whole numbers"):
+        paged_pass(**{name: np.array(value) if as_array else value})
+
+
+def test_indices_of_other_whole_types():
+    np = pytest.importorskip("numpy")
+    for t in (np.int64, np.uint32, np.int16, np.uint8, np.int32, np.float64):
+        got = jieyu_amd._int32s(np.array([[0, 7], [3, 100]], t)[:, ::-1], "tables")
+        assert got.dtype == np.int32 and got.flags.c_contiguous and got.tolist() == [[7, 0], [100, 3]]
+    assert jieyu_amd._int32s([], "pos").shape == (0,) and jieyu_amd._int32s([-1, (1 << 31) - 1], "pos").tolist() == [-1, (1 << 31) - 1]
