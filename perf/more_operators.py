@@ -17,8 +17,8 @@ A case is a plain dict.  Its "kind" says which operator runs:
             last `recent` among them, then PagePool.read of what stayed.
 
 "io" is the type of queries, new keys and values and outputs, "pool" the cache's: "i4" (two 4-bit numbers a
-byte, fp16 scale and lowest value per 32 elements), "i8" (one fp32 scale per vector), "f16", "bf16".  `own`
-chooses between the operators' plain form and the package's kernels.
+byte; per 32 elements their step, of seven bits, and their lowest value in fp16), "i8" (one fp32 scale
+per vector), "f16", "bf16".  `own` chooses between the operators' plain form and the package's kernels.
 """
 import math
 import random
@@ -139,8 +139,14 @@ def _shares(rng, case):
 
 
 def _groups(hd):
-    """4-bit groups of a vector as it is laid out: 32 elements each, their number a power of two"""
-    return 1 << max(0, (hd + 31) // 32 - 1).bit_length()
+    """4-bit groups of a vector as it is laid out: 32 elements each, 2, 4 or 8 of them"""
+    return 2 if hd <= 64 else 4 if hd <= 128 else 8
+
+
+def _seven_bits(x):
+    """fp32 numbers (not negative) rounded to seven significant bits, ties to even"""
+    u = x.view(torch.int32)
+    return ((u + 0xffff + ((u >> 17) & 1)) & ~0x1ffff).view(torch.float32)
 
 
 def _quantise4(x):
@@ -155,7 +161,8 @@ def _quantise4(x):
     high = torch.where(there, room, torch.full_like(room, -math.inf)).amax(-1)
     some = there.any(-1)
     low = torch.where(some, low, torch.zeros_like(low)).half().float()
-    scale = torch.where(some, (high - low) / torch.full_like(low, 15.0), torch.zeros_like(low)).half().float()
+    scale = torch.where(some, (high - low) / torch.full_like(low, 15.0), torch.zeros_like(low))
+    scale = _seven_bits(scale).half().float()
     inv = torch.where(scale > 0, torch.ones_like(scale) / scale, torch.zeros_like(scale))
     n = torch.round((room - low[..., None]) * inv[..., None]).clamp(0.0, 15.0)
     return torch.where(there, n, torch.zeros_like(n)), scale, low
@@ -528,7 +535,8 @@ def _held64(x, pool):
     for i in range(0, hd, 32):
         part = x[..., i:i + 32].double()
         low = part.amin(-1, keepdim=True).half().double()
-        step = ((part.amax(-1, keepdim=True) - low).float().double() / 15).float().half().double()
+        m, e = torch.frexp(((part.amax(-1, keepdim=True) - low).float().double() / 15).float().double())
+        step = torch.ldexp(torch.round(m * 128), e - 7).half().double()  # seven bits
         back = torch.where(step > 0, 1 / step, 0.0).float().double()
         n = torch.round(((part - low).float().double() * back).float().double()).clamp(0, 15)
         out[..., i:i + 32] = (n * step + low).float().double()
