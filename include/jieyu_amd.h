@@ -246,16 +246,26 @@ JYHIP_API int jyhip_wmat_time(jyhip_wmat* w, const float* x, int iters, double* 
  * device is refused. */
 
 /* element types */
-enum { JYHIP_T_F32 = 0, JYHIP_T_F16 = 1, JYHIP_T_BF16 = 2, JYHIP_T_I8 = 3 };
+enum { JYHIP_T_F32 = 0, JYHIP_T_F16 = 1, JYHIP_T_BF16 = 2, JYHIP_T_I8 = 3, JYHIP_T_I4 = 4 };
 
 /* One layer's pool of pages, `page_size` positions each:
  *   k, v              [num_pages][num_kv_heads][page_size][head_dim] of `type`
- *   k_scale, v_scale  fp32 [num_pages][num_kv_heads][page_size] with JYHIP_T_I8, else NULL
+ *   k_scale, v_scale  fp32 [num_pages][num_kv_heads][page_size] with JYHIP_T_I8, the groups'
+ *                     numbers below with JYHIP_T_I4, else NULL
  * head_dim: a multiple of 16 up to 256; page_size: 16, 32, 64, 128 or 256; type: JYHIP_T_I8,
- * JYHIP_T_F16 or JYHIP_T_BF16.  k and v are aligned to 16 bytes.  An int8 vector holds
+ * JYHIP_T_I4, JYHIP_T_F16 or JYHIP_T_BF16.  k and v are aligned to 16 bytes.  An int8 vector holds
  * q * scale by the rule of jyhip_kv (libs/model_libs/attention/attention_q8.h:29-35): scale =
  * absmax / 127, q = rint(x * (127 / absmax)), both fp32; zeros where absmax <= 1e-8.  A vector
- * with an infinity or a NaN in it is held as NaN (scale NaN), all of it. */
+ * with an infinity or a NaN in it is held as NaN (scale NaN), all of it.
+ *
+ * A JYHIP_T_I4 vector is laid out in G groups of 32 elements, G = 2 for a head_dim up to 64, 4 up to 128,
+ * 8 above: 16 G bytes, byte r G + g holding the numbers n of elements 32 g + 2 r (its low half) and
+ * 32 g + 2 r + 1 (what lies past head_dim holds zeros); so k, v are [num_pages][num_kv_heads][page_size][16 G]
+ * bytes.  k_scale, v_scale point to fp16 [num_pages][num_kv_heads][page_size][G][2], each group's step and
+ * lowest value: an element is n * step + low, with low = fp16(min x), step = fp16(round7((max x - low) / 15)),
+ * n = rint((x - low) * (1 / step)) in 0 .. 15 (0 where step is 0), in fp32; round7 rounds to seven significant
+ * bits, ties to even.  A vector with an element that is not finite or past +-30000 is held as NaN, all of it.
+ * Steps that are not of this kind (more than seven bits, over 4000) are within the rules of none of these calls. */
 typedef struct jyhip_pages {
     void* k;
     void* v;
@@ -344,6 +354,18 @@ JYHIP_API int jyhip_sample(const void* logits, int type, int rows, int vocab, lo
                            const float* temperature, const int* top_k, const float* top_p, const float* min_p,
                            int* ids, void* workspace, size_t workspace_bytes, int device, void* stream);
 JYHIP_API size_t jyhip_sample_workspace(int rows, int vocab);
+
+/* Rotary positions: turn the pairs of every head of `rows` rows of queries (q_heads heads) and keys (k_heads,
+ * 0 with k and k_out NULL: none).  Pair i of a head of row r turns by the angle pos[r] * freq[i] (fp64):
+ *   (x, y) -> (x c - y s, x s + y c),  c = factor * cos, s = factor * sin
+ * with (x, y) elements (i, i + pairs) or, interleaved, (2 i, 2 i + 1); a head's elements from 2 pairs on are
+ * copied.  q, k and the outputs hold elements of `type` (JYHIP_T_F32, _F16, _BF16); an output may be its own
+ * input (the same data and strides), else they do not overlap.  Products are fp32, rounded once; angles are
+ * good up to 2^40.  head_dim is at most 1024, 2 pairs at most head_dim, pairs at least 1. */
+JYHIP_API int jyhip_rope(const jyhip_vectors* q, const jyhip_vectors* q_out, int q_heads, const jyhip_vectors* k,
+                         const jyhip_vectors* k_out, int k_heads, int rows, int head_dim, const int* pos,
+                         const double* freq, int pairs, int interleaved, float factor, int type, int device,
+                         void* stream);
 
 /* One pass of a model over `rows` tokens of several sequences whose keys and values lie in pages: row r
  * is position pos[r] of sequence seq[r] (seq NULL: of sequence r).  X and out: host [rows][hidden], the

@@ -452,8 +452,8 @@ class WeightMatrix:
             pass
 
 
-from .batch import PagePool, sample  # noqa: E402
+from .batch import PagePool, rope, rope_frequencies, sample  # noqa: E402
 
-__all__ = ["PagePool", "sample", "lib", "last_error", "device_count", "GpuModel", "KVCache", "Q8Matrix", "WeightMatrix", "Stats", "JyError",
+__all__ = ["PagePool", "rope", "rope_frequencies", "sample", "lib", "last_error", "device_count", "GpuModel", "KVCache", "Q8Matrix", "WeightMatrix", "Stats", "JyError",
            "ModelDesc", "LayerWeights", "SynthConfig", "Synth", "synth_config", "CONFIGS", "JY_F32", "JY_F16",
            "JY_Q8_0", "JY_Q4_K", "JY_Q5_K", "JY_Q6_K"]

@@ -14,7 +14,7 @@ P = C.c_void_p
 I = C.c_int
 LL = C.c_longlong
 
-T_F32, T_F16, T_BF16, T_I8 = 0, 1, 2, 3
+T_F32, T_F16, T_BF16, T_I8, T_I4 = 0, 1, 2, 3, 4
 
 
 class _Pages(C.Structure):
@@ -41,7 +41,7 @@ class _Bound:
         L = lib()
         self.torch, self.int32 = torch, torch.int32
         self.io = {torch.float32: T_F32, torch.float16: T_F16, torch.bfloat16: T_BF16}
-        self.pool = {torch.int8: T_I8, torch.float16: T_F16, torch.bfloat16: T_BF16}
+        self.pool = {torch.uint8: T_I4, torch.int8: T_I8, torch.float16: T_F16, torch.bfloat16: T_BF16}
         # the address of the current stream of device i (without torch.cuda.Stream's object around it,
         # where this torch has that)
         self.stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
@@ -59,6 +59,8 @@ class _Bound:
         self.attend = proto("jyhip_pages_attend", I, ref(_Pages), ref(_Tables), P, I, I, C.c_float, ref(_Vectors),
                             ref(_Vectors), I, P, C.c_size_t, P)
         self.attend_workspace = proto("jyhip_pages_attend_workspace", C.c_size_t, ref(_Pages), I, I, I)
+        self.rope = proto("jyhip_rope", I, ref(_Vectors), ref(_Vectors), I, ref(_Vectors), ref(_Vectors), I, I, I, P, P, I, I,
+                          C.c_float, I, I, P)
         self.sample = proto("jyhip_sample", I, P, I, I, I, LL, P, P, P, P, P, P, P, C.c_size_t, I, P)
         self.sample_workspace = proto("jyhip_sample_workspace", C.c_size_t, I, I)
         self.error = L.jyhip_last_error
@@ -82,32 +84,60 @@ def _indices(b, t, n, device, name):
     return t.data_ptr()
 
 
+def _strided(t, shape, dtype, device, name):
+    """A device tensor of vectors, for the library."""
+    if t.shape != shape or t.dtype is not dtype or t.device != device:
+        raise JyError(f"{name}: a {dtype} tensor of {tuple(shape)} on {device} is needed")
+    row, head, one = t.stride()
+    if one != 1 and shape[2] > 1:
+        raise JyError(f"{name}: a vector's elements must lie side by side")
+    return _Vectors(t.data_ptr(), row, head)
+
+
+def _groups4(hd):
+    """groups of 32 elements that a 4-bit vector is laid out in"""
+    return 2 if hd <= 64 else 4 if hd <= 128 else 8
+
+
 class PagePool:
     """The pages of a key/value cache: k, v [layers][pages][kv heads][page size][head size] in int8
-    (then with fp32 scales [layers][pages][kv heads][page size]), float16 or bfloat16.  The tensors
-    stay the caller's, and the pool keeps a reference to them.
+    (then with fp32 scales [layers][pages][kv heads][page size]), float16 or bfloat16, or in 4 bits:
+    uint8 [layers][pages][kv heads][page size][16 groups], then with float16 scales [layers][pages]
+    [kv heads][page size][groups][2], 2 groups for a head size up to 64, 4 up to 128, 8 up to 256 (the
+    head size itself is `head_dim`, 32 groups unless given).  The tensors stay the caller's, and the
+    pool keeps a reference to them.
 
     `tables` (int32 [sequences][pages of each]) says which page holds a sequence's positions; an id
     outside the pool is a hole: its positions are not written, read as zeros, and left out of the
     attention."""
 
-    def __init__(self, k, v, k_scale=None, v_scale=None):
+    def __init__(self, k, v, k_scale=None, v_scale=None, head_dim=None):
         b = self._b = _bind()
+        torch = b.torch
         if k.dim() != 5 or not k.is_cuda or k.dtype not in b.pool:
             raise JyError("pool: k and v are device tensors [layers][pages][kv heads][page size][head size] in int8, "
-                          "float16 or bfloat16")
-        for t, shape, dtype, name in ((k, k.shape, k.dtype, "k"), (v, k.shape, k.dtype, "v"),
-                                      (k_scale, k.shape[:4], b.torch.float32, "k_scale"),
-                                      (v_scale, k.shape[:4], b.torch.float32, "v_scale")):
-            if t is None and name.endswith("scale") and k.dtype is not b.torch.int8:
-                continue
+                          "4 bits (uint8), float16 or bfloat16")
+        self.layers, self.pages, self.nkv, self.page_size, width = k.shape
+        scales = None
+        if k.dtype is torch.int8:
+            scales = (torch.float32, k.shape[:4])
+        elif k.dtype is torch.uint8:
+            self.hd = 2 * width if head_dim is None else head_dim
+            if width != 16 * _groups4(self.hd):
+                raise JyError(f"pool: 4-bit vectors of {self.hd} elements take {16 * _groups4(self.hd)} bytes")
+            scales = (torch.float16, (*k.shape[:4], width // 16, 2))
+        if k.dtype is not torch.uint8:
+            self.hd = width
+            if head_dim not in (None, width):
+                raise JyError("pool: head_dim is not the vectors' size")
+        for t, shape, dtype, name in ((k, k.shape, k.dtype, "k"), (v, k.shape, k.dtype, "v")) + (() if scales is None else (
+                (k_scale, scales[1], scales[0], "k_scale"), (v_scale, scales[1], scales[0], "v_scale"))):
             if t is None or t.shape != shape or t.dtype is not dtype or t.device != k.device or not t.is_contiguous():
                 raise JyError(f"pool: {name} must be a contiguous {dtype} tensor of {tuple(shape)} on {k.device}")
-            if t is not None and name.endswith("scale") and k.dtype is not b.torch.int8:
-                raise JyError("pool: 16-bit pages have no scales")
+        if scales is None and (k_scale is not None or v_scale is not None):
+            raise JyError("pool: 16-bit pages have no scales")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.device = k.device
-        self.layers, self.pages, self.nkv, self.page_size, self.hd = k.shape
         if not self.layers or not self.pages or not self.nkv:
             raise JyError("pool: no pages")
 
@@ -119,13 +149,19 @@ class PagePool:
 
     @classmethod
     def empty(cls, layers, pages, page_size, num_kv_heads, head_dim, dtype=None, device="cuda"):
-        """A new pool, int8 unless `dtype` says otherwise, without any contents of its own."""
+        """A new pool, int8 unless `dtype` says otherwise (torch.uint8: 4 bits), without any contents of its own."""
         torch = _bind().torch
         dtype = dtype or torch.int8
-        shape = (layers, pages, num_kv_heads, page_size, head_dim)
+        lead = (layers, pages, num_kv_heads, page_size)
+        groups = _groups4(head_dim)
         new = lambda s, t: torch.empty(s, dtype=t, device=device)  # noqa: E731
-        scales = [new(shape[:4], torch.float32) for _ in range(2)] if dtype is torch.int8 else [None, None]
-        return cls(new(shape, dtype), new(shape, dtype), *scales)
+        scales = [None, None]
+        if dtype is torch.int8:
+            scales = [new(lead, torch.float32) for _ in range(2)]
+        if dtype is torch.uint8:
+            scales = [new((*lead, groups, 2), torch.float16) for _ in range(2)]
+        shape = (*lead, 16 * groups if dtype is torch.uint8 else head_dim)
+        return cls(new(shape, dtype), new(shape, dtype), *scales, head_dim=head_dim)
 
     def _layer(self, layer):
         if not 0 <= layer < self.layers:
@@ -139,12 +175,7 @@ class PagePool:
         return _Tables(t.data_ptr(), *shape)
 
     def _vectors(self, t, shape, dtype, name):
-        if t.shape != shape or t.dtype is not dtype or t.device != self.device:
-            raise JyError(f"{name}: a {dtype} tensor of {shape} on {self.device} is needed")
-        row, head, one = t.stride()
-        if one != 1:
-            raise JyError(f"{name}: a vector's elements must lie side by side")
-        return _Vectors(t.data_ptr(), row, head)
+        return _strided(t, shape, dtype, self.device, name)
 
     def _move(self, fn, layer, k, v, tables, pos, seq):
         b, device, dtype, shape = self._b, self.device, k.dtype, k.shape
@@ -244,4 +275,61 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, out=
     return out
 
 
-__all__ = ["PagePool", "sample"]
+def rope_frequencies(dim, theta=10000.0, scaling=None, factor=1.0, trained=None, low=1.0, high=4.0, device="cuda"):
+    """The angle per position of each of dim / 2 pairs, float64: theta^(-2 i / dim), for `rope`.  For contexts
+    `factor` times as long as the trained one, `scaling` is
+      "linear"  every frequency over `factor`;
+      "base"    theta times factor^(dim / (dim - 2)): the slowest pair alone turns `factor` times slower;
+      "ramp"    over `factor` where a pair turns less than `low` times in the `trained` positions, as it is
+                where it turns more than `high` times, in between the mix that rises with the turns."""
+    torch = _bind().torch
+    if dim < 2 or dim % 2 or not theta > 0 or not factor > 0:
+        raise JyError("rope_frequencies: dim is even, theta and factor are positive")
+    if scaling == "base":
+        theta = theta * factor ** (dim / max(1, dim - 2))
+    f = theta ** (-torch.arange(dim // 2, dtype=torch.float64, device=device) * 2 / dim)
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "ramp":
+        if trained is None or not high > low:
+            raise JyError("rope_frequencies: the ramp needs the trained length and low < high")
+        mix = ((trained * f / (2 * math.pi) - low) / (high - low)).clamp(0.0, 1.0)
+        f = f * mix + f / factor * (1.0 - mix)
+    elif scaling not in (None, "base"):
+        raise JyError('rope_frequencies: scaling is None, "linear", "base" or "ramp"')
+    return f
+
+
+def rope(q, k, pos, freq, layout="half", factor=1.0, out=None):
+    """Rotary positions: (q, k) with the pairs of every head of q [rows][heads][head size] and k [rows][kv heads]
+    [head size] (or None) turned by pos[r] * freq[i] (int32, one a row, and float64, one a pair); float32, float16
+    or bfloat16.  layout "half" pairs element i with i + pairs, "interleaved" 2 i with 2 i + 1; elements from 2 pairs
+    on stay.  `factor` multiplies cosines and sines.  out: a pair of tensors, which may be q and k themselves."""
+    b = _bind()
+    dtype, device = q.dtype, q.device
+    code = b.io.get(dtype)
+    if code is None or q.dim() != 3 or not q.is_cuda:
+        raise JyError("rope: q is a device tensor [rows][heads][head size] in float32, float16 or bfloat16")
+    if layout not in ("half", "interleaved"):
+        raise JyError('rope: layout is "half" or "interleaved"')
+    rows, heads, hd = q.shape
+    if k is not None and k.dim() != 3:
+        raise JyError("rope: k [rows][kv heads][head size]")
+    qo, ko = out if out is not None else (q.new_empty(q.shape), None if k is None else k.new_empty(k.shape))
+    if (k is None) != (ko is None):
+        raise JyError("rope: an output for each input")
+    Q, QO = _strided(q, q.shape, dtype, device, "q"), _strided(qo, q.shape, dtype, device, "out of q")
+    K = KO = None
+    if k is not None:
+        shape = (rows, k.shape[1], hd)
+        K, KO = _strided(k, shape, dtype, device, "k"), _strided(ko, shape, dtype, device, "out of k")
+    p = _indices(b, pos, rows, device, "pos")
+    if freq.dtype is not b.torch.float64 or freq.dim() != 1 or freq.device != device or not freq.is_contiguous():
+        raise JyError(f"rope: freq must be a contiguous float64 tensor [pairs] on {device}")
+    if b.rope(Q, QO, heads, K, KO, 0 if k is None else k.shape[1], rows, hd, p, freq.data_ptr(), freq.shape[0],
+              layout == "interleaved", factor, code, device.index, b.stream(device.index)) != 0:
+        _failed(b)
+    return qo, ko
+
+
+__all__ = ["PagePool", "rope", "rope_frequencies", "sample"]

@@ -9,14 +9,15 @@
 #include "jieyu_amd.h"
 #include "jy_guard.h"
 #include "jy_paged.h"
+#include "jy_rope.h"
 #include "jy_sample.h"
 
 using namespace jy;
 
 void jy::check_pages(const jyhip_pages* p) {
     if (!p) fail("pages is NULL");
-    if (p->type != JYHIP_T_I8 && p->type != JYHIP_T_F16 && p->type != JYHIP_T_BF16)
-        fail("pages: the type must be int8, fp16 or bf16");
+    if (p->type != JYHIP_T_I8 && p->type != JYHIP_T_I4 && p->type != JYHIP_T_F16 && p->type != JYHIP_T_BF16)
+        fail("pages: the type must be int8, 4-bit, fp16 or bf16");
     if (p->num_pages < 1 || p->num_kv_heads < 1) fail("pages: num_pages and num_kv_heads must be positive");
     const int ps = p->page_size;
     if (ps != 16 && ps != 32 && ps != 64 && ps != 128 && ps != 256)
@@ -25,8 +26,8 @@ void jy::check_pages(const jyhip_pages* p) {
         fail("pages: head_dim must be a multiple of 16 up to 256");
     if (!p->k || !p->v) fail("pages: NULL k or v");
     if (((uintptr_t)p->k | (uintptr_t)p->v) % 16) fail("pages: k and v must be aligned to 16 bytes");
-    if (p->type == JYHIP_T_I8) {
-        if (!p->k_scale || !p->v_scale) fail("pages: int8 pages need scales");
+    if (p->type == JYHIP_T_I8 || p->type == JYHIP_T_I4) {
+        if (!p->k_scale || !p->v_scale) fail("pages: int8 and 4-bit pages need scales");
         if (((uintptr_t)p->k_scale | (uintptr_t)p->v_scale) % 16) fail("pages: scales must be aligned to 16 bytes");
     } else if (p->k_scale || p->v_scale) {
         fail("pages: 16-bit pages have no scales");
@@ -124,6 +125,7 @@ JYHIP_API int jyhip_pages_attend(const jyhip_pages* pages, const jyhip_page_tabl
         check_pages(pages);
         check_tables(tables);
         check_type(type);
+        if (pages->type == JYHIP_T_I4) fail("attend: the type of the pages must be int8, fp16 or bf16");
         if (!lens) fail("lens is NULL");
         if (max_len < 0 || max_len > MAX_LEN) fail("max_len must be between 0 and 2^30");
         if (num_heads < 1 || num_heads % pages->num_kv_heads)
@@ -150,6 +152,50 @@ JYHIP_API int jyhip_pages_attend(const jyhip_pages* pages, const jyhip_page_tabl
             fail("attend: too many sequences and heads for one call");
         const OnDevice on(pages->device, (hipStream_t)stream);
         launch_paged_attend(A, (hipStream_t)stream);
+        CK(hipGetLastError());
+        return 0;
+    }, -1);
+}
+
+JYHIP_API int jyhip_rope(const jyhip_vectors* q, const jyhip_vectors* q_out, int q_heads, const jyhip_vectors* k,
+                         const jyhip_vectors* k_out, int k_heads, int rows, int head_dim, const int* pos,
+                         const double* freq, int pairs, int interleaved, float factor, int type, int device,
+                         void* stream) {
+    return guarded([&]() {
+        check_type(type);
+        if (rows < 0 || q_heads < 0 || k_heads < 0) fail("rope: rows and heads must not be negative");
+        if (head_dim < 2 || head_dim > ROPE_MAX_HEAD) fail("rope: head_dim must be between 2 and 1024");
+        if (pairs < 1 || 2 * (int64_t)pairs > head_dim) fail("rope: 2 * pairs must be between 2 and head_dim");
+        if (((int64_t)q_heads + k_heads) * head_dim > 1 << 20) fail("rope: heads x head_dim is over 2^20");
+        if (rows == 0 || q_heads + k_heads == 0) return 0;
+        if (!pos || !freq) fail("rope: NULL pos or freq");
+        if ((uintptr_t)freq % 8 || (uintptr_t)pos % 4) fail("rope: pos or freq is not aligned to its elements");
+        RopeArgs A;
+        if (q_heads) {
+            check_vectors(q, type, "q");
+            check_vectors(q_out, type, "q_out");
+            A.q = *q;
+            A.q_out = *q_out;
+        }
+        if (k_heads) {
+            check_vectors(k, type, "k");
+            check_vectors(k_out, type, "k_out");
+            A.k = *k;
+            A.k_out = *k_out;
+        }
+        A.q_heads = q_heads;
+        A.k_heads = k_heads;
+        A.rows = rows;
+        A.hd = head_dim;
+        A.pos = pos;
+        A.freq = freq;
+        A.pairs = pairs;
+        A.interleaved = interleaved != 0;
+        A.factor = factor;
+        A.type = type;
+        if (rope_blocks(A) >= (1 << 24)) fail("rope: too many rows for one call");
+        const OnDevice on(device, (hipStream_t)stream);
+        launch_rope(A, (hipStream_t)stream);
         CK(hipGetLastError());
         return 0;
     }, -1);

@@ -26,6 +26,12 @@ void launch_paged_write(const jyhip_pages& P, const PageMap& M, int rows, const 
 void launch_paged_read(const jyhip_pages& P, const PageMap& M, int rows, const jyhip_vectors& k,
                        const jyhip_vectors& v, int type, hipStream_t st);
 
+// the same for 4-bit pages (jy_paged4.hip)
+void launch_paged4_write(const jyhip_pages& P, const PageMap& M, int rows, const jyhip_vectors& k,
+                         const jyhip_vectors& v, int type, hipStream_t st);
+void launch_paged4_read(const jyhip_pages& P, const PageMap& M, int rows, const jyhip_vectors& k,
+                        const jyhip_vectors& v, int type, hipStream_t st);
+
 // RoPE on the q and k heads of every row of qkv ([rows][width], q then k first) in place, row r at
 // position pos[r], the rotated pairs in rope_pack's order; head_dim a multiple of 16
 void launch_rope_rows(float* qkv, int rows, int width, const int* pos, int heads, int hd, const float* cos_t,

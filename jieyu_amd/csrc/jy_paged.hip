@@ -215,11 +215,13 @@ void launch_rope_rows(float* qkv, int rows, int width, const int* pos, int heads
 
 void launch_paged_write(const jyhip_pages& P, const PageMap& M, int rows, const jyhip_vectors& k,
                         const jyhip_vectors& v, int type, hipStream_t st) {
+    if (P.type == JYHIP_T_I4) return launch_paged4_write(P, M, rows, k, v, type, st);
     launch_moved<true>(P, M, rows, k, v, type, st);
 }
 
 void launch_paged_read(const jyhip_pages& P, const PageMap& M, int rows, const jyhip_vectors& k,
                        const jyhip_vectors& v, int type, hipStream_t st) {
+    if (P.type == JYHIP_T_I4) return launch_paged4_read(P, M, rows, k, v, type, st);
     launch_moved<false>(P, M, rows, k, v, type, st);
 }
 

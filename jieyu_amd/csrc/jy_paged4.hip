@@ -1,0 +1,216 @@
+// jy_paged4.hip — writing and reading 4-bit pages.
+//
+// A vector's elements come in groups of 32, each with its lowest value and step in fp16:
+//   low = fp16(min x), step = fp16((max x - low) / 15 in seven significant bits),
+//   n = rint((x - low) / step) in 0 .. 15; value n step + low
+// The numbers go by the rounded low and step, so those roundings bias nothing.  A step of seven bits times a
+// number of four is exact in fp16: the attention's products take it so.
+//
+// 16 lanes take a vector, and lane r elements 32 g + 2 r and 32 g + 2 r + 1 of every group g: its byte of
+// each group lies beside the others (byte r G + g of the vector, G groups), so a lane's bytes are one store,
+// and the attention's lanes, which take a vector's dims in the same shares, one load.  A group's lowest and
+// largest take four DPP moves within the row of lanes; the scales leave as one word a lane, lane g that of
+// group g.  The lanes take a head's key and value together.
+#include <hip/hip_runtime.h>
+
+#include "jy_device.h"
+#include "jy_paged_device.h"
+
+namespace jy {
+
+namespace {
+
+typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+
+// elements past it make a vector NaN: 16 steps of a group stay finite in fp16
+constexpr float kMax4 = 30000.0f;
+
+struct Moved4 {
+    jyhip_pages P;
+    PageMap M;
+    int rows, ps_log2;
+    jyhip_vectors k, v;
+};
+
+// minimum / maximum over a row of 16 lanes, in each of them
+__device__ __forceinline__ float row_min(float v) {
+    v = fminf(v, dpp_f<0xB1>(v));
+    v = fminf(v, dpp_f<0x4E>(v));
+    v = fminf(v, dpp_f<0x124>(v));
+    return fminf(v, dpp_f<0x128>(v));
+}
+__device__ __forceinline__ float row_max(float v) {
+    v = fmaxf(v, dpp_f<0xB1>(v));
+    v = fmaxf(v, dpp_f<0x4E>(v));
+    v = fmaxf(v, dpp_f<0x124>(v));
+    return fmaxf(v, dpp_f<0x128>(v));
+}
+
+// fp32 rounded to seven significant bits, ties to even
+__device__ __forceinline__ float seven_bits(float x) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    return __builtin_bit_cast(float, (u + 0xffffu + ((u >> 17) & 1u)) & ~0x1ffffu);
+}
+
+template <int G>
+using bytes_t = uint8_t __attribute__((ext_vector_type(G)));
+
+template <class E, int G>
+__device__ __forceinline__ void load_pairs(const E* p, int hd, bool pairs, float (&x)[2 * G]) {
+    const int r2 = (threadIdx.x & 15) * 2;
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+        const int d = 32 * g + r2;
+        const E* const at = p + (d < hd ? d : 0);  // (hd is a multiple of 16)
+        if (pairs) {
+            typedef E two __attribute__((ext_vector_type(2)));
+            const two v = *reinterpret_cast<const two*>(at);
+            x[2 * g] = (float)v[0];
+            x[2 * g + 1] = (float)v[1];
+        } else {
+            x[2 * g] = (float)at[0];
+            x[2 * g + 1] = (float)at[1];
+        }
+    }
+}
+
+// hold the 2 G elements of this lane as the vector at `vec`
+template <int G>
+__device__ __forceinline__ void hold4(void* pool, void* scales, int64_t vec, int hd, const float (&x)[2 * G]) {
+    const int r = threadIdx.x & 15;
+    float past = 0.0f;
+#pragma unroll
+    for (int g = 0; g < G; g++)
+        if (32 * g + 2 * r < hd) past = fmaxf(past, !(fabsf(x[2 * g]) <= kMax4) || !(fabsf(x[2 * g + 1]) <= kMax4) ? 1.0f : 0.0f);
+    const bool bad = row_max(past) > 0.0f;  // the whole vector is NaN
+    uint8_t bytes[G];
+    uint32_t word = 0;
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+        const bool on = 32 * g + 2 * r < hd;
+        const float lo = row_min(on ? fminf(x[2 * g], x[2 * g + 1]) : __builtin_inff());
+        const float hi = row_max(on ? fmaxf(x[2 * g], x[2 * g + 1]) : -__builtin_inff());
+        const bool some = 32 * g < hd;
+        const _Float16 low = some ? (_Float16)lo : (_Float16)0.0f;
+        const _Float16 step = some ? (_Float16)seven_bits((hi - (float)low) / 15.0f) : (_Float16)0.0f;
+        const float inv = (float)step > 0.0f ? 1.0f / (float)step : 0.0f;
+        uint32_t n[2];
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const float y = __builtin_rintf((x[2 * g + e] - (float)low) * inv);
+            n[e] = (uint32_t)(int)fminf(fmaxf(y, 0.0f), 15.0f);
+        }
+        bytes[g] = on && !bad ? (uint8_t)(n[0] | n[1] << 4) : (uint8_t)0;
+        const uint32_t nan = 0x7e007e00u;
+        const uint32_t w = bad && some ? nan : __builtin_bit_cast(uint32_t, h2_t{step, low});
+        word = r == g ? w : word;
+    }
+    bytes_t<G> b;
+#pragma unroll
+    for (int g = 0; g < G; g++) b[g] = bytes[g];
+    *reinterpret_cast<bytes_t<G>*>(static_cast<uint8_t*>(pool) + vec * (16 * G) + r * G) = b;
+    if (r < G) static_cast<uint32_t*>(scales)[vec * G + r] = word;
+}
+
+template <class E, int G>
+__device__ __forceinline__ void give4(const void* pool, const void* scales, int64_t vec, int hd, E* out, bool pairs) {
+    const int r = threadIdx.x & 15;
+    uint8_t bytes[G] = {};
+    uint32_t word[G] = {};
+    if (vec >= 0) {
+        const auto b = *reinterpret_cast<const bytes_t<G>*>(static_cast<const uint8_t*>(pool) + vec * (16 * G) + r * G);
+#pragma unroll
+        for (int g = 0; g < G; g++) bytes[g] = b[g];
+        constexpr int W = G > 4 ? 4 : G;
+        typedef uint32_t words __attribute__((ext_vector_type(W)));
+#pragma unroll
+        for (int c = 0; c < G; c += W) {
+            const words w = *reinterpret_cast<const words*>(static_cast<const uint32_t*>(scales) + vec * G + c);
+#pragma unroll
+            for (int g = 0; g < W; g++) word[c + g] = w[g];
+        }
+    }
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+        const int d = 32 * g + 2 * r;
+        if (d >= hd) continue;
+        const h2_t s = __builtin_bit_cast(h2_t, word[g]);
+        // (a number times a step is exact in fp32: one rounding)
+        const float a = __builtin_fmaf((float)(bytes[g] & 15), (float)s.x, (float)s.y);
+        const float b = __builtin_fmaf((float)(bytes[g] >> 4), (float)s.x, (float)s.y);
+        if (pairs) {
+            typedef E two __attribute__((ext_vector_type(2)));
+            *reinterpret_cast<two*>(out + d) = two{(E)a, (E)b};
+        } else {
+            out[d] = (E)a;
+            out[d + 1] = (E)b;
+        }
+    }
+}
+
+template <class E, int G, bool WRITE>
+__global__ __launch_bounds__(256) void paged4_kernel(Moved4 A, bool pairs) {
+    const jyhip_pages& P = A.P;
+    const unsigned i = blockIdx.x * 16 + (threadIdx.x >> 4), nkv = P.num_kv_heads;
+    const int row = (int)(i / nkv), head = (int)(i - row * nkv);
+    if (row >= A.rows) return;
+    E* const k = static_cast<E*>(A.k.data) + row * A.k.row_stride + head * A.k.head_stride;
+    E* const v = static_cast<E*>(A.v.data) + row * A.v.row_stride + head * A.v.head_stride;
+    const int64_t slot = slot_of(A.M, P.num_pages, A.ps_log2, A.M.seq ? A.M.seq[row] : row, A.M.pos[row]);
+    const int64_t vec =
+        slot < 0 ? -1 : (((slot >> A.ps_log2) * nkv + head) << A.ps_log2) + (slot & ((1 << A.ps_log2) - 1));
+    if constexpr (WRITE) {
+        float x[2 * G], y[2 * G];
+        load_pairs<E, G>(k, P.head_dim, pairs, x);
+        load_pairs<E, G>(v, P.head_dim, pairs, y);
+        if (vec < 0) return;
+        hold4<G>(P.k, P.k_scale, vec, P.head_dim, x);
+        hold4<G>(P.v, P.v_scale, vec, P.head_dim, y);
+    } else {
+        give4<E, G>(P.k, P.k_scale, vec, P.head_dim, k, pairs);
+        give4<E, G>(P.v, P.v_scale, vec, P.head_dim, v, pairs);
+    }
+}
+
+// whether every pair of elements starts at a multiple of its size
+bool paired(const jyhip_vectors& x, int type) {
+    const long long e = type == JYHIP_T_F32 ? 4 : 2;
+    return ((uintptr_t)x.data | (uintptr_t)(x.row_stride * e) | (uintptr_t)(x.head_stride * e)) % (2 * e) == 0;
+}
+
+template <class E, bool WRITE>
+void launch_groups(const Moved4& A, bool pairs, unsigned grid, hipStream_t st) {
+    switch (groups4(A.P.head_dim)) {
+        case 2: paged4_kernel<E, 2, WRITE><<<grid, 256, 0, st>>>(A, pairs); break;
+        case 4: paged4_kernel<E, 4, WRITE><<<grid, 256, 0, st>>>(A, pairs); break;
+        default: paged4_kernel<E, 8, WRITE><<<grid, 256, 0, st>>>(A, pairs);
+    }
+}
+
+template <bool WRITE>
+void launch_moved4(const jyhip_pages& P, const PageMap& M, int rows, const jyhip_vectors& k, const jyhip_vectors& v,
+                   int type, hipStream_t st) {
+    const Moved4 A{P, M, rows, __builtin_ctz(P.page_size), k, v};
+    const bool pairs = paired(k, type) && paired(v, type);
+    const unsigned grid = (unsigned)(((int64_t)rows * P.num_kv_heads + 15) / 16);
+    if (type == JYHIP_T_F32)
+        launch_groups<float, WRITE>(A, pairs, grid, st);
+    else if (type == JYHIP_T_F16)
+        launch_groups<_Float16, WRITE>(A, pairs, grid, st);
+    else
+        launch_groups<__bf16, WRITE>(A, pairs, grid, st);
+}
+
+}  // namespace
+
+void launch_paged4_write(const jyhip_pages& P, const PageMap& M, int rows, const jyhip_vectors& k,
+                         const jyhip_vectors& v, int type, hipStream_t st) {
+    launch_moved4<true>(P, M, rows, k, v, type, st);
+}
+
+void launch_paged4_read(const jyhip_pages& P, const PageMap& M, int rows, const jyhip_vectors& k,
+                        const jyhip_vectors& v, int type, hipStream_t st) {
+    launch_moved4<false>(P, M, rows, k, v, type, st);
+}
+
+}  // namespace jy

@@ -80,4 +80,8 @@ __device__ __forceinline__ int64_t slot_of(const PageMap& M, int num_pages, int 
     return ((int64_t)page << ps_log2) + (pos & ((1 << ps_log2) - 1));
 }
 
+// groups of 32 elements of a 4-bit vector as it is laid out, so that its bytes and its groups' words are
+// aligned to their sizes
+__host__ __device__ __forceinline__ int groups4(int hd) { return hd <= 64 ? 2 : hd <= 128 ? 4 : 8; }
+
 }  // namespace jy
