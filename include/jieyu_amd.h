@@ -355,6 +355,61 @@ JYHIP_API int jyhip_sample(const void* logits, int type, int rows, int vocab, lo
                            int* ids, void* workspace, size_t workspace_bytes, int device, void* stream);
 JYHIP_API size_t jyhip_sample_workspace(int rows, int vocab);
 
+/* What else makes a score, beside scale q . k:
+ *   cap     c > 0: a score s becomes c tanh(s / c), so it stays within +-c (0: as it is)
+ *   slopes  fp32 [num_heads]: then slope * |the row's position - the key's| is taken off (NULL: nothing)
+ *   first   int32, one per row: positions before it are left out (NULL: none; a window, a document's start)
+ *   last    int32, one per row: positions from it on are left out (NULL: those after the row's own; past it
+ *           for a prefix that is seen whole) */
+typedef struct jyhip_rules {
+    float cap;
+    const float* slopes;
+    const int* first;
+    const int* last;
+} jyhip_rules;
+
+/* jyhip_pages_attend with rules (NULL: none; `last` is not for it), the row of sequence s at position lens[s] - 1
+ * over positions first[s] .. lens[s] - 1.  With `first`, max_len is an upper bound of lens[s] - first[s], and of
+ * more positions the first max_len count.  With `weights`, fp32, the weights of position j, summed over the
+ * query heads of a kv head, are added to weights[s * weights_seq_stride + kv head * weights_head_stride + j]
+ * (strides in elements), for each position j < weights_len that s sees; sequences have elements of their own.  What is not finite: as in
+ * jyhip_pages_attend, but that what a row's rules leave out never reaches it; with a cap a score of +-infinity is
+ * +-cap. */
+JYHIP_API int jyhip_pages_attend_ruled(const jyhip_pages* pages, const jyhip_page_tables* tables, const int* lens,
+                                       int max_len, int num_heads, float scale, const jyhip_rules* rules,
+                                       const jyhip_vectors* q, const jyhip_vectors* out, int type, float* weights,
+                                       long long weights_seq_stride, long long weights_head_stride, int weights_len,
+                                       void* workspace, size_t workspace_bytes, void* stream);
+JYHIP_API size_t jyhip_pages_attend_ruled_workspace(const jyhip_pages* pages, int num_seqs, int num_heads, int max_len,
+                                                    int has_first, int has_weights);
+
+/* The same for runs of rows (prompts, drafted tokens): sequence s has the query rows starts[s] .. starts[s + 1] - 1 of
+ * q and out (starts: int32 [num_seqs + 1], ascending, on the device), and row r stands at position pos[r] and sees
+ * positions first[r] .. last[r] - 1 (0 and pos[r] + 1 without them) of its sequence, whose keys and values are in the
+ * pages.  A row that sees nothing gives zeros; rows before starts[0] and from starts[num_seqs] on are left as they
+ * are.  max_len is an upper bound of the positions that any row sees (last, or pos + 1): those past it are cut. */
+JYHIP_API int jyhip_pages_attend_rows(const jyhip_pages* pages, const jyhip_page_tables* tables, const int* starts,
+                                      const int* pos, int rows, int max_len, int num_heads, float scale,
+                                      const jyhip_rules* rules, const jyhip_vectors* q, const jyhip_vectors* out, int type,
+                                      void* workspace, size_t workspace_bytes, void* stream);
+JYHIP_API size_t jyhip_pages_attend_rows_workspace(const jyhip_pages* pages, int num_seqs, int rows, int num_heads,
+                                                   int max_len, int type);
+
+/* Evict what gets little attention: of the first n = min(lens[s], max_len) positions of every sequence (holes do not
+ * count) each kv head keeps min(keep, their number): those from n - recent on, and of the others the ones with the
+ * largest weights, equal ones by position (NaN counts as the least, a position past weights_len as 0).  weights: fp32,
+ * position j of kv head h at weights[s * weights_seq_stride + h * weights_head_stride + j], as jyhip_pages_attend_ruled adds them up.
+ * What stays moves, in order, to positions 0, 1, ... of the pages that `to` names, which are none that any of `tables`
+ * names (their contents would be unspecified): the caller frees the old ones afterwards.  kept [num_seqs][kv heads][keep]
+ * receives the old positions, -1 behind them; new_lens the new lengths (lens itself is not for it); new_weights, if not
+ * NULL, the weights of what stayed and zeros behind them, new_weights_len a head; it may be `weights` itself with the same
+ * strides and length.  0 <= recent <= keep, keep >= 1; sequences x kv heads x keep is at most 2^28 - 16. */
+JYHIP_API int jyhip_pages_evict(const jyhip_pages* pages, const jyhip_page_tables* tables, const jyhip_page_tables* to,
+                                const int* lens, int* new_lens, int max_len, int keep, int recent, const float* weights,
+                                long long weights_seq_stride, long long weights_head_stride, int weights_len,
+                                float* new_weights, long long new_seq_stride, long long new_head_stride,
+                                int new_weights_len, int* kept, void* stream);
+
 /* Rotary positions: turn the pairs of every head of `rows` rows of queries (q_heads heads) and keys (k_heads,
  * 0 with k and k_out NULL: none).  Pair i of a head of row r turns by the angle pos[r] * freq[i] (fp64):
  *   (x, y) -> (x c - y s, x s + y c),  c = factor * cos, s = factor * sin

@@ -30,6 +30,10 @@ class _Vectors(C.Structure):
     _fields_ = [("data", P), ("row_stride", LL), ("head_stride", LL)]
 
 
+class _Rules(C.Structure):
+    _fields_ = [("cap", C.c_float), ("slopes", P), ("first", P), ("last", P)]
+
+
 _bound = None
 
 
@@ -59,6 +63,15 @@ class _Bound:
         self.attend = proto("jyhip_pages_attend", I, ref(_Pages), ref(_Tables), P, I, I, C.c_float, ref(_Vectors),
                             ref(_Vectors), I, P, C.c_size_t, P)
         self.attend_workspace = proto("jyhip_pages_attend_workspace", C.c_size_t, ref(_Pages), I, I, I)
+        rules, seen = ref(_Rules), (ref(_Vectors), ref(_Vectors), I)
+        self.attend_ruled = proto("jyhip_pages_attend_ruled", I, ref(_Pages), ref(_Tables), P, I, I, C.c_float, rules, *seen, P,
+                                  LL, LL, I, P, C.c_size_t, P)
+        self.attend_ruled_workspace = proto("jyhip_pages_attend_ruled_workspace", C.c_size_t, ref(_Pages), I, I, I, I, I)
+        self.attend_rows = proto("jyhip_pages_attend_rows", I, ref(_Pages), ref(_Tables), P, P, I, I, I, C.c_float, rules, *seen,
+                                 P, C.c_size_t, P)
+        self.attend_rows_workspace = proto("jyhip_pages_attend_rows_workspace", C.c_size_t, ref(_Pages), I, I, I, I, I)
+        self.evict = proto("jyhip_pages_evict", I, ref(_Pages), ref(_Tables), ref(_Tables), P, P, I, I, I, P, LL, LL, I, P, LL, LL,
+                           I, P, P)
         self.rope = proto("jyhip_rope", I, ref(_Vectors), ref(_Vectors), I, ref(_Vectors), ref(_Vectors), I, I, I, P, P, I, I,
                           C.c_float, I, I, P)
         self.sample = proto("jyhip_sample", I, P, I, I, I, LL, P, P, P, P, P, P, P, C.c_size_t, I, P)
@@ -207,33 +220,124 @@ class PagePool:
         self._move(self._b.read, layer, out[0], out[1], tables, pos, seq)
         return out[0], out[1]
 
-    def attend(self, layer, q, tables, lens, max_len, scale=None, out=None):
+    def _queries(self, q, out):
+        """q's and out's vectors, their type and shape, and out"""
+        code = self._b.io.get(q.dtype)
+        if code is None or q.dim() != 3:
+            raise JyError("q: float32, float16 or bfloat16 [rows][heads][head size]")
+        rows, heads, _ = q.shape
+        shape = (rows, heads, self.hd)
+        if out is None:
+            out = q.new_empty(shape)
+        return self._vectors(q, shape, q.dtype, "q"), self._vectors(out, shape, q.dtype, "out"), code, rows, heads, out
+
+    def _rules(self, rows, heads, cap, slopes, first, last=None):
+        """The rules of a call, None without any."""
+        if cap is None and slopes is None and first is None and last is None:
+            return None
+        b = self._b
+        if slopes is not None and (slopes.dtype is not b.torch.float32 or slopes.shape != (heads,) or slopes.device != self.device
+                                   or not slopes.is_contiguous()):
+            raise JyError(f"slopes: {heads} contiguous float32 values on {self.device} are needed")
+        if cap is not None and not cap > 0:
+            raise JyError("cap: a positive number, or None")
+        return _Rules(0.0 if cap is None else cap, None if slopes is None else slopes.data_ptr(),
+                      None if first is None else _indices(b, first, rows, self.device, "first"),
+                      None if last is None else _indices(b, last, rows, self.device, "last"))
+
+    def attend(self, layer, q, tables, lens, max_len, scale=None, out=None, first=None, cap=None, slopes=None, weights=None):
         """Attention of q [sequences][heads][head size], one row per sequence, over the first lens[s]
         (int32) positions of each; zeros for a sequence without any.  `max_len`, an upper bound of
-        lens, sizes the launch: a longer one is cut to it.  scale: 1 / sqrt(head size) unless given."""
+        lens, sizes the launch: a longer one is cut to it.  scale: 1 / sqrt(head size) unless given.
+
+        first (int32): a sequence's positions before first[s] are left out, and max_len is an upper bound
+        of lens - first.  cap: a score s becomes cap * tanh(s / cap).  slopes (float32 [heads]): slope times the
+        distance to position lens[s] - 1 is taken off the scores.  weights (float32 [sequences][kv heads]
+        [positions]): the weights of each position, summed over the query heads of a kv head, are added to it (past its
+        last position they are not counted)."""
         b = self._b
         pages, T = self._layer(layer), self._tables(tables)
-        code = b.io.get(q.dtype)
-        if code is None or q.dim() != 3:
-            raise JyError("q: float32, float16 or bfloat16 [sequences][heads][head size]")
-        batch, heads, _ = q.shape
-        if out is None:
-            out = q.new_empty((batch, heads, self.hd))
-        shape = (batch, heads, self.hd)
-        Q, O = self._vectors(q, shape, q.dtype, "q"), self._vectors(out, shape, q.dtype, "out")
+        Q, O, code, batch, heads, out = self._queries(q, out)
         n = _indices(b, lens, batch, self.device, "lens")
         if T.num_seqs != batch:
             raise JyError("attend: one query row for each sequence of the tables")
         if not 0 <= max_len <= 1 << 30:
             raise JyError("attend: max_len must be between 0 and 2^30")
+        rules = self._rules(batch, heads, cap, slopes, first)
+        w = (None, 0, 0, 0) if weights is None else self._weights(weights, batch, "weights")
         if not batch:
             return out
-        need = b.attend_workspace(pages, batch, heads, max_len)
-        ws = q.new_empty(need, dtype=b.torch.uint8) if need else None
-        if b.attend(pages, T, n, max_len, heads, 1.0 / math.sqrt(self.hd) if scale is None else scale, Q, O, code,
-                    ws.data_ptr() if need else None, need, b.stream(self.device.index)) != 0:
+        scale = 1.0 / math.sqrt(self.hd) if scale is None else scale
+        stream = b.stream(self.device.index)
+        if rules is None and weights is None:
+            need = b.attend_workspace(pages, batch, heads, max_len)
+            ws = q.new_empty(need, dtype=b.torch.uint8) if need else None
+            rc = b.attend(pages, T, n, max_len, heads, scale, Q, O, code, ws.data_ptr() if need else None, need, stream)
+        else:
+            need = b.attend_ruled_workspace(pages, batch, heads, max_len, first is not None, weights is not None)
+            ws = q.new_empty(need, dtype=b.torch.uint8) if need else None
+            rc = b.attend_ruled(pages, T, n, max_len, heads, scale, rules, Q, O, code, *w, ws.data_ptr() if need else None, need,
+                                stream)
+        if rc != 0:
             _failed(b)
         return out
+
+    def attend_rows(self, layer, q, tables, starts, pos, max_len, scale=None, out=None, first=None, last=None, cap=None,
+                    slopes=None):
+        """Attention of runs of rows (prompts, drafted tokens): sequence s has rows starts[s] .. starts[s + 1] - 1 of
+        q [rows][heads][head size] (starts: int32 [sequences + 1], ascending), row r stands at position pos[r]
+        (int32) and sees positions first[r] .. last[r] - 1 of its sequence (int32; 0 and pos[r] + 1 unless given),
+        all of which are in the pages by then.  A row that sees nothing gives zeros; rows in no run are left as
+        they are.  `max_len` bounds last (pos + 1): what lies past it is cut.  scale, cap, slopes: as in attend."""
+        b = self._b
+        pages, T = self._layer(layer), self._tables(tables)
+        Q, O, code, rows, heads, out = self._queries(q, out)
+        s = _indices(b, starts, T.num_seqs + 1, self.device, "starts")
+        p = _indices(b, pos, rows, self.device, "pos")
+        if not 0 <= max_len <= 1 << 30:
+            raise JyError("attend_rows: max_len must be between 0 and 2^30")
+        rules = self._rules(rows, heads, cap, slopes, first, last)
+        if not rows:
+            return out
+        need = b.attend_rows_workspace(pages, T.num_seqs, rows, heads, max_len, code)
+        ws = q.new_empty(need, dtype=b.torch.uint8) if need else None
+        if b.attend_rows(pages, T, s, p, rows, max_len, heads, 1.0 / math.sqrt(self.hd) if scale is None else scale, rules, Q, O,
+                         code, ws.data_ptr() if need else None, need, b.stream(self.device.index)) != 0:
+            _failed(b)
+        return out
+
+
+    def _weights(self, t, batch, name):
+        """Weights of positions, for the library: address, strides and length."""
+        if (t.dtype is not self._b.torch.float32 or t.dim() != 3 or t.shape[:2] != (batch, self.nkv) or t.device != self.device
+                or (t.stride(2) != 1 and t.shape[2] > 1)):
+            raise JyError(f"{name}: a float32 tensor [sequences][kv heads][positions] on {self.device} is needed, positions "
+                          "side by side")
+        return (t.data_ptr(), *t.stride()[:2], t.shape[2])
+
+    def evict(self, layer, weights, tables, lens, keep, recent, max_len, new_tables, new_weights=None):
+        """Keep `keep` positions of each sequence and kv head: the last `recent` of its lens[s] (int32) and of the
+        others those with the largest weights (float32 [sequences][kv heads][positions], as `attend` adds them up; equal
+        ones by position).  What stays moves, in order, to the first positions of the pages that new_tables names, none
+        of them a page of `tables`.  (kept, lens, weights): the old positions int32 [sequences][kv heads][keep], -1 behind
+        them, the new lengths, and the weights of what stayed, zeros behind them, in new_weights (a new tensor unless
+        given; it may be `weights`).  `max_len`, an upper bound of lens: a longer one is cut to it."""
+        b = self._b
+        pages, T, to = self._layer(layer), self._tables(tables), self._tables(new_tables)
+        batch = T.num_seqs
+        n = _indices(b, lens, batch, self.device, "lens")
+        w = self._weights(weights, batch, "weights")
+        if not (0 <= max_len <= 1 << 30 and 1 <= keep <= 1 << 30 and 0 <= recent <= keep):
+            raise JyError("evict: max_len up to 2^30, 0 <= recent <= keep, keep from 1 to 2^30")
+        if new_weights is None:
+            new_weights = weights.new_empty(weights.shape)
+        nw = self._weights(new_weights, batch, "new_weights")
+        kept = tables.new_empty((batch, self.nkv, keep))
+        new_lens = lens.new_empty(batch)
+        if batch and b.evict(pages, T, to, n, new_lens.data_ptr(), max_len, keep, recent, *w, *nw, kept.data_ptr(),
+                             b.stream(self.device.index)) != 0:
+            _failed(b)
+        return kept, new_lens, new_weights
 
 
 def _settings(b, t, rows, device, dtype, name):

@@ -84,6 +84,58 @@ PageMap map_of(const jyhip_page_tables* t, const int* seq, const int* pos) {
     return m;
 }
 
+// whether attention over these pages is one that a workspace is given for
+bool shaped(const jyhip_pages& p, int num_heads, int max_len) {
+    return num_heads >= 1 && p.num_kv_heads >= 1 && max_len >= 0 && max_len <= MAX_LEN && num_heads % p.num_kv_heads == 0 &&
+           p.head_dim >= 16 && p.head_dim <= 256;
+}
+
+// what single rows and runs of rows have in common, checked
+RuledAttn ruled_args(const jyhip_pages* pages, const jyhip_page_tables* tables, int max_len, int num_heads, float scale,
+                     const jyhip_rules* rules, const jyhip_vectors* q, const jyhip_vectors* out, int type) {
+    check_pages(pages);
+    check_tables(tables);
+    check_type(type);
+    if (max_len < 0 || max_len > MAX_LEN) fail("max_len must be between 0 and 2^30");
+    if (num_heads < 1 || num_heads % pages->num_kv_heads) fail("the query heads must be a multiple of the key/value heads");
+    if (!std::isfinite(scale)) fail("scale must be finite");
+    check_vectors(q, type, "q");
+    check_vectors(out, type, "out");
+    RuledAttn A;
+    A.P = *pages;
+    A.M = map_of(tables, nullptr, nullptr);
+    A.span = std::max(max_len, 1);
+    A.most = max_len;
+    A.cap = (int)std::min<int64_t>(MAX_LEN, (int64_t)tables->table_stride * pages->page_size);
+    A.nh = num_heads;
+    A.scale = scale;
+    if (rules) {
+        if (!std::isfinite(rules->cap) || rules->cap < 0.0f) fail("the cap must be finite and not negative");
+        if (rules->cap != 0.0f && !std::isfinite(scale / rules->cap)) fail("scale over the cap must be finite");
+        if (((uintptr_t)rules->slopes | (uintptr_t)rules->first | (uintptr_t)rules->last) % 4)
+            fail("slopes, first or last are not aligned to their elements");
+        A.soft = rules->cap;
+        A.slopes = rules->slopes;
+        A.first = rules->first;
+        A.last = rules->last;
+    }
+    A.q = *q;
+    A.out = *out;
+    A.type = type;
+    return A;
+}
+
+void launch_checked(RuledAttn& A, void* workspace, size_t workspace_bytes, int device, hipStream_t st) {
+    A.part = static_cast<float*>(workspace);
+    const size_t need = ruled_attend_part_floats(A) * sizeof(float);
+    if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 16))
+        fail("attend: the workspace must hold " + std::to_string(need) + " bytes, aligned to 16");
+    if (ruled_attend_blocks(A) >= (1 << 24)) fail("attend: too many rows and heads for one call");
+    const OnDevice on(device, st);
+    launch_ruled_attend(A, st);
+    CK(hipGetLastError());
+}
+
 }  // namespace
 
 extern "C" {
@@ -125,7 +177,6 @@ JYHIP_API int jyhip_pages_attend(const jyhip_pages* pages, const jyhip_page_tabl
         check_pages(pages);
         check_tables(tables);
         check_type(type);
-        if (pages->type == JYHIP_T_I4) fail("attend: the type of the pages must be int8, fp16 or bf16");
         if (!lens) fail("lens is NULL");
         if (max_len < 0 || max_len > MAX_LEN) fail("max_len must be between 0 and 2^30");
         if (num_heads < 1 || num_heads % pages->num_kv_heads)
@@ -152,6 +203,133 @@ JYHIP_API int jyhip_pages_attend(const jyhip_pages* pages, const jyhip_page_tabl
             fail("attend: too many sequences and heads for one call");
         const OnDevice on(pages->device, (hipStream_t)stream);
         launch_paged_attend(A, (hipStream_t)stream);
+        CK(hipGetLastError());
+        return 0;
+    }, -1);
+}
+
+JYHIP_API size_t jyhip_pages_attend_ruled_workspace(const jyhip_pages* pages, int num_seqs, int num_heads, int max_len,
+                                                    int has_first, int has_weights) {
+    if (!pages || num_seqs < 1 || !shaped(*pages, num_heads, max_len)) return 0;
+    static const int some = 0;
+    static float any = 0.0f;
+    RuledAttn A;
+    A.P = *pages;
+    A.M.nseq = A.rows = num_seqs;
+    A.nh = num_heads;
+    A.span = std::max(max_len, 1);
+    A.first = has_first ? &some : nullptr;
+    A.weights = has_weights ? &any : nullptr;
+    return ruled_attend_part_floats(A) * sizeof(float);
+}
+
+JYHIP_API int jyhip_pages_attend_ruled(const jyhip_pages* pages, const jyhip_page_tables* tables, const int* lens,
+                                       int max_len, int num_heads, float scale, const jyhip_rules* rules,
+                                       const jyhip_vectors* q, const jyhip_vectors* out, int type, float* weights,
+                                       long long weights_seq_stride, long long weights_head_stride, int weights_len,
+                                       void* workspace, size_t workspace_bytes, void* stream) {
+    return guarded([&]() {
+        RuledAttn A = ruled_args(pages, tables, max_len, num_heads, scale, rules, q, out, type);
+        if (!lens) fail("lens is NULL");
+        if (rules && rules->last) fail("attend: one row per sequence ends at its length: last is for runs of rows");
+        if (weights && (weights_seq_stride < 0 || weights_head_stride < 0 || weights_len < 0))
+            fail("attend: a negative stride or length of the weights");
+        if ((uintptr_t)weights % 4) fail("attend: weights are not aligned to their elements");
+        A.lens = lens;
+        A.rows = tables->num_seqs;
+        if (!A.first) A.cap = std::min(A.cap, max_len);
+        A.weights = weights;
+        A.seq_stride = weights_seq_stride;
+        A.head_stride = weights_head_stride;
+        A.weights_len = weights_len;
+        launch_checked(A, workspace, workspace_bytes, pages->device, (hipStream_t)stream);
+        return 0;
+    }, -1);
+}
+
+JYHIP_API size_t jyhip_pages_attend_rows_workspace(const jyhip_pages* pages, int num_seqs, int rows, int num_heads,
+                                                   int max_len, int type) {
+    if (!pages || num_seqs < 1 || rows < 1 || !shaped(*pages, num_heads, max_len)) return 0;
+    static const int some = 0;
+    RuledAttn A;
+    A.P = *pages;
+    A.M.nseq = num_seqs;
+    A.rows = rows;
+    A.nh = num_heads;
+    A.span = std::max(max_len, 1);
+    A.starts = &some;
+    A.type = type;
+    return ruled_attend_part_floats(A) * sizeof(float);
+}
+
+JYHIP_API int jyhip_pages_attend_rows(const jyhip_pages* pages, const jyhip_page_tables* tables, const int* starts,
+                                      const int* pos, int rows, int max_len, int num_heads, float scale,
+                                      const jyhip_rules* rules, const jyhip_vectors* q, const jyhip_vectors* out, int type,
+                                      void* workspace, size_t workspace_bytes, void* stream) {
+    return guarded([&]() {
+        if (rows < 0) fail("rows must not be negative");
+        if (rows == 0) {
+            check_pages(pages);
+            check_tables(tables);
+            check_type(type);
+            return 0;
+        }
+        RuledAttn A = ruled_args(pages, tables, max_len, num_heads, scale, rules, q, out, type);
+        if (!starts || !pos) fail("attend_rows: NULL starts or pos");
+        A.starts = starts;
+        A.pos = pos;
+        A.rows = rows;
+        A.cap = std::min(A.cap, max_len);
+        launch_checked(A, workspace, workspace_bytes, pages->device, (hipStream_t)stream);
+        return 0;
+    }, -1);
+}
+
+JYHIP_API int jyhip_pages_evict(const jyhip_pages* pages, const jyhip_page_tables* tables, const jyhip_page_tables* to,
+                                const int* lens, int* new_lens, int max_len, int keep, int recent, const float* weights,
+                                long long weights_seq_stride, long long weights_head_stride, int weights_len,
+                                float* new_weights, long long new_seq_stride, long long new_head_stride,
+                                int new_weights_len, int* kept, void* stream) {
+    return guarded([&]() {
+        check_pages(pages);
+        check_tables(tables);
+        check_tables(to);
+        if (tables->num_seqs != to->num_seqs) fail("evict: the new tables are of other sequences");
+        if (!lens || !new_lens || (!weights && weights_len) || !kept) fail("evict: NULL lens, new_lens, weights or kept");
+        if (lens == new_lens) fail("evict: lens and new_lens must be apart");
+        if (((uintptr_t)lens | (uintptr_t)new_lens | (uintptr_t)weights | (uintptr_t)new_weights | (uintptr_t)kept) % 4)
+            fail("evict: a buffer is not aligned to its elements");
+        if (max_len < 0 || max_len > MAX_LEN) fail("max_len must be between 0 and 2^30");
+        if (keep < 1 || keep > MAX_LEN) fail("evict: keep must be between 1 and 2^30");
+        if (recent < 0 || recent > keep) fail("evict: recent must be between 0 and keep");
+        if (weights_seq_stride < 0 || weights_head_stride < 0 || weights_len < 0 || new_seq_stride < 0 || new_head_stride < 0 ||
+            new_weights_len < 0)
+            fail("evict: a negative stride or length of weights");
+        Eviction E;
+        E.P = *pages;
+        E.M = map_of(tables, nullptr, nullptr);
+        E.to = map_of(to, nullptr, nullptr);
+        E.lens = lens;
+        E.new_lens = new_lens;
+        E.cap = (int)std::min<int64_t>(max_len, (int64_t)tables->table_stride * pages->page_size);
+        E.keep = keep;
+        E.recent = recent;
+        if ((int64_t)to->table_stride * pages->page_size < std::min(keep, E.cap))
+            fail("evict: the new tables have too few pages for what stays");
+        const int64_t heads = (int64_t)tables->num_seqs * pages->num_kv_heads;
+        if (heads >= 1 << 22 || heads * std::min(keep, std::max(E.cap, 1)) > (1 << 28) - 16)
+            fail("evict: sequences x heads x keep is too large for one call");
+        E.weights = weights;
+        E.new_weights = new_weights;
+        E.seq_stride = weights_seq_stride;
+        E.head_stride = weights_head_stride;
+        E.weights_len = weights_len;
+        E.new_seq_stride = new_seq_stride;
+        E.new_head_stride = new_head_stride;
+        E.new_weights_len = new_weights_len;
+        E.kept = kept;
+        const OnDevice on(pages->device, (hipStream_t)stream);
+        launch_evict(E, (hipStream_t)stream);
         CK(hipGetLastError());
         return 0;
     }, -1);

@@ -54,4 +54,54 @@ size_t paged_attend_part_floats(const jyhip_pages& P, int nseq, int nh, int max_
 int64_t paged_attend_blocks(const jyhip_pages& P, int nseq, int nh, int max_len);
 void launch_paged_attend(const PagedAttn& A, hipStream_t st);
 
+// Attention with rules for scores, of one row per sequence (starts null: row s is sequence s, its positions
+// first[s] .. lens[s] - 1) or of runs of rows (sequence s has rows starts[s] .. starts[s + 1] - 1, row r at
+// position pos[r] over first[r] .. last[r] - 1).
+struct RuledAttn {
+    jyhip_pages P;
+    PageMap M;  // tables only
+    const int* lens = nullptr;
+    const int* starts = nullptr;
+    const int* pos = nullptr;
+    const int* first = nullptr;  // null: 0
+    const int* last = nullptr;   // null: pos + 1
+    int rows = 0;
+    int span = 0;  // at least 1: most positions that a row (starts null) or a run of rows may see, sizes the launch
+    int most = 0;  // with `first`, one row per sequence: positions past the first `most` do not count
+    int cap = 0;   // positions past it do not exist
+    int nh = 0;
+    float scale = 1.0f;
+    float soft = 0.0f;              // scores stay within +-soft (0: any)
+    const float* slopes = nullptr;  // [nh] null: no bias
+    jyhip_vectors q{}, out{};
+    int type = 0;
+    // one row per sequence: the weights of position j < weights_len are added to weights[s * seq_stride +
+    // kv head * head_stride + j]
+    float* weights = nullptr;
+    long long seq_stride = 0, head_stride = 0;
+    int weights_len = 0;
+    float* part = nullptr;  // ruled_attend_part_floats() floats
+};
+// rows, runs, heads and span as launch_ruled_attend gets them
+size_t ruled_attend_part_floats(const RuledAttn& A);
+int64_t ruled_attend_blocks(const RuledAttn& A);
+void launch_ruled_attend(const RuledAttn& A, hipStream_t st);
+
+// Eviction: of each sequence's positions the last `recent` and the heaviest of the others, `keep` in all, to
+// the front of the pages that new_tables names.
+struct Eviction {
+    jyhip_pages P;
+    PageMap M, to;  // tables only
+    const int* lens = nullptr;
+    int* new_lens = nullptr;
+    int cap = 0;  // positions past it do not exist
+    int keep = 0, recent = 0;
+    const float* weights = nullptr;  // [s * seq_stride + kv head * head_stride + position], weights_len of them
+    float* new_weights = nullptr;    // null: not wanted
+    long long seq_stride = 0, head_stride = 0, new_seq_stride = 0, new_head_stride = 0;
+    int weights_len = 0, new_weights_len = 0;
+    int* kept = nullptr;  // [nseq][kv heads][keep]
+};
+void launch_evict(const Eviction& E, hipStream_t st);
+
 }  // namespace jy

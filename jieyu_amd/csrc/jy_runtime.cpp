@@ -1749,7 +1749,6 @@ int forward_paged(jyhip_model* m, const jyhip_pages* pages, const float* X, floa
     if (!seq && rows > num_seqs) fail("forward_paged: without seq there is one row per sequence: more rows than sequences");
     for (int l = 0; l < m->L; l++) {
         check_pages(&pages[l]);
-        if (pages[l].type == JYHIP_T_I4) fail("forward_paged: the type of the pages must be int8, fp16 or bf16");
         if (pages[l].num_kv_heads != m->nkv || pages[l].head_dim != m->hd)
             fail("forward_paged: the pages' heads are not the model's");
         if (pages[l].device != m->device) fail("forward_paged: the pages are on another device than the model");
