@@ -111,7 +111,7 @@ RuledAttn ruled_args(const jyhip_pages* pages, const jyhip_page_tables* tables, 
     A.scale = scale;
     if (rules) {
         if (!std::isfinite(rules->cap) || rules->cap < 0.0f) fail("the cap must be finite and not negative");
-        if (rules->cap != 0.0f && !std::isfinite(scale / rules->cap)) fail("scale over the cap must be finite");
+        if (rules->cap != 0.0f && !std::isfinite(scale / rules->cap * 4.0f)) fail("scale over the cap must be finite");
         if (((uintptr_t)rules->slopes | (uintptr_t)rules->first | (uintptr_t)rules->last) % 4)
             fail("slopes, first or last are not aligned to their elements");
         A.soft = rules->cap;

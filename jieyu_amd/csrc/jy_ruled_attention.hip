@@ -22,6 +22,7 @@
 
 #include "jy_paged_attention.h"
 #include "jy_paged_attention4.h"
+#include "jy_ruled.h"
 
 namespace jy {
 
@@ -29,26 +30,13 @@ namespace {
 
 constexpr int kPages = 4096;  // positions whose pages the lanes hold at once
 
-struct Ruled {
-    RuledAttn A;
-    int ps_log2;
-    int hpg, rpg;   // heads and rows of a column group
-    int tiles;      // groups of heads per kv head
-    int groups;     // groups of rows: the most there can be
-    int chunk, splits;
-    int sstride;    // scores of one (row, head) in the workspace
-    float* part_o;  // [rows][nh][splits][hd]
-    float2* part_ml;
-    int* part_live;  // [rows] chunks that a row's group had
-    float2* ml;      // [rows][nh] the final maximum and sum
-    float* scores;   // [rows][nh][sstride], from the group's first multiple of 32 on
-};
-
 // Rows of a group: what fills 16 columns.  Single rows are groups of one.
 Ruled plan_of(const RuledAttn& A) {
     Ruled K;
     K.A = A;
     K.ps_log2 = __builtin_ctz(A.P.page_size);
+    K.sstride = 0;
+    if (plan_tiled(K)) return K;
     const int per = A.nh / A.P.num_kv_heads;
     K.hpg = std::min(per, 16);
     K.tiles = (per + 15) / 16;
@@ -89,19 +77,6 @@ size_t lay_out(Ruled& K, float* at) {
     return n;
 }
 
-// smallest / largest over a row of 16 lanes, in each of them
-template <int CTRL>
-__device__ __forceinline__ int dpp_i(int v) {
-    return __builtin_bit_cast(int, dpp_f<CTRL>(__builtin_bit_cast(float, v)));
-}
-__device__ __forceinline__ int cols_min(int v) {
-    v = min(v, dpp_i<0xB1>(v));
-    v = min(v, dpp_i<0x4E>(v));
-    v = min(v, dpp_i<0x124>(v));
-    return min(v, dpp_i<0x128>(v));
-}
-__device__ __forceinline__ int cols_max(int v) { return -cols_min(-v); }
-
 // tanh: 1 - 2 / (e^2y + 1), where that cancels the series to y^11 (its remainder under 2^-26 of tanh there)
 __device__ __forceinline__ float tanh_of(float y) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -117,43 +92,6 @@ __device__ __forceinline__ float tanh_of(float y) {
 #else
     return y;
 #endif
-}
-
-// The run and group of rows that group number `at` of the launch is: (sequence, first row), sequence -1 past
-// the last.  The lanes look at 64 runs at a time.
-struct Run {
-    int seq, row0, end;
-};
-__device__ __forceinline__ Run run_of(const Ruled& K, int at) {
-    Run r{-1, 0, 0};
-#if defined(__HIP_DEVICE_COMPILE__)
-    const int lane = threadIdx.x & 63, n = K.A.M.nseq;
-    for (int s0 = 0; s0 < n; s0 += 64) {
-        const int s = s0 + lane;
-        int a = 0, b = 0;
-        if (s < n) {
-            a = min(max(K.A.starts[s], 0), K.A.rows);
-            b = min(max(K.A.starts[s + 1], a), K.A.rows);
-        }
-        int sum = (b - a + K.rpg - 1) / K.rpg;
-        const int own = sum;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const int v = __shfl_up(sum, d);
-            if (lane >= d) sum += v;
-        }
-        const unsigned long long hit = __ballot(sum > at);
-        if (hit) {
-            const int l = __builtin_ctzll(hit);
-            r.seq = s0 + l;
-            r.row0 = __builtin_amdgcn_readlane(a, l) + (at - __builtin_amdgcn_readlane(sum - own, l)) * K.rpg;
-            r.end = __builtin_amdgcn_readlane(b, l);
-            return r;
-        }
-        at -= __builtin_amdgcn_readlane(sum, 63);
-    }
-#endif
-    return r;
 }
 
 template <int PT, int NC, bool WIDE>
@@ -670,7 +608,9 @@ void launch_ruled_attend(const RuledAttn& A, hipStream_t st) {
     Ruled K = plan_of(A);
     lay_out(K, A.part);
     const unsigned grid = (unsigned)((int64_t)K.groups * A.P.num_kv_heads * K.tiles * K.splits);
-    if (A.P.type == JYHIP_T_I4)
+    if (K.tiled)
+        launch_tiled(K, grid, st);
+    else if (A.P.type == JYHIP_T_I4)
         launch_wide<JYHIP_T_I4>(K, grid, st);
     else if (A.P.type == JYHIP_T_I8)
         launch_wide<JYHIP_T_I8>(K, grid, st);

@@ -82,15 +82,21 @@ class Cache:
         self.ka, self.va = cut(terms(k)), cut(terms(v))
 
 
-def attention64(c, b, q, pos, first, last, cap=0.0, slopes=None, scale=None, io=torch.float32):
+def attention64(c, b, q, pos, first, last, cap=0.0, slopes=None, scale=None, io=torch.float32, runs=False):
     """(out, room, p, room of p) of rows q [rows][nh][hd] of sequence b in 64 bits.
 
     fp32 scores: a sum of hd products of a query held in 24 bits is off by (hd + 2) 2^-24 S, S = scale sum |q| |k| at
     most, the factors, the cap (a tanh to 8 steps) and the bias B = slope x distance by 24 more of S and 8 of S + B.
     Weights: twice that relative, 2 n + 16 steps of the sums; 4-bit pages with bf16 queries take a weight times
     a step as one fp16 number, 2^-11 of it.  A weight far below the largest ends at 2^-39 of the largest weight times
-    value."""
+    value.
+
+    Runs of 16-bit rows: a tanh is off by 4 steps of 1, so 8 more of the cap for two scores; a weight is one number of
+    the product's type (fp16 over fp16 and 4-bit values, 2^-11; bf16 over the others, 2^-8, or 2^-16 in two parts where
+    the outputs are fp16), a 4-bit value one fp16 number, another 2^-11; and fp16 weights end at half a step of their
+    smallest, 2^-25 of the largest."""
     rows, nh, hd = q.shape
+    runs = runs and io is not torch.float32
     k, v, ka, va = c.k[b], c.v[b], c.ka[b], c.va[b]
     n, per = k.shape[0], nh // c.nkv
     scale = 1 / math.sqrt(hd) if scale is None else scale
@@ -114,12 +120,17 @@ def attention64(c, b, q, pos, first, last, cap=0.0, slopes=None, scale=None, io=
             if not m:
                 continue
             p = torch.softmax(s[r, at], 0)
-            ds = 2.0**-24 * ((hd + 24) * S[r, at].max() + 8 * (S[r, at] + B[r, at].abs()).max())
+            ds = 2.0**-24 * ((hd + 24) * S[r, at].max() + 8 * (S[r, at] + B[r, at].abs()).max() + (8 * cap if runs else 0.0))
             rel = float(2 * ds) + (2 * m + 16) * 2.0**-24
             vv, va_ = v[at][:, h // per], va[at][:, h // per]
             out[r, h] = p @ vv
             one = 2.0**-11 if c.kind == "i4" and io is torch.bfloat16 else 0.0
-            room[r, h] = (rel + one) * (p @ va_) + m * 2.0**-39 * va_.amax()
+            far = 2.0**-39
+            if runs:
+                half = c.kind in ("f16", "i4")
+                one = {"i4": 2.0**-10, "f16": 2.0**-11}[c.kind] if half else 2.0**-8 if io is torch.bfloat16 else 2.0**-16
+                far = 2.0**-25 if half else 2.0**-39
+            room[r, h] = (rel + one) * (p @ va_) + m * far * va_.amax()
             P[r, h, at], PR[r, h, at] = p, rel * p + 2.0**-126
     return out, room, P, PR
 
@@ -321,7 +332,7 @@ def test_runs(jy, mask, pool, io, nh, nkv, hd):
         at = list(range(p, p + a))
         f, l = bounds(mask, at, lens[b], rng)
         pos, first, last = pos + at, first + f, last + l
-        parts.append(attention64(c, b, q[starts[b]:starts[b + 1]], at, f, [min(x, lens[b]) for x in l], cap=6.0, slopes=slopes, io=q.dtype))
+        parts.append(attention64(c, b, q[starts[b]:starts[b + 1]], at, f, [min(x, lens[b]) for x in l], cap=6.0, slopes=slopes, io=q.dtype, runs=True))
     pos, first, last = pos + [0] * rest, first + [0] * rest, last + [1] * rest
     out = torch.full_like(q, 5.0).to(DEV)
     kw = {} if mask == "causal" else dict(first=ints(first), last=ints(last))
@@ -339,7 +350,7 @@ def test_runs_over_long_caches(jy, pool, io):
     q = torch.randn((16, 4, 64), generator=gen(4)).to(IO[io])
     starts, pos = [0, 2, 7, 16], [i for n, a in zip(lens, new) for i in range(n - a, n)]
     parts = [attention64(c, b, q[starts[b]:starts[b + 1]], pos[starts[b]:starts[b + 1]], [0] * new[b],
-                         [p + 1 for p in pos[starts[b]:starts[b + 1]]], io=q.dtype) for b in range(3)]
+                         [p + 1 for p in pos[starts[b]:starts[b + 1]]], io=q.dtype, runs=True) for b in range(3)]
     got = c.pool.attend_rows(c.layer, q.to(DEV), c.dtables, ints(starts), ints(pos), 5000)
     check(got, torch.cat([p[0] for p in parts]), torch.cat([p[1] for p in parts]))
 
@@ -354,8 +365,59 @@ def test_a_long_prompt_in_fp32(jy):
     check(got[at], want, room)
 
 
+@pytest.mark.parametrize("pool", list(POOL))
+@pytest.mark.parametrize("io", ["f16", "bf16"])
+@pytest.mark.parametrize("nh,nkv,hd,lens,new", [(32, 8, 128, [700], [700]), (4, 4, 64, [300, 129, 64], [300, 129, 1]), (24, 1, 80, [90, 65], [90, 3]),
+                                                (6, 3, 96, [3000], [200]), (8, 1, 256, [260], [260]), (14, 2, 64, [1000], [1]),
+                                                (150, 1, 16, [40, 70], [40, 7]), (2, 1, 240, [70], [66]), (28, 4, 128, [513, 5], [100, 5])])
+@pytest.mark.parametrize("rules", [False, True])
+def test_prompts(jy, pool, io, nh, nkv, hd, lens, new, rules):
+    """runs that fill the matrix products' columns, and some that do not"""
+    c = Cache(jy, lens, nkv, hd, 32, pool, seed=hd + nh)
+    total = sum(new)
+    q = torch.randn((total, nh, hd), generator=gen(4)).to(IO[io])
+    starts, pos = [0], [i for n, a in zip(lens, new) for i in range(n - a, n)]
+    for a in new:
+        starts.append(starts[-1] + a)
+    slopes = torch.rand(nh, generator=gen(1)) * 0.05
+    kw, mine = {}, {}
+    first = [max(0, p - 77) if rules else 0 for p in pos]
+    if rules:
+        kw, mine = dict(cap=5.0, slopes=slopes.to(DEV), first=ints(first)), dict(cap=5.0, slopes=slopes)
+    got = c.pool.attend_rows(c.layer, q.to(DEV), c.dtables, ints(starts), ints(pos), max(lens), **kw)
+    for b in range(len(lens)):
+        a, e = starts[b], starts[b + 1]
+        some = sorted({a, e - 1, *range(a, e, max(1, (e - a) // 40))})  # (rows all over the run)
+        want, room, _, _ = attention64(c, b, q[some], [pos[r] for r in some], [first[r] for r in some], [pos[r] + 1 for r in some],
+                                       io=q.dtype, runs=True, **mine)
+        check(got[some], want, room)
+
+
+@pytest.mark.parametrize("pool", list(POOL))
+@pytest.mark.parametrize("io", ["f32", "f16", "bf16"])
+def test_runs_over_holes(jy, pool, io):
+    """pages that do not exist are left out of a run's attention, and a run over nothing but holes gives zeros"""
+    lens = [150, 40]
+    c = Cache(jy, lens, 2, 64, 16, pool, seed=3)
+    t = c.tables.clone()
+    gone = {0: [0, 3, 4, 8], 1: [0, 1, 2]}
+    for b, pages in gone.items():
+        for i, pg in enumerate(pages):
+            t[b, pg] = [-1, 1 << 30, -(1 << 31)][i % 3]
+    q = torch.randn((190, 8, 64), generator=gen(4)).to(IO[io])
+    pos = list(range(150)) + list(range(40))
+    got = c.pool.attend_rows(c.layer, q.to(DEV), t.to(DEV), ints([0, 150, 190]), ints(pos), 150)
+    live = torch.tensor([p // 16 not in gone[0] for p in range(150)])
+    for x in ("k", "v", "ka", "va"):
+        getattr(c, x)[0] = getattr(c, x)[0][live]
+    last = [int(live[:p + 1].sum()) for p in range(150)]
+    want, room, _, _ = attention64(c, 0, q[:150], pos[:150], [0] * 150, last, io=q.dtype, runs=True)
+    check(got[:150], want, room)
+    assert not got[:16].any() and not got[150:].any()
+
+
 @pytest.mark.parametrize("pool", ["f16", "bf16", "i8", "i4"])
-@pytest.mark.parametrize("io", ["f32", "bf16"])
+@pytest.mark.parametrize("io", ["f32", "f16", "bf16"])
 def test_values_that_are_not_finite_reach_only_rows_that_see_them(jy, pool, io):
     n = 70
     c = Cache(jy, [n], 2, 64, 16, pool, seed=5)
@@ -419,6 +481,23 @@ def test_4bit_values_of_any_size(jy, size, io):
     c.k, c.v, c.ka, c.va = [k], [v], [3 * k.abs().amax(-1, keepdim=True).expand_as(k)], [3 * v.abs().amax(-1, keepdim=True).expand_as(v)]
     q = torch.randn((1, 4, 128), generator=gen(2)).to(IO[io])
     check(c.pool.attend(c.layer, q.to(DEV), c.dtables, c.dlens, 90), *single(c, q)[:2])
+
+
+@pytest.mark.parametrize("io", ["f16", "bf16"])
+@pytest.mark.parametrize("pool", list(POOL))
+def test_strides_of_prompts(jy, io, pool):
+    """heads that do not start at multiples of 16 bytes"""
+    c = Cache(jy, [70], 2, 48, 16, pool, seed=10)
+    fused = torch.randn((70, 6, 51), generator=gen(3)).to(IO[io]).to(DEV)
+    q = fused[:, 1:5, 1:49]
+    buf = torch.full((72, 4, 60), 7.0, dtype=IO[io], device=DEV)
+    out = buf[1:71, :, 3:51]
+    c.pool.attend_rows(c.layer, q, c.dtables, ints([0, 70]), ints(list(range(70))), 70, out=out)
+    want, room, _, _ = attention64(c, 0, q.cpu(), list(range(70)), [0] * 70, [i + 1 for i in range(70)], io=q.dtype, runs=True)
+    check(out, want, room)
+    left = buf.clone()
+    left[1:71, :, 3:51] = 7.0
+    assert (left == 7.0).all()
 
 
 @pytest.mark.parametrize("io", list(IO))
