@@ -81,6 +81,14 @@ struct Half<false> {
         return c;
 #endif
     }
+    // both numbers of a word added to l
+    static __device__ __forceinline__ float both(uint32_t w, float l) {
+#if defined(__HIP_DEVICE_COMPILE__)
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2_t, w), h2_t{(_Float16)1.0f, (_Float16)1.0f}, l, false);
+#else
+        return l;
+#endif
+    }
 };
 template <>
 struct Half<true> {
@@ -92,6 +100,9 @@ struct Half<true> {
 #else
         return c;
 #endif
+    }
+    static __device__ __forceinline__ float both(uint32_t w, float l) {
+        return l + __builtin_bit_cast(float, w << 16) + __builtin_bit_cast(float, w & 0xffff0000u);
     }
 };
 
@@ -123,6 +134,8 @@ struct Form {
     static constexpr int G = HDT == 1 ? 2 : HDT == 2 ? 4 : 8;  // groups of a 4-bit vector
     static constexpr int STEPS = HD / 16, DT = HD / 32;        // steps of the first product, tiles of outputs
     static constexpr int BYTES = I8 ? HD : I4 ? 16 * G : 2 * HD;  // of a vector in its page, at most
+    // where a chunk of key `key`'s values lies in its row: pairs of chunks side by side, those of 4 neighbouring keys apart
+    static __host__ __device__ __forceinline__ constexpr int vchunk(int key, int chunk) { return chunk ^ (2 * key & MASK); }
     // what a thread brings of a tile's keys (and as much of its values), in 16-byte units (4 bits: a key's quarter)
     static constexpr int UNITS = I4 ? (G + 3) / 4 : BN * (BYTES / 16) / NT;
 };
@@ -131,7 +144,7 @@ template <class F>
 struct Staged {
     u4_t k[F::UNITS], v[F::UNITS];
     u4_t kw[F::I4 ? (F::G + 3) / 4 : 1], vw[F::I4 ? (F::G + 3) / 4 : 1];
-    float ks, vs;  // int8: thread t < 64 has key t's
+    float ks, vs;  // int8: lane l < 16 of wave w has those of key 16 w + l
 };
 
 template <class F>
@@ -247,6 +260,7 @@ __global__ __launch_bounds__(NT, HDT <= 2 ? 2 : 1) void tiled_attend_kernel(Rule
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 y[e] = bad ? 0.0f : F::SCALED ? __builtin_ldexpf((float)x[s][e], e2) : (float)x[s][e];
+                if (A.scale < 0.0f) y[e] = -y[e];
                 a[e] = (typename HK::E)y[e];
                 if constexpr (F::I4) sum[s / 2] += y[e];
             }
@@ -267,24 +281,19 @@ __global__ __launch_bounds__(NT, HDT <= 2 ? 2 : 1) void tiled_attend_kernel(Rule
             sums = __builtin_bit_cast(u4_t, w);
         }
         const float unit = F::SCALED ? __builtin_ldexpf(1.0f, -e2) : 1.0f;
-        qf = bad ? __builtin_nanf("") : unit * (A.soft != 0.0f ? A.scale / A.soft * (2.0f * kLog2e) : A.scale * kLog2e);
+        qf = bad ? __builtin_nanf("") : unit * (A.soft != 0.0f ? fabsf(A.scale) / A.soft : fabsf(A.scale) * kLog2e);
     }
+    const bool simple = !(fabsf(A.scale) < 0x1p-60f);
     const float soft = A.soft * kLog2e, slope = A.slopes ? A.slopes[head] * kLog2e : 0.0f;
 
-    // LDS addresses, in bytes: of a key's chunks for the first product, and of the values' columns for the second
-    uint32_t koff[F::STEPS];
-#pragma unroll
-    for (int s = 0; s < F::STEPS; s++)
-        koff[s] = (uint32_t)((lane & 31) * F::ROW + (((2 * s + half) ^ (lane & F::MASK)) * 16));
-    uint32_t voff[2][F::DT];
+    // LDS addresses, in bytes: of a key's chunk of step 0 for the first product, and of the values' columns of tile 0
+    // (for keys 0 .. 3 and 8 .. 11 of a half) for the second.  Step s and tile t lie an exclusive or with 32 s or 64 t away.
+    const uint32_t koff = (uint32_t)((lane & 31) * F::ROW + ((half ^ (lane & F::MASK)) * 16));
+    uint32_t voff[2];
 #pragma unroll
     for (int e = 0; e < 2; e++) {
         const int key = 8 * e + 4 * half + (lane & 15) / 4;  // (a multiple of 16 further on in the reads)
-#pragma unroll
-        for (int t = 0; t < F::DT; t++) {
-            const int chunk = 4 * t + 2 * (lane >> 4 & 1) + (lane & 3) / 2;
-            voff[e][t] = (uint32_t)(key * F::ROW + ((chunk ^ (key & F::MASK)) * 16) + (lane & 1) * 8);
-        }
+        voff[e] = (uint32_t)(key * F::ROW + F::vchunk(key, 2 * (lane >> 4 & 1) + (lane & 3) / 2) * 16 + (lane & 1) * 8);
     }
 
     const int64_t first = (int64_t)kvh * P.page_size, page_rows = (int64_t)nkv * P.page_size;
@@ -292,75 +301,79 @@ __global__ __launch_bounds__(NT, HDT <= 2 ? 2 : 1) void tiled_attend_kernel(Rule
     const int row_bytes = F::I4 ? 16 * F::G : F::I8 ? hd : 2 * hd;
     const int units = row_bytes / 16;
 
-    // where a position lies, among the positions of all pages and heads (-1: nowhere, or not to be read)
-    auto place = [&](int j, int from, int to) -> int64_t {
-        if (j < from || j >= to) return -1;
-        const int i = j >> K.ps_log2;
-        if (i >= A.M.stride) return -1;
-        const int page = table[i];
-        if ((unsigned)page >= (unsigned)P.num_pages) return -1;
-        return page * page_rows + first + (j & (P.page_size - 1));
-    };
-    auto pages = [&](int t0) -> uint32_t {
+    // The page of each of a tile's four groups of 16 positions, in lanes 0 .. 3 (and again behind them).
+    auto pages = [&](int t0) -> int {
         const int i = (t0 + 16 * (lane & 3)) >> K.ps_log2;
-        return (uint32_t)__ballot(i < A.M.stride && (unsigned)table[min(i, A.M.stride - 1)] < (unsigned)P.num_pages) & 15u;
+        return i < A.M.stride ? table[i] : -1;
     };
-    auto bring = [&](Staged<F>& g, int t0, int from, int to) {
+    // A unit's loads lie within one group for all lanes of a wave, so they go through a buffer over the group's
+    // positions below `to`: others read as zeros.
+    constexpr int PER = F::I4 ? 4 : F::BYTES / 16;  // threads that share a key
+    const int key16 = tid / PER & 15;
+    const uint32_t voff_k = F::I4 ? (uint32_t)(key16 * row_bytes + (tid & 3) * 4 * F::G)
+                            : tid % PER < units ? (uint32_t)(key16 * row_bytes + tid % PER * 16)
+                                                : kNowhere;
+    auto bring = [&](Staged<F>& g, int ids, int t0, int from, int to) {
+        auto group = [&](int grp, int& live) -> int64_t {  // its first position among those of all pages and heads
+            const int page = __builtin_amdgcn_readlane(ids, grp), at = t0 + 16 * grp;
+            const bool here = (unsigned)page < (unsigned)P.num_pages;
+            live = __builtin_amdgcn_readfirstlane(here ? min(max(to - at, 0), 16) : 0);
+            return (here ? page * page_rows : 0) + first + (at & (P.page_size - 1));
+        };
+        auto buffer = [](const void* p, int bytes) {
+            return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, bytes, 0x00020000);
+        };
+        auto load16 = [](auto r, uint32_t off) { return __builtin_bit_cast(u4_t, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, 0)); };
+        auto load8 = [](auto r, uint32_t off) {
+            const u2_t x = __builtin_bit_cast(u2_t, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0));
+            return u4_t{x[0], x[1], 0, 0};
+        };
         if constexpr (F::I4) {
-            const int64_t r = place(t0 + tid / 4, from, to);
-            const int quarter = tid & 3;
+            int live;
+            const int64_t r = group(wave, live);
+            const bool out = key16 < from - (t0 + 16 * wave);
+            const uint32_t off = out ? kNowhere : voff_k, woff = out ? kNowhere : (uint32_t)(key16 * 4 * F::G);
+            const auto kr = buffer(static_cast<const char*>(P.k) + r * row_bytes, live * row_bytes);
+            const auto vr = buffer(static_cast<const char*>(P.v) + r * row_bytes, live * row_bytes);
+            const auto kwr = buffer(reinterpret_cast<const char*>(P.k_scale) + r * (4 * F::G), live * (4 * F::G));
+            const auto vwr = buffer(reinterpret_cast<const char*>(P.v_scale) + r * (4 * F::G), live * (4 * F::G));
+            if constexpr (F::G == 2) {
+                g.k[0] = load8(kr, off);
+                g.v[0] = load8(vr, off);
+                g.kw[0] = load8(kwr, woff);
+                g.vw[0] = load8(vwr, woff);
+            } else {
 #pragma unroll
-            for (int u = 0; u < F::UNITS; u++) g.k[u] = g.v[u] = u4_t{};
-#pragma unroll
-            for (int u = 0; u < (F::G + 3) / 4; u++) g.kw[u] = g.vw[u] = u4_t{};
-            if (r >= 0) {
-                const char* const k = static_cast<const char*>(P.k) + r * row_bytes + quarter * 4 * F::G;
-                const char* const v = static_cast<const char*>(P.v) + r * row_bytes + quarter * 4 * F::G;
-                const char* const kw = reinterpret_cast<const char*>(P.k_scale) + r * (4 * F::G);
-                const char* const vw = reinterpret_cast<const char*>(P.v_scale) + r * (4 * F::G);
-                if constexpr (F::G == 2) {
-                    const u2_t a = *reinterpret_cast<const u2_t*>(k), b = *reinterpret_cast<const u2_t*>(v);
-                    const u2_t c = *reinterpret_cast<const u2_t*>(kw), d = *reinterpret_cast<const u2_t*>(vw);
-                    g.k[0] = u4_t{a[0], a[1], 0, 0};
-                    g.v[0] = u4_t{b[0], b[1], 0, 0};
-                    g.kw[0] = u4_t{c[0], c[1], 0, 0};
-                    g.vw[0] = u4_t{d[0], d[1], 0, 0};
-                } else {
-#pragma unroll
-                    for (int u = 0; u < F::UNITS; u++) {
-                        g.k[u] = reinterpret_cast<const u4_t*>(k)[u];
-                        g.v[u] = reinterpret_cast<const u4_t*>(v)[u];
-                        g.kw[u] = reinterpret_cast<const u4_t*>(kw)[u];
-                        g.vw[u] = reinterpret_cast<const u4_t*>(vw)[u];
-                    }
+                for (int u = 0; u < F::UNITS; u++) {
+                    g.k[u] = load16(kr, off + 16 * u);
+                    g.v[u] = load16(vr, off + 16 * u);
+                    g.kw[u] = load16(kwr, woff + 16 * u);
+                    g.vw[u] = load16(vwr, woff + 16 * u);
                 }
             }
         } else {
-            constexpr int PER = F::BYTES / 16;  // units of a whole row
 #pragma unroll
             for (int u = 0; u < F::UNITS; u++) {
-                const int i = u * NT + tid, key = i / PER, c = i % PER;
-                const int64_t r = c < units ? place(t0 + key, from, to) : -1;
-                g.k[u] = g.v[u] = u4_t{};
-                if (r >= 0) {
-                    g.k[u] = reinterpret_cast<const u4_t*>(static_cast<const char*>(P.k) + r * row_bytes)[c];
-                    g.v[u] = reinterpret_cast<const u4_t*>(static_cast<const char*>(P.v) + r * row_bytes)[c];
-                }
+                const int grp = (u * NT + 64 * wave) / PER / 16;
+                int live;
+                const int64_t r = group(grp, live);
+                // (rows of 32 units: every other one is the group's second half)
+                const int key = key16 + (PER == 32 && (u & 1) ? 8 : 0);
+                const uint32_t off = key < from - (t0 + 16 * grp) ? kNowhere : voff_k + (uint32_t)(PER == 32 && (u & 1) ? 8 * row_bytes : 0);
+                g.k[u] = load16(buffer(static_cast<const char*>(P.k) + r * row_bytes, live * row_bytes), off);
+                g.v[u] = load16(buffer(static_cast<const char*>(P.v) + r * row_bytes, live * row_bytes), off);
             }
             if constexpr (F::I8) {
-                g.ks = g.vs = 0.0f;
-                if (tid < BN) {
-                    const int64_t r = place(t0 + tid, from, to);
-                    if (r >= 0) {
-                        g.ks = P.k_scale[r];
-                        g.vs = P.v_scale[r];
-                    }
-                }
+                int live;
+                const int64_t r = group(wave, live);
+                const uint32_t off = lane < 16 && lane >= from - (t0 + 16 * wave) ? (uint32_t)(4 * lane) : kNowhere;
+                g.ks = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(buffer(P.k_scale + r, 4 * live), off, 0, 0));
+                g.vs = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(buffer(P.v_scale + r, 4 * live), off, 0, 0));
             }
         }
     };
-    // into LDS as the products take it; whether a value is not finite
-    auto put = [&](const Staged<F>& g, int buf) -> bool {
+    // into LDS as the products take it; with `ask`, whether a value is not finite
+    auto put = [&](const Staged<F>& g, int buf, bool ask) -> bool {
         char* const ks = reinterpret_cast<char*>(sh.k[buf]);
         char* const vs = reinterpret_cast<char*>(sh.v[buf]);
         bool odd = false;
@@ -394,15 +407,16 @@ __global__ __launch_bounds__(NT, HDT <= 2 ? 2 : 1) void tiled_attend_kernel(Rule
                 if (32 * c + 8 * quarter >= hd) a = b = u4_t{};
                 const uint32_t off = (uint32_t)(key * F::ROW + (((4 * c + quarter) ^ (key & F::MASK)) * 16));
                 *reinterpret_cast<u4_t*>(ks + off) = a;
-                *reinterpret_cast<u4_t*>(vs + off) = b;
-                odd |= infinite16(b[0], false) || infinite16(b[1], false) || infinite16(b[2], false) || infinite16(b[3], false);
+                *reinterpret_cast<u4_t*>(vs + key * F::ROW + F::vchunk(key, 4 * c + quarter) * 16) = b;
+                if (ask)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) odd |= infinite16(b[i], false);
                 if (quarter == 0) sh.low[buf][key][c] = 32 * c < hd ? x.y : (_Float16)0.0f;
             }
             if (quarter == 0)
 #pragma unroll
                 for (int c = F::G; c < 8; c++) sh.low[buf][key][c] = (_Float16)0.0f;
         } else {
-            constexpr int PER = F::BYTES / 16;
 #pragma unroll
             for (int u = 0; u < F::UNITS; u++) {
                 const int i = u * NT + tid, key = i / PER, c = i % PER;
@@ -421,20 +435,21 @@ __global__ __launch_bounds__(NT, HDT <= 2 ? 2 : 1) void tiled_attend_kernel(Rule
                             *reinterpret_cast<u4_t*>(ks + off) = wide(g.k[u][2 * p], g.k[u][2 * p + 1], HK{});
                         else
                             *reinterpret_cast<u4_t*>(ks + off) = __builtin_bit_cast(u4_t, q8_to_h8(g.k[u][2 * p], g.k[u][2 * p + 1]));
-                        *reinterpret_cast<u4_t*>(vs + off) = wide(g.v[u][2 * p], g.v[u][2 * p + 1], HV{});
+                        *reinterpret_cast<u4_t*>(vs + key * F::ROW + F::vchunk(key, 2 * c + p) * 16) = wide(g.v[u][2 * p], g.v[u][2 * p + 1], HV{});
                     }
                 } else {
                     const uint32_t off = (uint32_t)(key * F::ROW + ((c ^ (key & F::MASK)) * 16));
                     *reinterpret_cast<u4_t*>(ks + off) = g.k[u];
-                    *reinterpret_cast<u4_t*>(vs + off) = g.v[u];
+                    *reinterpret_cast<u4_t*>(vs + key * F::ROW + F::vchunk(key, c) * 16) = g.v[u];
+                    if (ask)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) odd |= infinite16(g.v[u][i], F::VBF);
+                        for (int i = 0; i < 4; i++) odd |= infinite16(g.v[u][i], F::VBF);
                 }
             }
             if constexpr (F::I8)
-                if (tid < BN) {
-                    sh.ks[buf][tid] = g.ks;
-                    sh.vs[buf][tid] = g.vs;
+                if (lane < 16) {
+                    sh.ks[buf][16 * wave + lane] = g.ks;
+                    sh.vs[buf][16 * wave + lane] = g.vs;
                 }
         }
         return odd;
@@ -445,6 +460,8 @@ __global__ __launch_bounds__(NT, HDT <= 2 ? 2 : 1) void tiled_attend_kernel(Rule
     // one tile from LDS
     auto work = [&](int buf, int t0, uint32_t there) {
         const char* const ks = reinterpret_cast<const char*>(sh.k[buf]);
+        uint32_t ko = koff, vo[2] = {voff[0], voff[1]};
+        asm volatile("" : "+v"(ko), "+v"(vo[0]), "+v"(vo[1]));  // (the addresses made from them are not kept in registers)
         f16_t s[2];
 #pragma unroll
         for (int n = 0; n < 2; n++) {
@@ -455,49 +472,75 @@ __global__ __launch_bounds__(NT, HDT <= 2 ? 2 : 1) void tiled_attend_kernel(Rule
             }
 #pragma unroll
             for (int i = 0; i < F::STEPS; i++) {
-                const u4_t a = *reinterpret_cast<const u4_t*>(ks + 32 * n * F::ROW + koff[i]);
+                const u4_t a = *reinterpret_cast<const u4_t*>(ks + 32 * n * F::ROW + (ko ^ (32u * i)));
 #pragma unroll
                 for (int p = F::QP - 1; p >= 0; p--) s[n] = HK::mul(a, q[i][p], s[n]);
             }
         }
-        float top = kNone;
         const bool masked = t0 < w_all_lo || t0 + BN > w_all_hi || there != 15u;
+        auto mask = [&](float none) {
+            asm volatile("");  // (a branch)
 #pragma unroll
-        for (int n = 0; n < 2; n++) {
-#pragma unroll
-            for (int b = 0; b < 4; b++) {
-                f4_t f = {qf, qf, qf, qf};
-                if constexpr (F::I8) {
-                    const f4_t x = *reinterpret_cast<const f4_t*>(&sh.ks[buf][32 * n + 8 * b + 4 * half]);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) f[i] = qf * x[i];
-                }
-#pragma unroll
-                for (int i = 0; i < 4; i++) s[n][4 * b + i] *= f[i];
-            }
-            if (A.soft != 0.0f) {  // (qf has made it 2 log2 e times what the tanh is of)
-#pragma unroll
-                for (int i = 0; i < 16; i++)
-                    s[n][i] = __builtin_fmaf(-2.0f * soft, __builtin_amdgcn_rcpf(exp2_hw(s[n][i]) + 1.0f), soft);
-            }
-            if (A.slopes) {
-                const float d = (float)(pos - t0 - 32 * n - 4 * half);
-#pragma unroll
-                for (int i = 0; i < 16; i++)
-                    s[n][i] = __builtin_fmaf(-slope, fabsf(d - (float)(8 * (i >> 2) + (i & 3))), s[n][i]);
-            }
-            if (masked) {
-                asm volatile("");
+            for (int n = 0; n < 2; n++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     const int j = t0 + 32 * n + 8 * (i >> 2) + 4 * half + (i & 3);
-                    s[n][i] = j < lo || j >= hi || !(there >> (2 * n + (i >> 3)) & 1u) ? -__builtin_inff() : s[n][i];
+                    s[n][i] = j < lo || j >= hi || !(there >> (2 * n + (i >> 3)) & 1u) ? none : s[n][i];
+                }
+        };
+        auto largest = [&](float sign) {
+            float top = -__builtin_inff();
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) top = fmaxf(top, sign * s[n][i]);
+            return half_max(top);
+        };
+        if constexpr (F::I8) {
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int b = 0; b < 4; b++) {
+                    const f4_t x = *reinterpret_cast<const f4_t*>(&sh.ks[buf][32 * n + 8 * b + 4 * half]);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) s[n][4 * b + i] *= x[i];
+                }
+        }
+        // s becomes the exponents, scores in units of log2 e less the running maximum: without cap or bias by one fma (but
+        // where qf could be 0, which -infinity cannot be multiplied with); capped ones that all lie within half the cap by
+        // tanh y = y (c0 + c1 y^2 + c2 y^4 + c3 y^6) to 1.3e-7 (fitted), five operations; else step by step.
+        float top = largest(1.0f);
+        int way = A.slopes || (A.soft != 0.0f && masked) || !simple ? 2 : A.soft != 0.0f ? 1 : 0;
+        if (way == 1 && __any(!(fmaxf(top, largest(-1.0f)) * qf <= 0.5f))) way = 2;
+        const float sq = soft * qf, q2 = qf * qf;
+        auto rest = [&](float x) {
+            const float y = x * x * q2;
+            return __builtin_fmaf(y, __builtin_fmaf(y, __builtin_fmaf(y, -0.04337234f, 0.13145139f), -0.33320654f), 0.99999768f);
+        };
+        if (way == 2) {
+            const float twice = 2.0f * kLog2e;
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                if (A.soft != 0.0f) {  // 1 - 2 / (e^2y + 1)
+#pragma unroll
+                    for (int i = 0; i < 16; i++)
+                        s[n][i] = __builtin_fmaf(-2.0f * soft, __builtin_amdgcn_rcpf(exp2_hw(s[n][i] * qf * twice) + 1.0f), soft);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; i++) s[n][i] *= qf;
+                }
+                if (A.slopes) {
+                    const float d = (float)(pos - t0 - 32 * n - 4 * half);
+#pragma unroll
+                    for (int i = 0; i < 16; i++)
+                        s[n][i] = __builtin_fmaf(-slope, fabsf(d - (float)(8 * (i >> 2) + (i & 3))), s[n][i]);
                 }
             }
-#pragma unroll
-            for (int i = 0; i < 16; i++) top = fmaxf(top, s[n][i]);
         }
-        top = half_max(top);
+        if (masked) mask(-__builtin_inff());
+        if (way == 2 || masked) top = largest(1.0f);
+        top = way == 2 ? top : way == 1 ? top * sq * rest(top) : top * qf;
+        // the running maximum moves when the tile's is over it by more than 2^6, and at first
         if (__any(top > m + 6.0f)) {
             const float mn = top > m + 6.0f ? top : m;
             const float a = exp2_hw(m - mn);
@@ -508,6 +551,19 @@ __global__ __launch_bounds__(NT, HDT <= 2 ? 2 : 1) void tiled_attend_kernel(Rule
 #pragma unroll
                 for (int i = 0; i < 16; i++) o[t][i] *= a;
         }
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
+            if (way == 0) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) s[n][i] = __builtin_fmaf(s[n][i], qf, -m);
+            } else if (way == 1) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) s[n][i] = __builtin_fmaf(s[n][i] * sq, rest(s[n][i]), -m);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; i++) s[n][i] -= m;
+            }
+        }
         const char* const vs = reinterpret_cast<const char*>(sh.v[buf]);
 #pragma unroll
         for (int n = 0; n < 2; n++) {
@@ -517,7 +573,7 @@ __global__ __launch_bounds__(NT, HDT <= 2 ? 2 : 1) void tiled_attend_kernel(Rule
                 {
                     float w[8];
 #pragma unroll
-                    for (int e = 0; e < 8; e++) w[e] = exp2_hw(s[n][8 * c + e] - m);
+                    for (int e = 0; e < 8; e++) w[e] = exp2_hw(s[n][8 * c + e]);
                     if constexpr (F::I8) {
 #pragma unroll
                         for (int e = 0; e < 8; e++) l += w[e];
@@ -536,11 +592,11 @@ __global__ __launch_bounds__(NT, HDT <= 2 ? 2 : 1) void tiled_attend_kernel(Rule
                     } else {
                         typename HV::V a;
 #pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            a[e] = (typename HV::E)w[e];
-                            if constexpr (!F::I8) l += (float)a[e];
-                        }
+                        for (int e = 0; e < 8; e++) a[e] = (typename HV::E)w[e];
                         p[0] = __builtin_bit_cast(u4_t, a);
+                        if constexpr (!F::I8)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) l = HV::both(p[0][e], l);
                     }
                 }
 #pragma unroll
@@ -549,7 +605,7 @@ __global__ __launch_bounds__(NT, HDT <= 2 ? 2 : 1) void tiled_attend_kernel(Rule
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
                         const auto x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (__attribute__((address_space(3))) s4_t*)(vs + (32 * n + 16 * c) * F::ROW + voff[e][t]));
+                            (__attribute__((address_space(3))) s4_t*)(vs + (32 * n + 16 * c) * F::ROW + (vo[e] ^ (64u * t))));
                         const u2_t y = __builtin_bit_cast(u2_t, x);
                         a[2 * e] = y[0];
                         a[2 * e + 1] = y[1];
@@ -575,24 +631,23 @@ __global__ __launch_bounds__(NT, HDT <= 2 ? 2 : 1) void tiled_attend_kernel(Rule
         l = 0.0f;
         bool odd = false;
         Staged<F> g;
-        uint32_t there = 0, next = 0;  // which of a tile's four groups of 16 positions have a page
+        int ids = -1, next = -1;  // the pages of this tile and of the next
         if (c0 < end) {
             next = pages(c0);
-            bring(g, c0, s_from, s_to);
+            bring(g, next, c0, s_from, s_to);
         }
         for (int t0 = c0, buf = 0; t0 < end; t0 += BN, buf ^= 1) {
-            const bool some = put(g, buf);
-            if (!F::I8 && only < 0 && some && (t0 < all_lo || t0 + BN > all_hi)) sh.odd[buf] = 1;
+            ids = next;
+            if (t0 + BN < end) next = pages(t0 + BN);
+            const bool ask = !F::I8 && only < 0 && (t0 < all_lo || t0 + BN > all_hi);
+            if (put(g, buf, ask)) sh.odd[buf] = 1;
             __syncthreads();
-            if (!F::I8 && only < 0 && sh.odd[buf]) {  // (this buffer's flag is not set again before all have read it)
+            if (ask && sh.odd[buf]) {  // (this buffer's flag is not set again before all have read it)
                 odd = true;
                 break;
             }
-            there = next;
-            if (t0 + BN < end) {
-                next = pages(t0 + BN);
-                bring(g, t0 + BN, s_from, s_to);
-            }
+            if (t0 + BN < end) bring(g, next, t0 + BN, s_from, s_to);
+            const uint32_t there = (uint32_t)__ballot((unsigned)ids < (unsigned)P.num_pages) & 15u;
             if (t0 < w_to && t0 + BN > w_from) work(buf, t0, there);
         }
         if (odd) {
