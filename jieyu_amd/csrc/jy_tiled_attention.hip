@@ -102,7 +102,12 @@ struct Half<true> {
 #endif
     }
     static __device__ __forceinline__ float both(uint32_t w, float l) {
-        return l + __builtin_bit_cast(float, w << 16) + __builtin_bit_cast(float, w & 0xffff0000u);
+#if defined(__HIP_DEVICE_COMPILE__)
+        typedef __bf16 b2_t __attribute__((ext_vector_type(2)));
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2_t, w), b2_t{(__bf16)1.0f, (__bf16)1.0f}, l, false);
+#else
+        return l;
+#endif
     }
 };
 
@@ -285,6 +290,10 @@ __global__ __launch_bounds__(NT, HDT <= 2 ? 2 : 1) void tiled_attend_kernel(Rule
     }
     const bool simple = !(fabsf(A.scale) < 0x1p-60f);
     const float soft = A.soft * kLog2e, slope = A.slopes ? A.slopes[head] * kLog2e : 0.0f;
+
+    // cap tanh(qf x) of a raw score x within half the cap, as a polynomial: x (p0 + p1 x^2 + p2 x^4 + p3 x^6)
+    const float q2 = qf * qf, p0 = 0.99999768f * (soft * qf), p1 = -0.33320654f * (soft * qf) * q2;
+    const float p2 = 0.13145139f * (soft * qf) * q2 * q2, p3 = -0.04337234f * (soft * qf) * q2 * q2 * q2;
 
     // LDS addresses, in bytes: of a key's chunk of step 0 for the first product, and of the values' columns of tile 0
     // (for keys 0 .. 3 and 8 .. 11 of a half) for the second.  Step s and tile t lie an exclusive or with 32 s or 64 t away.
@@ -508,14 +517,15 @@ __global__ __launch_bounds__(NT, HDT <= 2 ? 2 : 1) void tiled_attend_kernel(Rule
         }
         // s becomes the exponents, scores in units of log2 e less the running maximum: without cap or bias by one fma (but
         // where qf could be 0, which -infinity cannot be multiplied with); capped ones that all lie within half the cap by
-        // tanh y = y (c0 + c1 y^2 + c2 y^4 + c3 y^6) to 1.3e-7 (fitted), five operations; else step by step.
+        // a polynomial (tanh to 1.3e-7, fitted) in five operations; else step by step.
         float top = largest(1.0f);
         int way = A.slopes || (A.soft != 0.0f && masked) || !simple ? 2 : A.soft != 0.0f ? 1 : 0;
-        if (way == 1 && __any(!(fmaxf(top, largest(-1.0f)) * qf <= 0.5f))) way = 2;
-        const float sq = soft * qf, q2 = qf * qf;
-        auto rest = [&](float x) {
-            const float y = x * x * q2;
-            return __builtin_fmaf(y, __builtin_fmaf(y, __builtin_fmaf(y, -0.04337234f, 0.13145139f), -0.33320654f), 0.99999768f);
+        // (the coefficients stay normal numbers for qf from 2^-16 on)
+        if (way == 1 && __any(!(fmaxf(top, largest(-1.0f)) * qf <= 0.5f && qf >= 0x1p-16f))) way = 2;
+        way = __builtin_amdgcn_readfirstlane(way);
+        auto capped = [&](float x, float less) {
+            const float x2 = x * x;
+            return __builtin_fmaf(x, __builtin_fmaf(x2, __builtin_fmaf(x2, __builtin_fmaf(x2, p3, p2), p1), p0), less);
         };
         if (way == 2) {
             const float twice = 2.0f * kLog2e;
@@ -539,7 +549,7 @@ __global__ __launch_bounds__(NT, HDT <= 2 ? 2 : 1) void tiled_attend_kernel(Rule
         }
         if (masked) mask(-__builtin_inff());
         if (way == 2 || masked) top = largest(1.0f);
-        top = way == 2 ? top : way == 1 ? top * sq * rest(top) : top * qf;
+        top = way == 2 ? top : way == 1 ? capped(top, 0.0f) : top * qf;
         // the running maximum moves when the tile's is over it by more than 2^6, and at first
         if (__any(top > m + 6.0f)) {
             const float mn = top > m + 6.0f ? top : m;
@@ -558,7 +568,7 @@ __global__ __launch_bounds__(NT, HDT <= 2 ? 2 : 1) void tiled_attend_kernel(Rule
                 for (int i = 0; i < 16; i++) s[n][i] = __builtin_fmaf(s[n][i], qf, -m);
             } else if (way == 1) {
 #pragma unroll
-                for (int i = 0; i < 16; i++) s[n][i] = __builtin_fmaf(s[n][i] * sq, rest(s[n][i]), -m);
+                for (int i = 0; i < 16; i++) s[n][i] = capped(s[n][i], -m);
             } else {
 #pragma unroll
                 for (int i = 0; i < 16; i++) s[n][i] -= m;
