@@ -4,7 +4,8 @@
 // need-th largest is found by three counts over its digits (12, 10 and 10 bits, bins in LDS, whole numbers: the
 // order of the atomics does not matter); the first digit is sign, exponent and three bits of the fraction, so
 // that the weights of a sequence spread over dozens of bins.  A last pass over the positions in order takes
-// what lies above that weight, of those equal to it the first, and the recent ones.
+// what lies above that weight, of those equal to it the first, and the recent ones.  Up to 35840 positions the
+// numbers stay in LDS and the weights are read once, 16 of a thread under way at a time.
 // Moving: 16 lanes a vector, key and value together, bytes as they are.
 #include <hip/hip_runtime.h>
 
@@ -17,113 +18,205 @@ namespace jy {
 
 namespace {
 
-constexpr int NT = 1024, PER = 4;  // threads; positions a thread takes at a time
+typedef uint32_t u4_t __attribute__((ext_vector_type(4)));
+typedef float f4_t __attribute__((ext_vector_type(4), aligned(4)));  // (four elements from any)
+
+constexpr int NT = 1024, PER = 4;  // threads; positions a thread takes side by side
+constexpr int AHEAD = 4;           // and so many times at once
 constexpr int BINS = 4096;
+constexpr int kHeld = 140 * 1024;  // bytes of LDS for ranks, beside the bins
 
 struct EvictArgs {
     Eviction E;
     int ps_log2;
 };
 
-// rises with the weight: NaN lowest, then -infinity .. +infinity, both zeros the same
+// rises with the weight, from 1 on: NaN lowest, then -infinity .. +infinity, both zeros the same; and back
 __device__ __forceinline__ uint32_t rank_of(float w) {
-    if (!(w == w)) return 0;
+    if (!(w == w)) return 1;
     const uint32_t u = __builtin_bit_cast(uint32_t, w + 0.0f);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// exclusive sum over the workgroup's threads, and the whole
-__device__ __forceinline__ uint32_t scan(uint32_t v, uint32_t* part, uint32_t& total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    uint32_t s = v;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const uint32_t x = __shfl_up(s, d);
-        if (lane >= d) s += x;
-    }
-    __syncthreads();  // (the last scan's parts are read)
-    if (lane == 63) part[wave] = s;
-    __syncthreads();
-    uint32_t before = 0;
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < NT / 64; w++) {
-        const uint32_t x = part[w];
-        before += w < wave ? x : 0;
-        total += x;
-    }
-    return before + s - v;
+__device__ __forceinline__ float weight_of(uint32_t r) {
+    return r == 1 ? __builtin_nanf("") : __builtin_bit_cast(float, r & 0x80000000u ? r ^ 0x80000000u : ~r);
 }
 
+// inclusive sum over the wave's lanes by DPP moves (within rows of 16, then each row's last to those behind it)
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);
+#endif
+    return v;
+}
+
+// exclusive sums over the workgroup's threads, of N numbers at once, and the whole
+template <int N>
+__device__ __forceinline__ void scan(uint32_t (&v)[N], uint32_t (*part)[NT / 64], uint32_t (&total)[N]) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    static_assert(NT == 1024, "one row of lanes holds the waves' sums");
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    uint32_t s[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) s[i] = wave_scan(v[i]);
+    __syncthreads();  // (the last scan's parts are read)
+    if (lane == 63)
+#pragma unroll
+        for (int i = 0; i < N; i++) part[i][wave] = s[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const uint32_t all = wave_scan(part[i][lane & 15]);  // (lane 15 has the whole)
+        total[i] = (uint32_t)__builtin_amdgcn_readlane((int)all, 15);
+        const uint32_t before = wave ? (uint32_t)__builtin_amdgcn_readlane((int)all, wave - 1) : 0u;
+        v[i] = before + s[i] - v[i];
+    }
+#endif
+}
+
+// The bin (into found[0]) in which the left-th largest lies, counted from the largest bin down; how many lie above it.
+__device__ __forceinline__ uint32_t border(const uint32_t* bins, int size, uint32_t left, uint32_t (*part)[NT / 64], uint32_t* found) {
+    const int per = (size + NT - 1) / NT;  // thread t has bins size - 1 - t per and down
+    uint32_t own = 0;
+    for (int i = 0; i < per; i++) {
+        const int b = size - 1 - ((int)threadIdx.x * per + i);
+        own += b >= 0 ? bins[b] : 0;
+    }
+    uint32_t at[1] = {own}, total[1];
+    scan<1>(at, part, total);
+    uint32_t above = at[0];
+    if (above < left && above + own >= left) {
+        for (int i = 0; i < per; i++) {
+            const int b = size - 1 - ((int)threadIdx.x * per + i);
+            if (above + bins[b] >= left) {
+                found[0] = (uint32_t)b;
+                found[1] = above;
+                break;
+            }
+            above += bins[b];
+        }
+    }
+    __syncthreads();
+    return found[1];
+}
+
+// HELD: the ranks of all positions stay in LDS (n of them behind the bins), so the weights are read once; else each
+// pass reads them again.
+template <bool HELD>
 __global__ __launch_bounds__(NT) void evict_select_kernel(EvictArgs K) {
+    extern __shared__ uint32_t ranks[];
     __shared__ uint32_t bins[BINS];
-    __shared__ uint32_t part[NT / 64];
+    __shared__ uint32_t part[AHEAD][NT / 64];
     __shared__ uint32_t found[2];
     const Eviction& E = K.E;
     const int nkv = E.P.num_kv_heads, s = blockIdx.x / nkv, h = blockIdx.x - s * nkv;
-    const int n = max(min(E.lens[s], E.cap), 0);
-    const int late = max(n - E.recent, 0);
+    const int n = max(min(E.lens[s], E.cap), 0), late = max(n - E.recent, 0);
     const float* const w = E.weights + s * E.seq_stride + h * E.head_stride;
     const int* const table = E.M.tables + (int64_t)s * E.M.stride;
-    auto exists = [&](int j) { return (unsigned)table[j >> K.ps_log2] < (unsigned)E.P.num_pages; };
-    auto weight = [&](int j) { return j < E.weights_len ? w[j] : 0.0f; };
 
-    // how many positions there are, and how many of them are recent
-    uint32_t count = 0;
-    for (int at = threadIdx.x << K.ps_log2; at < n; at += NT << K.ps_log2) {
-        if (!exists(at)) continue;
-        const int end = min(at + (1 << K.ps_log2), n);
-        count += (uint32_t)(end - at);
-    }
-    uint32_t there = 0, recent = 0;
-    scan(count, part, there);
-    count = 0;
-    for (int j = late + threadIdx.x; j < n; j += NT) count += exists(j);
-    scan(count, part, recent);
-    const int stay = min(E.keep, (int)there);
-    const bool all = (int)there <= E.keep;
-
-    // the need-th largest rank among the old positions: its digits from the top
-    uint32_t need = all ? 0 : (uint32_t)stay - recent, top = 0, ties = 0;
-    if (need > 0) {
-        int shift = 32;
-        uint32_t left = need;
+    // the ranks of positions j .. j + 3 (j a multiple of 4: one page), 0 where there is none
+    struct Four {
+        float w[4];
+        int page;
+    };
+    auto ask = [&](int j) {
+        Four f;
+        f.page = j < n ? table[j >> K.ps_log2] : -1;
+        if (j < n && j + 4 <= E.weights_len) {
+            const f4_t v = *reinterpret_cast<const f4_t*>(w + j);
 #pragma unroll
-        for (int digit = 0; digit < 3; digit++) {
-            const int bits = digit == 0 ? 12 : 10, size = 1 << bits;
-            shift -= bits;
-            for (int i = threadIdx.x; i < size; i += NT) bins[i] = 0;
-            __syncthreads();
-            for (int j = threadIdx.x; j < late; j += NT) {
-                if (!exists(j)) continue;
-                const uint32_t r = rank_of(weight(j));
-                if (digit == 0 || r >> (shift + bits) == top >> (shift + bits)) atomicAdd(&bins[(r >> shift) & (size - 1)], 1u);
-            }
-            __syncthreads();
-            // from the largest bin down: thread t has bins size - 1 - t per .. down
-            const int per = (size + NT - 1) / NT;
-            uint32_t own = 0;
-            for (int i = 0; i < per; i++) {
-                const int b = size - 1 - ((int)threadIdx.x * per + i);
-                own += b >= 0 ? bins[b] : 0;
-            }
-            uint32_t total;
-            uint32_t above = scan(own, part, total);
-            if (above < left && above + own >= left) {
-                for (int i = 0; i < per; i++) {
-                    const int b = size - 1 - ((int)threadIdx.x * per + i);
-                    if (above + bins[b] >= left) {
-                        found[0] = (uint32_t)b;
-                        found[1] = above;
-                        break;
-                    }
-                    above += bins[b];
+            for (int e = 0; e < 4; e++) f.w[e] = v[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) f.w[e] = j + e < min(n, E.weights_len) ? w[j + e] : 0.0f;
+        }
+        return f;
+    };
+    auto ranked = [&](const Four& f, int j, uint32_t (&r)[4]) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) r[e] = j + e < n && (unsigned)f.page < (unsigned)E.P.num_pages ? rank_of(f.w[e]) : 0u;
+    };
+    auto get = [&](int j, uint32_t (&r)[4]) {
+        if constexpr (HELD) {
+            const u4_t v = *reinterpret_cast<const u4_t*>(ranks + j);
+#pragma unroll
+            for (int e = 0; e < 4; e++) r[e] = v[e];
+        } else {
+            ranked(ask(j), j, r);
+        }
+    };
+    auto count = [&](uint32_t r, int shift, int bits) { atomicAdd(&bins[(r >> shift) & ((1u << bits) - 1u)], 1u); };
+
+    // how many positions there are and how many of them are recent, and the first digits of the others: 12 bits
+    for (int i = threadIdx.x; i < BINS; i += NT) bins[i] = 0;
+    __syncthreads();
+    uint32_t early = 0, latest = 0;
+    for (int c0 = 0; c0 < n; c0 += NT * PER * AHEAD) {
+        Four f[AHEAD];
+#pragma unroll
+        for (int a = 0; a < AHEAD; a++) f[a] = ask(c0 + (a * NT + (int)threadIdx.x) * PER);
+#pragma unroll
+        for (int a = 0; a < AHEAD; a++) {
+            const int j = c0 + (a * NT + (int)threadIdx.x) * PER;
+            if (j >= n) continue;
+            uint32_t r[4];
+            ranked(f[a], j, r);
+            if constexpr (HELD) *reinterpret_cast<u4_t*>(ranks + j) = u4_t{r[0], r[1], r[2], r[3]};
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if (r[e] == 0) continue;
+                if (j + e < late) {
+                    early++;
+                    count(r[e], 20, 12);
+                } else {
+                    latest++;
                 }
             }
+        }
+    }
+    uint32_t counts[2] = {early, latest}, sums[2];
+    scan<2>(counts, part, sums);
+    const uint32_t old = sums[0], recent = sums[1];
+    const int there = (int)(old + recent), stay = min(E.keep, there);
+    const bool all = there <= E.keep;
+
+    // the need-th largest rank among the old positions: its digits from the top
+    const uint32_t need = all ? 0 : (uint32_t)stay - recent;
+    uint32_t top = 0, ties = 0;
+    if (need > 0) {
+        uint32_t left = need;
+        left -= border(bins, BINS, left, part, found);
+        top = found[0] << 20;
+#pragma unroll
+        for (int shift = 10; shift >= 0; shift -= 10) {
             __syncthreads();
+            for (int i = threadIdx.x; i < 1024; i += NT) bins[i] = 0;
+            __syncthreads();
+            for (int c0 = 0; c0 < late; c0 += NT * PER * AHEAD) {
+                uint32_t r[AHEAD][4];
+#pragma unroll
+                for (int c = 0; c < AHEAD; c++) {
+                    const int j = c0 + (c * NT + (int)threadIdx.x) * PER;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) r[c][e] = 0;
+                    if (j < late) get(j, r[c]);
+                }
+#pragma unroll
+                for (int c = 0; c < AHEAD; c++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (r[c][e] >> (shift + 10) == top >> (shift + 10) && r[c][e] &&
+                            c0 + (c * NT + (int)threadIdx.x) * PER + e < late)
+                            count(r[c][e], shift, 10);
+            }
+            __syncthreads();
+            left -= border(bins, 1024, left, part, found);
             top |= found[0] << shift;
-            left -= found[1];
-            __syncthreads();
         }
         ties = left;  // of those whose rank is the border's, the first
     }
@@ -131,38 +224,70 @@ __global__ __launch_bounds__(NT) void evict_select_kernel(EvictArgs K) {
     int* const kept = E.kept + (int64_t)blockIdx.x * E.keep;
     float* const to = E.new_weights ? E.new_weights + s * E.new_seq_stride + h * E.new_head_stride : nullptr;
     uint32_t above = 0, equal = 0;  // positions over the border and on it, so far
-    for (int c0 = 0; c0 < n; c0 += NT * PER) {
-        const int j0 = c0 + threadIdx.x * PER;
-        float x[PER];
-        bool over[PER], on[PER];
-        uint32_t v = 0;
+    for (int c0 = 0; c0 < n; c0 += NT * PER * AHEAD) {
+        uint32_t r[AHEAD][4], before[AHEAD], total[AHEAD];
+        uint32_t over[AHEAD], on[AHEAD];  // a bit for each of the four
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
-            const int j = j0 + i;
-            const bool is = j < n && exists(j);
-            x[i] = is ? weight(j) : 0.0f;
-            const uint32_t r = rank_of(x[i]);
-            over[i] = is && (all || j >= late || (need > 0 && r > top));
-            on[i] = is && !over[i] && need > 0 && r == top;
-            v += (over[i] ? 1u : 0u) + (on[i] ? 0x10000u : 0u);
-        }
-        uint32_t total;
-        const uint32_t before = scan(v, part, total);
-        uint32_t a = above + (before & 0xffffu), e = equal + (before >> 16);
+        for (int c = 0; c < AHEAD; c++) {
+            const int j0 = c0 + (c * NT + (int)threadIdx.x) * PER;
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
-            if (over[i] || (on[i] && e < ties)) {
-                const uint32_t at = a + min(e, ties);
-                kept[at] = j0 + i;
-                if (to && (int)at < E.new_weights_len) to[at] = x[i];
+            for (int e = 0; e < 4; e++) r[c][e] = 0;
+            if (j0 < n) get(j0, r[c]);
+            over[c] = on[c] = 0;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const bool is = r[c][e] && (all || j0 + e >= late || (need > 0 && r[c][e] > top));
+                over[c] |= (uint32_t)is << e;
+                on[c] |= (uint32_t)(r[c][e] && !is && need > 0 && r[c][e] == top) << e;
             }
-            a += over[i];
-            e += on[i];
+            before[c] = (uint32_t)__builtin_popcount(over[c]) | (uint32_t)__builtin_popcount(on[c]) << 16;  // (4096 of each at most)
         }
-        above += total & 0xffffu;
-        equal += total >> 16;
+        scan<AHEAD>(before, part, total);  // (all of these positions' weights are read by now)
+#pragma unroll
+        for (int c = 0; c < AHEAD; c++) {
+            const int j0 = c0 + (c * NT + (int)threadIdx.x) * PER;
+            uint32_t a = above + (before[c] & 0xffffu), e0 = equal + (before[c] >> 16);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const bool is_over = over[c] >> e & 1, is_on = on[c] >> e & 1;
+                if (is_over || (is_on && e0 < ties)) {
+                    const uint32_t at = a + min(e0, ties);
+                    if constexpr (HELD) {
+                        ranks[at] = (uint32_t)(j0 + e);  // (over numbers that are used up: at is at most j0 + e)
+                    } else {
+                        kept[at] = j0 + e;
+                        if (to && (int)at < E.new_weights_len) to[at] = weight_of(r[c][e]);
+                    }
+                }
+                a += is_over;
+                e0 += is_on;
+            }
+            above += total[c] & 0xffffu;
+            equal += total[c] >> 16;
+        }
     }
     __syncthreads();
+    if constexpr (HELD) {  // the list as it lies: whole lines leave, where lanes scattered over the positions took 18 us for 32769
+        for (int c0 = 0; c0 < stay; c0 += NT * AHEAD) {
+            float x[AHEAD];
+#pragma unroll
+            for (int c = 0; c < AHEAD; c++) {
+                const int i = c0 + c * NT + (int)threadIdx.x;
+                x[c] = 0.0f;
+                if (i < stay) {
+                    const int j = (int)ranks[i];
+                    kept[i] = j;
+                    if (to && j < E.weights_len) x[c] = w[j];
+                }
+            }
+            __syncthreads();  // (new weights may take the place of the old: they are read first, and later ones lie further on)
+#pragma unroll
+            for (int c = 0; c < AHEAD; c++) {
+                const int i = c0 + c * NT + (int)threadIdx.x;
+                if (to && i < min(stay, E.new_weights_len)) to[i] = x[c];
+            }
+        }
+    }
     for (int i = stay + threadIdx.x; i < E.keep; i += NT) kept[i] = -1;
     if (to)
         for (int i = stay + threadIdx.x; i < E.new_weights_len; i += NT) to[i] = 0.0f;
@@ -176,26 +301,52 @@ __device__ __forceinline__ int64_t vector_at(const Eviction& E, const PageMap& M
     return (((slot >> ps_log2) * E.P.num_kv_heads + h) << ps_log2) + (slot & ((1 << ps_log2) - 1));
 }
 
-__global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs K, int width, int vec16, int words) {
+// 16 lanes take VECS vectors, keys and values, whose places are looked up together: a look-up is three loads, one
+// after the other, and there has to be enough under way meanwhile.
+constexpr int VECS = 2;
+template <int UNITS>
+__global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs K, int groups, int vec16, int words) {
     const Eviction& E = K.E;
     const unsigned id = blockIdx.x * 16 + (threadIdx.x >> 4);
-    const unsigned head = id / width, lane = threadIdx.x & 15;
-    const int i = (int)(id - head * width), nkv = E.P.num_kv_heads;
+    const unsigned head = id / groups, lane = threadIdx.x & 15;
+    const int i0 = (int)(id - head * groups) * VECS, nkv = E.P.num_kv_heads, width = min(E.keep, E.cap);
     if (head >= (unsigned)E.M.nseq * nkv) return;
     const int s = head / nkv, h = head % nkv;
-    const int pos = E.kept[(int64_t)head * E.keep + i];
-    const int64_t from = vector_at(E, E.M, K.ps_log2, s, h, pos), to = vector_at(E, E.to, K.ps_log2, s, h, i);
-    if (from < 0 || to < 0) return;
-    // 16 bytes a lane, the key's first; scales as words
-    for (int u = lane; u < 2 * vec16; u += 16) {
-        uint4* const p = static_cast<uint4*>(u < vec16 ? E.P.k : E.P.v);
-        const int at = u < vec16 ? u : u - vec16;
-        p[to * vec16 + at] = p[from * vec16 + at];
+    int64_t from[VECS], to[VECS];
+    int pos[VECS];
+#pragma unroll
+    for (int v = 0; v < VECS; v++) pos[v] = i0 + v < width ? E.kept[(int64_t)head * E.keep + i0 + v] : -1;
+#pragma unroll
+    for (int v = 0; v < VECS; v++) {
+        from[v] = vector_at(E, E.M, K.ps_log2, s, h, pos[v]);
+        to[v] = pos[v] < 0 ? -1 : vector_at(E, E.to, K.ps_log2, s, h, i0 + v);
     }
-    for (int u = lane; u < 2 * words; u += 16) {
-        float* const p = u < words ? E.P.k_scale : E.P.v_scale;
-        const int at = u < words ? u : u - words;
-        p[to * words + at] = p[from * words + at];
+    // 16 bytes a lane, the key's first; scales as words
+    u4_t x[VECS][UNITS];
+    float y[VECS];
+#pragma unroll
+    for (int v = 0; v < VECS; v++) {
+        const bool is = from[v] >= 0 && to[v] >= 0;
+#pragma unroll
+        for (int c = 0; c < UNITS; c++) {
+            const int u = 16 * c + (int)lane;
+            if (is && u < 2 * vec16)
+                x[v][c] = static_cast<const u4_t*>(u < vec16 ? E.P.k : E.P.v)[from[v] * vec16 + (u < vec16 ? u : u - vec16)];
+        }
+        const int u = lane;  // (at most 8 words a vector)
+        if (is && u < 2 * words) y[v] = (u < words ? E.P.k_scale : E.P.v_scale)[from[v] * words + (u < words ? u : u - words)];
+    }
+#pragma unroll
+    for (int v = 0; v < VECS; v++) {
+        const bool is = from[v] >= 0 && to[v] >= 0;
+#pragma unroll
+        for (int c = 0; c < UNITS; c++) {
+            const int u = 16 * c + (int)lane;
+            if (is && u < 2 * vec16)
+                static_cast<u4_t*>(u < vec16 ? E.P.k : E.P.v)[to[v] * vec16 + (u < vec16 ? u : u - vec16)] = x[v][c];
+        }
+        const int u = lane;
+        if (is && u < 2 * words) (u < words ? E.P.k_scale : E.P.v_scale)[to[v] * words + (u < words ? u : u - words)] = y[v];
     }
 }
 
@@ -203,14 +354,26 @@ __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs K, int width,
 
 void launch_evict(const Eviction& E, hipStream_t st) {
     const EvictArgs K{E, __builtin_ctz(E.P.page_size)};
-    evict_select_kernel<<<(unsigned)(E.M.nseq * E.P.num_kv_heads), NT, 0, st>>>(K);
+    const unsigned heads = (unsigned)(E.M.nseq * E.P.num_kv_heads);
+    const int held = (E.cap + 3) / 4 * 16;  // bytes of the ranks
+    if (held <= kHeld)
+        evict_select_kernel<true><<<heads, NT, held, st>>>(K);
+    else
+        evict_select_kernel<false><<<heads, NT, 0, st>>>(K);
     const int width = std::min(E.keep, E.cap);
     if (width == 0) return;
     const bool b4 = E.P.type == JYHIP_T_I4;
     const int bytes = b4 ? 16 * groups4(E.P.head_dim) : E.P.type == JYHIP_T_I8 ? E.P.head_dim : 2 * E.P.head_dim;
     const int words = b4 ? groups4(E.P.head_dim) : E.P.type == JYHIP_T_I8 ? 1 : 0;
-    const int64_t vectors = (int64_t)E.M.nseq * E.P.num_kv_heads * width;
-    evict_move_kernel<<<(unsigned)((vectors + 15) / 16), 256, 0, st>>>(K, width, bytes / 16, words);
+    const int groups = (width + VECS - 1) / VECS;
+    const unsigned grid = (unsigned)(((int64_t)heads * groups + 15) / 16);
+    const int units = (2 * bytes / 16 + 15) / 16;  // 1 to 4
+    if (units == 1)
+        evict_move_kernel<1><<<grid, 256, 0, st>>>(K, groups, bytes / 16, words);
+    else if (units == 2)
+        evict_move_kernel<2><<<grid, 256, 0, st>>>(K, groups, bytes / 16, words);
+    else
+        evict_move_kernel<4><<<grid, 256, 0, st>>>(K, groups, bytes / 16, words);
 }
 
 }  // namespace jy
