@@ -9,7 +9,7 @@
 // where the numbers' bytes, masked, are subnormal halves that one packed product makes n / 512 (as subnormal operands
 // they cost fp32 sums five digits: 4e-5 measured against 1e-7); the weight times the step goes in as one fp16 part
 // where queries and outputs are bf16 (at most 2^-11 of a term, of either sign) and as two where they have more digits,
-// relative to a power of two over the steps seen; and the second sum is 8 fmas a group on the vector unit.
+// relative to a power of two over the steps seen; and the second sum is one more product, the groups its rows.
 //
 // Lane l holds of key l & 15 the bytes of quarter l >> 4 (elements 8 (l >> 4) .. + 7 of every group) and that
 // key's words; of its 8 values j the byte of every group for elements 32 g + 2 (l & 15), + 1, and their words.
@@ -36,9 +36,13 @@ struct Tile<JYHIP_T_I4, NC> {
     uint32_t k[2][G];        // 4 G bytes of key l & 15
     uint32_t kw[2][G];       // its words (step, low)
     uint32_t v[8][VW];       // G bytes of each value
-    uint32_t vw[2][4 * G];   // the words of values 4 (l >> 4) + i of each 16
-    uint32_t top[2][G > 4 ? 2 : 1];  // the 16 values' words spread over the wave: lane l has some of value top_key(l)
-    static __device__ __forceinline__ int top_key(int lane) { return lane / (G == 2 ? 2 : 4); }
+    // The words of the 16 values, spread over the wave so that a row of 16 lanes holds those of its four values
+    // (4 (l >> 4) + i): word_lane(i, g) has group g's of value i, in vw[.][g / 4] (two groups: lanes 8 .. 15 repeat 0 .. 7).
+    static constexpr int VC = G > 4 ? 2 : 1;
+    uint32_t vw[2][VC];
+    static constexpr __device__ int word_lane(int i, int g) { return G == 2 ? 2 * i + g : 4 * i + (g & 3); }
+    // which of the row's values lane l has words of
+    static __device__ __forceinline__ int word_value(int lane) { return G == 2 ? lane >> 1 & 3 : lane >> 2 & 3; }
     int live[2];
 };
 
@@ -95,11 +99,9 @@ struct Loader<JYHIP_T_I4, NC> {
                     else
                         words<T::VW>(t.v[g * 4 + j], vr, off);
                 }
-                words<4 * G>(t.vw[g], vwr, (unsigned)(kg * 4 * G));
-                if constexpr (G == 2)
-                    words<1>(t.top[g], vwr, lane < 32 ? (unsigned)(lane * 4) : kNowhere);
-                else
-                    words<G / 4>(t.top[g], vwr, (unsigned)(lane * G));
+#pragma unroll
+                for (int c = 0; c < T::VC; c++)
+                    words<1>(&t.vw[g][c], vwr, (unsigned)(((kg + T::word_value(lane)) * G + (G == 2 ? key & 1 : key & 3) + 4 * c) * 4));
             }
         }
 #endif
@@ -162,17 +164,15 @@ struct Query<JYHIP_T_I4, KC, WIDE> {
     }
     static __device__ __forceinline__ float factor(float amax) { return __builtin_ldexpf(1.0f, -exponent(amax)); }
 
-    __device__ __forceinline__ void dot(const uint32_t (&k)[G], const uint32_t (&kw)[G], int groups, float (&s)[4]) const {
+    __device__ __forceinline__ void dot(const uint32_t (&k)[G], const uint32_t (&kw)[G], float (&s)[4]) const {
 #if defined(__HIP_DEVICE_COMPILE__)
         uint32_t w[4] = {};
 #pragma unroll
-        for (int g = 0; g < G; g += 2)  // the lows (a group past the head's end: zeros)
-            w[g / 2] = __builtin_amdgcn_perm(g + 1 < groups ? kw[g + 1] : 0u, g < groups ? kw[g] : 0u, 0x07060302u);
+        for (int g = 0; g < G; g += 2) w[g / 2] = __builtin_amdgcn_perm(kw[g + 1], kw[g], 0x07060302u);  // the lows
         f4_t d = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, i4_t{(int)w[0], (int)w[1], (int)w[2], (int)w[3]}),
                                                         sums, f4_t{}, 0, 0, 0);
 #pragma unroll
         for (int g = 0; g < G; g++) {
-            if (g >= groups) continue;
             const _Float16 s1 = as_h2(kw[g]).x * (_Float16)16.0f;
             const h2_t s16 = {s1, s1};
             uint32_t a[4];
@@ -199,15 +199,15 @@ struct State4 {
     static constexpr int G = 2 * NC, DL = 2 * G;
     typedef Tile<JYHIP_T_I4, NC> T;
     f4_t o[DL] = {};
-    float low[G] = {};  // this lane's part of sum p low
+    f4_t low = {};  // row g (as in o): 2^15 sum p low of group g
     float m = kNone, l = 0.0f;
     float vref = 0.0f, vinv = 0.0f;  // o counts in units of vref / 2^15 * 2^9; vinv = 2^15 / vref
 
     template <class Q>
-    static __device__ __forceinline__ void scores(const Q& q, float qf, const T& t, int groups, float (&s)[2][4]) {
+    static __device__ __forceinline__ void scores(const Q& q, float qf, const T& t, float (&s)[2][4]) {
 #pragma unroll
         for (int g = 0; g < 2; g++) {
-            q.dot(t.k[g], t.kw[g], groups, s[g]);
+            q.dot(t.k[g], t.kw[g], s[g]);
 #pragma unroll
             for (int i = 0; i < 4; i++) s[g][i] *= qf;
         }
@@ -220,14 +220,14 @@ struct State4 {
 #pragma unroll
         for (int g = 0; g < 2; g++)
 #pragma unroll
-            for (int i = 0; i < (G > 4 ? 2 : 1); i++) step = fmaxf(step, fabsf((float)as_h2(t.top[g][i]).x));
+            for (int i = 0; i < T::VC; i++) step = fmaxf(step, fabsf((float)as_h2(t.vw[g][i]).x));
         if (__any(most > m || step > vref)) {
             const float mn = fmaxf(m, head_max(most));
             float a = exp2_hw(m - mn);
             m = mn;
             l *= a;
 #pragma unroll
-            for (int g = 0; g < G; g++) low[g] *= a;
+            for (int i = 0; i < 4; i++) low[i] *= a;
             step = wave_max64(step);
             if (step > vref) {  // (the same in every lane)
                 const int e = min((int)(__builtin_bit_cast(uint32_t, step) >> 23) - 126, 100);
@@ -251,39 +251,89 @@ struct State4 {
         l += sum;
     }
 
-    // o and low with these weights
-    __device__ __forceinline__ void product(const T& t, const float (&p)[8], int groups) {
+    // 8 numbers as one or two fp16 parts.  (Two are cut, not rounded: a conversion that the compiler joins with the
+    // product that made the number rounds once where the remainder takes it as rounded twice.)
+    static __device__ __forceinline__ void parts(const float (&w)[8], h8_t& hi, h8_t& lo) {
+        if constexpr (WIDE) {
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+                const auto a = __builtin_amdgcn_cvt_pkrtz(w[j], w[j + 1]);
+                const auto b = __builtin_amdgcn_cvt_pkrtz(w[j] - (float)a[0], w[j + 1] - (float)a[1]);
+                hi[j] = (_Float16)a[0];
+                hi[j + 1] = (_Float16)a[1];
+                lo[j] = (_Float16)b[0];
+                lo[j + 1] = (_Float16)b[1];
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) hi[j] = (_Float16)w[j];
+        }
+    }
+
+    // Where some words are not finite in a tile that not all columns see whole: they count as zeros, and the columns
+    // that see them (`out`: which of its 8 positions this lane's does not) become NaN in all their dims, as such a vector is.
+    __device__ __forceinline__ void take_infinite(T& t, uint32_t out) {
 #if defined(__HIP_DEVICE_COMPILE__)
-        float pv[8];
+        const int lane = threadIdx.x & 63;
+        bool hit = false;
 #pragma unroll
-        for (int j = 0; j < 8; j++) pv[j] = p[j] * vinv;
+        for (int h = 0; h < 2; h++)
 #pragma unroll
-        for (int g = 0; g < G; g++) {
-            if (g >= groups) continue;
+            for (int c = 0; c < T::VC; c++) {
+                const h2_t x = as_h2(t.vw[h][c]);
+                const bool is = !(fabsf((float)x.x) <= 65504.0f) || !(fabsf((float)x.y) <= 65504.0f);
+                const uint32_t row = (uint32_t)(__ballot(is) >> (lane & 48)) & 0xffffu;
+                t.vw[h][c] = is ? 0u : t.vw[h][c];
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    hit |= !(out >> (4 * h + i) & 1u) && (row & (G == 2 ? 0x0303u << (2 * i) : 0xfu << (4 * i))) != 0;
+            }
+        if (head_max(hit ? 1.0f : 0.0f) > 0.0f)
+#pragma unroll
+            for (int d = 0; d < DL; d++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[d][i] = __builtin_nanf("");
+#endif
+    }
+
+    // o and low with these weights
+    __device__ __forceinline__ void product(const T& t, const float (&p)[8]) {
+#if defined(__HIP_DEVICE_COMPILE__)
+        // The lows: one product of the groups (its rows) by the weights.  Lane r of a row takes group r's words of the
+        // row's values by rotations.
+        {
+            uint32_t x[8];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                x[4 * h] = first<0>(t.vw[h]);
+                x[4 * h + 1] = first<1>(t.vw[h]);
+                x[4 * h + 2] = first<2>(t.vw[h]);
+                x[4 * h + 3] = first<3>(t.vw[h]);
+            }
+            i4_t A;
+#pragma unroll
+            for (int j = 0; j < 4; j++) A[j] = (int)__builtin_amdgcn_perm(x[2 * j + 1], x[2 * j], 0x07060302u);
             float w[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const h2_t x = as_h2(t.vw[j >> 2][(j & 3) * G + g]);
-                w[j] = (float)x.x * pv[j];
-                low[g] = __builtin_fmaf((float)x.y, p[j], low[g]);
-            }
+            for (int j = 0; j < 8; j++) w[j] = p[j] * 32768.0f;
             h8_t hi, lo;
-            if constexpr (WIDE) {
-                // (cut, not rounded: a conversion that the compiler joins with the product above rounds once where
-                // the remainder below takes it as rounded twice)
+            parts(w, hi, lo);
+            if constexpr (WIDE) low = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, A), lo, low, 0, 0, 0);
+            low = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8_t, A), hi, low, 0, 0, 0);
+        }
+        // the steps in the product's units; a lane takes each from the one that has it, by a move within its row that
+        // the multiplication does itself
+        float steps[2][T::VC];
 #pragma unroll
-                for (int j = 0; j < 8; j += 2) {
-                    const auto a = __builtin_amdgcn_cvt_pkrtz(w[j], w[j + 1]);
-                    const auto b = __builtin_amdgcn_cvt_pkrtz(w[j] - (float)a[0], w[j + 1] - (float)a[1]);
-                    hi[j] = (_Float16)a[0];
-                    hi[j + 1] = (_Float16)a[1];
-                    lo[j] = (_Float16)b[0];
-                    lo[j + 1] = (_Float16)b[1];
-                }
-            } else {
+        for (int h = 0; h < 2; h++)
 #pragma unroll
-                for (int j = 0; j < 8; j++) hi[j] = (_Float16)w[j];
-            }
+            for (int i = 0; i < T::VC; i++) steps[h][i] = (float)as_h2(t.vw[h][i]).x * vinv;
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+            float w[8];
+            values<0>(w, p, steps, g);
+            h8_t hi, lo;
+            parts(w, hi, lo);
             uint32_t b[4];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
@@ -309,6 +359,47 @@ struct State4 {
             }
         }
 #endif
+    }
+
+    // lane r of a row: the word of group r of the row's value I (other lanes past the last group: anything)
+    template <int I>
+    static __device__ __forceinline__ uint32_t first(const uint32_t (&vw)[T::VC]) {
+        constexpr int by = T::word_lane(I, 0), back = (16 - by) & 15;  // row_ror by 16 - n brings lane r + n's to lane r
+        uint32_t x = rotated<back>(vw[0]);
+        if constexpr (T::VC > 1) {
+            const uint32_t y = rotated<(back + 4) & 15>(vw[1]);  // (moved by all lanes, those that have the word among them)
+            x = (threadIdx.x & 15) < 4 ? x : y;
+        }
+        return x;
+    }
+    template <int N>
+    static __device__ __forceinline__ uint32_t rotated(uint32_t v) {
+        if constexpr (N == 0)
+            return v;
+        else
+            return __builtin_bit_cast(uint32_t, dpp_f<0x120 + N>(__builtin_bit_cast(float, v)));
+    }
+
+    // w[J ..]: the weights times the steps of group g
+    template <int J>
+    __device__ __forceinline__ void values(float (&w)[8], const float (&p)[8], const float (&steps)[2][T::VC], int g) {
+        if constexpr (J < 8) {
+            switch (g) {
+                case 0: value<J, 0>(w, p, steps); break;
+                case 1: value<J, 1>(w, p, steps); break;
+                case 2: value<J, 2>(w, p, steps); break;
+                case 3: value<J, 3>(w, p, steps); break;
+                case 4: value<J, 4>(w, p, steps); break;
+                case 5: value<J, 5>(w, p, steps); break;
+                case 6: value<J, 6>(w, p, steps); break;
+                default: value<J, 7>(w, p, steps);
+            }
+            values<J + 1>(w, p, steps, g);
+        }
+    }
+    template <int J, int GR>
+    __device__ __forceinline__ void value(float (&w)[8], const float (&p)[8], const float (&steps)[2][T::VC]) {
+        if constexpr (GR < G) w[J] = dpp_f<0x150 + T::word_lane(J & 3, GR)>(steps[J >> 2][GR / 4]) * p[J];  // row_newbcast
     }
 
     static __device__ __forceinline__ float exp2_hw(float x) {

@@ -162,7 +162,7 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void ruled_attend_kernel(Rule
     const RuledAttn& A = K.A;
     const jyhip_pages& P = A.P;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15;
-    const int hd = P.head_dim, nkv = P.num_kv_heads, per = A.nh / nkv, words4 = (hd + 31) / 32;
+    const int hd = P.head_dim, nkv = P.num_kv_heads, per = A.nh / nkv;
     // heads fastest, then groups of rows, the last (and longest) of a run first, then chunks
     unsigned id = blockIdx.x;
     const int hg = id % (nkv * K.tiles);
@@ -259,15 +259,16 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void ruled_attend_kernel(Rule
     float* const sc = K.sstride ? K.scores + ((int64_t)row * A.nh + head) * K.sstride - base : nullptr;
     bool asked = false;
 
-    // one tile; the next one's keys are asked for once this one's are used up, its values at the end
-    T t;
-    auto step = [&](int key0, auto&& next_keys, auto&& next_values) {
+    // One tile, its keys in t and its values in tv; the keys of a later one are asked for once these are used up, its
+    // values at the end.  DK, DV: two tiles of keys, of values are in registers at a time (what fits them)
+    constexpr bool DK = B4 || PT == JYHIP_T_I8 || (!WIDE && !RUNS && NC <= 2), DV = B4 && NC <= 2;
+    T ta, tb;
+    auto step = [&](T& t, T& tv, int key0, auto&& next_keys, auto&& next_values) {
         const int kg = (lane >> 4) * 4;
+        uint32_t outs = 0;
+        bool care = false;
         float s[2][4], p[8];
-        if constexpr (B4)
-            S::scores(q, qf, t, words4, s);
-        else
-            S::scores(q, qf, t, s);
+        S::scores(q, qf, t, s);
         const int live[2] = {t.live[0], t.live[1]};
         next_keys();
         if (A.soft != 0.0f) {
@@ -292,36 +293,39 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void ruled_attend_kernel(Rule
                     const int j = key0 + 16 * g + kg + i;
                     const bool out = j < lo || j >= hi || kg + i >= live[g];
                     s[g][i] = out ? -__builtin_inff() : s[g][i];
-                    if constexpr (PT == JYHIP_T_I8) t.vs[g][i] = out ? 0.0f : t.vs[g][i];
-                    if constexpr (B4) {
-#pragma unroll
-                        for (int w = 0; w < T::G; w++) t.vw[g][i * T::G + w] = out ? 0u : t.vw[g][i * T::G + w];
-                    }
+                    if constexpr (PT == JYHIP_T_I8) tv.vs[g][i] = out ? 0.0f : tv.vs[g][i];
+                    if constexpr (B4) outs |= (uint32_t)out << (4 * g + i);
                     if constexpr (PT == JYHIP_T_F16 || PT == JYHIP_T_BF16) {
                         // a value in front of everybody's first position (the ones behind were not loaded)
 #pragma unroll
-                        for (int w = 0; w < T::VW; w++) t.v[4 * g + i][w] = j < from ? 0u : t.v[4 * g + i][w];
+                        for (int w = 0; w < T::VW; w++) tv.v[4 * g + i][w] = j < from ? 0u : tv.v[4 * g + i][w];
                     }
                 }
                 if constexpr (B4) {
 #pragma unroll
-                    for (int w = 0; w < (T::G > 4 ? 2 : 1); w++)
-                        t.top[g][w] = key0 + 16 * g + T::top_key(lane) < from ? 0u : t.top[g][w];
+                    for (int w = 0; w < T::VC; w++) {
+                        // (what nobody sees has no say in the scale of the weights either)
+                        tv.vw[g][w] = key0 + 16 * g + kg + T::word_value(lane) < from ? 0u : tv.vw[g][w];
+                        const h2_t x = as_h2(tv.vw[g][w]);
+                        care |= __any(!(fabsf((float)x.x) <= 65504.0f) || !(fabsf((float)x.y) <= 65504.0f));
+                    }
                 }
             }
             if constexpr (B16)
-                if (rows > 1 && holds_infinite<PT, NC>(t)) take_infinite<PT, NC>(t, bad, key0, rows, K.hpg, lo, hi);
+                if (rows > 1 && holds_infinite<PT, NC>(tv)) take_infinite<PT, NC>(tv, bad, key0, rows, K.hpg, lo, hi);
         }
         if (sc && on) {
 #pragma unroll
             for (int g = 0; g < 2; g++)
                 *reinterpret_cast<f4_t*>(sc + key0 + 16 * g + kg) = f4_t{s[g][0], s[g][1], s[g][2], s[g][3]};
         }
-        st.weights(t, s, p);
-        if constexpr (B4)
-            st.product(t, p, words4);
-        else
-            S::product(t, p, st.o);
+        st.weights(tv, s, p);
+        if constexpr (B4) {
+            if (care) st.take_infinite(tv, outs);
+            st.product(tv, p);
+        } else {
+            S::product(tv, p, st.o);
+        }
         next_values();
     };
 
@@ -335,18 +339,20 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void ruled_attend_kernel(Rule
         }
         const int ntiles = stop > s0 ? (stop - s0 + 31) / 32 : 0;
         const int cnt = (ntiles - wave + 3) / 4;
-        auto keys = [&](int i) {
+        auto keys = [&](T& t, int i) {
+            if (i >= cnt) return;
             const int p0 = __builtin_amdgcn_readlane(ids, 2 * i), p1 = __builtin_amdgcn_readlane(ids, 2 * i + 1);
             ld.template load<true, false>(t, p0, p1, s0 + (wave + 4 * i) * 32, stop);
         };
-        auto values = [&](int i) {
+        auto values = [&](T& t, int i) {
+            if (i >= cnt) return;
             const int p0 = __builtin_amdgcn_readlane(ids, 2 * i), p1 = __builtin_amdgcn_readlane(ids, 2 * i + 1);
             ld.template load<false, true>(t, p0, p1, s0 + (wave + 4 * i) * 32, stop);
         };
-        if (cnt > 0) {
-            keys(0);
-            values(0);
-        }
+        keys(ta, 0);
+        values(ta, 0);
+        if constexpr (DK) keys(tb, 1);
+        if constexpr (DV) values(tb, 1);
         if (!asked) {  // the query as operands, while the first positions are on their way
             asked = true;
             float amax = 0.0f;
@@ -366,14 +372,17 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void ruled_attend_kernel(Rule
             q.load(x, amax);
             qf = bad ? __builtin_nanf("") : q.factor(amax) * (A.soft != 0.0f ? A.scale / A.soft : A.scale * kLog2e);
         }
-        for (int i = 0; i < cnt; i++)
-            step(s0 + (wave + 4 * i) * 32,
-                 [&] {
-                     if (i + 1 < cnt) keys(i + 1);
-                 },
-                 [&] {
-                     if (i + 1 < cnt) values(i + 1);
-                 });
+        auto at = [&](int i) { return s0 + (wave + 4 * i) * 32; };
+        if constexpr (DK) {
+            T& vb = DV ? tb : ta;
+            for (int i = 0; i < cnt; i += 2) {
+                step(ta, ta, at(i), [&] { keys(ta, i + 2); }, [&] { values(ta, DV ? i + 2 : i + 1); });
+                if (i + 1 >= cnt) break;
+                step(tb, vb, at(i + 1), [&] { keys(tb, i + 3); }, [&] { values(vb, DV ? i + 3 : i + 2); });
+            }
+        } else {
+            for (int i = 0; i < cnt; i++) step(ta, ta, at(i), [&] { keys(ta, i + 1); }, [&] { values(ta, i + 1); });
+        }
     }
 
     // join the waves
@@ -381,7 +390,7 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void ruled_attend_kernel(Rule
     if constexpr (B4) {
 #pragma unroll
         for (int g = 0; g < T::G; g++) {
-            const float low = head_sum(st.low[g]);
+            const float low = __shfl(st.low[g & 3], (g >> 2) * 16 + col) * (1.0f / 32768.0f);
 #pragma unroll
             for (int e = 0; e < 2; e++) {
                 const float unit = st.vref * (512.0f / 32768.0f);
