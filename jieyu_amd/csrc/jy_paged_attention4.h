@@ -179,7 +179,7 @@ struct Query<JYHIP_T_I4, KC, WIDE> {
 #pragma unroll
             for (int j = 0; j < 2; j++) {
                 const uint32_t b = two_bytes(k, 2 * j * G + g, (2 * j + 1) * G + g);
-                const uint32_t lo = (b << 6 & 0x03c003c0u) | 0x3c003c00u, hi = (b << 2 & 0x03c003c0u) | 0x3c003c00u;
+                const uint32_t lo = (b & 0x000f000fu) << 6 | 0x3c003c00u, hi = (b & 0x00f000f0u) << 2 | 0x3c003c00u;
                 a[2 * j] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(as_h2(lo), s16, -s16));
                 a[2 * j + 1] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(as_h2(hi), s16, -s16));
             }

@@ -171,10 +171,21 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void ruled_attend_kernel(Rule
     const int split = id / K.groups;
     const int kvh = hg / K.tiles, tile = hg % K.tiles;
     const int h0 = kvh * per + tile * 16, heads = min(K.hpg, per - tile * 16);
+    // the page of each of the wave's groups of 16 positions from s0 on: lane 2i + g has that of group g of its i-th tile
+    auto pages = [&](int b, int s0) {
+        const int i = (s0 + (wave + 4 * (lane >> 1)) * 32 + 16 * (lane & 1)) >> K.ps_log2;
+        return i < A.M.stride ? A.M.tables[(int64_t)b * A.M.stride + i] : -1;
+    };
     Run run{at, at, at + 1};
+    int early = -1;  // single rows from position 0 on: where their pages lie does not wait for their lengths
     if (A.starts) {
         run = run_of(K, K.groups - 1 - at);
         if (run.seq < 0) return;
+    } else {
+        // (a chunk that its sequence has not leaves at once: in a ragged batch those are most)
+        if (!A.first) early = pages(at, split * K.chunk);
+        const int f = A.first ? max(A.first[at], 0) & ~31 : 0;
+        if (split != 0 && f + split * K.chunk >= min(A.lens[at], A.cap)) return;
     }
     const int b = run.seq, rows = min(K.rpg, run.end - run.row0);
     // this lane's column
@@ -330,23 +341,18 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void ruled_attend_kernel(Rule
     };
 
     for (int s0 = c0; s0 < end || !asked; s0 += kPages) {
-        // the page of each of the wave's groups of 16 positions: lane 2i + g has that of group g of its i-th tile
         const int stop = min(end, s0 + kPages);
-        int ids = -1;
-        {
-            const int at = (s0 + (wave + 4 * (lane >> 1)) * 32 + 16 * (lane & 1)) >> K.ps_log2;
-            if (at < A.M.stride) ids = A.M.tables[(int64_t)b * A.M.stride + at];
-        }
+        const int ids = !A.starts && !A.first && s0 == c0 ? early : pages(b, s0);
         const int ntiles = stop > s0 ? (stop - s0 + 31) / 32 : 0;
         const int cnt = (ntiles - wave + 3) / 4;
+        // (Past the last tile nothing is fetched, but the loads are issued: were they under a condition, the waits for the
+        // earlier ones could not count on them and would wait for the whole queue.)
         auto keys = [&](T& t, int i) {
-            if (i >= cnt) return;
-            const int p0 = __builtin_amdgcn_readlane(ids, 2 * i), p1 = __builtin_amdgcn_readlane(ids, 2 * i + 1);
+            const int p0 = __builtin_amdgcn_readlane(ids, 2 * i & 63), p1 = __builtin_amdgcn_readlane(ids, (2 * i + 1) & 63);
             ld.template load<true, false>(t, p0, p1, s0 + (wave + 4 * i) * 32, stop);
         };
         auto values = [&](T& t, int i) {
-            if (i >= cnt) return;
-            const int p0 = __builtin_amdgcn_readlane(ids, 2 * i), p1 = __builtin_amdgcn_readlane(ids, 2 * i + 1);
+            const int p0 = __builtin_amdgcn_readlane(ids, 2 * i & 63), p1 = __builtin_amdgcn_readlane(ids, (2 * i + 1) & 63);
             ld.template load<false, true>(t, p0, p1, s0 + (wave + 4 * i) * 32, stop);
         };
         keys(ta, 0);
@@ -375,11 +381,13 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void ruled_attend_kernel(Rule
         auto at = [&](int i) { return s0 + (wave + 4 * i) * 32; };
         if constexpr (DK) {
             T& vb = DV ? tb : ta;
-            for (int i = 0; i < cnt; i += 2) {
+            // (in pairs without a way out between them, for the same reason)
+            int i = 0;
+            for (; i + 1 < cnt; i += 2) {
                 step(ta, ta, at(i), [&] { keys(ta, i + 2); }, [&] { values(ta, DV ? i + 2 : i + 1); });
-                if (i + 1 >= cnt) break;
                 step(tb, vb, at(i + 1), [&] { keys(tb, i + 3); }, [&] { values(vb, DV ? i + 3 : i + 2); });
             }
+            if (i < cnt) step(ta, ta, at(i), [] {}, [] {});
         } else {
             for (int i = 0; i < cnt; i++) step(ta, ta, at(i), [&] { keys(ta, i + 1); }, [&] { values(ta, i + 1); });
         }
