@@ -9,8 +9,8 @@
 // 16 lanes take a vector, and lane r elements 32 g + 2 r and 32 g + 2 r + 1 of every group g: its byte of
 // each group lies beside the others (byte r G + g of the vector, G groups), so a lane's bytes are one store,
 // and the attention's lanes, which take a vector's dims in the same shares, one load.  A group's lowest and
-// largest take four DPP moves within the row of lanes; the scales leave as one word a lane, lane g that of
-// group g.  The lanes take a head's key and value together.
+// largest take four DPP moves within the row of lanes, and lane i works out the words of one of the key's and
+// the value's groups.
 #include <hip/hip_runtime.h>
 
 #include "jy_device.h"
@@ -74,42 +74,65 @@ __device__ __forceinline__ void load_pairs(const E* p, int hd, bool pairs, float
     }
 }
 
-// hold the 2 G elements of this lane as the vector at `vec`
-template <int G>
-__device__ __forceinline__ void hold4(void* pool, void* scales, int64_t vec, int hd, const float (&x)[2 * G]) {
-    const int r = threadIdx.x & 15;
-    float past = 0.0f;
-#pragma unroll
-    for (int g = 0; g < G; g++)
-        if (32 * g + 2 * r < hd) past = fmaxf(past, !(fabsf(x[2 * g]) <= kMax4) || !(fabsf(x[2 * g + 1]) <= kMax4) ? 1.0f : 0.0f);
-    const bool bad = row_max(past) > 0.0f;  // the whole vector is NaN
-    uint8_t bytes[G];
-    uint32_t word = 0;
-#pragma unroll
-    for (int g = 0; g < G; g++) {
-        const bool on = 32 * g + 2 * r < hd;
-        const float lo = row_min(on ? fminf(x[2 * g], x[2 * g + 1]) : __builtin_inff());
-        const float hi = row_max(on ? fmaxf(x[2 * g], x[2 * g + 1]) : -__builtin_inff());
-        const bool some = 32 * g < hd;
-        const _Float16 low = some ? (_Float16)lo : (_Float16)0.0f;
-        const _Float16 step = some ? (_Float16)seven_bits((hi - (float)low) / 15.0f) : (_Float16)0.0f;
-        const float inv = (float)step > 0.0f ? 1.0f / (float)step : 0.0f;
+// v of lane L of the row
+template <int L>
+__device__ __forceinline__ float from_lane(float v) {
+    return dpp_f<0x150 + L>(v);  // row_newbcast
+}
+
+// the numbers of both sides' groups from group I on, by the lows and reciprocal steps that lane I of the row has
+template <int G, int I>
+__device__ __forceinline__ void numbers(const float (&x)[2][2 * G], float low, float inv, uint8_t (&bytes)[2][G]) {
+    if constexpr (I < 2 * G) {
+        const float lo = from_lane<I>(low), back = from_lane<I>(inv);
         uint32_t n[2];
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-            const float y = __builtin_rintf((x[2 * g + e] - (float)low) * inv);
+            const float y = __builtin_rintf((x[I / G][2 * (I % G) + e] - lo) * back);
             n[e] = (uint32_t)(int)fminf(fmaxf(y, 0.0f), 15.0f);
         }
-        bytes[g] = on && !bad ? (uint8_t)(n[0] | n[1] << 4) : (uint8_t)0;
-        const uint32_t nan = 0x7e007e00u;
-        const uint32_t w = bad && some ? nan : __builtin_bit_cast(uint32_t, h2_t{step, low});
-        word = r == g ? w : word;
+        bytes[I / G][I % G] = (uint8_t)(n[0] | n[1] << 4);
+        numbers<G, I + 1>(x, low, inv, bytes);
     }
-    bytes_t<G> b;
+}
+
+// Hold the 2 G elements that this lane has of a key (x[0]) and of its value (x[1]) as the vectors at `vec`.  Lane i of
+// the row works out the words of group i of the 2 G (the divisions once, not in every lane) and stores them.
+template <int G>
+__device__ __forceinline__ void hold4(const jyhip_pages& P, int64_t vec, const float (&x)[2][2 * G]) {
+    const int r = threadIdx.x & 15, hd = P.head_dim;
+    float lo = 0.0f, hi = 0.0f, past[2];
 #pragma unroll
-    for (int g = 0; g < G; g++) b[g] = bytes[g];
-    *reinterpret_cast<bytes_t<G>*>(static_cast<uint8_t*>(pool) + vec * (16 * G) + r * G) = b;
-    if (r < G) static_cast<uint32_t*>(scales)[vec * G + r] = word;
+    for (int s = 0; s < 2; s++) {
+        past[s] = 0.0f;
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+            const bool on = 32 * g + 2 * r < hd;
+            const float a = x[s][2 * g], b = x[s][2 * g + 1];
+            past[s] = on && !(fmaxf(fabsf(a), fabsf(b)) <= kMax4 && a == a && b == b) ? 1.0f : past[s];
+            const float least = row_min(on ? fminf(a, b) : __builtin_inff());
+            const float most = row_max(on ? fmaxf(a, b) : -__builtin_inff());
+            lo = r == s * G + g ? least : lo;
+            hi = r == s * G + g ? most : hi;
+        }
+        past[s] = row_max(past[s]);
+    }
+    const bool some = 32 * (r % G) < hd, second = r >= G;  // (lanes from 2 G on: anything)
+    const bool bad = (second ? past[1] : past[0]) > 0.0f;  // the whole vector is NaN
+    const _Float16 low = some ? (_Float16)lo : (_Float16)0.0f;
+    const _Float16 step = some ? (_Float16)seven_bits((hi - (float)low) / 15.0f) : (_Float16)0.0f;
+    const float inv = (float)step > 0.0f && !bad ? 1.0f / (float)step : 0.0f;
+    const uint32_t word = bad && some ? 0x7e007e00u : __builtin_bit_cast(uint32_t, h2_t{step, low});
+    uint8_t bytes[2][G];
+    numbers<G, 0>(x, (float)low, inv, bytes);
+#pragma unroll
+    for (int s = 0; s < 2; s++) {
+        bytes_t<G> b;
+#pragma unroll
+        for (int g = 0; g < G; g++) b[g] = 32 * g + 2 * r < hd && !(past[s] > 0.0f) ? bytes[s][g] : (uint8_t)0;
+        *reinterpret_cast<bytes_t<G>*>(static_cast<uint8_t*>(s ? P.v : P.k) + vec * (16 * G) + r * G) = b;
+    }
+    if (r < 2 * G) reinterpret_cast<uint32_t*>(second ? P.v_scale : P.k_scale)[vec * G + r % G] = word;
 }
 
 template <class E, int G>
@@ -160,12 +183,11 @@ __global__ __launch_bounds__(256) void paged4_kernel(Moved4 A, bool pairs) {
     const int64_t vec =
         slot < 0 ? -1 : (((slot >> A.ps_log2) * nkv + head) << A.ps_log2) + (slot & ((1 << A.ps_log2) - 1));
     if constexpr (WRITE) {
-        float x[2 * G], y[2 * G];
-        load_pairs<E, G>(k, P.head_dim, pairs, x);
-        load_pairs<E, G>(v, P.head_dim, pairs, y);
+        float x[2][2 * G];
+        load_pairs<E, G>(k, P.head_dim, pairs, x[0]);
+        load_pairs<E, G>(v, P.head_dim, pairs, x[1]);
         if (vec < 0) return;
-        hold4<G>(P.k, P.k_scale, vec, P.head_dim, x);
-        hold4<G>(P.v, P.v_scale, vec, P.head_dim, y);
+        hold4<G>(P, vec, x);
     } else {
         give4<E, G>(P.k, P.k_scale, vec, P.head_dim, k, pairs);
         give4<E, G>(P.v, P.v_scale, vec, P.head_dim, v, pairs);
