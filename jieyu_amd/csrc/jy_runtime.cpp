@@ -1785,11 +1785,14 @@ int forward_paged(jyhip_model* m, const jyhip_pages* pages, const float* X, floa
         const int* t = tables + (size_t)(seq ? seq[r] : r) * table_stride;
         h.insert(h.end(), t, t + table_stride);
     }
-    if (paged_attend_blocks(pages[0], rows, m->nh, max_len) >= (1 << 24)) fail("forward_paged: too many rows for one call");
+    size_t part = 0;  // (layers may hold different types, whose attention needs different workspaces)
+    for (int l = 0; l < m->L; l++) {
+        if (paged_attend_blocks(pages[l], rows, m->nh, max_len) >= (1 << 24)) fail("forward_paged: too many rows for one call");
+        part = std::max(part, paged_attend_part_floats(pages[l], rows, m->nh, max_len));
+    }
     check_moved_size(rows, m->nkv);
     const OnDevice on(m->device, nullptr);
     ensure_ws(m, rows);
-    const size_t part = paged_attend_part_floats(pages[0], rows, m->nh, max_len);
     if (m->paged_idx_n < h.size()) {
         dfree(m->paged_idx);
         m->paged_idx = nullptr;
