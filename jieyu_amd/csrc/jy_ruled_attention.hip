@@ -34,7 +34,7 @@ constexpr int kPages = 4096;  // positions whose pages the lanes hold at once
 Ruled plan_of(const RuledAttn& A) {
     Ruled K;
     K.A = A;
-    K.ps_log2 = __builtin_ctz(A.P.page_size);
+    K.ps_log2 = A.P.page_size > 0 ? __builtin_ctz(A.P.page_size) : 0;  // (a workspace is asked for before pages are checked)
     K.sstride = 0;
     if (plan_tiled(K)) return K;
     const int per = A.nh / A.P.num_kv_heads;

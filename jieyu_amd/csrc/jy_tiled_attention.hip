@@ -731,8 +731,12 @@ bool plan_tiled(Ruled& K) {
     const RuledAttn& A = K.A;
     if (!A.starts || A.type == JYHIP_T_F32) return false;
     const int per = A.nh / A.P.num_kv_heads;
-    // runs that fill a wave's columns at least
-    if ((int64_t)A.rows * per < (int64_t)32 * A.M.nseq) return false;
+    // Columns a run on average that pay for tiles of 128; the kernel of 16 columns reads a run's cache once for
+    // each 16.  32 heads over 8 of 128, 16 runs behind 4000 positions: 8 rows each (32 columns) 48 us there and 62
+    // here, 16 rows 66 and 74, 32 rows 95 and 91, 64 rows 155 and 132; prompts of 16 rows 17.5 and 12.9.  14 over 2
+    // of 64: 4 rows (28 columns) 25 and 26, 8 rows (56) 29 and 27, 16 rows 36 and 31.
+    const int pays = A.P.head_dim <= 64 ? 32 : 64;
+    if ((int64_t)A.rows * per < (int64_t)pays * A.M.nseq) return false;
     K.hpg = std::min(per, COLS);
     K.tiles = (per + COLS - 1) / COLS;
     K.rpg = per <= COLS ? COLS / per : 1;
