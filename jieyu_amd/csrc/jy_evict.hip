@@ -355,9 +355,9 @@ __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs K, int groups
 void launch_evict(const Eviction& E, hipStream_t st) {
     const EvictArgs K{E, __builtin_ctz(E.P.page_size)};
     const unsigned heads = (unsigned)(E.M.nseq * E.P.num_kv_heads);
-    const int held = (E.cap + 3) / 4 * 16;  // bytes of the ranks
+    const int64_t held = ((int64_t)E.cap + 3) / 4 * 16;  // bytes of the ranks
     if (held <= kHeld)
-        evict_select_kernel<true><<<heads, NT, held, st>>>(K);
+        evict_select_kernel<true><<<heads, NT, (unsigned)held, st>>>(K);
     else
         evict_select_kernel<false><<<heads, NT, 0, st>>>(K);
     const int width = std::min(E.keep, E.cap);

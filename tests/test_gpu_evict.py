@@ -311,3 +311,22 @@ def test_a_replayed_graph(jy):
         a, b, c, pages = kept.clone(), new_lens.clone(), new_w.clone(), p.k.clone()
         again = p.evict(0, w, dt, lens, 100, 10, 500, dto)
         assert torch.equal(a, again[0]) and torch.equal(b, again[1]) and torch.equal(c, again[2]) and torch.equal(pages, p.k)
+
+
+def test_a_table_of_2_to_the_30_positions(jy):
+    """an upper bound far past the sequence: the ranks of 100 positions, not of all that the table could hold"""
+    g = gen(4)
+    p = jy.PagePool.empty(1, 2, 256, 1, 16, dtype=torch.float16, device=DEV)
+    k, v = (torch.randn((100, 1, 16), generator=g).to(DEV) for _ in range(2))
+    t = torch.full((1, 1 << 22), -1, dtype=torch.int32, device=DEV)
+    t[0, 0] = 0
+    at, zero = ints(list(range(100))), ints([0] * 100)
+    p.write(0, k, v, t, at, seq=zero)
+    w = torch.rand((1, 1, 100), generator=g).to(DEV)
+    for bound in (1 << 29, 1 << 30):
+        kept, n, left = p.evict(0, w, t, ints([100]), 40, 10, bound, ints([[1]]))
+        want = stays(w[0, 0].tolist(), 100, 40, 10, [True] * 100)
+        assert kept[0, 0].tolist() == want and n.tolist() == [40]
+        assert torch.equal(left[0, 0, :40], w[0, 0, want]) and not left[0, 0, 40:].any()
+        got, _ = p.read(0, ints([[1]]), ints(list(range(40))), seq=ints([0] * 40))
+        assert torch.equal(got, k[want].half().float())
