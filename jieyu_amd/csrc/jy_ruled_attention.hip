@@ -184,8 +184,8 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void ruled_attend_kernel(Rule
     } else {
         // (a chunk that its sequence has not leaves at once: in a ragged batch those are most)
         if (!A.first) early = pages(at, split * K.chunk);
-        const int f = A.first ? max(A.first[at], 0) & ~31 : 0;
-        if (split != 0 && f + split * K.chunk >= min(A.lens[at], A.cap)) return;
+        const unsigned f = A.first ? max(A.first[at], 0) & ~31 : 0;
+        if (split != 0 && f + (unsigned)split * K.chunk >= (unsigned)max(min(A.lens[at], A.cap), 0)) return;
     }
     const int b = run.seq, rows = min(K.rpg, run.end - run.row0);
     // this lane's column
@@ -209,8 +209,9 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void ruled_attend_kernel(Rule
     const int all_lo = __builtin_amdgcn_readfirstlane(cols_max(sees ? lo : 0));
     const int all_hi = __builtin_amdgcn_readfirstlane(cols_min(sees ? hi : 0x7fffffff));
     const int base = to > 0 ? from & ~31 : 0;
+    // (both up to 2^30: their sum may pass 2^31)
+    if (split != 0 && (unsigned)base + (unsigned)split * K.chunk >= (unsigned)to) return;
     const int c0 = base + split * K.chunk;
-    if (split != 0 && c0 >= to) return;
     if (K.splits > 1 && split == 0 && hg == 0 && threadIdx.x < 16 && on && chead == 0)
         K.part_live[row] = max(1, (to - base + K.chunk - 1) / K.chunk);
 

@@ -220,8 +220,9 @@ __global__ __launch_bounds__(NT, HDT <= 2 ? 2 : 1) void tiled_attend_kernel(Rule
     from = __builtin_amdgcn_readfirstlane(from);
     to = __builtin_amdgcn_readfirstlane(to);
     const int base = to > 0 ? from & ~31 : 0;
+    // (both up to 2^30: their sum may pass 2^31)
+    if (split != 0 && (unsigned)base + (unsigned)split * K.chunk >= (unsigned)to) return;
     const int c0 = base + split * K.chunk;
-    if (split != 0 && c0 >= to) return;
     if (K.splits > 1 && split == 0 && hg == 0)
         for (int r = tid; r < rows; r += NT) K.part_live[run.row0 + r] = max(1, (to - base + K.chunk - 1) / K.chunk);
     const int end = K.splits > 1 ? min(to, c0 + K.chunk) : to;

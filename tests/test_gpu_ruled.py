@@ -555,3 +555,35 @@ def test_no_rows(jy):
     c = Cache(jy, [5], 2, 64, 16, "i4", seed=12)
     e = torch.empty((0, 4, 64), device=DEV)
     assert c.pool.attend_rows(c.layer, e, c.dtables, ints([0, 0]), ints([]), 5).shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("pool", ["i4", "bf16"])
+@pytest.mark.parametrize("first", [0, (1 << 30) - 4096, (1 << 30) - 100])
+def test_windows_at_the_far_end(jy, pool, first):
+    """a window near position 2^30 with bounds as large: positions and pieces whose sum passes 31 bits"""
+    n = 1 << 30
+    p = jy.PagePool.empty(1, 2, 256, 1, 64, dtype=POOL[pool], device=DEV)
+    t = torch.full((1, n // 256), -1, dtype=torch.int32, device=DEV)
+    t[0, -1], t[0, 3] = 1, 0
+    g = gen(3)
+    k, v = (torch.randn((2, 1, 64), generator=g).to(DEV) for _ in range(2))
+    for pg in range(2):
+        p.k[0, pg], p.v[0, pg] = 0, 0
+        if p.k_scale is not None:
+            p.k_scale[0, pg], p.v_scale[0, pg] = 0, 0
+    where, zero = ints([n - 1, 800]), ints([0, 0])
+    p.write(0, k, v, t, where, seq=zero)
+    kk, vv = p.read(0, t, where, seq=zero)
+    q = torch.randn((1, 1, 64), generator=g).to(DEV)
+    seen = 512 if first == 0 else min(n - first, 256)  # (all the rest are holes)
+    s = torch.zeros(seen, dtype=torch.float64)
+    s[0] = (q[0, 0].double() @ kk[0, 0].double()).cpu() / 8
+    if first == 0:
+        s[1] = (q[0, 0].double() @ kk[1, 0].double()).cpu() / 8
+    w = torch.softmax(s, 0)
+    want = w[0] * vv[0, 0].double().cpu() + (w[1] * vv[1, 0].double().cpu() if first == 0 else 0)
+    rows = q.expand(1, 1, 64).contiguous()
+    # (a sum of two products, whose weights are off by 2^-20 of 1 at scores of a few: far under 1e-5 of values of a few)
+    for got in (p.attend(0, rows, t, ints([n]), n, first=ints([first])),
+                p.attend_rows(0, rows, t, ints([0, 1]), ints([n - 1]), n, first=ints([first]))):
+        assert (got[0, 0].double().cpu() - want).abs().max() < 1e-5
