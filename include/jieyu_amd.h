@@ -372,7 +372,8 @@ typedef struct jyhip_rules {
  * over positions first[s] .. lens[s] - 1.  With `first`, max_len is an upper bound of lens[s] - first[s], and of
  * more positions the first max_len count.  With `weights`, fp32, the weights of position j, summed over the
  * query heads of a kv head, are added to weights[s * weights_seq_stride + kv head * weights_head_stride + j]
- * (strides in elements), for each position j < weights_len that s sees; sequences have elements of their own.  What is not finite: as in
+ * (strides in elements), for each position j < weights_len that s sees; each sequence and head has elements of its own (strides
+ * that say otherwise are refused).  What is not finite: as in
  * jyhip_pages_attend, but that what a row's rules leave out never reaches it; with a cap a score of +-infinity is
  * +-cap. */
 JYHIP_API int jyhip_pages_attend_ruled(const jyhip_pages* pages, const jyhip_page_tables* tables, const int* lens,

@@ -125,6 +125,15 @@ RuledAttn ruled_args(const jyhip_pages* pages, const jyhip_page_tables* tables, 
     return A;
 }
 
+// whether weights that are written [seqs][heads][len] have an element each
+bool apart(long long seq_stride, int seqs, long long head_stride, int heads, int len) {
+    if (len == 0) return true;
+    auto nested = [len](long long inner, int a, long long outer, int b) {
+        return (a == 1 || inner >= len) && (b == 1 || (__int128)outer >= (a == 1 ? 0 : (__int128)inner * (a - 1)) + len);
+    };
+    return nested(head_stride, heads, seq_stride, seqs) || nested(seq_stride, seqs, head_stride, heads);
+}
+
 void launch_checked(RuledAttn& A, void* workspace, size_t workspace_bytes, int device, hipStream_t st) {
     A.part = static_cast<float*>(workspace);
     const size_t need = ruled_attend_part_floats(A) * sizeof(float);
@@ -235,6 +244,8 @@ JYHIP_API int jyhip_pages_attend_ruled(const jyhip_pages* pages, const jyhip_pag
         if (weights && (weights_seq_stride < 0 || weights_head_stride < 0 || weights_len < 0))
             fail("attend: a negative stride or length of the weights");
         if ((uintptr_t)weights % 4) fail("attend: weights are not aligned to their elements");
+        if (weights && !apart(weights_seq_stride, tables->num_seqs, weights_head_stride, pages->num_kv_heads, weights_len))
+            fail("attend: the weights of two sequences or heads share elements");
         A.lens = lens;
         A.rows = tables->num_seqs;
         if (!A.first) A.cap = std::min(A.cap, max_len);
@@ -305,6 +316,8 @@ JYHIP_API int jyhip_pages_evict(const jyhip_pages* pages, const jyhip_page_table
         if (weights_seq_stride < 0 || weights_head_stride < 0 || weights_len < 0 || new_seq_stride < 0 || new_head_stride < 0 ||
             new_weights_len < 0)
             fail("evict: a negative stride or length of weights");
+        if (new_weights && !apart(new_seq_stride, tables->num_seqs, new_head_stride, pages->num_kv_heads, new_weights_len))
+            fail("evict: the new weights of two sequences or heads share elements");
         Eviction E;
         E.P = *pages;
         E.M = map_of(tables, nullptr, nullptr);

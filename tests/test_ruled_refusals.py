@@ -116,3 +116,15 @@ def test_4bit_pools_want_their_layout():
     x = torch.zeros((1, 2, 2, 16, 32), dtype=torch.uint8)
     with pytest.raises(jieyu_amd.JyError, match="device tensors"):
         jieyu_amd.PagePool(x, x, None, None)
+
+
+@pytest.mark.parametrize("ws,hs,wn,ok", [(0, 32, 32, False), (64, 0, 32, False), (64, 32, 33, False), (63, 32, 32, False), (32, 96, 32, True),
+                                         (32, 95, 32, False), (31, 96, 32, False), (1 << 62, 1 << 62, 5, False), (0, 0, 0, True)])
+def test_weights_that_are_written_share_no_elements(b, ws, hs, wn, ok):
+    """3 sequences of 2 heads, in either order"""
+    bad = dict(bytes=0, max_len=5000) if ok else {}  # (good strides reach the check of the workspace)
+    assert one(b, w=0x1000, ws=ws, hs=hs, wn=wn, **bad) == -1
+    assert ("workspace" if ok else "share") in b.error().decode()
+    if not ok:
+        assert evict(b, nw=0x1000, ns=ws, nh=hs, nn=wn) == -1
+        assert "share" in b.error().decode()
