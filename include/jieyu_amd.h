@@ -253,7 +253,7 @@ enum { JYHIP_T_F32 = 0, JYHIP_T_F16 = 1, JYHIP_T_BF16 = 2, JYHIP_T_I8 = 3, JYHIP
  *   k_scale, v_scale  fp32 [num_pages][num_kv_heads][page_size] with JYHIP_T_I8, the groups'
  *                     numbers below with JYHIP_T_I4, else NULL
  * head_dim: a multiple of 16 up to 256; page_size: 16, 32, 64, 128 or 256; type: JYHIP_T_I8,
- * JYHIP_T_I4, JYHIP_T_F16 or JYHIP_T_BF16.  k and v are aligned to 16 bytes.  An int8 vector holds
+ * JYHIP_T_I4, JYHIP_T_F16 or JYHIP_T_BF16.  k and v are aligned to 16 bytes, as 4-bit pages' scales are.  An int8 vector holds
  * q * scale by the rule of jyhip_kv (libs/model_libs/attention/attention_q8.h:29-35): scale =
  * absmax / 127, q = rint(x * (127 / absmax)), both fp32; zeros where absmax <= 1e-8.  A vector
  * with an infinity or a NaN in it is held as NaN (scale NaN), all of it.
@@ -388,7 +388,11 @@ JYHIP_API size_t jyhip_pages_attend_ruled_workspace(const jyhip_pages* pages, in
  * q and out (starts: int32 [num_seqs + 1], ascending, on the device), and row r stands at position pos[r] and sees
  * positions first[r] .. last[r] - 1 (0 and pos[r] + 1 without them) of its sequence, whose keys and values are in the
  * pages.  A row that sees nothing gives zeros; rows before starts[0] and from starts[num_seqs] on are left as they
- * are.  max_len is an upper bound of the positions that any row sees (last, or pos + 1): those past it are cut. */
+ * are.  max_len is an upper bound of the positions that any row sees (last, or pos + 1): those past it are cut.
+ * Long runs of 16-bit rows take a weight as one number of the second product's type: fp16 over fp16 and 4-bit pages
+ * (under 2^-25 of its row's largest it may count as 0; a 4-bit value is rounded to fp16 there), else bf16, in two
+ * parts where the outputs are fp16; sums are fp32.  Which runs are long is decided by the call's rows, query heads and
+ * sequences.  What is not finite: as with single rows, for each row by what it sees. */
 JYHIP_API int jyhip_pages_attend_rows(const jyhip_pages* pages, const jyhip_page_tables* tables, const int* starts,
                                       const int* pos, int rows, int max_len, int num_heads, float scale,
                                       const jyhip_rules* rules, const jyhip_vectors* q, const jyhip_vectors* out, int type,
@@ -426,8 +430,8 @@ JYHIP_API int jyhip_rope(const jyhip_vectors* q, const jyhip_vectors* q_out, int
 /* One pass of a model over `rows` tokens of several sequences whose keys and values lie in pages: row r
  * is position pos[r] of sequence seq[r] (seq NULL: of sequence r).  X and out: host [rows][hidden], the
  * tokens' embeddings and their final-normed hidden states, as in jyhip_forward_cached_to (out may be X).
- * pages: one pool per layer of the model (pages[0 .. num_layers)), all of one shape, on the model's
- * device, its heads the model's.  tables, seq and pos are HOST arrays here ([num_seqs][table_stride],
+ * pages: one pool per layer of the model (pages[0 .. num_layers)), of one number and size of pages (the types
+ * may differ), on the model's device, its heads the model's.  tables, seq and pos are HOST arrays here ([num_seqs][table_stride],
  * [rows], [rows]).  Each layer writes the rows' keys and values into the pages, then every row attends
  * over positions 0 .. pos[r] of its sequence, so several new positions of one sequence may come in one
  * call (a prompt) as long as the earlier ones are in the pages or in the call; each row reads its positions

@@ -1,5 +1,6 @@
-"""Operators of a decode step over several sequences at once (include/jieyu_amd.h), on torch
-tensors in device memory: a paged key/value cache, attention over it, and sampling.
+"""Operators of a step over several sequences at once (include/jieyu_amd.h), on torch tensors in device
+memory: rotary positions, a paged key/value cache (down to 4 bits an element), attention of single rows and of
+runs of rows over it, eviction from it, and sampling.
 
 Everything runs on torch's current stream of the tensors' device and nothing waits for it, so
 calls can be recorded into a graph.  Workspaces come from torch's allocator, call by call.  There are
@@ -254,7 +255,7 @@ class PagePool:
         of lens - first.  cap: a score s becomes cap * tanh(s / cap).  slopes (float32 [heads]): slope times the
         distance to position lens[s] - 1 is taken off the scores.  weights (float32 [sequences][kv heads]
         [positions]): the weights of each position, summed over the query heads of a kv head, are added to it (past its
-        last position they are not counted)."""
+        last position they are not counted; each sequence and head has elements of its own)."""
         b = self._b
         pages, T = self._layer(layer), self._tables(tables)
         Q, O, code, batch, heads, out = self._queries(q, out)
@@ -305,7 +306,6 @@ class PagePool:
                          code, ws.data_ptr() if need else None, need, b.stream(self.device.index)) != 0:
             _failed(b)
         return out
-
 
     def _weights(self, t, batch, name):
         """Weights of positions, for the library: address, strides and length."""

@@ -10,7 +10,9 @@
 // each group lies beside the others (byte r G + g of the vector, G groups), so a lane's bytes are one store,
 // and the attention's lanes, which take a vector's dims in the same shares, one load.  A group's lowest and
 // largest take four DPP moves within the row of lanes, and lane i works out the words of one of the key's and
-// the value's groups.
+// the value's groups (each lane dividing for itself: 29 us against 25 for 8191 rows of 8 heads of 128 in bf16,
+// which read 34 MB and write 10).  Its vector instructions bound the write; the same rows read back take 13 us,
+// 3.4 TB/s.
 #include <hip/hip_runtime.h>
 
 #include "jy_device.h"

