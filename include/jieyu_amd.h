@@ -392,7 +392,7 @@ JYHIP_API size_t jyhip_pages_attend_ruled_workspace(const jyhip_pages* pages, in
  * Long runs of 16-bit rows take a weight as one number of the second product's type: fp16 over fp16 and 4-bit pages
  * (under 2^-25 of its row's largest it may count as 0; a 4-bit value is rounded to fp16 there), else bf16, in two
  * parts where the outputs are fp16; sums are fp32.  Which runs are long is decided by the call's rows, query heads and
- * sequences.  What is not finite: as with single rows, for each row by what it sees. */
+ * sequences.  What is not finite: as with single rows, for each row by what it sees.  rows x num_heads is less than 2^22. */
 JYHIP_API int jyhip_pages_attend_rows(const jyhip_pages* pages, const jyhip_page_tables* tables, const int* starts,
                                       const int* pos, int rows, int max_len, int num_heads, float scale,
                                       const jyhip_rules* rules, const jyhip_vectors* q, const jyhip_vectors* out, int type,

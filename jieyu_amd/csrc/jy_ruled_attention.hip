@@ -18,7 +18,7 @@
 //
 // 64 sequences of 200 to 8190, 32 heads over 8 of 128, 4 bits: 75 to 81 us, 2.5 TB/s (4.1 where all are of one
 // length: in the ragged batch the longest end alone); the vector instructions of a tile are as long as its loads.
-// 8 of 1000 to 16001 in int8 with cap and weights: 46 us, 6.6 of join, 6.5 of weighing.  77 drafted rows of 16
+// 8 of 1000 to 16001 in int8 with cap and weights: 46 us, 4.9 of join, 6.3 of weighing.  77 drafted rows of 16
 // sequences behind 4000 positions in int8: 35 us.
 #include <hip/hip_runtime.h>
 
@@ -644,7 +644,9 @@ void launch_ruled_attend(const RuledAttn& A, hipStream_t st) {
     if (K.splits > 1) {
         const int quads = A.P.head_dim / 4;
         const int64_t rows = (int64_t)A.rows * A.nh;
-        if (K.splits <= 16)
+        // 8 sequences of 32 heads of 128: 16 chunks 4.7 us with a workgroup a row, 6.7 with a thread for four dims; the
+        // latter takes 4.8 for 64 sequences of 8 chunks, with fewer workgroups to start
+        if (K.splits <= 8)
             ruled_join_few_kernel<<<(unsigned)((rows * quads + 255) / 256), 256, 0, st>>>(K);
         else if (K.splits * quads <= 4 * 256)
             ruled_join_kernel<256><<<(unsigned)rows, 256, 0, st>>>(K);
