@@ -173,26 +173,39 @@ __device__ __forceinline__ void give4(const void* pool, const void* scales, int6
     }
 }
 
-template <class E, int G, bool WRITE>
+// 16 lanes take VECS vectors: what the later ones wait for is under way with the first's
+template <class E, int G, bool WRITE, int VECS>
 __global__ __launch_bounds__(256) void paged4_kernel(Moved4 A, bool pairs) {
     const jyhip_pages& P = A.P;
-    const unsigned i = blockIdx.x * 16 + (threadIdx.x >> 4), nkv = P.num_kv_heads;
-    const int row = (int)(i / nkv), head = (int)(i - row * nkv);
-    if (row >= A.rows) return;
-    E* const k = static_cast<E*>(A.k.data) + row * A.k.row_stride + head * A.k.head_stride;
-    E* const v = static_cast<E*>(A.v.data) + row * A.v.row_stride + head * A.v.head_stride;
-    const int64_t slot = slot_of(A.M, P.num_pages, A.ps_log2, A.M.seq ? A.M.seq[row] : row, A.M.pos[row]);
-    const int64_t vec =
-        slot < 0 ? -1 : (((slot >> A.ps_log2) * nkv + head) << A.ps_log2) + (slot & ((1 << A.ps_log2) - 1));
+    const unsigned i0 = (blockIdx.x * 16 + (threadIdx.x >> 4)) * VECS, nkv = P.num_kv_heads, total = A.rows * nkv;
+    E *k[VECS], *v[VECS];
+    int64_t vec[VECS];
+#pragma unroll
+    for (int c = 0; c < VECS; c++) {
+        const unsigned i = i0 + c < total ? i0 + c : total - 1;
+        const int row = (int)(i / nkv), head = (int)(i - row * nkv);
+        k[c] = static_cast<E*>(A.k.data) + row * A.k.row_stride + head * A.k.head_stride;
+        v[c] = static_cast<E*>(A.v.data) + row * A.v.row_stride + head * A.v.head_stride;
+        const int64_t slot = slot_of(A.M, P.num_pages, A.ps_log2, A.M.seq ? A.M.seq[row] : row, A.M.pos[row]);
+        vec[c] = slot < 0 ? -1 : (((slot >> A.ps_log2) * nkv + head) << A.ps_log2) + (slot & ((1 << A.ps_log2) - 1));
+    }
     if constexpr (WRITE) {
-        float x[2][2 * G];
-        load_pairs<E, G>(k, P.head_dim, pairs, x[0]);
-        load_pairs<E, G>(v, P.head_dim, pairs, x[1]);
-        if (vec < 0) return;
-        hold4<G>(P, vec, x);
+        float x[VECS][2][2 * G];
+#pragma unroll
+        for (int c = 0; c < VECS; c++) {
+            load_pairs<E, G>(k[c], P.head_dim, pairs, x[c][0]);
+            load_pairs<E, G>(v[c], P.head_dim, pairs, x[c][1]);
+        }
+#pragma unroll
+        for (int c = 0; c < VECS; c++)
+            if (vec[c] >= 0 && i0 + c < total) hold4<G>(P, vec[c], x[c]);
     } else {
-        give4<E, G>(P.k, P.k_scale, vec, P.head_dim, k, pairs);
-        give4<E, G>(P.v, P.v_scale, vec, P.head_dim, v, pairs);
+#pragma unroll
+        for (int c = 0; c < VECS; c++) {
+            if (i0 + c >= total) return;
+            give4<E, G>(P.k, P.k_scale, vec[c], P.head_dim, k[c], pairs);
+            give4<E, G>(P.v, P.v_scale, vec[c], P.head_dim, v[c], pairs);
+        }
     }
 }
 
@@ -202,39 +215,41 @@ bool paired(const jyhip_vectors& x, int type) {
     return ((uintptr_t)x.data | (uintptr_t)(x.row_stride * e) | (uintptr_t)(x.head_stride * e)) % (2 * e) == 0;
 }
 
-template <class E, bool WRITE>
+template <class E, bool WRITE, int VECS>
 void launch_groups(const Moved4& A, bool pairs, unsigned grid, hipStream_t st) {
     switch (groups4(A.P.head_dim)) {
-        case 2: paged4_kernel<E, 2, WRITE><<<grid, 256, 0, st>>>(A, pairs); break;
-        case 4: paged4_kernel<E, 4, WRITE><<<grid, 256, 0, st>>>(A, pairs); break;
-        default: paged4_kernel<E, 8, WRITE><<<grid, 256, 0, st>>>(A, pairs);
+        case 2: paged4_kernel<E, 2, WRITE, VECS><<<grid, 256, 0, st>>>(A, pairs); break;
+        case 4: paged4_kernel<E, 4, WRITE, VECS><<<grid, 256, 0, st>>>(A, pairs); break;
+        default: paged4_kernel<E, 8, WRITE, VECS><<<grid, 256, 0, st>>>(A, pairs);
     }
 }
 
-template <bool WRITE>
-void launch_moved4(const jyhip_pages& P, const PageMap& M, int rows, const jyhip_vectors& k, const jyhip_vectors& v,
-                   int type, hipStream_t st) {
-    const Moved4 A{P, M, rows, __builtin_ctz(P.page_size), k, v};
-    const bool pairs = paired(k, type) && paired(v, type);
-    const unsigned grid = (unsigned)(((int64_t)rows * P.num_kv_heads + 15) / 16);
+template <bool WRITE, int VECS>
+void launch_vectors(const Moved4& A, int type, hipStream_t st) {
+    const bool pairs = paired(A.k, type) && paired(A.v, type);
+    const unsigned grid = (unsigned)(((int64_t)A.rows * A.P.num_kv_heads + 16 * VECS - 1) / (16 * VECS));
     if (type == JYHIP_T_F32)
-        launch_groups<float, WRITE>(A, pairs, grid, st);
+        launch_groups<float, WRITE, VECS>(A, pairs, grid, st);
     else if (type == JYHIP_T_F16)
-        launch_groups<_Float16, WRITE>(A, pairs, grid, st);
+        launch_groups<_Float16, WRITE, VECS>(A, pairs, grid, st);
     else
-        launch_groups<__bf16, WRITE>(A, pairs, grid, st);
+        launch_groups<__bf16, WRITE, VECS>(A, pairs, grid, st);
 }
 
 }  // namespace
 
 void launch_paged4_write(const jyhip_pages& P, const PageMap& M, int rows, const jyhip_vectors& k,
                          const jyhip_vectors& v, int type, hipStream_t st) {
-    launch_moved4<true>(P, M, rows, k, v, type, st);
+    const Moved4 A{P, M, rows, __builtin_ctz(P.page_size), k, v};
+    if ((int64_t)rows * P.num_kv_heads >= 32768)
+        launch_vectors<true, 2>(A, type, st);
+    else
+        launch_vectors<true, 1>(A, type, st);
 }
 
 void launch_paged4_read(const jyhip_pages& P, const PageMap& M, int rows, const jyhip_vectors& k,
                         const jyhip_vectors& v, int type, hipStream_t st) {
-    launch_moved4<false>(P, M, rows, k, v, type, st);
+    launch_vectors<false, 1>(Moved4{P, M, rows, __builtin_ctz(P.page_size), k, v}, type, st);
 }
 
 }  // namespace jy
