@@ -291,7 +291,11 @@ __global__ __launch_bounds__(NT, HDT <= 2 ? 2 : 1) void tiled_attend_kernel(Rule
             sums = __builtin_bit_cast(u4_t, w);
         }
         const float unit = F::SCALED ? __builtin_ldexpf(1.0f, -e2) : 1.0f;
-        qf = bad ? __builtin_nanf("") : unit * (A.soft != 0.0f ? fabsf(A.scale) / A.soft : fabsf(A.scale) * kLog2e);
+        qf = unit * (A.soft != 0.0f ? fabsf(A.scale) / A.soft : fabsf(A.scale) * kLog2e);
+        // Queries and scales so small that this would be 0, which a masked score of -infinity cannot be multiplied with: raw
+        // scores are under 2^40 here, so these scores are 0 either way.
+        if constexpr (F::SCALED) qf = fmaxf(qf, 0x1p-126f);
+        if (bad) qf = __builtin_nanf("");
     }
     const bool simple = !(fabsf(A.scale) < 0x1p-60f);
     const float soft = A.soft * kLog2e, slope = A.slopes ? A.slopes[head] * kLog2e : 0.0f;
@@ -521,7 +525,7 @@ __global__ __launch_bounds__(NT, HDT <= 2 ? 2 : 1) void tiled_attend_kernel(Rule
                 }
         }
         // s becomes the exponents, scores in units of log2 e less the running maximum: without cap or bias by one fma (but
-        // where qf could be 0, which -infinity cannot be multiplied with); capped ones that all lie within half the cap by
+        // where the scale is 0 or close to it, as -infinity cannot be multiplied with 0); capped ones that all lie within half the cap by
         // a polynomial (tanh to 1.3e-7, fitted) in five operations; else step by step.
         float top = largest(1.0f);
         int way = A.slopes || (A.soft != 0.0f && masked) || !simple ? 2 : A.soft != 0.0f ? 1 : 0;

@@ -1,0 +1,46 @@
+"""Runs of 16-bit rows at the ends of their numbers' ranges, rule by rule, and beside single tokens, against the
+definition in 64 bits."""
+import math
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from test_gpu_ruled import DEV, POOL, Cache, attention64, check, gen, ints, jy  # noqa: E402, F401
+
+pytestmark = pytest.mark.gpu
+
+IO16 = {"f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def room16(c, b, p, room, last, first, far=2.0**-25):
+    """The room of 32-bit scores and sums, and what a weight's rounding to the product's type adds: fp16 over fp16 and
+    4-bit values (half a step 2^-11; a 4-bit value is one fp16 number, another 2^-11; `far` of the largest weight is where
+    fp16 ends), else bf16, 2^-8, or two of them, 2^-16."""
+    va, per = c.va[b], p.shape[1] // c.nkv
+    out = room.clone()
+    for r in range(p.shape[0]):
+        lo, hi = max(first[r], 0), last[r]
+        for h in range(p.shape[1]):
+            v = va[lo:hi, h // per]
+            out[r, h] += c.one * (p[r, h, lo:hi] @ v) + (hi - lo) * (far if c.kind in ("f16", "i4") else 2.0**-39) * v.amax()
+    return out
+
+
+def tiles64(c, b, q, pos, first, last, far=2.0**-25, **kw):
+    """(want, room): a cap's tanh is off by 8 steps of itself, not of the cap"""
+    want, room, p, _ = attention64(c, b, q, pos, first, last, **kw)
+    c.one = {"i4": 2.0**-10, "f16": 2.0**-11}.get(c.kind, 2.0**-8 if q.dtype is torch.bfloat16 else 2.0**-16)
+    return want, room16(c, b, p, room, last, first, far)
+
+
+@pytest.mark.parametrize("pool", list(POOL))
+@pytest.mark.parametrize("scale", [2.0**-30, 2.0**-45, -2.0**-30])
+def test_queries_so_small_that_scores_are_zeros(jy, pool, scale):
+    """tiles that are cut by the diagonal: the factor of such scores is under fp32's smallest number"""
+    n = 150
+    c = Cache(jy, [n], 2, 64, 16, pool, seed=3)
+    q = (torch.randn((n, 8, 64), generator=gen(4)) * 2.0**-120).bfloat16()
+    at = list(range(n))
+    got = c.pool.attend_rows(c.layer, q.to(DEV), c.dtables, ints([0, n]), ints(at), n, scale=scale)
+    check(got, *tiles64(c, 0, q, at, [0] * n, [p + 1 for p in at], scale=scale))
