@@ -170,7 +170,11 @@ __device__ __forceinline__ bool infinite16(uint32_t w, bool bf) {
     return (w & e) == e || (w >> 16 & e) == e;
 }
 
-template <int PT, int HDT, bool BIO>
+// FINE: tanh to 8 steps of itself.  1 - 2 / (e^2y + 1) cancels at small y and is off by 4 steps of 1, so scores under a cap c
+// by c 2^-22: up to caps of 64 that is 2e-5 of a weight.  As a branch of one kernel the other form made those that do not
+// take it 2 to 3% slower (slopes without a cap 849 -> 873 us, the prompt above).
+constexpr float kFineCap = 64.0f;
+template <int PT, int HDT, bool BIO, bool FINE>
 __global__ __launch_bounds__(NT, HDT <= 2 ? 2 : 1) void tiled_attend_kernel(Ruled K) {
 #if defined(__HIP_DEVICE_COMPILE__)
     typedef Form<PT, HDT, BIO> F;
@@ -300,9 +304,11 @@ __global__ __launch_bounds__(NT, HDT <= 2 ? 2 : 1) void tiled_attend_kernel(Rule
     const bool simple = !(fabsf(A.scale) < 0x1p-60f);
     const float soft = A.soft * kLog2e, slope = A.slopes ? A.slopes[head] * kLog2e : 0.0f;
 
-    // cap tanh(qf x) of a raw score x within half the cap, as a polynomial: x (p0 + p1 x^2 + p2 x^4 + p3 x^6)
-    const float q2 = qf * qf, p0 = 0.99999768f * (soft * qf), p1 = -0.33320654f * (soft * qf) * q2;
-    const float p2 = 0.13145139f * (soft * qf) * q2 * q2, p3 = -0.04337234f * (soft * qf) * q2 * q2 * q2;
+    // tanh y = y (1 + t1 y^2 + t2 y^4 + t3 y^6) for y up to 0.45, off by 2.9e-7 of itself at most (fitted; the first
+    // coefficient is 1, so that scores that are a small part of the cap lose nothing), and its coefficients for raw scores:
+    // cap tanh(qf x) = x (p0 + p1 x^2 + p2 x^4 + p3 x^6)
+    constexpr float kSmall = 0.45f, t1 = -0.333304852f, t2 = 0.13246648f, t3 = -0.0463218503f;
+    const float q2 = qf * qf, p0 = soft * qf, p1 = t1 * p0 * q2, p2 = t2 * p0 * q2 * q2, p3 = t3 * p0 * q2 * q2 * q2;
 
     // LDS addresses, in bytes: of a key's chunk of step 0 for the first product, and of the values' columns of tile 0
     // (for keys 0 .. 3 and 8 .. 11 of a half) for the second.  Step s and tile t lie an exclusive or with 32 s or 64 t away.
@@ -525,12 +531,12 @@ __global__ __launch_bounds__(NT, HDT <= 2 ? 2 : 1) void tiled_attend_kernel(Rule
                 }
         }
         // s becomes the exponents, scores in units of log2 e less the running maximum: without cap or bias by one fma (but
-        // where the scale is 0 or close to it, as -infinity cannot be multiplied with 0); capped ones that all lie within half the cap by
-        // a polynomial (tanh to 1.3e-7, fitted) in five operations; else step by step.
+        // where the scale is 0 or close to it, as -infinity cannot be multiplied with 0); capped ones that are all within
+        // 0.45 of the cap by the polynomial in five operations; else step by step.
         float top = largest(1.0f);
         int way = A.slopes || (A.soft != 0.0f && masked) || !simple ? 2 : A.soft != 0.0f ? 1 : 0;
-        // (the coefficients stay normal numbers for qf from 2^-16 on)
-        if (way == 1 && __any(!(fmaxf(top, largest(-1.0f)) * qf <= 0.5f && qf >= 0x1p-16f))) way = 2;
+        // (the polynomial's coefficients stay normal numbers for qf from 2^-16 on)
+        if (way == 1 && __any(!(fmaxf(top, largest(-1.0f)) * qf <= kSmall && qf >= 0x1p-16f))) way = 2;
         way = __builtin_amdgcn_readfirstlane(way);
         auto capped = [&](float x, float less) {
             const float x2 = x * x;
@@ -540,7 +546,15 @@ __global__ __launch_bounds__(NT, HDT <= 2 ? 2 : 1) void tiled_attend_kernel(Rule
             const float twice = 2.0f * kLog2e;
 #pragma unroll
             for (int n = 0; n < 2; n++) {
-                if (A.soft != 0.0f) {  // 1 - 2 / (e^2y + 1)
+                if (FINE) {
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const float y = s[n][i] * qf, y2 = y * y;
+                        const float x = __builtin_fmaf(-2.0f * soft, __builtin_amdgcn_rcpf(exp2_hw(fabsf(y) * twice) + 1.0f), soft);
+                        const float z = soft * y * __builtin_fmaf(y2, __builtin_fmaf(y2, __builtin_fmaf(y2, t3, t2), t1), 1.0f);
+                        s[n][i] = fabsf(y) <= kSmall ? z : __builtin_copysignf(x, y);
+                    }
+                } else if (A.soft != 0.0f) {  // 1 - 2 / (e^2y + 1)
 #pragma unroll
                     for (int i = 0; i < 16; i++)
                         s[n][i] = __builtin_fmaf(-2.0f * soft, __builtin_amdgcn_rcpf(exp2_hw(s[n][i] * qf * twice) + 1.0f), soft);
@@ -715,23 +729,31 @@ __global__ __launch_bounds__(NT, HDT <= 2 ? 2 : 1) void tiled_attend_kernel(Rule
 #endif
 }
 
-template <int PT, bool BIO>
+template <int PT, bool BIO, bool FINE>
 void launch_hd(const Ruled& K, unsigned grid, hipStream_t st) {
     const int hd = K.A.P.head_dim;
     if (hd <= 64)
-        tiled_attend_kernel<PT, 1, BIO><<<grid, NT, 0, st>>>(K);
+        tiled_attend_kernel<PT, 1, BIO, FINE><<<grid, NT, 0, st>>>(K);
     else if (hd <= 128)
-        tiled_attend_kernel<PT, 2, BIO><<<grid, NT, 0, st>>>(K);
+        tiled_attend_kernel<PT, 2, BIO, FINE><<<grid, NT, 0, st>>>(K);
     else
-        tiled_attend_kernel<PT, 4, BIO><<<grid, NT, 0, st>>>(K);
+        tiled_attend_kernel<PT, 4, BIO, FINE><<<grid, NT, 0, st>>>(K);
+}
+
+template <int PT, bool FINE>
+void launch_io(const Ruled& K, unsigned grid, hipStream_t st) {
+    if (K.A.type == JYHIP_T_BF16)
+        launch_hd<PT, true, FINE>(K, grid, st);
+    else
+        launch_hd<PT, false, FINE>(K, grid, st);
 }
 
 template <int PT>
-void launch_io(const Ruled& K, unsigned grid, hipStream_t st) {
-    if (K.A.type == JYHIP_T_BF16)
-        launch_hd<PT, true>(K, grid, st);
+void launch_fine(const Ruled& K, unsigned grid, hipStream_t st) {
+    if (K.A.soft > kFineCap)
+        launch_io<PT, true>(K, grid, st);
     else
-        launch_hd<PT, false>(K, grid, st);
+        launch_io<PT, false>(K, grid, st);
 }
 
 }  // namespace
@@ -766,13 +788,13 @@ bool plan_tiled(Ruled& K) {
 
 void launch_tiled(const Ruled& K, unsigned grid, hipStream_t st) {
     if (K.A.P.type == JYHIP_T_I4)
-        launch_io<JYHIP_T_I4>(K, grid, st);
+        launch_fine<JYHIP_T_I4>(K, grid, st);
     else if (K.A.P.type == JYHIP_T_I8)
-        launch_io<JYHIP_T_I8>(K, grid, st);
+        launch_fine<JYHIP_T_I8>(K, grid, st);
     else if (K.A.P.type == JYHIP_T_F16)
-        launch_io<JYHIP_T_F16>(K, grid, st);
+        launch_fine<JYHIP_T_F16>(K, grid, st);
     else
-        launch_io<JYHIP_T_BF16>(K, grid, st);
+        launch_fine<JYHIP_T_BF16>(K, grid, st);
 }
 
 }  // namespace jy

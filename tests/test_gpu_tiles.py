@@ -44,3 +44,38 @@ def test_queries_so_small_that_scores_are_zeros(jy, pool, scale):
     at = list(range(n))
     got = c.pool.attend_rows(c.layer, q.to(DEV), c.dtables, ints([0, n]), ints(at), n, scale=scale)
     check(got, *tiles64(c, 0, q, at, [0] * n, [p + 1 for p in at], scale=scale))
+
+
+def prompt(jy, pool, io, nh, nkv, hd, n, new, q_size=1.0, first=None, far=2.0**-25, every=7, **kw):
+    """a run of `new` rows behind n - new positions under rules, some of its rows against the definition"""
+    c = Cache(jy, [n], nkv, hd, 32, pool, seed=hd + n)
+    q = (torch.randn((new, nh, hd), generator=gen(4)) * q_size).to(IO16[io])
+    pos = list(range(n - new, n))
+    lo = [0 if first is None else max(0, p - first) for p in pos]
+    mine = dict(kw)
+    if kw.get("slopes") is not None:
+        kw["slopes"] = kw["slopes"].to(DEV)
+    if first is not None:
+        kw["first"] = ints(lo)
+    got = c.pool.attend_rows(c.layer, q.to(DEV), c.dtables, ints([0, new]), ints(pos), n, **kw)
+    some = sorted({0, new - 1, *range(0, new, every)})
+    want, room = tiles64(c, 0, q[some], [pos[r] for r in some], [lo[r] for r in some], [pos[r] + 1 for r in some], far=far, **mine)
+    check(got[some], want, room)
+
+
+@pytest.mark.parametrize("pool", list(POOL))
+@pytest.mark.parametrize("io", list(IO16))
+@pytest.mark.parametrize("cap", [1e3, 1e4, 1e5, 1e6])
+@pytest.mark.parametrize("slopes", [False, True])
+def test_large_caps(jy, pool, io, cap, slopes):
+    """scores that are a small part of the cap keep their digits, on the diagonal and off it"""
+    prompt(jy, pool, io, 8, 2, 64, 300, 200, 2.0, cap=cap, slopes=torch.rand(8, generator=gen(1)) * 0.02 if slopes else None)
+
+
+@pytest.mark.parametrize("pool", list(POOL))
+@pytest.mark.parametrize("io", list(IO16))
+@pytest.mark.parametrize("cap,size", [(30.0, 1.0), (50.0, 1.0), (50.0, 8.0), (6.0, 1.0), (6.0, 2.5), (0.5, 1.0)])
+@pytest.mark.parametrize("scale", [None, -0.1])
+def test_caps_alone(jy, pool, io, cap, size, scale):
+    """scores all within half the cap, some past it, most at it; tiles seen whole among them"""
+    prompt(jy, pool, io, 8, 2, 64, 400, 130, size, cap=cap, scale=scale)
