@@ -502,15 +502,17 @@ __global__ __launch_bounds__(NT, HDT <= 2 ? 2 : 1) void tiled_attend_kernel(Rule
             }
         }
         const bool masked = t0 < w_all_lo || t0 + BN > w_all_hi || there != 15u;
+        // whether the column does not see the position of its score s[n][i]
+        auto outside = [&](int n, int i) {
+            const int j = t0 + 32 * n + 8 * (i >> 2) + 4 * half + (i & 3);
+            return j < lo || j >= hi || !(there >> (2 * n + (i >> 3)) & 1u);
+        };
         auto mask = [&](float none) {
             asm volatile("");  // (a branch)
 #pragma unroll
             for (int n = 0; n < 2; n++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const int j = t0 + 32 * n + 8 * (i >> 2) + 4 * half + (i & 3);
-                    s[n][i] = j < lo || j >= hi || !(there >> (2 * n + (i >> 3)) & 1u) ? none : s[n][i];
-                }
+                for (int i = 0; i < 16; i++) s[n][i] = outside(n, i) ? none : s[n][i];
         };
         auto largest = [&](float sign) {
             float top = -__builtin_inff();
@@ -614,7 +616,12 @@ __global__ __launch_bounds__(NT, HDT <= 2 ? 2 : 1) void tiled_attend_kernel(Rule
                         for (int b = 0; b < 2; b++) {
                             const f4_t x = *reinterpret_cast<const f4_t*>(&sh.vs[buf][32 * n + 16 * c + 8 * b + 4 * half]);
 #pragma unroll
-                            for (int i = 0; i < 4; i++) w[4 * b + i] = masked && !(w[4 * b + i] > 0.0f) ? 0.0f : w[4 * b + i] * x[i];
+                            for (int i = 0; i < 4; i++) w[4 * b + i] *= x[i];
+                        }
+                        if (masked) {  // 0 times a scale that is NaN, where the row does not see it
+                            asm volatile("");
+#pragma unroll
+                            for (int e = 0; e < 8; e++) w[e] = outside(n, 8 * c + e) ? 0.0f : w[e];
                         }
                     }
                     if constexpr (F::PP == 2) {

@@ -79,3 +79,18 @@ def test_large_caps(jy, pool, io, cap, slopes):
 def test_caps_alone(jy, pool, io, cap, size, scale):
     """scores all within half the cap, some past it, most at it; tiles seen whole among them"""
     prompt(jy, pool, io, 8, 2, 64, 400, 130, size, cap=cap, scale=scale)
+
+
+@pytest.mark.parametrize("pool", list(POOL))
+@pytest.mark.parametrize("io", ["f32", "f16", "bf16"])
+def test_a_value_of_no_weight_that_is_not_finite(jy, pool, io):
+    """the rows that see it are NaN all the same, on the diagonal and off it, and no others"""
+    n = 200
+    c = Cache(jy, [n], 2, 64, 16, pool, seed=5)
+    k, v = torch.full((1, 2, 64), -60.0), torch.randn((1, 2, 64), generator=gen(1))
+    v[0, 1] = math.nan
+    c.pool.write(c.layer, k.to(DEV), v.to(DEV), c.dtables, ints([20]))
+    q = torch.ones((n, 8, 64)).to({"f32": torch.float32, **IO16}[io])
+    got = c.pool.attend_rows(c.layer, q.to(DEV), c.dtables, ints([0, n]), ints(list(range(n))), n)
+    assert torch.isfinite(got[:, :4]).all() and torch.isfinite(got[:20]).all()
+    assert torch.isnan(got[20:, 4:]).all()
