@@ -240,8 +240,8 @@ class PagePool:
         if slopes is not None and (slopes.dtype is not b.torch.float32 or slopes.shape != (heads,) or slopes.device != self.device
                                    or not slopes.is_contiguous()):
             raise JyError(f"slopes: {heads} contiguous float32 values on {self.device} are needed")
-        if cap is not None and not cap > 0:
-            raise JyError("cap: a positive number, or None")
+        if cap is not None and not C.c_float(cap).value > 0:  # (a smaller one than fp32 holds would count as none)
+            raise JyError("cap: a positive number that float32 holds, or None")
         return _Rules(0.0 if cap is None else cap, None if slopes is None else slopes.data_ptr(),
                       None if first is None else _indices(b, first, rows, self.device, "first"),
                       None if last is None else _indices(b, last, rows, self.device, "last"))
