@@ -356,7 +356,7 @@ JYHIP_API int jyhip_sample(const void* logits, int type, int rows, int vocab, lo
 JYHIP_API size_t jyhip_sample_workspace(int rows, int vocab);
 
 /* What else makes a score, beside scale q . k:
- *   cap     c > 0: a score s becomes c tanh(s / c), so it stays within +-c (0: as it is)
+ *   cap     c > 0: a score s becomes c tanh(s / c), so it stays within +-c (0: as it is; over 2^64: 2^64)
  *   slopes  fp32 [num_heads]: then slope * |the row's position - the key's| is taken off (NULL: nothing)
  *   first   int32, one per row: positions before it are left out (NULL: none; a window, a document's start)
  *   last    int32, one per row: positions from it on are left out (NULL: those after the row's own; past it

@@ -114,7 +114,7 @@ RuledAttn ruled_args(const jyhip_pages* pages, const jyhip_page_tables* tables, 
         if (rules->cap != 0.0f && !std::isfinite(scale / rules->cap * 4.0f)) fail("scale over the cap must be finite");
         if (((uintptr_t)rules->slopes | (uintptr_t)rules->first | (uintptr_t)rules->last) % 4)
             fail("slopes, first or last are not aligned to their elements");
-        A.soft = rules->cap;
+        A.soft = std::min(rules->cap, 0x1p64f);
         A.slopes = rules->slopes;
         A.first = rules->first;
         A.last = rules->last;

@@ -382,7 +382,9 @@ __global__ __launch_bounds__(256, NC <= 2 ? 2 : 1) void ruled_attend_kernel(Rule
                 amax = 0.0f;
             }
             q.load(x, amax);
-            qf = bad ? __builtin_nanf("") : q.factor(amax) * (A.soft != 0.0f ? A.scale / A.soft : A.scale * kLog2e);
+            qf = q.factor(amax) * (A.soft != 0.0f ? A.scale / A.soft : A.scale * kLog2e);
+            // (a small cap: an infinite factor would make NaN of a score of 0)
+            qf = bad ? __builtin_nanf("") : fminf(fmaxf(qf, -3.402823466e38f), 3.402823466e38f);
         }
         auto at = [&](int i) { return s0 + (wave + 4 * i) * 32; };
         if constexpr (DK) {

@@ -299,6 +299,7 @@ __global__ __launch_bounds__(NT, HDT <= 2 ? 2 : 1) void tiled_attend_kernel(Rule
         // Queries and scales so small that this would be 0, which a masked score of -infinity cannot be multiplied with: raw
         // scores are under 2^40 here, so these scores are 0 either way.
         if constexpr (F::SCALED) qf = fmaxf(qf, 0x1p-126f);
+        qf = fminf(qf, 3.402823466e38f);  // (a small cap: an infinite factor would make NaN of a score of 0)
         if (bad) qf = __builtin_nanf("");
     }
     const bool simple = !(fabsf(A.scale) < 0x1p-60f);
@@ -537,8 +538,8 @@ __global__ __launch_bounds__(NT, HDT <= 2 ? 2 : 1) void tiled_attend_kernel(Rule
         // 0.45 of the cap by the polynomial in five operations; else step by step.
         float top = largest(1.0f);
         int way = A.slopes || (A.soft != 0.0f && masked) || !simple ? 2 : A.soft != 0.0f ? 1 : 0;
-        // (the polynomial's coefficients stay normal numbers for qf from 2^-16 on)
-        if (way == 1 && __any(!(fmaxf(top, largest(-1.0f)) * qf <= kSmall && qf >= 0x1p-16f))) way = 2;
+        // (between these the polynomial's coefficients are finite and normal numbers)
+        if (way == 1 && __any(!(fmaxf(top, largest(-1.0f)) * qf <= kSmall && qf >= 0x1p-16f && qf <= 0x1p16f))) way = 2;
         way = __builtin_amdgcn_readfirstlane(way);
         auto capped = [&](float x, float less) {
             const float x2 = x * x;

@@ -94,3 +94,44 @@ def test_a_value_of_no_weight_that_is_not_finite(jy, pool, io):
     got = c.pool.attend_rows(c.layer, q.to(DEV), c.dtables, ints([0, n]), ints(list(range(n))), n)
     assert torch.isfinite(got[:, :4]).all() and torch.isfinite(got[:20]).all()
     assert torch.isnan(got[20:, 4:]).all()
+
+
+@pytest.mark.parametrize("pool", list(POOL))
+@pytest.mark.parametrize("io", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("single", [False, True])
+def test_caps_at_the_ends_of_their_type(jy, pool, io, single):
+    """tiny caps make every weight the same, of queries of any size and of zeros; huge ones change nothing"""
+    n = 200
+    c = Cache(jy, [n], 2, 64, 16, pool, seed=5)
+    dtype = {"f32": torch.float32, **IO16}[io]
+    kz = torch.zeros((3, 2, 64))
+    c.pool.write(c.layer, kz.to(DEV), torch.ones((3, 2, 64)).to(DEV), c.dtables, ints([4, 90, 150]), ints([0, 0, 0]))
+    at = ints(list(range(n)))
+    k, v = (t.double().cpu() for t in c.pool.read(c.layer, c.dtables, at, ints([0] * n)))
+    c.k[0], c.v[0] = k, v
+    c.va[0] = torch.maximum(c.va[0], v.abs())
+    size = 1.0 if io == "f16" else 1e30
+    rows = [n - 1] if single else list(range(n))
+
+    def run(q, **kw):
+        if single:
+            return c.pool.attend(c.layer, q.to(DEV), c.dtables, c.dlens, n, **kw)
+        return c.pool.attend_rows(c.layer, q.to(DEV), c.dtables, ints([0, n]), at, n, **kw)
+
+    def mean(scores=None):
+        """(want, room) of weights that are all the same, in 32 bits or as one number of 16"""
+        want = torch.stack([v[:r + 1].mean(0) for r in rows]).repeat_interleave(4, 1)
+        room = torch.stack([c.va[0][:r + 1].mean(0) for r in rows]).repeat_interleave(4, 1)
+        # (a 4-bit value is one fp16 number; a weight times an int8 value's scale one bf16 number, or two; weights of 1 are exact)
+        one = 2.0**-8 if pool == "i8" else 2.0**-10
+        return want, room * ((2 * n + 16) * 2.0**-24 + one)
+
+    for cap, x in ((1e-8, 0.0), (1e-20, 0.0), (1e-8, 1.0), (1e-20, size)):
+        q = torch.randn((len(rows), 8, 64), generator=gen(2)).mul(x).to(dtype)
+        check(run(q, cap=cap), *mean())
+    q = torch.randn((len(rows), 8, 64), generator=gen(3)).to(dtype)
+    some = list(range(0, len(rows), 9))
+    pos = [rows[r] for r in some]
+    for cap in (1e9, 1e19, 1e25, 1e36, 3e38):
+        want, room = tiles64(c, 0, q[some], pos, [0] * len(some), [p + 1 for p in pos])
+        check(run(q, cap=cap)[some], want, room)
