@@ -390,7 +390,7 @@ JYHIP_API size_t jyhip_pages_attend_ruled_workspace(const jyhip_pages* pages, in
  * pages.  A row that sees nothing gives zeros; rows before starts[0] and from starts[num_seqs] on are left as they
  * are.  max_len is an upper bound of the positions that any row sees (last, or pos + 1): those past it are cut.
  * Long runs of 16-bit rows take a weight as one number of the second product's type: fp16 over fp16 and 4-bit pages
- * (under 2^-25 of its row's largest it may count as 0; a 4-bit value is rounded to fp16 there), else bf16, in two
+ * (under 2^-34 of its row's largest it may count as 0; a 4-bit value is rounded to fp16 there), else bf16, in two
  * parts where the outputs are fp16; sums are fp32.  Which runs are long is decided by the call's rows, query heads and
  * sequences.  What is not finite: as with single rows, for each row by what it sees.  rows x num_heads is less than 2^22. */
 JYHIP_API int jyhip_pages_attend_rows(const jyhip_pages* pages, const jyhip_page_tables* tables, const int* starts,

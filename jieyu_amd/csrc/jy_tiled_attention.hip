@@ -138,6 +138,9 @@ struct Form {
     static constexpr int QP = BF && !BIO ? 2 : 1;              // parts of a query
     static constexpr int PP = (BF || I8) && !BIO ? 2 : 1;      // of a weight
     static constexpr bool SCALED = (F16 && BIO) || I4;         // queries by a power of two
+    // Weights, at most 2^6 as the maximum moves late, by this power of two more, in outputs and sums alike: fp16 ones then
+    // reach 2^15, and lose digits only from 2^-23 of the largest down.
+    static constexpr float LIFT = VBF ? 0.0f : 9.0f;
     static constexpr int HD = 64 * HDT, ROW = 2 * HD;          // elements and bytes of a staged row
     static constexpr int MASK = HDT == 1 ? 7 : 15;             // of a key's bits that move its chunks of 16 bytes
     static constexpr int G = HDT == 1 ? 2 : HDT == 2 ? 4 : 8;  // groups of a 4-bit vector
@@ -587,17 +590,18 @@ __global__ __launch_bounds__(NT, HDT <= 2 ? 2 : 1) void tiled_attend_kernel(Rule
 #pragma unroll
                 for (int i = 0; i < 16; i++) o[t][i] *= a;
         }
+        const float less = F::LIFT - m;
 #pragma unroll
         for (int n = 0; n < 2; n++) {
             if (way == 0) {
 #pragma unroll
-                for (int i = 0; i < 16; i++) s[n][i] = __builtin_fmaf(s[n][i], qf, -m);
+                for (int i = 0; i < 16; i++) s[n][i] = __builtin_fmaf(s[n][i], qf, less);
             } else if (way == 1) {
 #pragma unroll
-                for (int i = 0; i < 16; i++) s[n][i] = capped(s[n][i], -m);
+                for (int i = 0; i < 16; i++) s[n][i] = capped(s[n][i], less);
             } else {
 #pragma unroll
-                for (int i = 0; i < 16; i++) s[n][i] -= m;
+                for (int i = 0; i < 16; i++) s[n][i] += less;
             }
         }
         const char* const vs = reinterpret_cast<const char*>(sh.v[buf]);

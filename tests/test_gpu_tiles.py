@@ -135,3 +135,30 @@ def test_caps_at_the_ends_of_their_type(jy, pool, io, single):
     for cap in (1e9, 1e19, 1e25, 1e36, 3e38):
         want, room = tiles64(c, 0, q[some], pos, [0] * len(some), [p + 1 for p in pos])
         check(run(q, cap=cap)[some], want, room)
+
+
+@pytest.mark.parametrize("pool", list(POOL))
+@pytest.mark.parametrize("io", list(IO16))
+@pytest.mark.parametrize("below", [15, 20, 26, 30])
+def test_many_small_weights_beside_a_large_one(jy, pool, io, below):
+    """thousands of positions of 2^-below of the largest weight each, which alone make some dims of the output"""
+    n, new, hd = 6000, 40, 64
+    c = Cache(jy, [n], 1, hd, 256, pool, seed=2)
+    k, v = torch.zeros((n, 1, hd)), torch.zeros((n, 1, hd))
+    k[7, 0, 0] = 1.0
+    v[:, 0, :32] = torch.rand((n, 32), generator=gen(1)) + 1.0
+    v[7, 0, :32], v[7, 0, 32:] = 0.0, 1.0
+    at = ints(list(range(n)))
+    c.pool.write(c.layer, k.to(DEV), v.to(DEV), c.dtables, at, ints([0] * n))
+    c.k[0], c.v[0] = (t.double().cpu() for t in c.pool.read(c.layer, c.dtables, at, ints([0] * n)))
+    c.ka[0] = c.k[0].abs()
+    c.va[0] = c.v[0].abs()  # (a 4-bit group here: its low 0 or 1, a number times a step of at most 1)
+    q = torch.zeros((new, 1, hd))
+    q[:, :, 0] = below * math.log(2.0)
+    q = q.repeat(1, 4, 1).to(IO16[io])
+    pos = list(range(n - new, n))
+    got = c.pool.attend_rows(c.layer, q.to(DEV), c.dtables, ints([0, new]), ints(pos), n, scale=1.0)
+    some = [0, 1, 17, new - 1]
+    want, room = tiles64(c, 0, q[some], [pos[r] for r in some], [0] * 4, [pos[r] + 1 for r in some], far=2.0**-34, scale=1.0)
+    # (dims of the small ones alone: the large one's value there is 0, so that `far` counts the small values alone)
+    check(got[some], want, room)
