@@ -10,9 +10,9 @@
 // each group lies beside the others (byte r G + g of the vector, G groups), so a lane's bytes are one store,
 // and the attention's lanes, which take a vector's dims in the same shares, one load.  A group's lowest and
 // largest take four DPP moves within the row of lanes, and lane i works out the words of one of the key's and
-// the value's groups (each lane dividing for itself: 29 us against 25 for 8191 rows of 8 heads of 128 in bf16,
-// which read 34 MB and write 10).  Its vector instructions bound the write; the same rows read back take 13 us,
-// 3.4 TB/s.
+// the value's groups (each lane dividing for itself took 16% longer).  8191 rows of 8 heads of 128 in bf16, which read
+// 34 MB and write 10: 20.5 us from launch to launch, bound by vector instructions; two vectors a group of lanes, with more
+// loads under way, took 25.7, and 91.6 against 76 for 32768 rows.  The same rows read back take 12 us, 3.6 TB/s.
 #include <hip/hip_runtime.h>
 
 #include "jy_device.h"
@@ -57,22 +57,30 @@ __device__ __forceinline__ float seven_bits(float x) {
 template <int G>
 using bytes_t = uint8_t __attribute__((ext_vector_type(G)));
 
+// (one branch around all loads: around each, every one is waited for before the next)
 template <class E, int G>
-__device__ __forceinline__ void load_pairs(const E* p, int hd, bool pairs, float (&x)[2 * G]) {
+__device__ __forceinline__ void load_pairs(const E* k, const E* v, int hd, bool pairs, float (&x)[2][2 * G]) {
     const int r2 = (threadIdx.x & 15) * 2;
-#pragma unroll
-    for (int g = 0; g < G; g++) {
+    auto at = [&](int s, int g) {
         const int d = 32 * g + r2;
-        const E* const at = p + (d < hd ? d : 0);  // (hd is a multiple of 16)
-        if (pairs) {
-            typedef E two __attribute__((ext_vector_type(2)));
-            const two v = *reinterpret_cast<const two*>(at);
-            x[2 * g] = (float)v[0];
-            x[2 * g + 1] = (float)v[1];
-        } else {
-            x[2 * g] = (float)at[0];
-            x[2 * g + 1] = (float)at[1];
-        }
+        return (s ? v : k) + (d < hd ? d : 0);  // (hd is a multiple of 16)
+    };
+    if (pairs) {
+        typedef E two __attribute__((ext_vector_type(2)));
+        two y[2][G];
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int g = 0; g < G; g++) y[s][g] = *reinterpret_cast<const two*>(at(s, g));
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int e = 0; e < 2 * G; e++) x[s][e] = (float)y[s][e / 2][e % 2];
+    } else {
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int e = 0; e < 2 * G; e++) x[s][e] = (float)at(s, e / 2)[e % 2];
     }
 }
 
@@ -111,7 +119,8 @@ __device__ __forceinline__ void hold4(const jyhip_pages& P, int64_t vec, const f
         for (int g = 0; g < G; g++) {
             const bool on = 32 * g + 2 * r < hd;
             const float a = x[s][2 * g], b = x[s][2 * g + 1];
-            past[s] = on && !(fmaxf(fabsf(a), fabsf(b)) <= kMax4 && a == a && b == b) ? 1.0f : past[s];
+            // (without branches)
+            past[s] = on & !((fmaxf(fabsf(a), fabsf(b)) <= kMax4) & (a == a) & (b == b)) ? 1.0f : past[s];
             const float least = row_min(on ? fminf(a, b) : __builtin_inff());
             const float most = row_max(on ? fmaxf(a, b) : -__builtin_inff());
             lo = r == s * G + g ? least : lo;
@@ -131,7 +140,7 @@ __device__ __forceinline__ void hold4(const jyhip_pages& P, int64_t vec, const f
     for (int s = 0; s < 2; s++) {
         bytes_t<G> b;
 #pragma unroll
-        for (int g = 0; g < G; g++) b[g] = 32 * g + 2 * r < hd && !(past[s] > 0.0f) ? bytes[s][g] : (uint8_t)0;
+        for (int g = 0; g < G; g++) b[g] = (32 * g + 2 * r < hd) & !(past[s] > 0.0f) ? bytes[s][g] : (uint8_t)0;
         *reinterpret_cast<bytes_t<G>*>(static_cast<uint8_t*>(s ? P.v : P.k) + vec * (16 * G) + r * G) = b;
     }
     if (r < 2 * G) reinterpret_cast<uint32_t*>(second ? P.v_scale : P.k_scale)[vec * G + r % G] = word;
@@ -173,39 +182,25 @@ __device__ __forceinline__ void give4(const void* pool, const void* scales, int6
     }
 }
 
-// 16 lanes take VECS vectors: what the later ones wait for is under way with the first's
-template <class E, int G, bool WRITE, int VECS>
+template <class E, int G, bool WRITE>
 __global__ __launch_bounds__(256) void paged4_kernel(Moved4 A, bool pairs) {
     const jyhip_pages& P = A.P;
-    const unsigned i0 = (blockIdx.x * 16 + (threadIdx.x >> 4)) * VECS, nkv = P.num_kv_heads, total = A.rows * nkv;
-    E *k[VECS], *v[VECS];
-    int64_t vec[VECS];
-#pragma unroll
-    for (int c = 0; c < VECS; c++) {
-        const unsigned i = i0 + c < total ? i0 + c : total - 1;
-        const int row = (int)(i / nkv), head = (int)(i - row * nkv);
-        k[c] = static_cast<E*>(A.k.data) + row * A.k.row_stride + head * A.k.head_stride;
-        v[c] = static_cast<E*>(A.v.data) + row * A.v.row_stride + head * A.v.head_stride;
-        const int64_t slot = slot_of(A.M, P.num_pages, A.ps_log2, A.M.seq ? A.M.seq[row] : row, A.M.pos[row]);
-        vec[c] = slot < 0 ? -1 : (((slot >> A.ps_log2) * nkv + head) << A.ps_log2) + (slot & ((1 << A.ps_log2) - 1));
-    }
+    const unsigned at = blockIdx.x * 16 + (threadIdx.x >> 4), nkv = P.num_kv_heads, total = A.rows * nkv;
+    const unsigned i = min(at, total - 1);  // (lanes past the end look at the last vector)
+    const int row = (int)(i / nkv), head = (int)(i - row * nkv);
+    E* const k = static_cast<E*>(A.k.data) + row * A.k.row_stride + head * A.k.head_stride;
+    E* const v = static_cast<E*>(A.v.data) + row * A.v.row_stride + head * A.v.head_stride;
+    const int64_t slot = slot_of(A.M, P.num_pages, A.ps_log2, A.M.seq ? A.M.seq[row] : row, A.M.pos[row]);
+    const int64_t vec =
+        slot < 0 ? -1 : (((slot >> A.ps_log2) * nkv + head) << A.ps_log2) + (slot & ((1 << A.ps_log2) - 1));
     if constexpr (WRITE) {
-        float x[VECS][2][2 * G];
-#pragma unroll
-        for (int c = 0; c < VECS; c++) {
-            load_pairs<E, G>(k[c], P.head_dim, pairs, x[c][0]);
-            load_pairs<E, G>(v[c], P.head_dim, pairs, x[c][1]);
-        }
-#pragma unroll
-        for (int c = 0; c < VECS; c++)
-            if (vec[c] >= 0 && i0 + c < total) hold4<G>(P, vec[c], x[c]);
+        float x[2][2 * G];
+        load_pairs<E, G>(k, v, P.head_dim, pairs, x);
+        if (vec >= 0 && at < total) hold4<G>(P, vec, x);
     } else {
-#pragma unroll
-        for (int c = 0; c < VECS; c++) {
-            if (i0 + c >= total) return;
-            give4<E, G>(P.k, P.k_scale, vec[c], P.head_dim, k[c], pairs);
-            give4<E, G>(P.v, P.v_scale, vec[c], P.head_dim, v[c], pairs);
-        }
+        if (at >= total) return;
+        give4<E, G>(P.k, P.k_scale, vec, P.head_dim, k, pairs);
+        give4<E, G>(P.v, P.v_scale, vec, P.head_dim, v, pairs);
     }
 }
 
@@ -215,41 +210,39 @@ bool paired(const jyhip_vectors& x, int type) {
     return ((uintptr_t)x.data | (uintptr_t)(x.row_stride * e) | (uintptr_t)(x.head_stride * e)) % (2 * e) == 0;
 }
 
-template <class E, bool WRITE, int VECS>
+template <class E, bool WRITE>
 void launch_groups(const Moved4& A, bool pairs, unsigned grid, hipStream_t st) {
     switch (groups4(A.P.head_dim)) {
-        case 2: paged4_kernel<E, 2, WRITE, VECS><<<grid, 256, 0, st>>>(A, pairs); break;
-        case 4: paged4_kernel<E, 4, WRITE, VECS><<<grid, 256, 0, st>>>(A, pairs); break;
-        default: paged4_kernel<E, 8, WRITE, VECS><<<grid, 256, 0, st>>>(A, pairs);
+        case 2: paged4_kernel<E, 2, WRITE><<<grid, 256, 0, st>>>(A, pairs); break;
+        case 4: paged4_kernel<E, 4, WRITE><<<grid, 256, 0, st>>>(A, pairs); break;
+        default: paged4_kernel<E, 8, WRITE><<<grid, 256, 0, st>>>(A, pairs);
     }
 }
 
-template <bool WRITE, int VECS>
-void launch_vectors(const Moved4& A, int type, hipStream_t st) {
-    const bool pairs = paired(A.k, type) && paired(A.v, type);
-    const unsigned grid = (unsigned)(((int64_t)A.rows * A.P.num_kv_heads + 16 * VECS - 1) / (16 * VECS));
+template <bool WRITE>
+void launch_moved4(const jyhip_pages& P, const PageMap& M, int rows, const jyhip_vectors& k, const jyhip_vectors& v,
+                   int type, hipStream_t st) {
+    const Moved4 A{P, M, rows, __builtin_ctz(P.page_size), k, v};
+    const bool pairs = paired(k, type) && paired(v, type);
+    const unsigned grid = (unsigned)(((int64_t)rows * P.num_kv_heads + 15) / 16);
     if (type == JYHIP_T_F32)
-        launch_groups<float, WRITE, VECS>(A, pairs, grid, st);
+        launch_groups<float, WRITE>(A, pairs, grid, st);
     else if (type == JYHIP_T_F16)
-        launch_groups<_Float16, WRITE, VECS>(A, pairs, grid, st);
+        launch_groups<_Float16, WRITE>(A, pairs, grid, st);
     else
-        launch_groups<__bf16, WRITE, VECS>(A, pairs, grid, st);
+        launch_groups<__bf16, WRITE>(A, pairs, grid, st);
 }
 
 }  // namespace
 
 void launch_paged4_write(const jyhip_pages& P, const PageMap& M, int rows, const jyhip_vectors& k,
                          const jyhip_vectors& v, int type, hipStream_t st) {
-    const Moved4 A{P, M, rows, __builtin_ctz(P.page_size), k, v};
-    if ((int64_t)rows * P.num_kv_heads >= 32768)
-        launch_vectors<true, 2>(A, type, st);
-    else
-        launch_vectors<true, 1>(A, type, st);
+    launch_moved4<true>(P, M, rows, k, v, type, st);
 }
 
 void launch_paged4_read(const jyhip_pages& P, const PageMap& M, int rows, const jyhip_vectors& k,
                         const jyhip_vectors& v, int type, hipStream_t st) {
-    launch_vectors<false, 1>(Moved4{P, M, rows, __builtin_ctz(P.page_size), k, v}, type, st);
+    launch_moved4<false>(P, M, rows, k, v, type, st);
 }
 
 }  // namespace jy
