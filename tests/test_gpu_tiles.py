@@ -162,3 +162,45 @@ def test_many_small_weights_beside_a_large_one(jy, pool, io, below):
     want, room = tiles64(c, 0, q[some], [pos[r] for r in some], [0] * 4, [pos[r] + 1 for r in some], far=2.0**-34, scale=1.0)
     # (dims of the small ones alone: the large one's value there is 0, so that `far` counts the small values alone)
     check(got[some], want, room)
+
+
+@pytest.mark.parametrize("pool", list(POOL))
+@pytest.mark.parametrize("io", list(IO16))
+@pytest.mark.parametrize("rule", ["none", "slopes", "first", "scale", "rising"])
+def test_each_rule_alone(jy, pool, io, rule):
+    """tiles seen whole and tiles that are cut, under one rule at a time"""
+    kw = {}
+    if rule == "slopes":
+        kw = dict(slopes=torch.tensor([0.0, 0.5, -0.01, 0.03, 1.0, 0.002, 0.1, 0.004]))
+    if rule == "first":
+        kw = dict(first=150)
+    if rule == "scale":
+        kw = dict(scale=-0.2)
+    if rule == "rising":  # the maximum grows from tile to tile
+        kw = dict(slopes=torch.full((8,), 0.2))
+    prompt(jy, pool, io, 8, 2, 64, 500, 140, 1.5, **kw)
+
+
+@pytest.mark.parametrize("pool", list(POOL))
+@pytest.mark.parametrize("io", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows", [512, 1000])
+def test_a_prompt_beside_single_tokens(jy, pool, io, rows):
+    """one prompt and 63 sequences of one new token in a call: whichever kernel the call's average columns choose"""
+    g = gen(rows)
+    past = [0] + torch.randint(0, 700, (63,), generator=g).tolist()
+    new = [rows] + [1] * 63
+    lens = [a + b for a, b in zip(past, new)]
+    c = Cache(jy, lens, 2, 64, 32, pool, seed=rows)
+    q = torch.randn((sum(new), 8, 64), generator=g).to({"f32": torch.float32, **IO16}[io])
+    starts = [0]
+    for a in new:
+        starts.append(starts[-1] + a)
+    pos = [i for n, a in zip(lens, new) for i in range(n - a, n)]
+    got = c.pool.attend_rows(c.layer, q.to(DEV), c.dtables, ints(starts), ints(pos), max(lens))
+    for b in range(64):
+        some = list(range(0, rows, 37)) + [rows - 1] if b == 0 else [starts[b]]
+        at = [pos[r] for r in some]
+        want, room = tiles64(c, b, q[some], at, [0] * len(at), [p + 1 for p in at])
+        check(got[some], want, room)
+    again = c.pool.attend_rows(c.layer, q.to(DEV), c.dtables, ints(starts), ints(pos), max(lens))
+    assert torch.equal(got, again)
