@@ -485,6 +485,7 @@ __global__ __launch_bounds__(NT, HDT <= 2 ? 2 : 1) void tiled_attend_kernel(Rule
 
     f16_t o[F::DT];
     float m, l;
+    bool far;  // the wave has a running maximum past 2^20
     // one tile from LDS
     auto work = [&](int buf, int t0, uint32_t there) {
         const char* const ks = reinterpret_cast<const char*>(sh.k[buf]);
@@ -540,7 +541,7 @@ __global__ __launch_bounds__(NT, HDT <= 2 ? 2 : 1) void tiled_attend_kernel(Rule
         // where the scale is 0 or close to it, as -infinity cannot be multiplied with 0); capped ones that are all within
         // 0.45 of the cap by the polynomial in five operations; else step by step.
         float top = largest(1.0f);
-        int way = A.slopes || (A.soft != 0.0f && masked) || !simple ? 2 : A.soft != 0.0f ? 1 : 0;
+        int way = A.slopes || (A.soft != 0.0f && masked) || !simple || far ? 2 : A.soft != 0.0f ? 1 : 0;
         // (between these the polynomial's coefficients are finite and normal numbers)
         if (way == 1 && __any(!(fmaxf(top, largest(-1.0f)) * qf <= kSmall && qf >= 0x1p-16f && qf <= 0x1p16f))) way = 2;
         way = __builtin_amdgcn_readfirstlane(way);
@@ -580,10 +581,20 @@ __global__ __launch_bounds__(NT, HDT <= 2 ? 2 : 1) void tiled_attend_kernel(Rule
         if (way == 2 || masked) top = largest(1.0f);
         top = way == 2 ? top : way == 1 ? capped(top, 0.0f) : top * qf;
         // the running maximum moves when the tile's is over it by more than 2^6, and at first
-        if (__any(top > m + 6.0f)) {
-            const float mn = top > m + 6.0f ? top : m;
+        if (__any(top - m > 6.0f)) {
+            const float mn = top - m > 6.0f ? top : m;
             const float a = exp2_hw(m - mn);
             m = mn;
+            // Past 2^20 scores are rounded before the maximum is taken off: it is one of them, and what it lost by its own
+            // rounding, which grows with it, must not be left over as an exponent.
+            far = __any(fabsf(m) > 0x1p20f && m > kNone);
+            if (__builtin_expect(far && way != 2, 0)) {
+#pragma unroll
+                for (int n = 0; n < 2; n++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) s[n][i] = way == 1 ? capped(s[n][i], 0.0f) : s[n][i] * qf;
+                way = 2;
+            }
             l *= a;
 #pragma unroll
             for (int t = 0; t < F::DT; t++)
@@ -599,9 +610,12 @@ __global__ __launch_bounds__(NT, HDT <= 2 ? 2 : 1) void tiled_attend_kernel(Rule
             } else if (way == 1) {
 #pragma unroll
                 for (int i = 0; i < 16; i++) s[n][i] = capped(s[n][i], less);
-            } else {
+            } else if (__builtin_expect(!far, 1)) {
 #pragma unroll
                 for (int i = 0; i < 16; i++) s[n][i] += less;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; i++) s[n][i] = (s[n][i] - m) + F::LIFT;
             }
         }
         const char* const vs = reinterpret_cast<const char*>(sh.v[buf]);
@@ -674,6 +688,7 @@ __global__ __launch_bounds__(NT, HDT <= 2 ? 2 : 1) void tiled_attend_kernel(Rule
         for (int t = 0; t < F::DT; t++) o[t] = f16_t{};
         m = kNone;
         l = 0.0f;
+        far = false;
         bool odd = false;
         Staged<F> g;
         int ids = -1, next = -1;  // the pages of this tile and of the next

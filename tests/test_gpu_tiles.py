@@ -204,3 +204,37 @@ def test_a_prompt_beside_single_tokens(jy, pool, io, rows):
         check(got[some], want, room)
     again = c.pool.attend_rows(c.layer, q.to(DEV), c.dtables, ints(starts), ints(pos), max(lens))
     assert torch.equal(got, again)
+
+
+@pytest.mark.parametrize("pool", list(POOL))
+@pytest.mark.parametrize("io", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("power", [0, 8, 14, 20, 26, 50, 100])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("cap", [None, 1e9])
+def test_scores_of_any_size(jy, pool, io, power, sign, cap):
+    """scores far apart and up to 2^114, above or under 0: the row is the value of its largest (a cap keeps their order,
+    or makes the largest ones the same where they are past it)"""
+    n = 300
+    if cap and power > 14:
+        pytest.skip("scores past the cap are all the same")
+    c = Cache(jy, [n], 1, 64, 32, pool, seed=6)
+    a = torch.randperm(n, generator=gen(power)).float() % 150 + 1.0
+    k = (sign * a)[:, None, None].expand(n, 1, 64).contiguous()
+    v = torch.randn((n, 1, 64), generator=gen(2))
+    at = ints(list(range(n)))
+    c.pool.write(c.layer, k.to(DEV), v.to(DEV), c.dtables, at, ints([0] * n))
+    v = c.pool.read(c.layer, c.dtables, at, ints([0] * n))[1].double().cpu()
+    q = torch.ones((n, 4, 64)).to({"f32": torch.float32, **IO16}[io])
+    got = c.pool.attend_rows(c.layer, q.to(DEV), c.dtables, ints([0, n]), at, n, scale=2.0**power, cap=cap)
+    assert torch.isfinite(got).all()
+    # Scores are 64 2^power a: of two that differ the smaller is 1/150 and more below, 64 and more.  Equal ones share; a cap's
+    # tanh is off by 8 steps of 2^-24 of a score of 10^8, that is 50, in tiles that are cut and others by different steps, so
+    # there equal ones may weigh anything, and the row lies between their values.
+    for r in range(n):
+        top = (sign * a[:r + 1])
+        equal = v[:r + 1][top == top.max()]
+        # (at most two share: their weights are the same number; 4-bit values are one fp16 number in tiles)
+        limit = (2.0**-9 + {torch.float16: 2.0**-11, torch.bfloat16: 2.0**-8}.get(q.dtype, 0)) * v[:r + 1].abs().amax()
+        if cap:
+            limit = limit + (equal.amax(0) - equal.amin(0)) / 2
+        assert ((got[r].double().cpu() - equal.mean(0)).abs() <= limit).all(), r
