@@ -139,8 +139,9 @@ struct Form {
     static constexpr int PP = (BF || I8) && !BIO ? 2 : 1;      // of a weight
     static constexpr bool SCALED = (F16 && BIO) || I4;         // queries by a power of two
     // Weights, at most 2^6 as the maximum moves late, by this power of two more, in outputs and sums alike: fp16 ones then
-    // reach 2^15, and lose digits only from 2^-23 of the largest down.
-    static constexpr float LIFT = VBF ? 0.0f : 9.0f;
+    // reach 2^15, and lose digits only from 2^-23 of the largest down; bf16 ones reach 1, so that they times a value stay
+    // finite where the value is.
+    static constexpr float LIFT = VBF ? -6.0f : 9.0f;
     static constexpr int HD = 64 * HDT, ROW = 2 * HD;          // elements and bytes of a staged row
     static constexpr int MASK = HDT == 1 ? 7 : 15;             // of a key's bits that move its chunks of 16 bytes
     static constexpr int G = HDT == 1 ? 2 : HDT == 2 ? 4 : 8;  // groups of a 4-bit vector

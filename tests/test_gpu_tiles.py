@@ -208,15 +208,12 @@ def test_a_prompt_beside_single_tokens(jy, pool, io, rows):
 
 @pytest.mark.parametrize("pool", list(POOL))
 @pytest.mark.parametrize("io", ["f32", "f16", "bf16"])
-@pytest.mark.parametrize("power", [0, 8, 14, 20, 26, 50, 100])
+@pytest.mark.parametrize("power,cap", [(0, None), (8, None), (14, None), (20, None), (26, None), (50, None), (100, None),
+                                       (0, 1e9), (8, 1e9), (14, 1e9)])
 @pytest.mark.parametrize("sign", [1, -1])
-@pytest.mark.parametrize("cap", [None, 1e9])
 def test_scores_of_any_size(jy, pool, io, power, sign, cap):
-    """scores far apart and up to 2^114, above or under 0: the row is the value of its largest (a cap keeps their order,
-    or makes the largest ones the same where they are past it)"""
+    """scores far apart and up to 2^114, above or under 0, within a cap: the row is the value of its largest"""
     n = 300
-    if cap and power > 14:
-        pytest.skip("scores past the cap are all the same")
     c = Cache(jy, [n], 1, 64, 32, pool, seed=6)
     a = torch.randperm(n, generator=gen(power)).float() % 150 + 1.0
     k = (sign * a)[:, None, None].expand(n, 1, 64).contiguous()
@@ -238,3 +235,25 @@ def test_scores_of_any_size(jy, pool, io, power, sign, cap):
         if cap:
             limit = limit + (equal.amax(0) - equal.amin(0)) / 2
         assert ((got[r].double().cpu() - equal.mean(0)).abs() <= limit).all(), r
+
+
+@pytest.mark.parametrize("pool", ["bf16", "i8"])
+@pytest.mark.parametrize("below", [0.5, 3.0, 5.5, 7.0])
+def test_large_values_of_the_largest_weight(jy, pool, below):
+    """a value near the type's largest number that weighs a little more than what came before it"""
+    n = 200
+    c = Cache(jy, [n], 1, 64, 32, pool, seed=6)
+    k, v = torch.zeros((n, 1, 64)), torch.zeros((n, 1, 64))
+    k[100, 0, 0] = 1.0
+    v[100] = 1e38
+    at = ints(list(range(n)))
+    c.pool.write(c.layer, k.to(DEV), v.to(DEV), c.dtables, at, ints([0] * n))
+    c.k[0], c.v[0] = (t.double().cpu() for t in c.pool.read(c.layer, c.dtables, at, ints([0] * n)))
+    c.ka[0], c.va[0] = c.k[0].abs(), c.v[0].abs()
+    q = torch.zeros((n, 4, 64))
+    q[:, :, 0] = below * math.log(2.0)
+    q = q.bfloat16()
+    pos = list(range(n))
+    got = c.pool.attend_rows(c.layer, q.to(DEV), c.dtables, ints([0, n]), at, n, scale=1.0)
+    want, room = tiles64(c, 0, q, pos, [0] * n, [p + 1 for p in pos], scale=1.0)
+    check(got, want, room)
