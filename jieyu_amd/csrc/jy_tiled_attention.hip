@@ -602,7 +602,14 @@ __global__ __launch_bounds__(NT, HDT <= 2 ? 2 : 1) void tiled_attend_kernel(Rule
 #pragma unroll
                 for (int i = 0; i < 16; i++) o[t][i] *= a;
         }
-        const float less = F::LIFT - m;
+        float less = F::LIFT - m;
+        if (__builtin_expect(far, 0)) {  // (always way 2)
+            less = F::LIFT;
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) s[n][i] -= m;
+        }
 #pragma unroll
         for (int n = 0; n < 2; n++) {
             if (way == 0) {
@@ -611,12 +618,9 @@ __global__ __launch_bounds__(NT, HDT <= 2 ? 2 : 1) void tiled_attend_kernel(Rule
             } else if (way == 1) {
 #pragma unroll
                 for (int i = 0; i < 16; i++) s[n][i] = capped(s[n][i], less);
-            } else if (__builtin_expect(!far, 1)) {
-#pragma unroll
-                for (int i = 0; i < 16; i++) s[n][i] += less;
             } else {
 #pragma unroll
-                for (int i = 0; i < 16; i++) s[n][i] = (s[n][i] - m) + F::LIFT;
+                for (int i = 0; i < 16; i++) s[n][i] += less;
             }
         }
         const char* const vs = reinterpret_cast<const char*>(sh.v[buf]);
