@@ -6,7 +6,7 @@
 //
 // The angle is an fp64 product: at position 2^20 an fp32 one would be off by 2^-4.  It is reduced to
 // [-pi/4, pi/4] in fp64 (pi/2 in two parts) and from there on fp32 Taylor polynomials do (their
-// remainders are under 2^-27).  That is 40 fp64 operations a pair, for 32 to 64 pairs a row; everything
+// remainders are under 2^-27).  That is some fifteen fp64 operations a pair, for 32 to 64 pairs a row; everything
 // else is one read and one write of the heads, so memory bounds long calls and the launch short ones: 8191 rows of
 // 32 + 8 heads of 128 in bf16 30 us (168 MB, 5.6 TB/s), one row of 14 + 2 heads of 64 2 us.
 #include <hip/hip_runtime.h>

@@ -16,7 +16,7 @@
 // The weights of single rows need the softmax's final maximum and sum: the scores go to the workspace (a
 // sixteenth of an int8 cache's bytes at four query heads a kv head), and a last kernel adds up what they weigh.
 //
-// 64 sequences of 200 to 8190, 32 heads over 8 of 128, 4 bits: 75 to 81 us, 2.5 TB/s (4.1 where all are of one
+// 64 sequences of 200 to 8190, 32 heads over 8 of 128, 4 bits: 71 to 81 us, 2.5 TB/s (4.1 where all are of one
 // length: in the ragged batch the longest end alone); the vector instructions of a tile are as long as its loads.
 // 8 of 1000 to 16001 in int8 with cap and weights: 46 us, 4.9 of join, 6.3 of weighing.  77 drafted rows of 16
 // sequences behind 4000 positions in int8: 35 us.

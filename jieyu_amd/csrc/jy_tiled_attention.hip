@@ -18,16 +18,19 @@
 // in two bf16 parts (fp16 ones).  int8 pages: the whole numbers, exact in 16 bits; a key's scale multiplies its
 // scores, a value's its weight, which is carried in bf16 (in two parts for fp16 outputs).  4-bit pages: a key's
 // number times step, exact in fp16, its low by one more product with the query's sums over the groups; a value
-// rounded to fp16.  A weight is rounded to the product's 16 bits, and the sum adds up what was rounded (over int8
-// values the weights themselves).
+// rounded to fp16, once more than its outputs are.  A weight is rounded to the product's 16 bits, and the sum adds up
+// what was rounded (over int8 values the weights themselves), so that only the roundings' differences are left: for bf16
+// outputs bf16 weights are off 2.1e-3 of the largest output from the formula in 64 bits where the outputs' own rounding
+// alone leaves 1.6e-3.  Two bf16 parts leave 1.6e-3 and take 1111 us for 850 (the prompt below).
 //
 // What a row does not see has to leave it alone even where its values are not finite (0 times that is NaN).
 // Positions that no row of the workgroup sees are staged as zeros.  Where some rows see a tile whole and others do not
 // (on the diagonal) and a value in it is not finite, the workgroup starts again row by row, staging what each sees.
 //
-// A prompt of 8191 rows, 32 heads over 8 of 128, bf16, cap 30: 839 us, 655 TFLOP/s (a large product: 1335).  A tile
-// is 1024 cycles of matrix instructions a wave and 1950 of vector ones (15 a score with a cap), and only the two
-// workgroups of a CU cover each other.
+// A prompt of 8191 rows, 32 heads over 8 of 128, bf16, cap 30: 840 to 890 us from card to card, 620 to 655 TFLOP/s (a
+// large product: 1335); over int8 without a cap 767.  A tile is 1024 cycles of matrix instructions a wave and 1950 of
+// vector ones (15 a score with a cap), each wave reads all of it from LDS, and only the two workgroups of a CU cover
+// each other.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
